@@ -44,7 +44,6 @@
  *   tile_pack_kernel, dequant_tiled_kernel, quantize_kernel: the load-time re-layout and the
  *                       checks of it
  */
-#include <hip/hip_ext.h>
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -55,9 +54,36 @@
 #include <mutex>
 
 #include "common.h"
+#include "launch.h"
 #include "rows_shape.h"
 
 using namespace w4a16;
+
+namespace w4a16 {
+
+thread_local hipEvent_t t_next_launch_events[2] = {nullptr, nullptr};
+thread_local int t_launches_to_skip = 0;
+
+int hip_status(hipError_t e, const char *what) {
+    if (e == hipSuccess) return W4A16_OK;
+    return set_error(W4A16_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
+}
+
+int device_cus() {
+    static int cus[64] = {0};
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+    if (cus[dev] == 0) {
+        int n = 0;
+        if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess ||
+            n <= 0)
+            n = 256;
+        cus[dev] = n;
+    }
+    return cus[dev];
+}
+
+} // namespace w4a16
 
 namespace {
 
@@ -2223,34 +2249,6 @@ __global__ __launch_bounds__(256) void quantize_kernel(const float *__restrict__
     }
 }
 
-int hip_status(hipError_t e, const char *what) {
-    if (e == hipSuccess) return W4A16_OK;
-    return set_error(W4A16_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
-}
-
-/* Events that time one of the calling thread's next kernel launches (w4a16_time_next_launch): it
- * goes through hipExtLaunchKernel, whose events take the dispatch's own start and end times
- * (the times a kernel trace reports), and the pair is then forgotten. */
-thread_local hipEvent_t t_next_launch_events[2] = {nullptr, nullptr};
-thread_local int t_launches_to_skip = 0;
-
-template <typename... Params, typename... Args>
-void launch_k(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, hipStream_t stream,
-              Args... args) {
-    hipEvent_t start = t_next_launch_events[0], stop = t_next_launch_events[1];
-    if ((start || stop) && t_launches_to_skip > 0) {
-        --t_launches_to_skip;
-        start = stop = nullptr;
-    }
-    if (start || stop) {
-        t_next_launch_events[0] = t_next_launch_events[1] = nullptr;
-        hipExtLaunchKernelGGL(kernel, grid, block, (uint32_t)smem, stream, start, stop, 0u,
-                              static_cast<Params>(args)...);
-    } else {
-        hipLaunchKernelGGL(kernel, grid, block, smem, stream, static_cast<Params>(args)...);
-    }
-}
-
 int grid_for(long long work, int block) {
     long long g = (work + block - 1) / block;
     if (g > 65535LL * 16) g = 65535LL * 16;
@@ -2454,8 +2452,6 @@ int launch_rows16_nl(const uint16_t *x, int M, const uint8_t *w, const uint16_t 
                        dim3(TP * SK * 64), smem, stream, x, M, w, s, out, N, K, TP, SK, cm);
     return hip_status(hipGetLastError(), "gemv rows16 launch");
 }
-
-int device_cus();
 
 template <bool OUT_F32, bool CM, int NL>
 int launch_rows16x_nl(const uint16_t *x, int M, const uint8_t *w, const uint16_t *s, void *out,
@@ -2678,21 +2674,6 @@ int launch_rows(const uint16_t *x, int M, const uint8_t *w, const uint16_t *s, v
     return 1;
 }
 
-/* Compute units of the current device (cached per device; 256 if the query fails). */
-int device_cus() {
-    static int cus[64] = {0};
-    int dev = 0;
-    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
-    if (cus[dev] == 0) {
-        int n = 0;
-        if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess ||
-            n <= 0)
-            n = 256;
-        cus[dev] = n;
-    }
-    return cus[dev];
-}
-
 /* Split-K scratch for the MFMA form: FP32 partials and per-tile-pair arrival counters, one set
  * per device, grown on demand (growth allocates, so it cannot happen under graph capture, and
  * synchronises the device; counters are zeroed when allocated and every kernel leaves them
@@ -2894,17 +2875,6 @@ int launch_mfma(const uint16_t *x, int M, const uint8_t *w, const uint16_t *s, v
         case 2: return launch_mfma_x<OUT, 2>(p, x, M, w, s, out, N, K, partial, counters, stream, residual, cm);
         default: return launch_mfma_x<OUT, 4>(p, x, M, w, s, out, N, K, partial, counters, stream, residual, cm);
     }
-}
-
-/* Every device buffer of the compute entry points starts on a 16-byte boundary: the kernels
- * move 16 bytes a lane (buffer and direct-to-LDS loads). Allocator pointers always do. */
-bool misaligned(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
-
-/* Whether byte ranges [a, a + an) and [b, b + bn) share a byte. A kernel that reads one while
- * its other blocks write the other would race, so such pairs are refused. */
-bool overlap(const void *a, size_t an, const void *b, size_t bn) {
-    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-    return an && bn && x < y + bn && y < x + an;
 }
 
 /* Shape refusals of the reference wrapper (csrc/kernels/gemm_quant.cu:204-231), plus the

@@ -96,6 +96,14 @@ _SIGNATURES = {
                                                  _vp]),
     "test_gemm_int4": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i]),
     "test_silu_mul_packed": (_i, [_vp, _vp, _i, _i]),
+    "w4a16_kv_write_bf16": (_i, [_vp, _vp, _vp, _ll, _ll, _vp, _ll, _ll, _vp]),
+    "w4a16_kv_read_bf16": (_i, [_vp, _vp, _vp, _vp, _vp]),
+    "w4a16_paged_attention_workspace": (_i, [_vp, _vp, _i, ctypes.POINTER(ctypes.c_size_t)]),
+    "w4a16_paged_attention_bf16": (_i, [_vp, _vp, _vp, _ll, _ll, _i, ctypes.c_float, _i, _i, _vp, _ll, _ll, _vp, _vp,
+                                        ctypes.c_size_t, _vp]),
+    "w4a16_verify_drafts_workspace": (_i, [_i, _i, _i, ctypes.POINTER(ctypes.c_size_t)]),
+    "w4a16_verify_drafts_f32": (_i, [_vp, _ll, _ll, _vp, _ll, _ll, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp,
+                                     ctypes.c_size_t, _vp]),
 }
 
 
@@ -607,3 +615,226 @@ class Engine:
                                                     eps, op, m, _stream(stream)),
                "engine_ffn_forward_residual_norm")
         return out
+
+
+# ----------------------------------------------------------------------------------------------
+# Paged KV cache, attention over it, verification of drafted tokens
+# ----------------------------------------------------------------------------------------------
+
+KV_FORMATS = {"bf16": 0, "int8": 1, "fp8": 2}
+
+
+class _KvCacheStruct(ctypes.Structure):
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("format", _i), ("num_pages", _i),
+                ("page_size", _i), ("kv_heads", _i), ("head_dim", _i)]
+
+
+class _KvBatchStruct(ctypes.Structure):
+    _fields_ = [("page_table", _vp), ("kv_lens", _vp), ("starts", _vp), ("seqs", _i), ("rows", _i), ("table_pages", _i),
+                ("table_stride", _i), ("max_new", _i), ("max_kv", _i)]
+
+
+def _refuse(what):
+    raise W4A16Error(W4A16_ERR_CONFIG, what)
+
+
+def _on_current(device, what):
+    """The library launches on the current device: tensors of another one are refused."""
+    import torch
+
+    if device.type != "cuda" or device.index != torch.cuda.current_device():
+        _refuse(f"{what}: tensors on {device}, which is not the current GPU")
+
+
+def _rows3(t, rows, heads, dim, device, what):
+    """Address and strides of a [rows, heads, dim] tensor of BF16 values whose last axis is dense."""
+    if not hasattr(t, "is_cuda") or not t.is_cuda or t.device != device:
+        _refuse(f"{what}: expected a tensor on {device}")
+    if t.dim() != 3 or t.shape[0] != rows or t.shape[1] != heads or t.shape[2] != dim:
+        _refuse(f"{what}: shape {tuple(t.shape)}, the call needs {(rows, heads, dim)}")
+    if t.element_size() != 2 or t.is_complex():
+        _refuse(f"{what}: {t.dtype} is not BF16 (or its bits)")
+    row, head, one = t.stride()
+    if one != 1:
+        _refuse(f"{what}: the last axis is strided")
+    return t.data_ptr(), row, head
+
+
+class KvCache:
+    """A paged cache over tensors of the caller: k, v [pages, kv_heads, page_size, head_dim] of
+    torch.bfloat16, int8 or float8_e4m3fn, with FP32 scales [pages, kv_heads, page_size] for the
+    8-bit ones. The handle keeps the tensors; it holds nothing else."""
+
+    def __init__(self, k, v, k_scale=None, v_scale=None):
+        import torch
+
+        formats = {torch.bfloat16: 0, torch.int8: 1, torch.float8_e4m3fn: 2}
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.dtype not in formats:
+            _refuse(f"KvCache: k {tuple(k.shape)} {k.dtype} and v {tuple(v.shape)} {v.dtype} are no cache")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.device = k.device
+        self.num_pages, self.kv_heads, self.page_size, self.head_dim = k.shape
+        size = k.numel() * k.element_size()
+        scales = [None, None]
+        if formats[k.dtype]:
+            if any(s is None or s.dtype != torch.float32 for s in (k_scale, v_scale)):
+                _refuse("KvCache: an 8-bit cache has FP32 scales for keys and values")
+            scales = [_dev(s, k.numel() // self.head_dim * 4, 4, "KvCache scales", k.device) for s in (k_scale, v_scale)]
+        self._c = _KvCacheStruct(_dev(k, size, k.element_size(), "KvCache k"),
+                                 _dev(v, size, v.element_size(), "KvCache v", k.device), scales[0], scales[1],
+                                 formats[k.dtype], self.num_pages, self.page_size, self.kv_heads, self.head_dim)
+        self._ref = ctypes.addressof(self._c)
+
+    @classmethod
+    def empty(cls, num_pages, page_size, kv_heads, head_dim, format="bf16", device="cuda"):
+        import torch
+
+        if format not in KV_FORMATS:
+            _refuse(f"KvCache: format {format!r} is none of {sorted(KV_FORMATS)}")
+        dtype = {"bf16": torch.bfloat16, "int8": torch.int8, "fp8": torch.float8_e4m3fn}[format]
+        shape = (num_pages, kv_heads, page_size, head_dim)
+        k, v = torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device)
+        if format == "bf16":
+            return cls(k, v)
+        return cls(k, v, torch.empty(shape[:3], device=device), torch.empty(shape[:3], device=device))
+
+    def write(self, k, v, batch, stream=None):
+        """Writes the batch's rows of k and v [rows, kv_heads, head_dim] (strided views are fine)."""
+        _on_current(self.device, "KvCache.write")
+        batch.check(self.device, "KvCache.write")
+        kp, k_row, k_head = _rows3(k, batch.rows, self.kv_heads, self.head_dim, self.device, "KvCache.write k")
+        vp, v_row, v_head = _rows3(v, batch.rows, self.kv_heads, self.head_dim, self.device, "KvCache.write v")
+        _check(lib.w4a16_kv_write_bf16(self._ref, batch._ref, kp, k_row, k_head, vp, v_row, v_head, _stream(stream)),
+               "KvCache.write")
+
+    def read(self, batch, out=None, stream=None):
+        """The batch's rows out of the cache: (k, v) as BF16 [rows, kv_heads, head_dim]. Without
+        `out` rows of no sequence are zeros; with it they are left as they were."""
+        import torch
+
+        _on_current(self.device, "KvCache.read")
+        batch.check(self.device, "KvCache.read")
+        shape = (batch.rows, self.kv_heads, self.head_dim)
+        if out is None:
+            make = torch.zeros if batch.padded else torch.empty
+            out = tuple(make(shape, dtype=torch.bfloat16, device=self.device) for _ in range(2))
+        size = batch.rows * self.kv_heads * self.head_dim * 2
+        k, v = (_dev(t, size, 2, "KvCache.read out", self.device) for t in out)
+        _check(lib.w4a16_kv_read_bf16(self._ref, batch._ref, k, v, _stream(stream)), "KvCache.read")
+        return out
+
+
+class KvBatch:
+    """The sequences of a call: page_table [seqs, pages] (its rows may be strided), kv_lens [seqs]
+    and starts [seqs + 1], int32 on the device and read there at run time. Rows starts[s] ..
+    starts[s + 1] - 1 of the call's tensors are the last tokens of sequence s, kv_lens counting
+    them. `rows` is the tensors' row count; `padded` says that it is more than the sequences have.
+    max_new and max_kv bound the new tokens and the lengths of any sequence (0: rows, and what the
+    table holds): they plan the launches, nothing else."""
+
+    def __init__(self, page_table, kv_lens, starts, rows, max_new=0, max_kv=0, padded=False):
+        import torch
+
+        for name, t, dims in (("page_table", page_table, 2), ("kv_lens", kv_lens, 1), ("starts", starts, 1)):
+            if not hasattr(t, "is_cuda") or not t.is_cuda or t.dtype != torch.int32 or t.dim() != dims:
+                _refuse(f"KvBatch: {name} is no int32 CUDA tensor of {dims} axes")
+            if t.device != kv_lens.device or (t.numel() > 0 and t.shape[-1] > 1 and t.stride(-1) != 1):
+                _refuse(f"KvBatch: {name} is on another device, or strided")
+        seqs, pages = page_table.shape
+        if kv_lens.shape[0] != seqs or starts.shape[0] != seqs + 1:
+            _refuse(f"KvBatch: {seqs} rows of the table, {kv_lens.shape[0]} lengths, {starts.shape[0]} starts")
+        if rows < 0:
+            _refuse(f"KvBatch: rows={rows}")
+        self.page_table, self.kv_lens, self.starts = page_table, kv_lens, starts
+        self.device, self.rows, self.padded = kv_lens.device, rows, padded
+        stride = page_table.stride(0) if seqs > 1 else pages
+        self._c = _KvBatchStruct(page_table.data_ptr(), kv_lens.data_ptr(), starts.data_ptr(), seqs, rows, pages,
+                                 stride, max_new, max_kv)
+        self._ref = ctypes.addressof(self._c)
+
+    def check(self, device, what):
+        if self.device != device:
+            _refuse(f"{what}: the batch is on {self.device}, the call on {device}")
+
+
+def paged_attention(q, cache, batch, scale=None, causal=True, window=0, out=None, return_lse=False, workspace=None,
+                    stream=None):
+    """Attention of the batch's rows of q [rows, q_heads, head_dim] (BF16; strided views are fine)
+    over the cache, their own keys and values written already. scale: 1 / sqrt(head_dim) unless it
+    is given. Returns out [rows, q_heads, head_dim], or (out, lse [rows, q_heads]). `workspace`: a
+    uint8 tensor to use instead of a new one, not shared with a call that may still run."""
+    import torch
+
+    device = cache.device
+    _on_current(device, "paged_attention")
+    batch.check(device, "paged_attention")
+    q_heads = q.shape[1] if q.dim() == 3 else 0
+    qp, q_row, q_head = _rows3(q, batch.rows, q_heads, cache.head_dim, device, "paged_attention q")
+    if out is None:
+        make = torch.zeros if batch.padded else torch.empty
+        out = make((batch.rows, q_heads, cache.head_dim), dtype=torch.bfloat16, device=device)
+    op, o_row, o_head = _rows3(out, batch.rows, q_heads, cache.head_dim, device, "paged_attention out")
+    lse = None
+    if return_lse:
+        lse = torch.full((batch.rows, q_heads), float("-inf"), device=device) if batch.padded else \
+            torch.empty((batch.rows, q_heads), dtype=torch.float32, device=device)
+    need = ctypes.c_size_t(0)
+    _check(lib.w4a16_paged_attention_workspace(cache._ref, batch._ref, q_heads, ctypes.byref(need)), "paged_attention")
+    if need.value and workspace is None:
+        workspace = torch.empty(need.value, dtype=torch.uint8, device=device)
+    wp = _dev(workspace, need.value, 1, "paged_attention workspace", device) if need.value else None
+    _check(lib.w4a16_paged_attention_bf16(cache._ref, batch._ref, qp, q_row, q_head, q_heads,
+                                          cache.head_dim ** -0.5 if scale is None else scale, int(causal), window, op,
+                                          o_row, o_head, None if lse is None else lse.data_ptr(), wp, need.value,
+                                          _stream(stream)), "paged_attention")
+    return (out, lse) if return_lse else out
+
+
+def _floats3(t, what, device):
+    import torch
+
+    if not hasattr(t, "is_cuda") or not t.is_cuda or t.device != device:
+        _refuse(f"{what}: expected a tensor on {device}")
+    if t.dtype != torch.float32 or t.dim() != 3 or (t.shape[-1] > 1 and t.stride(-1) != 1):
+        _refuse(f"{what}: expected FP32 [seqs, rows, vocab] with a dense last axis, got {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr(), t.stride(0), t.stride(1)
+
+
+def verify_drafts(target, draft_tokens, uniforms, draft=None, lens=None, workspace=None, stream=None):
+    """Verification of drafted tokens (see include/w4a16.h): target [seqs, steps + 1, vocab] and,
+    where the tokens were drawn, draft [seqs, steps, vocab] probabilities in FP32, draft_tokens
+    [seqs, steps] int32, uniforms [seqs, steps + 1] FP32, lens [seqs] int32 or None. Returns
+    (accepted [seqs], tokens [seqs, steps + 1]), int32."""
+    import torch
+
+    device = target.device
+    _on_current(device, "verify_drafts")
+    tp, t_seq, t_row = _floats3(target, "verify_drafts target", device)
+    seqs, rows, vocab = target.shape
+    steps = rows - 1
+    if steps < 0:
+        _refuse("verify_drafts: the target has no rows")
+    dp, d_seq, d_row = None, 0, 0
+    if draft is not None and steps > 0:
+        dp, d_seq, d_row = _floats3(draft, "verify_drafts draft", device)
+        if tuple(draft.shape) != (seqs, steps, vocab):
+            _refuse(f"verify_drafts: draft {tuple(draft.shape)}, the call needs {(seqs, steps, vocab)}")
+    for name, t, shape, dtype in (("draft_tokens", draft_tokens, (seqs, steps), torch.int32),
+                                  ("uniforms", uniforms, (seqs, rows), torch.float32),
+                                  ("lens", lens, (seqs,), torch.int32)):
+        if t is not None and (tuple(t.shape) != shape or t.dtype != dtype):
+            _refuse(f"verify_drafts: {name} {tuple(t.shape)} {t.dtype}, the call needs {shape} {dtype}")
+    ip = _dev(draft_tokens, seqs * steps * 4, 4, "verify_drafts draft_tokens", device)
+    up = _dev(uniforms, seqs * rows * 4, 4, "verify_drafts uniforms", device)
+    lp = None if lens is None else _dev(lens, seqs * 4, 4, "verify_drafts lens", device)
+    accepted = torch.empty(seqs, dtype=torch.int32, device=device)
+    tokens = torch.empty((seqs, rows), dtype=torch.int32, device=device)
+    need = ctypes.c_size_t(0)
+    _check(lib.w4a16_verify_drafts_workspace(seqs, steps, vocab, ctypes.byref(need)), "verify_drafts")
+    if workspace is None:
+        workspace = torch.empty(need.value, dtype=torch.uint8, device=device)
+    wp = _dev(workspace, need.value, 1, "verify_drafts workspace", device)
+    _check(lib.w4a16_verify_drafts_f32(tp, t_seq, t_row, dp, d_seq, d_row, ip, lp, up, accepted.data_ptr(),
+                                       tokens.data_ptr(), seqs, steps, vocab, wp, need.value, _stream(stream)),
+           "verify_drafts")
+    return accepted, tokens

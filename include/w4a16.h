@@ -1,5 +1,6 @@
 /*
- * w4a16.h - C ABI of the MI355X (gfx950) weight-only INT4 dense-FFN decode path.
+ * w4a16.h - C ABI of the MI355X (gfx950) weight-only INT4 dense-FFN decode path, and of the paged
+ * KV cache, its attention and the draft verification of the same decode and verify steps.
  *
  * The artifact format is the reference's frozen INT4 format (reference
  * csrc/include/linear_weight.h:5-13): symmetric signed INT4 codes in 128-wide K groups, BF16
@@ -334,6 +335,119 @@ int engine_ffn_forward_residual_norm(W4A16Store *store, int layer, uint16_t *res
                                      const uint16_t *sublayer, const uint16_t *norm_w,
                                      int norm_style, float eps, uint16_t *out, int tokens,
                                      void *stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Paged KV cache, attention over it and verification of drafted tokens: what stands around the
+ * FFN in a decode or verify step (no counterpart in the reference's C ABI,
+ * whose entry points take whole steps).
+ *
+ * The cache. A page holds page_size tokens of every key head, keys and values in buffers of
+ * their own: k, v [num_pages][kv_heads][page_size][head_dim], of BF16 values or of 8-bit codes
+ * with an FP32 scale a token and head, k_scale, v_scale [num_pages][kv_heads][page_size].
+ * head_dim is 64, 128 or 256, page_size a power of two from 8 to 65536, and
+ * num_pages * page_size fits 31 bits. A row x of D values is held in 8 bits as
+ *   top = 127 (INT8) or 448 (FP8, OCP e4m3), a = max|x|,
+ *   scale = a / top, code = round to nearest even(x * (top / a)), the two quotients and the
+ *   product rounded to FP32;
+ * a row with a < 2^-117 is held as zeros (scale 0), one with an infinity or a NaN as zero codes
+ * with a NaN scale, so it reads back as NaN and no attention masks that out by accident.
+ *
+ * The batch. page_table[s * table_stride + i] is the page of tokens i * page_size .. of sequence
+ * s (i < table_pages), kv_lens[s] the tokens it has in the cache, the call's own among them.
+ * Rows starts[s] .. starts[s + 1] - 1 of the call's tensors are sequence s's last tokens: row
+ * starts[s] + i stands at position kv_lens[s] - (starts[s + 1] - starts[s]) + i. starts does not
+ * decrease; rows outside starts[0] .. starts[seqs] - 1 are left as they were. These arrays are
+ * read on the device at run time (a captured graph sees their values of each replay); they start
+ * on a 4-byte boundary. max_new and max_kv bound the new tokens and kv_lens of any sequence
+ * (0: rows, and what the table holds); they only plan the launch, so a loose bound costs speed and a wrong one is no fault. Tokens
+ * past the table (or past 2^30) and pages outside the cache are seen as tokens that are not there: not written,
+ * read as zeros, masked in the attention. A page that one call writes through two sequences
+ * holds either's rows.
+ *
+ * Strides are in elements; a token's heads and a head's values stand apart by multiples of 8
+ * elements, values next to each other. Tensors that are read and written by one call must not
+ * share memory unless it says so.
+ * ------------------------------------------------------------------------------------- */
+#define W4A16_KV_BF16 0
+#define W4A16_KV_INT8 1
+#define W4A16_KV_FP8 2
+
+typedef struct W4A16KvCache {
+    void *k;
+    void *v;
+    float *k_scale; /* NULL for W4A16_KV_BF16 */
+    float *v_scale;
+    int format; /* W4A16_KV_* */
+    int num_pages;
+    int page_size;
+    int kv_heads;
+    int head_dim;
+} W4A16KvCache;
+
+typedef struct W4A16KvBatch {
+    const int32_t *page_table; /* [seqs][table_stride], table_pages of each row used */
+    const int32_t *kv_lens;    /* [seqs] */
+    const int32_t *starts;     /* [seqs + 1] */
+    int seqs;
+    int rows; /* rows of the call's tensors, up to 2^25 */
+    int table_pages;
+    int table_stride;
+    int max_new;
+    int max_kv;
+} W4A16KvBatch;
+
+/* Writes the batch's rows of k and v [rows][kv_heads][head_dim] into the cache. */
+int w4a16_kv_write_bf16(const W4A16KvCache *cache, const W4A16KvBatch *batch, const uint16_t *k,
+                        long long k_row_stride, long long k_head_stride, const uint16_t *v,
+                        long long v_row_stride, long long v_head_stride, void *stream);
+
+/* Reads the batch's rows out of the cache as BF16: code * scale, rounded to nearest even once.
+ * k, v: [rows][kv_heads][head_dim], contiguous. */
+int w4a16_kv_read_bf16(const W4A16KvCache *cache, const W4A16KvBatch *batch, uint16_t *k,
+                       uint16_t *v, void *stream);
+
+/* Attention of the batch's rows of q [rows][q_heads][head_dim] over the cache, to which the rows'
+ * own keys and values have been written: out_i = sum_j softmax_j(scale * <q_i, k_j>) v_j. Query
+ * head h reads key head h / (q_heads / kv_heads). causal: a row sees positions up to its own;
+ * window > 0: only its last `window` ones of them (its own included). Scores, statistics and
+ * sums are FP32; the weights are rounded to BF16 before the product with V (and after a V
+ * scale's multiplication), the output once. A row that sees nothing gets zeros, and -infinity as
+ * lse. lse (optional): [rows][q_heads], log of the sum of exp of the scaled scores.
+ * ws: device memory of at least the bytes w4a16_paged_attention_workspace gives for the same
+ * arguments (on the same device), for this call alone until it has run; NULL if that is 0.
+ * out may be q itself (the same strides). */
+int w4a16_paged_attention_workspace(const W4A16KvCache *cache, const W4A16KvBatch *batch,
+                                    int q_heads, size_t *bytes);
+int w4a16_paged_attention_bf16(const W4A16KvCache *cache, const W4A16KvBatch *batch,
+                               const uint16_t *q, long long q_row_stride, long long q_head_stride,
+                               int q_heads, float scale, int causal, int window, uint16_t *out,
+                               long long out_row_stride, long long out_head_stride, float *lse,
+                               void *ws, size_t ws_bytes, void *stream);
+
+/* Verification of drafted tokens against the target's probabilities, from given random numbers.
+ * Sequence s has lens[s] drafted tokens (lens NULL: `steps` each; clipped to 0..steps) in
+ * draft_tokens[s * steps + i]. Its target row i (i = 0..steps) of `vocab` probabilities is at
+ * target + s * target_seq_stride + i * target_row_stride, the draft's row i likewise (i < steps).
+ * uniforms: [seqs][steps + 1]. Token i is taken while
+ *   uniforms[s][i] * draft_i(token) < target_i(token)
+ * (the product exact), up to the first that is not, or to the end; one more token is then drawn
+ * from the weights max(target_n - draft_n, 0) of the refused row n, or, if all were taken (or
+ * those weights are all zero), from target row n: the first index at which the running sum of
+ * weights (FP64) passes uniforms[s][steps] times their sum. draft NULL: the drafted tokens were
+ * chosen, not drawn (a draft distribution that is 1 at the token). Weights that are not
+ * positive and finite count as zero; a token outside the vocabulary is refused and takes nothing
+ * out of the weights.
+ * accepted[s]: the tokens taken. tokens [seqs][steps + 1]: those, the drawn one (-1 if no weight
+ * is positive), and -1 behind it. Every float row starts on a 4-byte boundary.
+ * ws: w4a16_verify_drafts_workspace bytes of device memory, for this call alone until it has
+ * run. */
+int w4a16_verify_drafts_workspace(int seqs, int steps, int vocab, size_t *bytes);
+int w4a16_verify_drafts_f32(const float *target, long long target_seq_stride,
+                            long long target_row_stride, const float *draft,
+                            long long draft_seq_stride, long long draft_row_stride,
+                            const int32_t *draft_tokens, const int32_t *lens,
+                            const float *uniforms, int32_t *accepted, int32_t *tokens, int seqs,
+                            int steps, int vocab, void *ws, size_t ws_bytes, void *stream);
 
 /* ---------------------------------------------------------------------------------------
  * Status of the split-K combines (no counterpart in the reference, whose kernels have no
