@@ -16,6 +16,8 @@
  * An 8-bit cache's codes are BF16 values; their scales multiply the scores (K) and the weights (V)
  * in FP32.
  */
+#include <cmath>
+
 #include "kv.h"
 
 using namespace w4a16;
@@ -24,6 +26,7 @@ namespace {
 
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 struct AttnArgs {
     KvView kv;
@@ -33,7 +36,9 @@ struct AttnArgs {
     long long q_row, q_head, out_row, out_head;
     int group, q_heads, causal, window;
     int splits, items;
-    float scale; /* times log2(e) */
+    int over, upto;   /* only sequences of over < rows <= upto (token, head) rows */
+    float scale;      /* |scale| log2(e) */
+    uint32_t flip;    /* sign bits of a BF16 pair of q: a negative scale turns its sign over */
 };
 
 constexpr int kFewestTokens = 256; /* of a split */
@@ -66,6 +71,7 @@ __device__ __forceinline__ bool find_tile(const AttnArgs &a, int item, int split
             first = a.kv.starts[s];
             const int last = a.kv.starts[s + 1];
             if (first >= 0 && last <= a.kv.rows && last > first) news = last - first;
+            if (news * a.group <= a.over || news * a.group > a.upto) news = 0;
         }
         const int tiles = (news * a.group + RM - 1) / RM;
         int upto = tiles;
@@ -147,29 +153,146 @@ __device__ __forceinline__ float *partial_of(const AttnArgs &a, int item, int he
     return a.ws + (((long long)item * a.kv.heads + head) * a.splits + split) * (RM * (D + 2));
 }
 
+/* Codes 2 * HALF and 2 * HALF + 1 of one token's dword x and its neighbour's y, as pairs of one value of
+ * both tokens: FP16, in which the codes of both formats are exact. An INT8 code's bits with the sign
+ * flipped, 0 to 255, are the low bits of 1024 + 128 + code. */
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+
+template <int FMT, int HALF>
+__device__ __forceinline__ void code_pairs(uint32_t x, uint32_t y, uint32_t *even, uint32_t *odd) {
+    if constexpr (FMT == W4A16_KV_FP8) {
+        const uint32_t a = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, HALF));
+        const uint32_t b = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(y, 1.0f, HALF));
+        *even = __builtin_amdgcn_perm(b, a, 0x05040100u);
+        *odd = __builtin_amdgcn_perm(b, a, 0x07060302u);
+    } else {
+        const h2 off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
+        const uint32_t a = __builtin_amdgcn_perm(y, x, HALF ? 0x0C060C02u : 0x0C040C00u) ^ 0x64806480u;
+        const uint32_t b = __builtin_amdgcn_perm(y, x, HALF ? 0x0C070C03u : 0x0C050C01u) ^ 0x64806480u;
+        *even = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, a) + off);
+        *odd = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, b) + off);
+    }
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(kv_f2{a, b}, h2));
+}
+
+/* The V product: BF16 values with BF16 weights, or codes with FP16 weights. */
+template <bool CODED>
+__device__ __forceinline__ f4 mfma_v(const uint32_t *v, const uint32_t *w, f4 acc) {
+    if constexpr (CODED)
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, make_uint4(v[0], v[1], v[2], v[3])),
+                                                      __builtin_bit_cast(h8, make_uint4(w[0], w[1], w[2], w[3])), acc, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf8(v[0], v[1], v[2], v[3]), as_bf8(w[0], w[1], w[2], w[3]), acc, 0, 0, 0);
+}
+
+__device__ __forceinline__ float power_of_two(int biased) { return __builtin_bit_cast(float, (uint32_t)biased << 23); }
+
 /*
  * Few rows: a block of four waves has RT tiles of 16 rows and one split of the keys; its waves
  * take 32 tokens at a time in turn, each with statistics of its own, and are joined in LDS at the
  * end. K and V go from memory into the registers that the products take them from; no LDS in the
- * loop.
+ * loop. The next tokens' K is loaded into its registers as soon as the score product has read
+ * them, V behind the second product, and the pages a step ahead of both, so that a load has most
+ * of a step to arrive.
  *
- * v_mfma_f32_16x16x32_bf16. K: a lane's row is token l % 16 of two groups of 16, its values the
- * 8 or 16 that lane group g = l / 16 has of each step. S^T gives a lane tokens 16 a + 4 g + i of row
- * l % 16, and those are the eight that it holds of P^T (a, i from 0 to 1, 3) and has to load of V^T: 16
+ * v_mfma_f32_16x16x32. K: a lane's row is token l % 16 of two groups of 16, its values the
+ * 8 or 16 that lane group g = l / 16 has of each step. S^T gives a lane tokens 16 c + 4 g + i of row
+ * l % 16, and those are the eight that it holds of P^T (c, i from 0 to 1, 3) and has to load of V^T: 16
  * lanes load a token's whole row, E = D / 16 values each, which stand at E neighbouring
  * columns; a transposition of 8 tokens x 2 values at a time by byte permutations makes them the
  * operand of value e's product.
+ *
+ * A BF16 cache's weights are rounded to BF16, whose largest, 1, is exact. Those of an 8-bit cache
+ * carry V's scale, so they are FP16 (codes are exact in it), scaled by a power of two that
+ * holds the largest scale so far in [1, 2): eight times less rounding than BF16, and for INT8
+ * fewer instructions to widen.
  */
 template <int D, int FMT, int RT>
 __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
     constexpr int RM = 16 * RT, E = D / 16, KS = D / 32; /* values of V a lane has; steps of the K product */
     constexpr bool kCoded = FMT != W4A16_KV_BF16;
-    constexpr int kVWords = kCoded ? E / 4 : E / 2;
+    constexpr int kVWords = kCoded ? E / 4 : E / 2, kKLoads = kCoded ? KS / 2 : KS;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
     const int head = blockIdx.x % a.kv.heads, item = blockIdx.x / a.kv.heads, split = blockIdx.y;
     Tile t;
     if (!find_tile<RM>(a, item, split, &t)) return;
     if (split >= t.active) return;
+
+    const int32_t *table = a.kv.table + (long long)t.seq * a.kv.table_stride;
+    const int mask = (1 << a.kv.shift) - 1;
+    /* Pages of this lane's K tokens and V tokens (page sizes are multiples of 8, so four
+     * neighbours from a multiple of 4 share one). Tokens that are not there read token 0 of page 0
+     * and are masked. */
+    int kpage[2], vpage[2];
+    auto load_pages = [&](int t0) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const int kt = t0 + 16 * c + n, vt = t0 + 16 * c + 4 * g;
+            kpage[c] = kt < t.length ? table[kt >> a.kv.shift] : -1;
+            vpage[c] = vt < t.length ? table[vt >> a.kv.shift] : -1;
+        }
+    };
+    auto slot_of = [&](int page, int token) -> long long {
+        return (unsigned)page < (unsigned)a.kv.pages ? (((long long)page * a.kv.heads + head) << a.kv.shift) + (token & mask) : 0;
+    };
+    u4 kraw[2][kKLoads];
+    uint32_t v[8][kVWords];
+    f4 ks[2], vs[2];
+    auto load_k = [&](int t0) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const uint8_t *p = static_cast<const uint8_t *>(a.kv.k) + slot_of(kpage[c], t0 + 16 * c + n) * (kCoded ? D : 2 * D) + 16 * g;
+#pragma unroll
+            for (int s = 0; s < kKLoads; ++s) kraw[c][s] = *reinterpret_cast<const u4 *>(p + 64 * s);
+        }
+    };
+    auto load_v = [&](int t0) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const long long slot = slot_of(vpage[c], t0 + 16 * c + 4 * g);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint8_t *p = static_cast<const uint8_t *>(a.kv.v) + (slot + i) * (kCoded ? D : 2 * D) + n * (4 * kVWords);
+                if constexpr (kVWords == 1) {
+                    v[4 * c + i][0] = *reinterpret_cast<const uint32_t *>(p);
+                } else if constexpr (kVWords == 2) {
+                    const uint2 x = *reinterpret_cast<const uint2 *>(p);
+                    v[4 * c + i][0] = x.x;
+                    v[4 * c + i][1] = x.y;
+                } else {
+#pragma unroll
+                    for (int w = 0; w < kVWords; w += 4) {
+                        const u4 x = *reinterpret_cast<const u4 *>(p + 4 * w);
+                        v[4 * c + i][w] = x.x;
+                        v[4 * c + i][w + 1] = x.y;
+                        v[4 * c + i][w + 2] = x.z;
+                        v[4 * c + i][w + 3] = x.w;
+                    }
+                }
+            }
+        }
+    };
+    auto load_scales = [&](int t0, f4 *k_of, f4 *v_of) {
+        if constexpr (kCoded) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const long long slot = slot_of(vpage[c], t0 + 16 * c + 4 * g);
+                k_of[c] = *reinterpret_cast<const f4 *>(a.kv.k_scale + slot);
+                v_of[c] = *reinterpret_cast<const f4 *>(a.kv.v_scale + slot);
+            }
+        }
+    };
+    int t0 = t.begin + 32 * wave;
+    if (t0 < t.end) {
+        load_pages(t0);
+        load_k(t0);
+        load_scales(t0, ks, vs);
+        load_v(t0);
+    }
 
     /* this lane's rows: their queries as the products' operand, and the keys they see */
     bf8 q[RT][KS];
@@ -186,12 +309,13 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
             const int d = kCoded ? 64 * (s / 2) + 16 * g + 8 * (s % 2) : 32 * s + 8 * g;
             uint4 x = make_uint4(0u, 0u, 0u, 0u);
             if (real) x = *reinterpret_cast<const uint4 *>(a.q + (t.first_row + token) * a.q_row + h * a.q_head + d);
-            q[r][s] = __builtin_bit_cast(bf8, x);
+            q[r][s] = as_bf8(x.x ^ a.flip, x.y ^ a.flip, x.z ^ a.flip, x.w ^ a.flip);
         }
     }
 
     f4 acc[RT][E];
     float m[RT], l[RT];
+    int v_exp = 1; /* biased exponent that the weights are scaled by (8-bit caches) */
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
         m[r] = -__builtin_inff();
@@ -200,58 +324,39 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
         for (int e = 0; e < E; ++e) acc[r][e] = f4{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    const int32_t *table = a.kv.table + (long long)t.seq * a.kv.table_stride;
-    const int mask = (1 << a.kv.shift) - 1;
-    for (int t0 = t.begin + 32 * wave; t0 < t.end; t0 += 128) {
-        /* pages of this lane's K tokens and V tokens (page sizes are multiples of 8, so four
-         * neighbours from a multiple of 4 share one); tokens out of range read token 0 of page 0
-         * and are masked below */
-        long long kslot[2], vslot[2];
+    for (; t0 < t.end; t0 += 128) {
         bool there[2];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            const int kt = t0 + 16 * c + n, vt = t0 + 16 * c + 4 * g;
-            const int kp = kt < t.length ? table[kt >> a.kv.shift] : -1;
-            const int vp = vt < t.length ? table[vt >> a.kv.shift] : -1;
-            const bool kin = (unsigned)kp < (unsigned)a.kv.pages;
-            there[c] = (unsigned)vp < (unsigned)a.kv.pages;
-            kslot[c] = kin ? (((long long)kp * a.kv.heads + head) << a.kv.shift) + (kt & mask) : 0;
-            vslot[c] = there[c] ? (((long long)vp * a.kv.heads + head) << a.kv.shift) + (vt & mask) : 0;
-        }
-        /* K */
-        bf8 k[2][KS];
+        for (int c = 0; c < 2; ++c) there[c] = (unsigned)vpage[c] < (unsigned)a.kv.pages;
+        const int next = t0 + 128;
+        const bool more = next < t.end;
+        if (more) load_pages(next);
+        f4 s[RT][2];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
+            bf8 k[KS];
             if constexpr (kCoded) {
-                const uint8_t *p = static_cast<const uint8_t *>(a.kv.k) + kslot[c] * D + 16 * g;
 #pragma unroll
-                for (int s = 0; s < KS / 2; ++s) {
-                    const uint4 x = *reinterpret_cast<const uint4 *>(p + 64 * s);
-                    k[c][2 * s] = as_bf8(kv_widen<FMT, 0>(x.x), kv_widen<FMT, 1>(x.x), kv_widen<FMT, 0>(x.y), kv_widen<FMT, 1>(x.y));
-                    k[c][2 * s + 1] = as_bf8(kv_widen<FMT, 0>(x.z), kv_widen<FMT, 1>(x.z), kv_widen<FMT, 0>(x.w), kv_widen<FMT, 1>(x.w));
+                for (int j = 0; j < KS / 2; ++j) {
+                    const u4 x = kraw[c][j];
+                    k[2 * j] = as_bf8(kv_widen<FMT, 0>(x.x), kv_widen<FMT, 1>(x.x), kv_widen<FMT, 0>(x.y), kv_widen<FMT, 1>(x.y));
+                    k[2 * j + 1] = as_bf8(kv_widen<FMT, 0>(x.z), kv_widen<FMT, 1>(x.z), kv_widen<FMT, 0>(x.w), kv_widen<FMT, 1>(x.w));
                 }
             } else {
-                const uint16_t *p = static_cast<const uint16_t *>(a.kv.k) + kslot[c] * D + 8 * g;
 #pragma unroll
-                for (int s = 0; s < KS; ++s) k[c][s] = *reinterpret_cast<const bf8 *>(p + 32 * s);
+                for (int j = 0; j < KS; ++j) k[j] = __builtin_bit_cast(bf8, kraw[c][j]);
+            }
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                s[r][c] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int j = 0; j < KS; ++j) s[r][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[j], q[r][j], s[r][c], 0, 0, 0);
             }
         }
-        /* V: tokens vt, vt + 1, .. of both groups, E values of each */
-        uint32_t v[8][kVWords];
-        f4 ks[2], vs[2];
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t *p = reinterpret_cast<const uint32_t *>(static_cast<const uint8_t *>(a.kv.v) +
-                                        (vslot[c] + i) * (kCoded ? D : 2 * D)) + n * kVWords;
-#pragma unroll
-                for (int w = 0; w < kVWords; ++w) v[4 * c + i][w] = p[w];
-            }
-            if constexpr (kCoded) {
-                ks[c] = *reinterpret_cast<const f4 *>(a.kv.k_scale + vslot[c]) * a.scale;
-                vs[c] = *reinterpret_cast<const f4 *>(a.kv.v_scale + vslot[c]);
-            }
+        f4 ks_next[2], vs_next[2];
+        if (more) {
+            load_k(next);
+            load_scales(next, ks_next, vs_next);
         }
         /* tokens that some row does not see, or that are not there: their V is not multiplied */
         const bool cut = t0 < t.all_lo || t0 + 32 > t.all_hi || __any(!there[0] || !there[1]);
@@ -262,84 +367,107 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int at = t0 + 16 * c + 4 * g + i;
-                    if (!there[c] || at < t.lo || at >= t.hi)
+                    if (!there[c] || at < t.lo || at >= t.hi) {
 #pragma unroll
                         for (int w = 0; w < kVWords; ++w) v[4 * c + i][w] = 0u;
+                        if constexpr (kCoded) vs[c][i] = 0.0f;
+                    }
                     if constexpr (!kCoded)
 #pragma unroll
                         for (int w = 0; w < kVWords; ++w) odd = odd || nonfinite2(v[4 * c + i][w]);
                 }
             odd = __any(odd);
         }
+        if constexpr (kCoded) {
+            /* the scales are positive, or not numbers: those are no measure of the others */
+            float most = 0.0f;
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) most = fmaxf(most, vs[c][i] < __builtin_inff() ? vs[c][i] : 0.0f);
+            most = lane_max32(lane_max16(most));
+            int exp = (int)(__builtin_bit_cast(uint32_t, most) >> 23);
+            exp = __builtin_amdgcn_readfirstlane(exp > 253 ? 1 : exp);
+            if (exp > v_exp) {
+                const int fall = exp - v_exp > 126 ? 126 : exp - v_exp;
+                const float by = power_of_two(127 - fall);
+#pragma unroll
+                for (int r = 0; r < RT; ++r)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) acc[r][e] *= by;
+                v_exp = exp;
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c) vs[c] *= power_of_two(254 - v_exp);
+        }
+        uint32_t p[RT][4];
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-            f4 s[2];
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                s[c] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+                if constexpr (kCoded) s[r][c] *= ks[c];
+                s[r][c] *= a.scale;
+                if (cut)
 #pragma unroll
-                for (int j = 0; j < KS; ++j) s[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[c][j], q[r][j], s[c], 0, 0, 0);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    s[c][i] *= kCoded ? ks[c][i] : a.scale;
-                    if (cut) {
+                    for (int i = 0; i < 4; ++i) {
                         const int at = t0 + 16 * c + 4 * g + i;
-                        if (!there[c] || at < lo[r] || at >= hi[r]) s[c][i] = -__builtin_inff();
+                        if (!there[c] || at < lo[r] || at >= hi[r]) s[r][c][i] = -__builtin_inff();
                     }
-                }
             }
-            float most = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
-                               fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+            float most = fmaxf(fmaxf(fmaxf(s[r][0][0], s[r][0][1]), fmaxf(s[r][0][2], s[r][0][3])),
+                               fmaxf(fmaxf(s[r][1][0], s[r][1][1]), fmaxf(s[r][1][2], s[r][1][3])));
             most = lane_max32(lane_max16(most));
-            const float next = fmaxf(m[r], most);
-            const float base = next == -__builtin_inff() ? 0.0f : next;
-            const float grow = __builtin_amdgcn_exp2f(m[r] - base);
-            m[r] = next;
-            uint32_t p[4];
-            float sum = 0.0f;
+            if (__any(most > m[r] + 8.0f)) {
+                const float upto = fmaxf(m[r], most);
+                const float grow = __builtin_amdgcn_exp2f(m[r] - (upto == -__builtin_inff() ? 0.0f : upto));
+                m[r] = upto;
+                l[r] *= grow;
+#pragma unroll
+                for (int e = 0; e < E; ++e) acc[r][e] *= grow;
+            }
+            const float base = m[r] == -__builtin_inff() ? 0.0f : m[r];
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 float w[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    w[i] = __builtin_amdgcn_exp2f(s[c][i] - base);
-                    sum += w[i];
+                    w[i] = __builtin_amdgcn_exp2f(s[r][c][i] - base);
+                    l[r] += w[i];
                     if constexpr (kCoded) {
                         w[i] *= vs[c][i];
-                        if (cut && s[c][i] == -__builtin_inff()) w[i] = 0.0f;
+                        if (cut && s[r][c][i] == -__builtin_inff()) w[i] = 0.0f;
                     }
                 }
-                p[2 * c] = kv_pack_bf16(w[0], w[1]);
-                p[2 * c + 1] = kv_pack_bf16(w[2], w[3]);
+                p[r][2 * c] = kCoded ? pack_f16(w[0], w[1]) : kv_pack_bf16(w[0], w[1]);
+                p[r][2 * c + 1] = kCoded ? pack_f16(w[2], w[3]) : kv_pack_bf16(w[2], w[3]);
             }
-            l[r] = l[r] * grow + sum;
+        }
+        if (!odd) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) acc[r][e] *= grow;
-            const bf8 weights = as_bf8(p[0], p[1], p[2], p[3]);
-            if (!odd) {
+            for (int e = 0; e < E; e += 2) {
+                uint32_t even[4], odds[4];
 #pragma unroll
-                for (int e = 0; e < E; e += 2) {
-                    uint32_t even[4], odds[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        uint32_t x, y; /* values e, e + 1 of tokens 2 j and 2 j + 1 */
-                        if constexpr (kCoded) {
-                            x = e % 4 ? kv_widen<FMT, 1>(v[2 * j][e / 4]) : kv_widen<FMT, 0>(v[2 * j][e / 4]);
-                            y = e % 4 ? kv_widen<FMT, 1>(v[2 * j + 1][e / 4]) : kv_widen<FMT, 0>(v[2 * j + 1][e / 4]);
-                        } else {
-                            x = v[2 * j][e / 2];
-                            y = v[2 * j + 1][e / 2];
-                        }
-                        even[j] = __builtin_amdgcn_perm(y, x, 0x05040100u);
-                        odds[j] = __builtin_amdgcn_perm(y, x, 0x07060302u);
+                for (int j = 0; j < 4; ++j) { /* values e, e + 1 of tokens 2 j and 2 j + 1 */
+                    if constexpr (kCoded) {
+                        if (e % 4) code_pairs<FMT, 1>(v[2 * j][e / 4], v[2 * j + 1][e / 4], &even[j], &odds[j]);
+                        else code_pairs<FMT, 0>(v[2 * j][e / 4], v[2 * j + 1][e / 4], &even[j], &odds[j]);
+                    } else {
+                        even[j] = __builtin_amdgcn_perm(v[2 * j + 1][e / 2], v[2 * j][e / 2], 0x05040100u);
+                        odds[j] = __builtin_amdgcn_perm(v[2 * j + 1][e / 2], v[2 * j][e / 2], 0x07060302u);
                     }
-                    acc[r][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf8(even[0], even[1], even[2], even[3]), weights, acc[r][e], 0, 0, 0);
-                    acc[r][e + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf8(odds[0], odds[1], odds[2], odds[3]), weights, acc[r][e + 1], 0, 0, 0);
                 }
-            } else if constexpr (!kCoded) {
-                /* an infinity or a NaN among values that not every row sees: 0 times it would
-                 * reach the rows that do not, so each row's product is formed apart, without
-                 * the tokens that it does not see */
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                    acc[r][e] = mfma_v<kCoded>(even, p[r], acc[r][e]);
+                    acc[r][e + 1] = mfma_v<kCoded>(odds, p[r], acc[r][e + 1]);
+                }
+            }
+        } else if constexpr (!kCoded) {
+            /* an infinity or a NaN among values that not every row sees: 0 times it would
+             * reach the rows that do not, so each row's product is formed apart, without
+             * the tokens that it does not see */
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
                 for (int one = 0; one < 16; ++one) {
                     const int o_lo = __shfl(lo[r], one), o_hi = __shfl(hi[r], one);
 #pragma unroll
@@ -350,15 +478,29 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
                             const int at = t0 + 16 * (j / 2) + 4 * g + 2 * (j % 2);
                             const uint32_t x = at >= o_lo && at < o_hi ? v[2 * j][e / 2] : 0u;
                             const uint32_t y = at + 1 >= o_lo && at + 1 < o_hi ? v[2 * j + 1][e / 2] : 0u;
-                            pair[j] = e % 2 ? __builtin_amdgcn_perm(y, x, 0x07060302u) : __builtin_amdgcn_perm(y, x, 0x05040100u);
+                            pair[j] = __builtin_amdgcn_perm(y, x, e % 2 ? 0x07060302u : 0x05040100u);
                         }
-                        const f4 got = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf8(pair[0], pair[1], pair[2], pair[3]), weights, acc[r][e], 0, 0, 0);
+                        const f4 got = mfma_v<kCoded>(pair, p[r], acc[r][e]);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) acc[r][e][i] = n == one ? got[i] : acc[r][e][i];
                     }
                 }
+        }
+        if (more) load_v(next);
+        if constexpr (kCoded) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                ks[c] = ks_next[c];
+                vs[c] = vs_next[c];
             }
         }
+    }
+    if constexpr (kCoded) {
+        const float by = power_of_two(v_exp);
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[r][e] *= by;
     }
 
     /* the four waves together: 128 values of 16 rows at a time */
@@ -427,83 +569,547 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
     }
 }
 
-/* Joins the splits of a tile that has more than one: 16 lanes a row. */
-template <int D, int RM>
-__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
-    constexpr int kPer = D / 16;
-    const int head = blockIdx.x % a.kv.heads, item = blockIdx.x / a.kv.heads;
-    Tile t;
-    if (!find_tile<RM>(a, item, 0, &t) || t.active < 2) return;
-    for (int i = threadIdx.x >> 4; i < t.rows; i += 16) {
-        const float *from = partial_of<D, RM>(a, item, head, 0);
-        float top = -__builtin_inff();
-        for (int s = 0; s < t.active; ++s) top = fmaxf(top, from[s * (RM * (D + 2)) + RM * D + 2 * i]);
-        const float base = top == -__builtin_inff() ? 0.0f : top;
-        float total = 0.0f, o[kPer];
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) o[j] = 0.0f;
-        const int part = (threadIdx.x & 15) * kPer;
-        for (int s = 0; s < t.active; ++s) {
-            const float *p = from + (long long)s * (RM * (D + 2));
-            const float f = __builtin_amdgcn_exp2f(p[RM * D + 2 * i] - base);
-            total += f * p[RM * D + 2 * i + 1];
-#pragma unroll
-            for (int j = 0; j < kPer; j += 4) {
-                const f4 x = *reinterpret_cast<const f4 *>(p + (long long)i * D + part + j);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) o[j + c] += f * x[c];
-            }
-        }
-        const int token = (t.start + i) / a.group, h = head * a.group + (t.start + i) % a.group;
-        const float by = total == 0.0f ? 0.0f : 1.0f / total;
-        uint32_t *to = reinterpret_cast<uint32_t *>(a.out + (t.first_row + token) * a.out_row + h * a.out_head + part);
-#pragma unroll
-        for (int j = 0; j < kPer; j += 2) to[j / 2] = kv_pack_bf16(o[j] * by, o[j + 1] * by);
-        if (a.lse && part == 0)
-            a.lse[(long long)(t.first_row + token) * a.q_heads + h] =
-                total == 0.0f ? -__builtin_inff() : (top + __builtin_amdgcn_logf(total)) * kLn2;
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+
+/* Codes 2 * HALF and 2 * HALF + 1 of a dword as an FP16 pair. */
+template <int FMT, int HALF>
+__device__ __forceinline__ uint32_t widen_f16(uint32_t codes) {
+    if constexpr (FMT == W4A16_KV_FP8) {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, 1.0f, HALF));
+    } else {
+        const h2 off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
+        const uint32_t x = __builtin_amdgcn_perm(codes, codes, HALF ? 0x0C030C02u : 0x0C010C00u) ^ 0x64806480u;
+        return __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, x) + off);
     }
 }
 
-/* How a call is cut: tiles of 16 rt rows, at most `items` of them a key head, `splits` a tile. */
+/*
+ * Many rows: a block of four waves has 128 (token, head) rows, 32 a wave, and goes through its
+ * keys BN at a time. The tile's K and V stand in LDS, BF16 (V of an 8-bit cache FP16), twice:
+ * while one is multiplied the next is on its way from memory into registers, widened there once
+ * for all four waves and written behind the products; one barrier a step.
+ *
+ * v_mfma_f32_32x32x16. S^T = K Q^T: a lane's column is row l % 32, its 16 values tokens
+ * 8 (i / 4) + 4 (l / 32) + i % 4 of 32, so that the first eight of them are what the lane holds of
+ * P^T in a product over 16 tokens, and the next eight in the following one; V^T comes out
+ * of LDS with the transposing read (four tokens of a column to each lane). A row's maximum is over
+ * a lane's own values and those of lane l ^ 32. The sums are rescaled only when a maximum has
+ * grown by more than 2^8 since the last time, which rounds nothing more: weights up to 2^8
+ * are as exact in BF16, FP16 and FP32 as those up to 1.
+ *
+ * 16-byte pieces of a token's K are exchanged by its number (XOR), pairs of pieces of its V by
+ * the same, so that the eight lanes of a step of a read fall on different banks.
+ */
+template <int D, int FMT>
+struct Chunk {
+    static constexpr bool kCoded = FMT != W4A16_KV_BF16;
+    static constexpr int kRows = 128, BN = D == 256 ? 32 : 64;
+    static constexpr int kPieces = D / 8;                              /* of 8 values a token */
+    static constexpr int kLoads = BN * D * (kCoded ? 1 : 2) / (256 * 16); /* 16-byte loads a thread and matrix */
+    static constexpr int kSwizzle = kPieces < 16 ? kPieces - 1 : 15;
+    /* LDS: [2]{K, V}, then scales [2][2][BN], pages [3][BN], flags */
+    static constexpr int kTile = BN * D * 2;
+    static constexpr int kScales = 4 * kTile, kPages = kScales + (kCoded ? 4 * BN * 4 : 0);
+    static constexpr int kFlags = kPages + 3 * BN * 4, kBytes = kFlags + 16;
+};
+
+/* 16 bytes a lane from memory to LDS, lane after lane from `to` (the same on every lane). */
+__device__ __forceinline__ void load_to_lds(const uint8_t *from, uint8_t *to) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
+                                     (__attribute__((address_space(3))) void *)to, 16, 0, 0);
+}
+
+/* Before the barrier behind which other waves read what load_to_lds wrote. */
+__device__ __forceinline__ void wait_for_lds_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+template <int D, int FMT>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_chunk_kernel(AttnArgs a) {
+    using C = Chunk<D, FMT>;
+    constexpr bool kCoded = C::kCoded;
+    constexpr int BN = C::BN, RM = C::kRows, kHalves = BN / 32, KS = D / 16, DB = D / 32;
+    extern __shared__ uint4 smem4[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>(smem4);
+    float *scales = reinterpret_cast<float *>(smem + C::kScales); /* [buffer][k, v][BN] */
+    int *pages = reinterpret_cast<int *>(smem + C::kPages);       /* [step % 3][BN] */
+    int *bad = reinterpret_cast<int *>(smem + C::kFlags);         /* [step % 3]: a token without a page */
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 31, half = lane >> 5;
+    const int head = blockIdx.x % a.kv.heads, split = blockIdx.y;
+    /* the last tiles of a sequence see the most keys: those first */
+    const int item = a.items - 1 - (int)(blockIdx.x / a.kv.heads);
+    Tile t;
+    if (!find_tile<RM>(a, item, split, &t)) return;
+    if (split >= t.active) return;
+
+    const int32_t *table = a.kv.table + (long long)t.seq * a.kv.table_stride;
+    const int mask = (1 << a.kv.shift) - 1;
+    const int steps = t.end > t.begin ? (t.end - t.begin + BN - 1) / BN : 0;
+
+    /* the page of token tid of a step, -1 where there is none */
+    auto page_of = [&](int step) {
+        const int at = t.begin + step * BN + tid;
+        int page = -1;
+        if (at >= t.lo && at < t.hi) page = table[at >> a.kv.shift];
+        return (unsigned)page < (unsigned)a.kv.pages ? page : -1;
+    };
+    auto put_page = [&](int step, int page) {
+        if (tid < BN) pages[(step % 3) * BN + tid] = page;
+        const bool none = __any(tid < BN && page < 0);
+        if (lane == 0) bad[step % 3] = none;
+    };
+    /* 8-bit: through registers, widened on the way into LDS. BF16: straight into LDS, a wave's 1 KiB at
+     * a time; a lane fetches the piece that belongs where it writes. */
+    u4 kr[C::kLoads], vr[C::kLoads];
+    float scale_r = 0.0f;
+    bool there_r[C::kLoads];
+    constexpr int kLanes = D * (kCoded ? 1 : 2) / 16; /* a token's 16-byte loads */
+    auto slot_of = [&](int step, int at, int page) -> long long {
+        return page >= 0 ? (((long long)page * a.kv.heads + head) << a.kv.shift) + ((t.begin + step * BN + at) & mask) : 0;
+    };
+    auto load_tile = [&](int step) {
+        const uint8_t *k = static_cast<const uint8_t *>(a.kv.k), *v = static_cast<const uint8_t *>(a.kv.v);
+        if constexpr (kCoded) {
+#pragma unroll
+            for (int x = 0; x < C::kLoads; ++x) {
+                const int at = (x * 256 + tid) / kLanes, part = (x * 256 + tid) % kLanes;
+                const int page = pages[(step % 3) * BN + at];
+                there_r[x] = page >= 0;
+                const long long slot = slot_of(step, at, page);
+                kr[x] = *reinterpret_cast<const u4 *>(k + slot * D + part * 16);
+                vr[x] = *reinterpret_cast<const u4 *>(v + slot * D + part * 16);
+            }
+            if (tid < 2 * BN) {
+                const int at = tid % BN, page = pages[(step % 3) * BN + at];
+                const long long slot = slot_of(step, at, page);
+                scale_r = page < 0 ? 0.0f : tid < BN ? a.kv.k_scale[slot] * a.scale : a.kv.v_scale[slot];
+            }
+        } else {
+            const int wave_u = __builtin_amdgcn_readfirstlane(wave);
+            uint8_t *to = smem + (step & 1) * 2 * C::kTile + wave_u * 1024;
+#pragma unroll
+            for (int x = 0; x < C::kLoads; ++x) {
+                const int at = (x * 256 + tid) / kLanes, part = (x * 256 + tid) % kLanes;
+                const long long slot = slot_of(step, at, pages[(step % 3) * BN + at]);
+                load_to_lds(k + slot * (2 * D) + (part ^ (at & C::kSwizzle)) * 16, to + x * 4096);
+                load_to_lds(v + slot * (2 * D) + (part ^ ((2 * at) & C::kSwizzle)) * 16, to + C::kTile + x * 4096);
+            }
+        }
+    };
+    auto store_tile = [&](int step) {
+        if constexpr (kCoded) {
+            uint8_t *k = smem + (step & 1) * 2 * C::kTile, *v = k + C::kTile;
+#pragma unroll
+            for (int x = 0; x < C::kLoads; ++x) {
+                const int at = (x * 256 + tid) / kLanes, part = (x * 256 + tid) % kLanes;
+                const u4 vx = there_r[x] ? vr[x] : u4{0u, 0u, 0u, 0u};
+                const int ks = at & C::kSwizzle, vs = (2 * at) & C::kSwizzle;
+                const u4 k0 = {kv_widen<FMT, 0>(kr[x].x), kv_widen<FMT, 1>(kr[x].x), kv_widen<FMT, 0>(kr[x].y), kv_widen<FMT, 1>(kr[x].y)};
+                const u4 k1 = {kv_widen<FMT, 0>(kr[x].z), kv_widen<FMT, 1>(kr[x].z), kv_widen<FMT, 0>(kr[x].w), kv_widen<FMT, 1>(kr[x].w)};
+                *reinterpret_cast<u4 *>(k + at * 2 * D + ((2 * part) ^ ks) * 16) = k0;
+                *reinterpret_cast<u4 *>(k + at * 2 * D + ((2 * part + 1) ^ ks) * 16) = k1;
+                const u4 v0 = {widen_f16<FMT, 0>(vx.x), widen_f16<FMT, 1>(vx.x), widen_f16<FMT, 0>(vx.y), widen_f16<FMT, 1>(vx.y)};
+                const u4 v1 = {widen_f16<FMT, 0>(vx.z), widen_f16<FMT, 1>(vx.z), widen_f16<FMT, 0>(vx.w), widen_f16<FMT, 1>(vx.w)};
+                *reinterpret_cast<u4 *>(v + at * 2 * D + ((2 * part) ^ vs) * 16) = v0;
+                *reinterpret_cast<u4 *>(v + at * 2 * D + ((2 * part + 1) ^ vs) * 16) = v1;
+            }
+            if (tid < 2 * BN) scales[(step & 1) * 2 * BN + tid] = scale_r;
+        } else {
+            wait_for_lds_loads();
+        }
+    };
+
+    if (steps > 0) {
+        if (tid < 64) {
+            put_page(0, tid < BN ? page_of(0) : 0);
+            if (steps > 1) put_page(1, tid < BN ? page_of(1) : 0);
+        }
+        __syncthreads();
+        load_tile(0);
+    }
+
+    /* this lane's row: its queries and the keys it sees */
+    const int i_row = wave * 32 + n, token = (t.start + i_row) / a.group, h = head * a.group + (t.start + i_row) % a.group;
+    const bool real = i_row < t.rows;
+    const int place = t.length - t.news + token;
+    const int hi = !real ? 0 : a.causal ? place + 1 : t.length, lo = t.window ? place - t.window + 1 : 0;
+    bf8 q[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+        uint4 x = make_uint4(0u, 0u, 0u, 0u);
+        if (real) x = *reinterpret_cast<const uint4 *>(a.q + (t.first_row + token) * a.q_row + h * a.q_head + 16 * s + 8 * half);
+        q[s] = as_bf8(x.x ^ a.flip, x.y ^ a.flip, x.z ^ a.flip, x.w ^ a.flip);
+    }
+    f16v acc[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[d][i] = 0.0f;
+    float m = -__builtin_inff(), l = 0.0f;
+    int v_exp = 1;
+    if (steps > 0) {
+        store_tile(0);
+        __syncthreads();
+    }
+
+    /* This lane's places in a tile of K: piece `half` of token n (that of step j, 2 j + half, is an XOR
+     * away); and in one of V, for the transposing read: row (lane % 16) / 4 of four tokens, four of
+     * 16 columns. */
+    const int k_at = n * 2 * D + ((half ^ (n & C::kSwizzle)) * 16);
+    const int v_row = 4 * half + ((lane >> 2) & 3), v_piece = 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
+    const int v_at = v_row * 2 * D + ((v_piece ^ ((2 * v_row) & C::kSwizzle)) * 16) + 8 * (lane & 1);
+    for (int step = 0; step < steps; ++step) {
+        const bool more = step + 1 < steps;
+        int page = 0;
+        if (more) load_tile(step + 1);
+        const bool look = tid < 64 && step + 2 < steps;
+        if (look && tid < BN) page = page_of(step + 2);
+        const int t0 = t.begin + step * BN;
+        const uint8_t *kt = smem + (step & 1) * 2 * C::kTile, *vt = kt + C::kTile;
+        const float *sc = scales + (step & 1) * 2 * BN;
+        f16v s[kHalves];
+#pragma unroll
+        for (int c = 0; c < kHalves; ++c) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[c][i] = 0.0f;
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int j = 0; j < KS; ++j) {
+                const bf8 k = *reinterpret_cast<const bf8 *>(kt + (k_at ^ (32 * j)) + 32 * c * 2 * D);
+                s[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, q[j], s[c], 0, 0, 0);
+            }
+        }
+        if constexpr (kCoded) {
+#pragma unroll
+            for (int c = 0; c < kHalves; ++c)
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    const f4 x = *reinterpret_cast<const f4 *>(sc + 32 * c + 8 * b + 4 * half);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[c][4 * b + i] *= x[i];
+                }
+        }
+        const bool cut = (t0 < t.all_lo) | (t0 + BN > t.all_hi) | (__builtin_amdgcn_readfirstlane(bad[step % 3]) != 0);
+        if (cut) {
+#pragma unroll
+            for (int c = 0; c < kHalves; ++c)
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    const int in = 32 * c + 8 * b + 4 * half;
+                    const int4 page = *reinterpret_cast<const int4 *>(pages + (step % 3) * BN + in);
+                    const int each[4] = {page.x, page.y, page.z, page.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const bool hidden = (t0 + in + i < lo) | (t0 + in + i >= hi) | (each[i] < 0);
+                        s[c][4 * b + i] = hidden ? -__builtin_inff() : s[c][4 * b + i];
+                    }
+                }
+        }
+        float most = s[0][0];
+#pragma unroll
+        for (int c = 0; c < kHalves; ++c)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) most = fmaxf(most, s[c][i]);
+        most = lane_max32(most);
+        if constexpr (!kCoded) most *= a.scale;
+        if (__any(most > m + 8.0f)) {
+            const float upto = fmaxf(m, most);
+            const float grow = __builtin_amdgcn_exp2f(m - (upto == -__builtin_inff() ? 0.0f : upto));
+            m = upto;
+            l *= grow;
+#pragma unroll
+            for (int d = 0; d < DB; ++d) acc[d] *= grow;
+        }
+        const float base = m == -__builtin_inff() ? 0.0f : m;
+        float v_by = 1.0f;
+        if constexpr (kCoded) {
+            /* V's largest scale of the step, as in attn_rows_kernel */
+            float top = lane < BN ? sc[BN + lane] : 0.0f;
+            int exp = (int)(__builtin_bit_cast(uint32_t, top) >> 23);
+            exp = exp > 253 ? 1 : exp;
+#pragma unroll
+            for (int x = 1; x < 64; x *= 2) {
+                const int o = __shfl_xor(exp, x);
+                exp = exp > o ? exp : o;
+            }
+            exp = __builtin_amdgcn_readfirstlane(exp);
+            if (exp > v_exp) {
+                const int fall = exp - v_exp > 126 ? 126 : exp - v_exp;
+                const float by = power_of_two(127 - fall);
+#pragma unroll
+                for (int d = 0; d < DB; ++d) acc[d] *= by;
+                v_exp = exp;
+            }
+            v_by = power_of_two(254 - v_exp);
+        }
+        uint32_t p[kHalves][8];
+#pragma unroll
+        for (int c = 0; c < kHalves; ++c)
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                float w[4];
+                f4 x = {1.0f, 1.0f, 1.0f, 1.0f};
+                if constexpr (kCoded) x = *reinterpret_cast<const f4 *>(sc + BN + 32 * c + 8 * b + 4 * half);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float score = s[c][4 * b + i];
+                    w[i] = __builtin_amdgcn_exp2f(kCoded ? score - base : fmaf(score, a.scale, -base));
+                    l += w[i];
+                    if constexpr (kCoded) {
+                        w[i] *= x[i] * v_by;
+                        if (cut && score == -__builtin_inff()) w[i] = 0.0f;
+                    }
+                }
+                p[c][2 * b] = kCoded ? pack_f16(w[0], w[1]) : kv_pack_bf16(w[0], w[1]);
+                p[c][2 * b + 1] = kCoded ? pack_f16(w[2], w[3]) : kv_pack_bf16(w[2], w[3]);
+            }
+        if constexpr (!kCoded) {
+            /* Tokens that are not there weigh nothing, and what memory holds for them is taken
+             * out. An infinity or a NaN among values that not every row sees: 0 times it would
+             * reach the rows that do not. Those that do have it added as it is, and the product
+             * goes without it. */
+            if (cut) {
+                uint32_t *tile = reinterpret_cast<uint32_t *>(smem + (step & 1) * 2 * C::kTile + C::kTile);
+                bool odd = false;
+                for (int x = tid; x < C::kTile / 4; x += 256) {
+                    if (pages[(step % 3) * BN + x / (D / 2)] < 0) tile[x] = 0u;
+                    else odd = odd || nonfinite2(tile[x]);
+                }
+                if (__syncthreads_or(odd)) {
+                    for (int in = 0; in < BN; ++in) {
+                        const bool sees = t0 + in >= lo && t0 + in < hi;
+#pragma unroll
+                        for (int d = 0; d < DB; ++d)
+#pragma unroll
+                            for (int b = 0; b < 4; ++b) {
+                                __builtin_amdgcn_sched_barrier(0); /* one piece at a time: registers */
+                                const uint2 x = *reinterpret_cast<const uint2 *>(vt + in * 2 * D + ((4 * d + b) ^ ((2 * in) & C::kSwizzle)) * 16 + 8 * half);
+                                const uint32_t f[4] = {x.x << 16, x.x & 0xFFFF0000u, x.y << 16, x.y & 0xFFFF0000u};
+#pragma unroll
+                                for (int i = 0; i < 4; ++i)
+                                    if (sees && (f[i] & 0x7F800000u) == 0x7F800000u) acc[d][4 * b + i] += __builtin_bit_cast(float, f[i]);
+                            }
+                    }
+                    __syncthreads();
+                    for (int x = tid; x < C::kTile / 4; x += 256) {
+                        const uint32_t pair = tile[x];
+                        tile[x] = ((pair & 0x7F80u) == 0x7F80u ? 0u : pair & 0xFFFFu) | ((pair & 0x7F800000u) == 0x7F800000u ? 0u : pair & 0xFFFF0000u);
+                    }
+                    __syncthreads();
+                }
+            }
+        }
+        /* O^T: 16 tokens and 32 values a product */
+#pragma unroll
+        for (int u = 0; u < BN / 16; ++u) {
+            const uint32_t *w = &p[u / 2][4 * (u % 2)];
+            if (u % 2 == 0) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+                uint32_t v[4];
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    const uint2 got = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (__attribute__((address_space(3))) s4 *)(vt + (v_at ^ (64 * d)) + (16 * u + 8 * y) * 2 * D)));
+                    v[2 * y] = got.x;
+                    v[2 * y + 1] = got.y;
+                }
+                if constexpr (kCoded) {
+                    acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, make_uint4(v[0], v[1], v[2], v[3])),
+                                                                    __builtin_bit_cast(h8, make_uint4(w[0], w[1], w[2], w[3])), acc[d], 0, 0, 0);
+                } else {
+                    acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf8(v[0], v[1], v[2], v[3]), as_bf8(w[0], w[1], w[2], w[3]), acc[d], 0, 0, 0);
+                }
+            }
+        }
+        if (more) store_tile(step + 1);
+        if (look) put_page(step + 2, page);
+        __syncthreads();
+    }
+
+    /* a lane has values 32 d + 8 b + 4 half .. + 3 of its row; so does lane ^ 32 the four between */
+    const float total = lane_sum32(l);
+    if (!real) return;
+    float by = kCoded ? power_of_two(v_exp) : 1.0f;
+    float *partial = t.active > 1 ? partial_of<D, RM>(a, item, head, split) : nullptr;
+    if (partial) {
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+                *reinterpret_cast<f4 *>(partial + (long long)i_row * D + 32 * d + 8 * b + 4 * half) =
+                    f4{acc[d][4 * b], acc[d][4 * b + 1], acc[d][4 * b + 2], acc[d][4 * b + 3]} * by;
+        if (half == 0) {
+            partial[RM * D + 2 * i_row] = m;
+            partial[RM * D + 2 * i_row + 1] = total;
+        }
+        return;
+    }
+    by = total == 0.0f ? 0.0f : by / total;
+    uint16_t *to = a.out + (t.first_row + token) * a.out_row + h * a.out_head + 4 * half;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+            *reinterpret_cast<uint2 *>(to + 32 * d + 8 * b) = make_uint2(kv_pack_bf16(acc[d][4 * b] * by, acc[d][4 * b + 1] * by),
+                                                                        kv_pack_bf16(acc[d][4 * b + 2] * by, acc[d][4 * b + 3] * by));
+    if (a.lse && half == 0)
+        a.lse[(long long)(t.first_row + token) * a.q_heads + h] =
+            total == 0.0f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(total)) * kLn2;
+}
+
+/* Joins the splits of a tile that has more than one. A block has 16 / SUB rows (blockIdx.y of
+ * them), 16 lanes a row and part of its splits: with many splits the sum over them is what takes
+ * time, so SUB parts of it run side by side and meet in LDS. */
+template <int D, int RM, int SUB>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
+    constexpr int kPer = D / 16, kRows = 16 / SUB;
+    const int head = blockIdx.x % a.kv.heads, item = blockIdx.x / a.kv.heads;
+    Tile t;
+    if (!find_tile<RM>(a, item, 0, &t) || t.active < 2 || (int)blockIdx.y * kRows >= t.rows) return;
+    const int lane = threadIdx.x & 15, unit = threadIdx.x >> 4, sub = unit / kRows, i = blockIdx.y * kRows + unit % kRows;
+    const float *from = partial_of<D, RM>(a, item, head, 0);
+    constexpr long long kStep = RM * (D + 2);
+    const int row = i < t.rows ? i : t.rows - 1;
+    const float *ml = from + RM * D + 2 * row, *values = from + (long long)row * D + lane * kPer;
+    float top = -__builtin_inff();
+    for (int s = lane; s < t.active; s += 16) top = fmaxf(top, ml[s * kStep]);
+#pragma unroll
+    for (int x = 1; x < 16; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
+    const float base = top == -__builtin_inff() ? 0.0f : top;
+    float total = 0.0f, o[kPer];
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) o[j] = 0.0f;
+#pragma unroll 4
+    for (int s = sub; s < t.active; s += SUB) {
+        const float f = __builtin_amdgcn_exp2f(ml[s * kStep] - base);
+        total += f * ml[s * kStep + 1];
+#pragma unroll
+        for (int j = 0; j < kPer; j += 4) {
+            const f4 x = *reinterpret_cast<const f4 *>(values + s * kStep + j);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) o[j + c] += f * x[c];
+        }
+    }
+    if constexpr (SUB > 1) {
+        __shared__ float parts[16][D + 4], totals[16];
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) parts[unit][lane * kPer + j] = o[j];
+        if (lane == 0) totals[unit] = total;
+        __syncthreads();
+        if (sub) return;
+#pragma unroll
+        for (int s = 1; s < SUB; ++s) {
+            total += totals[unit + s * kRows];
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) o[j] += parts[unit + s * kRows][lane * kPer + j];
+        }
+    }
+    if (i >= t.rows) return;
+    const int token = (t.start + i) / a.group, h = head * a.group + (t.start + i) % a.group;
+    const float by = total == 0.0f ? 0.0f : 1.0f / total;
+    uint32_t *to = reinterpret_cast<uint32_t *>(a.out + (t.first_row + token) * a.out_row + h * a.out_head + lane * kPer);
+#pragma unroll
+    for (int j = 0; j < kPer; j += 2) to[j / 2] = kv_pack_bf16(o[j] * by, o[j + 1] * by);
+    if (a.lse && lane == 0)
+        a.lse[(long long)(t.first_row + token) * a.q_heads + h] =
+            total == 0.0f ? -__builtin_inff() : (top + __builtin_amdgcn_logf(total)) * kLn2;
+}
+
+/* How a call is cut: sequences of few (token, head) rows into tiles of 16 rt rows, the others into
+ * tiles of 128; at most `items` tiles a key head, `splits` of each, and where their partial results
+ * begin in the workspace. */
+struct Part {
+    int items, splits, over, upto;
+    size_t ws_at;
+};
 struct Plan {
-    int rt, items, splits;
+    int rt;
+    Part few, many; /* items 0: not launched */
     size_t ws_bytes;
 };
 
+constexpr int kChunkRows = 128;
+
 Plan plan_of(const W4A16KvCache *c, const W4A16KvBatch *b, int q_heads) {
-    Plan p;
-    const int group = q_heads / c->kv_heads;
-    const long long most = (long long)(b->max_new ? b->max_new : b->rows) * group;
-    p.rt = most <= 16 ? 1 : most <= 32 ? 2 : 4;
+    Plan p = {};
+    const int group = q_heads / c->kv_heads, dim = c->head_dim;
+    const int max_new = b->max_new ? b->max_new : b->rows;
+    const long long rows = (long long)b->rows * group, longest = (long long)max_new * group;
+    const long long seqs = b->seqs < b->rows ? b->seqs : b->rows;
+    /* attn_rows_kernel has registers for 32 rows, or 16 of 256 values */
+    const int limit = dim == 256 ? 16 : 32;
+    p.rt = longest <= 16 || dim == 256 ? 1 : 2;
     const int rm = 16 * p.rt;
-    p.items = (int)((long long)b->rows * group / rm + (b->seqs < b->rows ? b->seqs : b->rows));
-    /* four blocks a CU */
-    const long long blocks = (long long)p.items * c->kv_heads, wanted = 4LL * device_cus();
+    p.few = {0, 1, 0, INT32_MAX, 0};
+    p.many = {0, 1, 0, INT32_MAX, 0};
+    if (longest <= limit) {
+        p.few.items = (int)(rows / rm + seqs);
+    } else if ((long long)b->seqs * max_new == b->rows || group > limit) {
+        /* all alike (whatever the bound says, this launch takes every sequence) */
+        p.many.items = (int)(rows / kChunkRows + seqs);
+    } else {
+        p.few.items = (int)seqs;
+        p.few.upto = p.many.over = rm;
+        p.many.items = (int)(rows / kChunkRows + (rows / (rm + 1) < seqs ? rows / (rm + 1) : seqs));
+    }
     const long long tokens = b->max_kv ? b->max_kv : (long long)b->table_pages * c->page_size;
-    const long long longest = (tokens + kFewestTokens - 1) / kFewestTokens;
-    long long splits = blocks > 0 ? (wanted + blocks - 1) / blocks : 1;
-    if (splits > longest) splits = longest;
-    if (splits > 256) splits = 256;
-    p.splits = splits < 1 ? 1 : (int)splits;
-    p.ws_bytes = p.splits > 1 ? (size_t)blocks * p.splits * rm * (c->head_dim + 2) * 4 : 0;
+    const long long most = (tokens + kFewestTokens - 1) / kFewestTokens;
+    for (Part *x : {&p.few, &p.many}) {
+        const bool few = x == &p.few;
+        const long long blocks = (long long)x->items * c->kv_heads, wanted = (few ? 4LL : 2LL) * device_cus();
+        long long splits = blocks > 0 ? (wanted + blocks - 1) / blocks : 1;
+        if (splits > most) splits = most;
+        if (splits > 256) splits = 256;
+        x->splits = splits < 1 ? 1 : (int)splits;
+        x->ws_at = p.ws_bytes;
+        if (x->splits > 1) p.ws_bytes += (size_t)blocks * x->splits * (few ? rm : kChunkRows) * (dim + 2) * 4;
+    }
     return p;
 }
 
-template <int D, int RT>
-void launch_rows(int format, const Plan &p, const AttnArgs &a, hipStream_t s) {
-    auto kernel = format == W4A16_KV_BF16   ? attn_rows_kernel<D, W4A16_KV_BF16, RT>
-                  : format == W4A16_KV_INT8 ? attn_rows_kernel<D, W4A16_KV_INT8, RT>
-                                            : attn_rows_kernel<D, W4A16_KV_FP8, RT>;
-    launch_k(kernel, dim3(a.kv.heads * p.items, p.splits), dim3(256), 0, s, a);
-    if (p.splits > 1) launch_k(attn_join_kernel<D, 16 * RT>, dim3(a.kv.heads * p.items), dim3(256), 0, s, a);
+template <int D, int RM>
+void launch_join(const Part &p, const AttnArgs &a, hipStream_t s) {
+    const unsigned x = a.kv.heads * p.items;
+    if (p.splits > 16) launch_k(attn_join_kernel<D, RM, 16>, dim3(x, RM), dim3(256), 0, s, a);
+    else if (p.splits > 4) launch_k(attn_join_kernel<D, RM, 4>, dim3(x, RM / 4), dim3(256), 0, s, a);
+    else if (p.splits > 1) launch_k(attn_join_kernel<D, RM, 1>, dim3(x, RM / 16), dim3(256), 0, s, a);
+}
+
+AttnArgs part_args(const AttnArgs &all, const Part &p) {
+    AttnArgs a = all;
+    a.items = p.items;
+    a.splits = p.splits;
+    a.over = p.over;
+    a.upto = p.upto;
+    a.ws += p.ws_at / 4;
+    return a;
+}
+
+template <int D, int FMT>
+void launch_format(const Plan &p, const AttnArgs &all, hipStream_t s) {
+    if (p.many.items) {
+        const AttnArgs a = part_args(all, p.many);
+        launch_k(attn_chunk_kernel<D, FMT>, dim3(a.kv.heads * a.items, a.splits), dim3(256), Chunk<D, FMT>::kBytes, s, a);
+        launch_join<D, kChunkRows>(p.many, a, s);
+    }
+    if (p.few.items) {
+        const AttnArgs a = part_args(all, p.few);
+        const dim3 grid(a.kv.heads * a.items, a.splits);
+        if constexpr (D <= 128)
+            if (p.rt == 2) {
+                launch_k(attn_rows_kernel<D, FMT, 2>, grid, dim3(256), 0, s, a);
+                return launch_join<D, 32>(p.few, a, s);
+            }
+        launch_k(attn_rows_kernel<D, FMT, 1>, grid, dim3(256), 0, s, a);
+        launch_join<D, 16>(p.few, a, s);
+    }
 }
 
 template <int D>
 void launch_dim(int format, const Plan &p, const AttnArgs &a, hipStream_t s) {
-    if (p.rt == 1) launch_rows<D, 1>(format, p, a, s);
-    else if (p.rt == 2) launch_rows<D, 2>(format, p, a, s);
-    else launch_rows<D, 4>(format, p, a, s);
+    if (format == W4A16_KV_BF16) launch_format<D, W4A16_KV_BF16>(p, a, s);
+    else if (format == W4A16_KV_INT8) launch_format<D, W4A16_KV_INT8>(p, a, s);
+    else launch_format<D, W4A16_KV_FP8>(p, a, s);
 }
 
 int check_heads(const KvView &kv, int q_heads, const char *what) {
@@ -574,9 +1180,9 @@ extern "C" int w4a16_paged_attention_bf16(const W4A16KvCache *cache, const W4A16
         for (int j = 0; j < i; ++j) clash = clash || overlap(writes[i].p, writes[i].n, writes[j].p, writes[j].n);
     }
     if (clash) return set_error(W4A16_ERR_CONFIG, "%s: an output or the workspace overlaps another buffer", what);
-    if ((long long)p.items * kv.heads > 1 << 23)
-        return set_error(W4A16_ERR_CONFIG, "%s: %lld tiles of rows: at most 2^23 a call", what,
-                         (long long)p.items * kv.heads);
+    const long long tiles = (long long)(p.few.items > p.many.items ? p.few.items : p.many.items) * kv.heads;
+    if (tiles > 1 << 23)
+        return set_error(W4A16_ERR_CONFIG, "%s: %lld tiles of rows: at most 2^23 a call", what, tiles);
     AttnArgs a;
     a.kv = kv;
     a.q = q;
@@ -591,9 +1197,9 @@ extern "C" int w4a16_paged_attention_bf16(const W4A16KvCache *cache, const W4A16
     a.q_heads = q_heads;
     a.causal = causal != 0;
     a.window = window;
-    a.splits = p.splits;
-    a.items = p.items;
-    a.scale = scale * 1.4426950408889634f;
+    a.splits = a.items = a.over = a.upto = 0; /* part_args */
+    a.scale = fabsf(scale) * 1.4426950408889634f;
+    a.flip = scale < 0.0f ? 0x80008000u : 0u;
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (dim == 64) launch_dim<64>(cache->format, p, a, s);
     else if (dim == 128) launch_dim<128>(cache->format, p, a, s);
