@@ -41,7 +41,8 @@ struct AttnArgs {
     uint32_t flip;    /* sign bits of a BF16 pair of q: a negative scale turns its sign over */
 };
 
-constexpr int kFewestTokens = 256; /* of a split */
+constexpr int kFewestTokens = 256; /* of a split of the chunk kernel */
+constexpr int kUnit = 128;         /* tokens that a block of the few-row kernel takes at a time */
 constexpr float kLn2 = 0.69314718055994531f;
 
 /* What a tile's block works on: a sequence, its rows in the tile, the keys that any of them
@@ -58,6 +59,36 @@ struct Tile {
     int seq;
 };
 
+/* The rest of a tile from its sequence, length, rows and start. */
+template <int RM>
+__device__ __forceinline__ void fill_tile(const AttnArgs &a, Tile *t) {
+    const int all = t->news * a.group;
+    t->rows = all - t->start < RM ? all - t->start : RM;
+    const int t0 = t->start / a.group, t1 = (t->start + t->rows - 1) / a.group, old = t->length - t->news;
+    t->window = a.window <= t->length ? a.window : 0;
+    t->hi = a.causal ? old + t1 + 1 : t->length;
+    t->all_hi = a.causal ? old + t0 + 1 : t->length;
+    t->lo = t->window ? old + t0 - t->window + 1 : 0;
+    t->all_lo = t->window ? old + t1 - t->window + 1 : 0;
+    if (t->lo < 0) t->lo = 0;
+    if (t->hi < t->lo) t->hi = t->lo;
+}
+
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_or_zero(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false); }
+
+/* The sum of v over the lanes up to and with this one: row shifts within 16 lanes, then the rows'
+ * last lanes carried to the rows behind (six VALU moves; shuffles are six round trips through LDS). */
+__device__ __forceinline__ int wave_upto(int v) {
+    v += dpp_or_zero<0x111, 0xF>(v);
+    v += dpp_or_zero<0x112, 0xF>(v);
+    v += dpp_or_zero<0x114, 0xF>(v);
+    v += dpp_or_zero<0x118, 0xF>(v);
+    v += dpp_or_zero<0x142, 0xA>(v); /* row_bcast:15 into rows 1 and 3 */
+    v += dpp_or_zero<0x143, 0xC>(v); /* row_bcast:31 into rows 2 and 3 */
+    return v;
+}
+
 /* Finds the `item`th tile of RM rows: the sequences' tiles are counted 64 sequences at a time.
  * Sequences whose rows do not lie in the call's tensors have none. */
 template <int RM>
@@ -73,13 +104,7 @@ __device__ __forceinline__ bool find_tile(const AttnArgs &a, int item, int split
             if (first >= 0 && last <= a.kv.rows && last > first) news = last - first;
             if (news * a.group <= a.over || news * a.group > a.upto) news = 0;
         }
-        const int tiles = (news * a.group + RM - 1) / RM;
-        int upto = tiles;
-#pragma unroll
-        for (int m = 1; m < 64; m *= 2) {
-            const int o = __shfl_up(upto, m);
-            if (lane >= m) upto += o;
-        }
+        const int tiles = (news * a.group + RM - 1) / RM, upto = wave_upto(tiles);
         const unsigned long long here = __ballot(upto > left);
         if (here) {
             const int l = __ffsll(here) - 1;
@@ -93,17 +118,8 @@ __device__ __forceinline__ bool find_tile(const AttnArgs &a, int item, int split
         if (base + 64 >= a.kv.seqs) return false;
     }
     t->seq = __builtin_amdgcn_readfirstlane(t->seq);
-    const int all = t->news * a.group;
-    t->rows = all - t->start < RM ? all - t->start : RM;
     t->length = __builtin_amdgcn_readfirstlane(kv_length(a.kv, t->seq));
-    const int t0 = t->start / a.group, t1 = (t->start + t->rows - 1) / a.group, old = t->length - t->news;
-    t->window = a.window <= t->length ? a.window : 0;
-    t->hi = a.causal ? old + t1 + 1 : t->length;
-    t->all_hi = a.causal ? old + t0 + 1 : t->length;
-    t->lo = t->window ? old + t0 - t->window + 1 : 0;
-    t->all_lo = t->window ? old + t1 - t->window + 1 : 0;
-    if (t->lo < 0) t->lo = 0;
-    if (t->hi < t->lo) t->hi = t->lo;
+    fill_tile<RM>(a, t);
     /* splits begin at multiples of 32 tokens and have at least kFewestTokens */
     const int from = t->lo & ~31, span = t->hi - from;
     int per = (span + a.splits - 1) / a.splits;
@@ -114,6 +130,96 @@ __device__ __forceinline__ bool find_tile(const AttnArgs &a, int item, int split
     t->begin = from + split * per;
     t->end = t->begin + per < t->hi ? t->begin + per : t->hi;
     return true;
+}
+
+/*
+ * The few-row kernel's work is cut by the lengths that it finds: with N units of kUnit tokens over
+ * all (tile, head) pairs and a.splits blocks wanted, every pair is cut into parts of
+ * ceil(N / a.splits) units, so that long sequences have many parts and none is much longer
+ * than another. The parts are counted through the sequences; a part is a block's, and its place in
+ * the workspace.
+ */
+struct Seqs { /* 64 sequences, one a lane */
+    int first, news, length, from; /* from: where the first key that any of its rows sees is cut */
+    int pairs, units;              /* its (tile, head) pairs, units of each */
+};
+
+template <int RM>
+__device__ __forceinline__ Seqs load_seqs(const AttnArgs &a, int base) {
+    const int s = base + (threadIdx.x & 63);
+    Seqs q = {0, 0, 0, 0, 0, 1};
+    if (s < a.kv.seqs) {
+        q.first = a.kv.starts[s];
+        const int last = a.kv.starts[s + 1];
+        q.length = kv_length(a.kv, s);
+        if (q.first >= 0 && last <= a.kv.rows && last > q.first) q.news = last - q.first;
+        if (q.news * a.group <= a.over || q.news * a.group > a.upto) q.news = 0;
+        const int old = q.length - q.news;
+        if (a.window && a.window <= q.length && old - a.window + 1 > 0) q.from = (old - a.window + 1) & ~31;
+        if (q.length > q.from) q.units = (q.length - q.from + kUnit - 1) / kUnit;
+        q.pairs = (q.news * a.group + RM - 1) / RM * a.kv.heads;
+    }
+    return q;
+}
+
+/* Units of a part; *q is left with the first 64 sequences. N / (blocks wanted) where that makes no
+ * more parts than blocks; each pair's last part is on average half as long. */
+template <int RM>
+__device__ __forceinline__ int part_units(const AttnArgs &a, Seqs *q) {
+    *q = load_seqs<RM>(a, 0);
+    /* n < 2^47 in two pieces, whose sums over 64 lanes fit 32 bits */
+    unsigned long long total = 0;
+    long long pairs = 0;
+    Seqs s = *q;
+    for (int base = 0;;) {
+        const unsigned long long n = (unsigned long long)s.pairs * s.units;
+        total += (uint32_t)__builtin_amdgcn_readlane(wave_upto((int)(n & 0xFFFFFF)), 63);
+        total += (unsigned long long)(uint32_t)__builtin_amdgcn_readlane(wave_upto((int)(n >> 24)), 63) << 24;
+        pairs += __builtin_amdgcn_readlane(wave_upto(s.pairs), 63);
+        base += 64;
+        if (base >= a.kv.seqs) break;
+        s = load_seqs<RM>(a, base);
+    }
+    const unsigned long long wanted = pairs < a.splits ? a.splits - pairs / 2 : a.splits;
+    const unsigned long long each = (total + wanted - 1) / wanted;
+    return each < 1 ? 1 : each > 1 << 23 ? 1 << 23 : (int)each;
+}
+
+/* The part of this block (PAIR false) or the (tile, head) pair of number `index` (true): the tile, its head, its number of
+ * parts, and the number of its first one. */
+template <int RM, bool PAIR>
+__device__ __forceinline__ bool find_part(const AttnArgs &a, int index, Tile *t, int *head, int *first_part) {
+    Seqs q;
+    const int each = part_units<RM>(a, &q);
+    int left = index, before = 0; /* parts of the sequences before */
+    for (int base = 0;;) {
+        const int per = (q.units + each - 1) / each, parts = q.pairs * per;
+        const int upto_parts = wave_upto(parts), upto = PAIR ? wave_upto(q.pairs) : upto_parts;
+        const unsigned long long here = __ballot(upto > left);
+        if (here) {
+            const int l = __ffsll((long long)here) - 1;
+            t->seq = base + l;
+            t->first_row = __builtin_amdgcn_readlane(q.first, l);
+            t->news = __builtin_amdgcn_readlane(q.news, l);
+            t->length = __builtin_amdgcn_readlane(q.length, l);
+            const int from = __builtin_amdgcn_readlane(q.from, l);
+            t->active = __builtin_amdgcn_readlane(per, l);
+            const int in_seq = left - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(PAIR ? q.pairs : parts, l));
+            const int pair = PAIR ? in_seq : in_seq / t->active, part = PAIR ? 0 : in_seq - pair * t->active;
+            *first_part = before + __builtin_amdgcn_readlane(upto_parts, l) - __builtin_amdgcn_readlane(parts, l) + pair * t->active;
+            *head = pair % a.kv.heads;
+            t->start = pair / a.kv.heads * RM;
+            fill_tile<RM>(a, t);
+            t->begin = from + part * each * kUnit;
+            t->end = part + 1 < t->active && t->begin + each * kUnit < t->hi ? t->begin + each * kUnit : t->hi;
+            return true;
+        }
+        left -= __builtin_amdgcn_readlane(upto, 63);
+        before += __builtin_amdgcn_readlane(upto_parts, 63);
+        base += 64;
+        if (base >= a.kv.seqs) return false;
+        q = load_seqs<RM>(a, base);
+    }
 }
 
 /* max of v and its value in lanes l ^ 16, l ^ 32 (as the sums of kernels.hip by lane swaps). */
@@ -146,11 +252,10 @@ __device__ __forceinline__ bool nonfinite2(uint32_t pair) {
     return (pair & 0x7F80u) == 0x7F80u || (pair & 0x7F800000u) == 0x7F800000u;
 }
 
-/* Where a partial result of (tile item, key head, split) stands in the workspace: RM rows of D
- * values, then RM pairs (m, l). */
+/* A partial result in the workspace: RM rows of D values, then RM pairs (m, l). */
 template <int D, int RM>
-__device__ __forceinline__ float *partial_of(const AttnArgs &a, int item, int head, int split) {
-    return a.ws + (((long long)item * a.kv.heads + head) * a.splits + split) * (RM * (D + 2));
+__device__ __forceinline__ float *partial_at(const AttnArgs &a, long long index) {
+    return a.ws + index * (RM * (D + 2));
 }
 
 /* Codes 2 * HALF and 2 * HALF + 1 of one token's dword x and its neighbour's y, as pairs of one value of
@@ -191,6 +296,13 @@ __device__ __forceinline__ f4 mfma_v(const uint32_t *v, const uint32_t *w, f4 ac
 
 __device__ __forceinline__ float power_of_two(int biased) { return __builtin_bit_cast(float, (uint32_t)biased << 23); }
 
+/* Blocks of attn_rows_kernel that a CU is to hold: as many as its registers allow without spilling.
+ * More waves are what hides the latency of its loads: RT = 2, D = 128, FP8, 96 sequences' worth
+ * of verify rows: 40.0 us at one block, 29.0 at two; D = 256, 2 x 100003 tokens: 107 and 82. */
+constexpr int rows_blocks(int dim, int format, int rt) {
+    return dim == 256 ? (format == W4A16_KV_BF16 ? 1 : 2) : dim == 128 ? (rt == 1 ? 3 : 2) : rt == 1 ? 4 : 3;
+}
+
 /*
  * Few rows: a block of four waves has RT tiles of 16 rows and one split of the keys; its waves
  * take 32 tokens at a time in turn, each with statistics of its own, and are joined in LDS at the
@@ -212,18 +324,17 @@ __device__ __forceinline__ float power_of_two(int biased) { return __builtin_bit
  * fewer instructions to widen.
  */
 template <int D, int FMT, int RT>
-__global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel(AttnArgs a) {
     constexpr int RM = 16 * RT, E = D / 16, KS = D / 32; /* values of V a lane has; steps of the K product */
     constexpr bool kCoded = FMT != W4A16_KV_BF16;
     constexpr int kVWords = kCoded ? E / 4 : E / 2, kKLoads = kCoded ? KS / 2 : KS;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
-    const int head = blockIdx.x % a.kv.heads, item = blockIdx.x / a.kv.heads, split = blockIdx.y;
+    const int mask = (1 << a.kv.shift) - 1;
     Tile t;
-    if (!find_tile<RM>(a, item, split, &t)) return;
-    if (split >= t.active) return;
+    int head, first_part;
+    if (!find_part<RM, false>(a, blockIdx.x, &t, &head, &first_part)) return;
 
     const int32_t *table = a.kv.table + (long long)t.seq * a.kv.table_stride;
-    const int mask = (1 << a.kv.shift) - 1;
     /* Pages of this lane's K tokens and V tokens (page sizes are multiples of 8, so four
      * neighbours from a multiple of 4 share one). Tokens that are not there read token 0 of page 0
      * and are masked. */
@@ -334,23 +445,24 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
         f4 s[RT][2];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-            bf8 k[KS];
-            if constexpr (kCoded) {
 #pragma unroll
-                for (int j = 0; j < KS / 2; ++j) {
-                    const u4 x = kraw[c][j];
-                    k[2 * j] = as_bf8(kv_widen<FMT, 0>(x.x), kv_widen<FMT, 1>(x.x), kv_widen<FMT, 0>(x.y), kv_widen<FMT, 1>(x.y));
-                    k[2 * j + 1] = as_bf8(kv_widen<FMT, 0>(x.z), kv_widen<FMT, 1>(x.z), kv_widen<FMT, 0>(x.w), kv_widen<FMT, 1>(x.w));
+            for (int r = 0; r < RT; ++r) s[r][c] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int j = 0; j < kKLoads; ++j) {
+                u4 x = kraw[c][j];
+                if constexpr (kCoded) {
+                    asm volatile("" : "+v"(x)); /* or the bytes are carried apart, each in a register */
+                    const bf8 k0 = as_bf8(kv_widen<FMT, 0>(x.x), kv_widen<FMT, 1>(x.x), kv_widen<FMT, 0>(x.y), kv_widen<FMT, 1>(x.y));
+                    const bf8 k1 = as_bf8(kv_widen<FMT, 0>(x.z), kv_widen<FMT, 1>(x.z), kv_widen<FMT, 0>(x.w), kv_widen<FMT, 1>(x.w));
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) {
+                        s[r][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, q[r][2 * j], s[r][c], 0, 0, 0);
+                        s[r][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, q[r][2 * j + 1], s[r][c], 0, 0, 0);
+                    }
+                } else {
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) s[r][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, x), q[r][j], s[r][c], 0, 0, 0);
                 }
-            } else {
-#pragma unroll
-                for (int j = 0; j < KS; ++j) k[j] = __builtin_bit_cast(bf8, kraw[c][j]);
-            }
-#pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                s[r][c] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int j = 0; j < KS; ++j) s[r][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[j], q[r][j], s[r][c], 0, 0, 0);
             }
         }
         f4 ks_next[2], vs_next[2];
@@ -358,6 +470,11 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
             load_k(next);
             load_scales(next, ks_next, vs_next);
         }
+        if constexpr (kCoded)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int w = 0; w < kVWords; ++w) asm volatile("" : "+v"(v[i][w]));
         /* tokens that some row does not see, or that are not there: their V is not multiplied */
         const bool cut = t0 < t.all_lo || t0 + 32 > t.all_hi || __any(!there[0] || !there[1]);
         bool odd = false;
@@ -507,7 +624,7 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnArgs a) {
     constexpr int kPart = D < 128 ? D : 128, kPad = kPart + 4, kPer = kPart / 16;
     __shared__ float o_all[4][16][kPad];
     __shared__ float m_all[4][16], l_all[4][16];
-    float *partial = t.active > 1 ? partial_of<D, RM>(a, item, head, split) : nullptr;
+    float *partial = t.active > 1 ? partial_at<D, RM>(a, blockIdx.x) : nullptr;
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
         const float sum = lane_sum32(lane_sum16(l[r]));
@@ -930,7 +1047,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_chunk_kernel(AttnA
     const float total = lane_sum32(l);
     if (!real) return;
     float by = kCoded ? power_of_two(v_exp) : 1.0f;
-    float *partial = t.active > 1 ? partial_of<D, RM>(a, item, head, split) : nullptr;
+    float *partial = t.active > 1 ? partial_at<D, RM>(a, ((long long)item * a.kv.heads + head) * a.splits + split) : nullptr;
     if (partial) {
 #pragma unroll
         for (int d = 0; d < DB; ++d)
@@ -957,22 +1074,27 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_chunk_kernel(AttnA
             total == 0.0f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(total)) * kLn2;
 }
 
-/* Joins the splits of a tile that has more than one. A block has 16 / SUB rows (blockIdx.y of
+/* Joins the parts of a (tile, head) that has more than one: the splits of the chunk kernel, or the
+ * parts of the few-row kernel (EVEN). A block has 16 / SUB rows (blockIdx.y of
  * them), 16 lanes a row and part of its splits: with many splits the sum over them is what takes
  * time, so SUB parts of it run side by side and meet in LDS. */
-template <int D, int RM, int SUB>
+template <int D, int RM, int SUB, bool EVEN>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     constexpr int kPer = D / 16, kRows = 16 / SUB;
-    const int head = blockIdx.x % a.kv.heads, item = blockIdx.x / a.kv.heads;
     Tile t;
-    if (!find_tile<RM>(a, item, 0, &t) || t.active < 2 || (int)blockIdx.y * kRows >= t.rows) return;
+    int head, first_part = 0;
+    if constexpr (EVEN) {
+        if (!find_part<RM, true>(a, blockIdx.x, &t, &head, &first_part)) return;
+    } else {
+        head = blockIdx.x % a.kv.heads;
+        if (!find_tile<RM>(a, blockIdx.x / a.kv.heads, 0, &t)) return;
+    }
+    if (t.active < 2 || (int)blockIdx.y * kRows >= t.rows) return;
     const int lane = threadIdx.x & 15, unit = threadIdx.x >> 4, sub = unit / kRows, i = blockIdx.y * kRows + unit % kRows;
-    const float *from = partial_of<D, RM>(a, item, head, 0);
-    constexpr long long kStep = RM * (D + 2);
     const int row = i < t.rows ? i : t.rows - 1;
-    const float *ml = from + RM * D + 2 * row, *values = from + (long long)row * D + lane * kPer;
+    auto part_of = [&](int s) { return partial_at<D, RM>(a, (EVEN ? first_part : (long long)blockIdx.x * a.splits) + s); };
     float top = -__builtin_inff();
-    for (int s = lane; s < t.active; s += 16) top = fmaxf(top, ml[s * kStep]);
+    for (int s = lane; s < t.active; s += 16) top = fmaxf(top, part_of(s)[RM * D + 2 * row]);
 #pragma unroll
     for (int x = 1; x < 16; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
     const float base = top == -__builtin_inff() ? 0.0f : top;
@@ -981,11 +1103,12 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     for (int j = 0; j < kPer; ++j) o[j] = 0.0f;
 #pragma unroll 4
     for (int s = sub; s < t.active; s += SUB) {
-        const float f = __builtin_amdgcn_exp2f(ml[s * kStep] - base);
-        total += f * ml[s * kStep + 1];
+        const float *from = part_of(s), *ml = from + RM * D + 2 * row, *values = from + row * D + lane * kPer;
+        const float f = __builtin_amdgcn_exp2f(ml[0] - base);
+        total += f * ml[1];
 #pragma unroll
         for (int j = 0; j < kPer; j += 4) {
-            const f4 x = *reinterpret_cast<const f4 *>(values + s * kStep + j);
+            const f4 x = *reinterpret_cast<const f4 *>(values + j);
 #pragma unroll
             for (int c = 0; c < 4; ++c) o[j + c] += f * x[c];
         }
@@ -1016,11 +1139,12 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
 }
 
 /* How a call is cut: sequences of few (token, head) rows into tiles of 16 rt rows, the others into
- * tiles of 128; at most `items` tiles a key head, `splits` of each, and where their partial results
- * begin in the workspace. */
+ * tiles of 128; at most `items` tiles a key head, `splits` of each (for few rows, of all), and
+ * where their partial results begin in the workspace. */
 struct Part {
     int items, splits, over, upto;
     size_t ws_at;
+    long long blocks; /* few rows */
 };
 struct Plan {
     int rt;
@@ -1040,8 +1164,8 @@ Plan plan_of(const W4A16KvCache *c, const W4A16KvBatch *b, int q_heads) {
     const int limit = dim == 256 ? 16 : 32;
     p.rt = longest <= 16 || dim == 256 ? 1 : 2;
     const int rm = 16 * p.rt;
-    p.few = {0, 1, 0, INT32_MAX, 0};
-    p.many = {0, 1, 0, INT32_MAX, 0};
+    p.few = {0, 1, 0, INT32_MAX, 0, 0};
+    p.many = {0, 1, 0, INT32_MAX, 0, 0};
     if (longest <= limit) {
         p.few.items = (int)(rows / rm + seqs);
     } else if ((long long)b->seqs * max_new == b->rows || group > limit) {
@@ -1053,26 +1177,35 @@ Plan plan_of(const W4A16KvCache *c, const W4A16KvBatch *b, int q_heads) {
         p.many.items = (int)(rows / kChunkRows + (rows / (rm + 1) < seqs ? rows / (rm + 1) : seqs));
     }
     const long long tokens = b->max_kv ? b->max_kv : (long long)b->table_pages * c->page_size;
-    const long long most = (tokens + kFewestTokens - 1) / kFewestTokens;
-    for (Part *x : {&p.few, &p.many}) {
-        const bool few = x == &p.few;
-        const long long blocks = (long long)x->items * c->kv_heads, wanted = (few ? 4LL : 2LL) * device_cus();
-        long long splits = blocks > 0 ? (wanted + blocks - 1) / blocks : 1;
+    if (p.few.items) {
+        /* One round of blocks (48 ragged sequences of up to 8192 tokens, INT8: 91.0 us; one and a
+         * half: 100.5, two: 85.8; 16 with verify rows, FP8: 22.0 / 25.8 / 24.0; 2 of 100003 tokens,
+         * D = 256: 77.8 / 89.7 / 82.8), and no more than there are units. */
+        const long long blocks = (long long)rows_blocks(dim, c->format, p.rt) * device_cus();
+        const long long pairs = (long long)p.few.items * c->kv_heads, units = pairs * ((tokens + kUnit - 1) / kUnit);
+        p.few.splits = (int)(units < 1 ? 1 : units < blocks ? units : blocks);
+        p.few.blocks = p.few.splits + pairs;
+        p.ws_bytes = (size_t)p.few.blocks * rm * (dim + 2) * 4;
+    }
+    if (p.many.items) {
+        const long long blocks = (long long)p.many.items * c->kv_heads, wanted = 2LL * device_cus();
+        const long long most = (tokens + kFewestTokens - 1) / kFewestTokens;
+        long long splits = (wanted + blocks - 1) / blocks;
         if (splits > most) splits = most;
         if (splits > 256) splits = 256;
-        x->splits = splits < 1 ? 1 : (int)splits;
-        x->ws_at = p.ws_bytes;
-        if (x->splits > 1) p.ws_bytes += (size_t)blocks * x->splits * (few ? rm : kChunkRows) * (dim + 2) * 4;
+        p.many.splits = splits < 1 ? 1 : (int)splits;
+        p.many.ws_at = p.ws_bytes;
+        if (p.many.splits > 1) p.ws_bytes += (size_t)blocks * p.many.splits * kChunkRows * (dim + 2) * 4;
     }
     return p;
 }
 
-template <int D, int RM>
-void launch_join(const Part &p, const AttnArgs &a, hipStream_t s) {
-    const unsigned x = a.kv.heads * p.items;
-    if (p.splits > 16) launch_k(attn_join_kernel<D, RM, 16>, dim3(x, RM), dim3(256), 0, s, a);
-    else if (p.splits > 4) launch_k(attn_join_kernel<D, RM, 4>, dim3(x, RM / 4), dim3(256), 0, s, a);
-    else if (p.splits > 1) launch_k(attn_join_kernel<D, RM, 1>, dim3(x, RM / 16), dim3(256), 0, s, a);
+template <int D, int RM, bool EVEN>
+void launch_join(int parts, const AttnArgs &a, hipStream_t s) {
+    const unsigned x = a.kv.heads * a.items;
+    if (parts > 16) launch_k(attn_join_kernel<D, RM, 16, EVEN>, dim3(x, RM), dim3(256), 0, s, a);
+    else if (parts > 4) launch_k(attn_join_kernel<D, RM, 4, EVEN>, dim3(x, RM / 4), dim3(256), 0, s, a);
+    else if (parts > 1) launch_k(attn_join_kernel<D, RM, 1, EVEN>, dim3(x, RM / 16), dim3(256), 0, s, a);
 }
 
 AttnArgs part_args(const AttnArgs &all, const Part &p) {
@@ -1090,18 +1223,18 @@ void launch_format(const Plan &p, const AttnArgs &all, hipStream_t s) {
     if (p.many.items) {
         const AttnArgs a = part_args(all, p.many);
         launch_k(attn_chunk_kernel<D, FMT>, dim3(a.kv.heads * a.items, a.splits), dim3(256), Chunk<D, FMT>::kBytes, s, a);
-        launch_join<D, kChunkRows>(p.many, a, s);
+        launch_join<D, kChunkRows, false>(a.splits, a, s);
     }
     if (p.few.items) {
         const AttnArgs a = part_args(all, p.few);
-        const dim3 grid(a.kv.heads * a.items, a.splits);
+        const int parts = (a.splits + a.items * a.kv.heads - 1) / (a.items * a.kv.heads) + 1; /* of each, about */
         if constexpr (D <= 128)
             if (p.rt == 2) {
-                launch_k(attn_rows_kernel<D, FMT, 2>, grid, dim3(256), 0, s, a);
-                return launch_join<D, 32>(p.few, a, s);
+                launch_k(attn_rows_kernel<D, FMT, 2>, dim3((unsigned)p.few.blocks), dim3(256), 0, s, a);
+                return launch_join<D, 32, true>(parts, a, s);
             }
-        launch_k(attn_rows_kernel<D, FMT, 1>, grid, dim3(256), 0, s, a);
-        launch_join<D, 16>(p.few, a, s);
+        launch_k(attn_rows_kernel<D, FMT, 1>, dim3((unsigned)p.few.blocks), dim3(256), 0, s, a);
+        launch_join<D, 16, true>(parts, a, s);
     }
 }
 

@@ -108,10 +108,15 @@ def test_workspaces():
     need = ctypes.c_size_t(7)
     one = cache(num_pages=1 << 20)
     lib = w4a16.lib
-    assert lib.w4a16_paged_attention_workspace(ctypes.byref(one), ctypes.byref(batch(max_kv=100)), 4, ctypes.byref(need)) == 0
-    assert need.value == 0  # one split
-    assert lib.w4a16_paged_attention_workspace(ctypes.byref(one), ctypes.byref(batch(max_kv=50000)), 4, ctypes.byref(need)) == 0
-    assert need.value > 0
+    sizes = []
+    for most in (100, 50000):
+        assert lib.w4a16_paged_attention_workspace(ctypes.byref(one), ctypes.byref(batch(max_kv=most)), 4, ctypes.byref(need)) == 0
+        sizes.append(need.value)
+    assert 0 < sizes[0] < sizes[1]
+    # many rows in many tiles: nothing to join
+    many = batch(rows=1 << 16, seqs=1, max_new=1 << 16)
+    assert lib.w4a16_paged_attention_workspace(ctypes.byref(one), ctypes.byref(many), 4, ctypes.byref(need)) == 0
+    assert need.value == 0
     assert lib.w4a16_paged_attention_workspace(ctypes.byref(one), ctypes.byref(batch()), 4, None) == CONFIG
     assert lib.w4a16_paged_attention_workspace(None, ctypes.byref(batch()), 4, ctypes.byref(need)) == CONFIG
     assert lib.w4a16_verify_drafts_workspace(3, 2, 100000, ctypes.byref(need)) == 0 and need.value >= 3 * 16
