@@ -20,8 +20,11 @@ using namespace w4a16;
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kPerThread = 16;
-constexpr int kPiece = kThreads * kPerThread; /* weights a block sums */
+constexpr int kQuads = 4;                     /* of neighbouring weights, a thread's: quad j of thread t is at 4 (256 j + t) */
+constexpr int kPiece = kThreads * kQuads * 4; /* weights a block sums */
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f4_loose __attribute__((ext_vector_type(4), aligned(4))); /* rows start anywhere */
 
 struct DraftArgs {
     const float *target, *draft;
@@ -30,11 +33,14 @@ struct DraftArgs {
     const float *uniforms;
     int32_t *accepted, *tokens;
     double *sums; /* [seqs][pieces][2]: of the weights, of the target's row */
+    int2 *found;  /* [seqs]: tokens taken; where one was refused, it (INT32_MIN: none) */
     int steps, vocab, pieces;
 };
 
-/* How many of the sequence's tokens are taken, and whether one was refused behind them: by one
- * wave, 64 tokens at a time. */
+constexpr int kNone = INT32_MIN;
+
+/* How many of the sequence's tokens are taken, and the one refused behind them (kNone: all taken):
+ * by one wave, 64 tokens at a time. */
 __device__ __forceinline__ int taken_of(const DraftArgs &a, int seq, int *refused) {
     const int lane = threadIdx.x & 63;
     int n = a.lens ? a.lens[seq] : a.steps;
@@ -42,22 +48,25 @@ __device__ __forceinline__ int taken_of(const DraftArgs &a, int seq, int *refuse
     for (int base = 0; base < n; base += 64) {
         const int i = base + lane;
         bool take = true;
+        int x = 0;
         if (i < n) {
-            const int x = a.draft_tokens[(long long)seq * a.steps + i];
+            x = a.draft_tokens[(long long)seq * a.steps + i];
             take = false;
             if ((unsigned)x < (unsigned)a.vocab) {
                 const double p = a.target[seq * a.target_seq + i * a.target_row + x];
                 const double q = a.draft ? a.draft[seq * a.draft_seq + i * a.draft_row + x] : 1.0f;
                 take = (double)a.uniforms[(long long)seq * (a.steps + 1) + i] * q < p;
             }
+            x = x == kNone ? -1 : x; /* outside the vocabulary either way */
         }
         const unsigned long long no = __ballot(!take);
         if (no) {
-            *refused = 1;
-            return base + __ffsll(no) - 1;
+            const int l = __ffsll((long long)no) - 1;
+            *refused = __builtin_amdgcn_readlane(x, l);
+            return base + l;
         }
     }
-    *refused = 0;
+    *refused = kNone;
     return n;
 }
 
@@ -66,6 +75,16 @@ __device__ __forceinline__ float weight(float w) { return w > 0.0f && w < __buil
 /* The weight of token i in the row that is drawn from, and the target's own. */
 __device__ __forceinline__ float rest_of(float p, float q, bool has_q, int i, int chosen) {
     return has_q ? weight(p - q) : i == chosen ? 0.0f : weight(p);
+}
+
+/* Weights i .. i + 3 of a row of n; zeros behind it. */
+__device__ __forceinline__ f4 load_quad(const float *row, int i, int n) {
+    if (i + 4 <= n) return *reinterpret_cast<const f4_loose *>(row + i);
+    f4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int c = 0; c < 3; ++c)
+        if (i + c < n) v[c] = row[i + c];
+    return v;
 }
 
 /* The row drawn from: the target's, what is taken off it, and the one token that is where the
@@ -77,59 +96,73 @@ struct Row {
 
 __device__ __forceinline__ Row row_of(const DraftArgs &a, int seq, int taken, int refused) {
     Row r = {a.target + seq * a.target_seq + taken * a.target_row, nullptr, -1};
-    if (refused) {
-        const int x = a.draft_tokens[(long long)seq * a.steps + taken];
+    if (refused != kNone) {
         if (a.draft)
             r.q = a.draft + seq * a.draft_seq + taken * a.draft_row;
         else
-            r.chosen = x;
+            r.chosen = refused;
     }
     return r;
 }
 
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-    for (int m = 32; m; m /= 2) v += __shfl_xor(v, m);
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_or_zero(double v) {
+    const uint2 b = __builtin_bit_cast(uint2, v);
+    return __builtin_bit_cast(double, make_uint2((uint32_t)__builtin_amdgcn_update_dpp(0, (int)b.x, CTRL, ROWS, 0xF, false),
+                                                 (uint32_t)__builtin_amdgcn_update_dpp(0, (int)b.y, CTRL, ROWS, 0xF, false)));
+}
+
+/* Sum of v over the lanes up to and with this one, by VALU moves: row shifts within 16 lanes, then the
+ * rows' last lanes carried to the rows behind. */
+__device__ __forceinline__ double wave_scan(double v) {
+    v += dpp_or_zero<0x111, 0xF>(v);
+    v += dpp_or_zero<0x112, 0xF>(v);
+    v += dpp_or_zero<0x114, 0xF>(v);
+    v += dpp_or_zero<0x118, 0xF>(v);
+    v += dpp_or_zero<0x142, 0xA>(v); /* row_bcast:15 into rows 1 and 3 */
+    v += dpp_or_zero<0x143, 0xC>(v); /* row_bcast:31 into rows 2 and 3 */
     return v;
 }
 
-/* Sum of v over the lanes up to and with this one. */
-__device__ __forceinline__ double wave_scan(double v) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int m = 1; m < 64; m *= 2) {
-        const double o = __shfl_up(v, m);
-        if (lane >= m) v += o;
-    }
-    return v;
+__device__ __forceinline__ double lane_f64(double v, int lane) {
+    const uint2 b = __builtin_bit_cast(uint2, v);
+    return __builtin_bit_cast(double, make_uint2((uint32_t)__builtin_amdgcn_readlane((int)b.x, lane),
+                                                 (uint32_t)__builtin_amdgcn_readlane((int)b.y, lane)));
 }
+
+__device__ __forceinline__ double wave_sum(double v) { return lane_f64(wave_scan(v), 63); }
 
 __global__ __launch_bounds__(kThreads) void drafts_sum_kernel(DraftArgs a) {
     const int seq = blockIdx.y, piece = blockIdx.x, tid = threadIdx.x;
     int refused;
     const int taken = taken_of(a, seq, &refused);
     if (piece == 0) {
-        if (tid == 0) a.accepted[seq] = taken;
+        if (tid == 0) {
+            a.accepted[seq] = taken;
+            a.found[seq] = make_int2(taken, refused);
+        }
         for (int i = tid; i <= a.steps; i += kThreads)
             if (i != taken)
                 a.tokens[(long long)seq * (a.steps + 1) + i] =
                     i < taken ? a.draft_tokens[(long long)seq * a.steps + i] : -1;
     }
     const Row r = row_of(a, seq, taken, refused);
-    float p[kPerThread], q[kPerThread];
+    f4 p[kQuads], q[kQuads];
 #pragma unroll
-    for (int j = 0; j < kPerThread; ++j) {
-        const int i = piece * kPiece + j * kThreads + tid;
-        p[j] = i < a.vocab ? r.p[i] : 0.0f;
-        q[j] = r.q && i < a.vocab ? r.q[i] : 0.0f;
+    for (int j = 0; j < kQuads; ++j) {
+        const int i = piece * kPiece + (j * kThreads + tid) * 4;
+        p[j] = load_quad(r.p, i, a.vocab);
+        q[j] = r.q ? load_quad(r.q, i, a.vocab) : f4{0.0f, 0.0f, 0.0f, 0.0f};
     }
     double rest = 0.0, all = 0.0;
 #pragma unroll
-    for (int j = 0; j < kPerThread; ++j) {
-        const int i = piece * kPiece + j * kThreads + tid;
-        rest += (double)rest_of(p[j], q[j], r.q != nullptr, i, r.chosen);
-        all += (double)weight(p[j]);
-    }
+    for (int j = 0; j < kQuads; ++j)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const int i = piece * kPiece + (j * kThreads + tid) * 4 + c;
+            rest += (double)rest_of(p[j][c], q[j][c], r.q != nullptr, i, r.chosen);
+            all += (double)weight(p[j][c]);
+        }
     __shared__ double part[2][kThreads / 64];
     rest = wave_sum(rest);
     all = wave_sum(all);
@@ -147,22 +180,24 @@ __global__ __launch_bounds__(kThreads) void drafts_sum_kernel(DraftArgs a) {
 
 __global__ __launch_bounds__(kThreads) void drafts_draw_kernel(DraftArgs a) {
     const int seq = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
-    const double *sums = a.sums + (long long)seq * a.pieces * 2;
-    int refused;
-    const int taken = taken_of(a, seq, &refused);
-    const Row r = row_of(a, seq, taken, refused);
+    const double2 *sums = reinterpret_cast<const double2 *>(a.sums) + (long long)seq * a.pieces;
+    const int2 got = a.found[seq];
+    const float uniform = a.uniforms[(long long)seq * (a.steps + 1) + a.steps];
     /* every wave does the same over the pieces' sums */
-    double rest = 0.0, all = 0.0;
-    for (int i = lane; i < a.pieces; i += 64) {
-        rest += sums[2 * i];
-        all += sums[2 * i + 1];
+    double2 first_sums = lane < a.pieces ? sums[lane] : double2{0.0, 0.0};
+    double rest = first_sums.x, all = first_sums.y;
+    for (int i = lane + 64; i < a.pieces; i += 64) {
+        const double2 s = sums[i];
+        rest += s.x;
+        all += s.y;
     }
     rest = wave_sum(rest);
     all = wave_sum(all);
-    const int which = rest > 0.0 ? 0 : 1;
+    const Row r = row_of(a, seq, got.x, got.y);
+    const bool which = !(rest > 0.0); /* from the target's own weights */
     const double total = which ? all : rest;
-    const double pass = (double)a.uniforms[(long long)seq * (a.steps + 1) + a.steps] * total;
-    int32_t *out = a.tokens + (long long)seq * (a.steps + 1) + taken;
+    const double pass = (double)uniform * total;
+    int32_t *out = a.tokens + (long long)seq * (a.steps + 1) + got.x;
     if (!(total > 0.0)) {
         if (tid == 0) *out = -1;
         return;
@@ -171,48 +206,70 @@ __global__ __launch_bounds__(kThreads) void drafts_draw_kernel(DraftArgs a) {
     double before = 0.0, start = 0.0;
     int piece = -1;
     for (int base = 0; base < a.pieces; base += 64) {
-        const double v = base + lane < a.pieces ? sums[2 * (base + lane) + which] : 0.0;
+        if (base) first_sums = base + lane < a.pieces ? sums[base + lane] : double2{0.0, 0.0};
+        const double v = which ? first_sums.y : first_sums.x;
         const double upto = before + wave_scan(v);
         const unsigned long long here = __ballot(v > 0.0), passing = __ballot(v > 0.0 && upto > pass);
-        const unsigned long long pick = passing ? passing & -passing : here ? 1ULL << (63 - __clzll(here)) : 0ULL;
+        const unsigned long long pick = passing ? passing & -passing : here ? 1ULL << (63 - __clzll((long long)here)) : 0ULL;
         if (pick) {
-            const int l = __ffsll(pick) - 1;
+            const int l = __ffsll((long long)pick) - 1;
             piece = base + l;
-            const double previous = l ? __shfl(upto, l - 1) : before;
-            start = previous;
+            start = l ? lane_f64(upto, l - 1) : before;
         }
-        before = __shfl(upto, 63);
+        before = lane_f64(upto, 63);
         if (passing) break;
     }
-    /* through that piece: a thread's own neighbours in order, then the waves, then the block */
-    const int first = piece * kPiece + tid * kPerThread;
-    double own[kPerThread], sum = 0.0;
+    /* Through that piece in order: 1024 weights a round j, of them 256 a wave, of them 4 a lane. A
+     * quad's running sum is what stands before the piece, the (round, wave) pairs before its own,
+     * the lanes before it. */
+    f4 own[kQuads], q[kQuads];
 #pragma unroll
-    for (int j = 0; j < kPerThread; ++j) {
-        const int i = first + j;
-        float w = 0.0f;
-        if (i < a.vocab) w = which ? weight(r.p[i]) : rest_of(r.p[i], r.q ? r.q[i] : 0.0f, r.q != nullptr, i, r.chosen);
-        own[j] = w;
-        sum += own[j];
+    for (int j = 0; j < kQuads; ++j) {
+        const int i = piece * kPiece + (j * kThreads + tid) * 4;
+        own[j] = load_quad(r.p, i, a.vocab);
+        q[j] = r.q && !which ? load_quad(r.q, i, a.vocab) : f4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    __shared__ double waves[kThreads / 64];
+    constexpr int kWaves = kThreads / 64;
+    __shared__ double before_of[kQuads * kWaves];
     __shared__ int found, last;
-    const double upto = wave_scan(sum);
-    if (lane == 63) waves[tid >> 6] = upto;
+    double upto[kQuads];
+#pragma unroll
+    for (int j = 0; j < kQuads; ++j) {
+        double sum = 0.0;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const int i = piece * kPiece + (j * kThreads + tid) * 4 + c;
+            own[j][c] = which ? weight(own[j][c]) : rest_of(own[j][c], q[j][c], r.q != nullptr, i, r.chosen);
+            sum += (double)own[j][c];
+        }
+        upto[j] = wave_scan(sum);
+        if (lane == 63) before_of[j * kWaves + (tid >> 6)] = upto[j];
+        upto[j] -= sum; /* before this quad */
+    }
     if (tid == 0) {
         found = INT32_MAX;
         last = -1;
     }
     __syncthreads();
-    double run = start + upto - sum;
-    for (int w = 0; w < (tid >> 6); ++w) run += waves[w];
     int mine = INT32_MAX, behind = -1;
+    double run_before = start;
 #pragma unroll
-    for (int j = 0; j < kPerThread; ++j) {
-        run += own[j];
-        if (own[j] > 0.0) {
-            behind = first + j;
-            if (run > pass && mine == INT32_MAX) mine = first + j;
+    for (int j = 0; j < kQuads; ++j) {
+        double run = run_before + upto[j];
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const double of = before_of[j * kWaves + w];
+            if (w < (tid >> 6)) run += of;
+            run_before += of;
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const int i = piece * kPiece + (j * kThreads + tid) * 4 + c;
+            run += (double)own[j][c];
+            if (own[j][c] > 0.0f) {
+                behind = i;
+                if (run > pass && mine == INT32_MAX) mine = i;
+            }
         }
     }
     if (mine != INT32_MAX) atomicMin(&found, mine);
@@ -228,7 +285,7 @@ extern "C" int w4a16_verify_drafts_workspace(int seqs, int steps, int vocab, siz
     if (seqs < 0 || seqs > 65535 || steps < 0 || steps > 65535 || vocab < 1 || vocab > (1 << 28))
         return set_error(W4A16_ERR_CONFIG, "w4a16_verify_drafts: bad extents seqs=%d steps=%d vocab=%d (seqs and steps "
                          "up to 65535, vocab 1 to 2^28)", seqs, steps, vocab);
-    *bytes = (size_t)seqs * ((vocab + kPiece - 1) / kPiece) * 16;
+    *bytes = (size_t)seqs * ((size_t)((vocab + kPiece - 1) / kPiece) * 16 + 16);
     return W4A16_OK;
 }
 
@@ -273,7 +330,7 @@ extern "C" int w4a16_verify_drafts_f32(const float *target, long long target_seq
     const int pieces = (vocab + kPiece - 1) / kPiece;
     const DraftArgs a = {target, steps > 0 ? draft : nullptr, target_seq_stride, target_row_stride, draft_seq_stride,
                          draft_row_stride, draft_tokens, lens, uniforms, accepted, tokens, static_cast<double *>(ws),
-                         steps, vocab, pieces};
+                         reinterpret_cast<int2 *>(static_cast<double *>(ws) + (size_t)seqs * pieces * 2), steps, vocab, pieces};
     hipStream_t s = static_cast<hipStream_t>(stream);
     launch_k(drafts_sum_kernel, dim3(pieces, seqs), dim3(kThreads), 0, s, a);
     launch_k(drafts_draw_kernel, dim3(seqs), dim3(kThreads), 0, s, a);

@@ -639,25 +639,46 @@ def _refuse(what):
 
 
 def _on_current(device, what):
-    """The library launches on the current device: tensors of another one are refused."""
+    """The library launches on the current device: tensors of another one are refused. Returns the
+    device's index."""
     import torch
 
     if device.type != "cuda" or device.index != torch.cuda.current_device():
         _refuse(f"{what}: tensors on {device}, which is not the current GPU")
+    return device.index
 
 
-def _rows3(t, rows, heads, dim, device, what):
+def _raw_stream(stream, index):
+    """As _stream, where the current device's index is known already."""
+    if stream is None:
+        raw = getattr(_torch_c(), "_cuda_getCurrentRawStream", None)
+        if raw is not None:
+            return raw(index)
+    return _stream(stream)
+
+
+def _torch_c():
+    import torch
+
+    return torch._C
+
+
+def _rows3(t, shape, device, what):
     """Address and strides of a [rows, heads, dim] tensor of BF16 values whose last axis is dense."""
+    try:
+        if t.shape == shape and t.device == device and t.element_size() == 2:
+            row, head, one = t.stride()
+            if one == 1:
+                return t.data_ptr(), row, head
+    except (AttributeError, TypeError, ValueError):
+        pass  # named below
     if not hasattr(t, "is_cuda") or not t.is_cuda or t.device != device:
         _refuse(f"{what}: expected a tensor on {device}")
-    if t.dim() != 3 or t.shape[0] != rows or t.shape[1] != heads or t.shape[2] != dim:
-        _refuse(f"{what}: shape {tuple(t.shape)}, the call needs {(rows, heads, dim)}")
-    if t.element_size() != 2 or t.is_complex():
+    if t.shape != shape:
+        _refuse(f"{what}: shape {tuple(t.shape)}, the call needs {shape}")
+    if t.element_size() != 2:
         _refuse(f"{what}: {t.dtype} is not BF16 (or its bits)")
-    row, head, one = t.stride()
-    if one != 1:
-        _refuse(f"{what}: the last axis is strided")
-    return t.data_ptr(), row, head
+    _refuse(f"{what}: the last axis is strided")
 
 
 class KvCache:
@@ -684,6 +705,7 @@ class KvCache:
                                  _dev(v, size, v.element_size(), "KvCache v", k.device), scales[0], scales[1],
                                  formats[k.dtype], self.num_pages, self.page_size, self.kv_heads, self.head_dim)
         self._ref = ctypes.addressof(self._c)
+        self._plan = tuple(k.shape) + (formats[k.dtype],)
 
     @classmethod
     def empty(cls, num_pages, page_size, kv_heads, head_dim, format="bf16", device="cuda"):
@@ -700,19 +722,21 @@ class KvCache:
 
     def write(self, k, v, batch, stream=None):
         """Writes the batch's rows of k and v [rows, kv_heads, head_dim] (strided views are fine)."""
-        _on_current(self.device, "KvCache.write")
+        index = _on_current(self.device, "KvCache.write")
         batch.check(self.device, "KvCache.write")
-        kp, k_row, k_head = _rows3(k, batch.rows, self.kv_heads, self.head_dim, self.device, "KvCache.write k")
-        vp, v_row, v_head = _rows3(v, batch.rows, self.kv_heads, self.head_dim, self.device, "KvCache.write v")
-        _check(lib.w4a16_kv_write_bf16(self._ref, batch._ref, kp, k_row, k_head, vp, v_row, v_head, _stream(stream)),
-               "KvCache.write")
+        shape = (batch.rows, self.kv_heads, self.head_dim)
+        kp, k_row, k_head = _rows3(k, shape, self.device, "KvCache.write k")
+        vp, v_row, v_head = _rows3(v, shape, self.device, "KvCache.write v")
+        st = lib.w4a16_kv_write_bf16(self._ref, batch._ref, kp, k_row, k_head, vp, v_row, v_head, _raw_stream(stream, index))
+        if st:
+            _check(st, "KvCache.write")
 
     def read(self, batch, out=None, stream=None):
         """The batch's rows out of the cache: (k, v) as BF16 [rows, kv_heads, head_dim]. Without
         `out` rows of no sequence are zeros; with it they are left as they were."""
         import torch
 
-        _on_current(self.device, "KvCache.read")
+        index = _on_current(self.device, "KvCache.read")
         batch.check(self.device, "KvCache.read")
         shape = (batch.rows, self.kv_heads, self.head_dim)
         if out is None:
@@ -720,7 +744,7 @@ class KvCache:
             out = tuple(make(shape, dtype=torch.bfloat16, device=self.device) for _ in range(2))
         size = batch.rows * self.kv_heads * self.head_dim * 2
         k, v = (_dev(t, size, 2, "KvCache.read out", self.device) for t in out)
-        _check(lib.w4a16_kv_read_bf16(self._ref, batch._ref, k, v, _stream(stream)), "KvCache.read")
+        _check(lib.w4a16_kv_read_bf16(self._ref, batch._ref, k, v, _raw_stream(stream, index)), "KvCache.read")
         return out
 
 
@@ -751,6 +775,7 @@ class KvBatch:
         self._c = _KvBatchStruct(page_table.data_ptr(), kv_lens.data_ptr(), starts.data_ptr(), seqs, rows, pages,
                                  stride, max_new, max_kv)
         self._ref = ctypes.addressof(self._c)
+        self._workspaces = {}  # bytes that paged_attention needs, by the cache's sizes and the query heads
 
     def check(self, device, what):
         if self.device != device:
@@ -766,27 +791,43 @@ def paged_attention(q, cache, batch, scale=None, causal=True, window=0, out=None
     import torch
 
     device = cache.device
-    _on_current(device, "paged_attention")
+    index = _on_current(device, "paged_attention")
     batch.check(device, "paged_attention")
-    q_heads = q.shape[1] if q.dim() == 3 else 0
-    qp, q_row, q_head = _rows3(q, batch.rows, q_heads, cache.head_dim, device, "paged_attention q")
+    rows, dim = batch.rows, cache.head_dim
+    q_heads = q.shape[1] if len(q.shape) == 3 else 0
+    shape = (rows, q_heads, dim)
+    qp, q_row, q_head = _rows3(q, shape, device, "paged_attention q")
     if out is None:
-        make = torch.zeros if batch.padded else torch.empty
-        out = make((batch.rows, q_heads, cache.head_dim), dtype=torch.bfloat16, device=device)
-    op, o_row, o_head = _rows3(out, batch.rows, q_heads, cache.head_dim, device, "paged_attention out")
+        if batch.padded or q.dtype != torch.bfloat16:
+            out = torch.zeros(shape, dtype=torch.bfloat16, device=device)
+        else:
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        op, o_row, o_head = out.data_ptr(), q_heads * dim, dim
+    else:
+        op, o_row, o_head = _rows3(out, shape, device, "paged_attention out")
     lse = None
     if return_lse:
-        lse = torch.full((batch.rows, q_heads), float("-inf"), device=device) if batch.padded else \
-            torch.empty((batch.rows, q_heads), dtype=torch.float32, device=device)
-    need = ctypes.c_size_t(0)
-    _check(lib.w4a16_paged_attention_workspace(cache._ref, batch._ref, q_heads, ctypes.byref(need)), "paged_attention")
-    if need.value and workspace is None:
-        workspace = torch.empty(need.value, dtype=torch.uint8, device=device)
-    wp = _dev(workspace, need.value, 1, "paged_attention workspace", device) if need.value else None
-    _check(lib.w4a16_paged_attention_bf16(cache._ref, batch._ref, qp, q_row, q_head, q_heads,
-                                          cache.head_dim ** -0.5 if scale is None else scale, int(causal), window, op,
-                                          o_row, o_head, None if lse is None else lse.data_ptr(), wp, need.value,
-                                          _stream(stream)), "paged_attention")
+        lse = torch.full((rows, q_heads), float("-inf"), device=device) if batch.padded else \
+            torch.empty((rows, q_heads), dtype=torch.float32, device=device)
+    key = (cache._plan, q_heads)
+    need = batch._workspaces.get(key)  # by the sizes alone
+    if need is None:
+        size = ctypes.c_size_t(0)
+        _check(lib.w4a16_paged_attention_workspace(cache._ref, batch._ref, q_heads, ctypes.byref(size)), "paged_attention")
+        need = batch._workspaces[key] = size.value
+    wp = None
+    if need:
+        if workspace is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=device)
+            wp = workspace.data_ptr()
+        else:
+            wp = _dev(workspace, need, 1, "paged_attention workspace", device)
+    st = lib.w4a16_paged_attention_bf16(cache._ref, batch._ref, qp, q_row, q_head, q_heads,
+                                        dim ** -0.5 if scale is None else scale, 1 if causal else 0, window, op, o_row,
+                                        o_head, None if lse is None else lse.data_ptr(), wp, need,
+                                        _raw_stream(stream, index))
+    if st:
+        _check(st, "paged_attention")
     return (out, lse) if return_lse else out
 
 
@@ -800,6 +841,14 @@ def _floats3(t, what, device):
     return t.data_ptr(), t.stride(0), t.stride(1)
 
 
+def _exactly(t, shape, dtype, device, what):
+    """Address of a contiguous tensor of this shape and type."""
+    if not hasattr(t, "is_cuda") or t.shape != shape or t.dtype != dtype or t.device != device or not t.is_contiguous():
+        _refuse(f"{what}: expected a contiguous {dtype} {shape} on {device}, got "
+                f"{tuple(getattr(t, 'shape', ()))} {getattr(t, 'dtype', type(t).__name__)}")
+    return t.data_ptr()
+
+
 def verify_drafts(target, draft_tokens, uniforms, draft=None, lens=None, workspace=None, stream=None):
     """Verification of drafted tokens (see include/w4a16.h): target [seqs, steps + 1, vocab] and,
     where the tokens were drawn, draft [seqs, steps, vocab] probabilities in FP32, draft_tokens
@@ -808,7 +857,7 @@ def verify_drafts(target, draft_tokens, uniforms, draft=None, lens=None, workspa
     import torch
 
     device = target.device
-    _on_current(device, "verify_drafts")
+    index = _on_current(device, "verify_drafts")
     tp, t_seq, t_row = _floats3(target, "verify_drafts target", device)
     seqs, rows, vocab = target.shape
     steps = rows - 1
@@ -817,24 +866,23 @@ def verify_drafts(target, draft_tokens, uniforms, draft=None, lens=None, workspa
     dp, d_seq, d_row = None, 0, 0
     if draft is not None and steps > 0:
         dp, d_seq, d_row = _floats3(draft, "verify_drafts draft", device)
-        if tuple(draft.shape) != (seqs, steps, vocab):
+        if draft.shape != (seqs, steps, vocab):
             _refuse(f"verify_drafts: draft {tuple(draft.shape)}, the call needs {(seqs, steps, vocab)}")
-    for name, t, shape, dtype in (("draft_tokens", draft_tokens, (seqs, steps), torch.int32),
-                                  ("uniforms", uniforms, (seqs, rows), torch.float32),
-                                  ("lens", lens, (seqs,), torch.int32)):
-        if t is not None and (tuple(t.shape) != shape or t.dtype != dtype):
-            _refuse(f"verify_drafts: {name} {tuple(t.shape)} {t.dtype}, the call needs {shape} {dtype}")
-    ip = _dev(draft_tokens, seqs * steps * 4, 4, "verify_drafts draft_tokens", device)
-    up = _dev(uniforms, seqs * rows * 4, 4, "verify_drafts uniforms", device)
-    lp = None if lens is None else _dev(lens, seqs * 4, 4, "verify_drafts lens", device)
+    ip = _exactly(draft_tokens, (seqs, steps), torch.int32, device, "verify_drafts draft_tokens")
+    up = _exactly(uniforms, (seqs, rows), torch.float32, device, "verify_drafts uniforms")
+    lp = None if lens is None else _exactly(lens, (seqs,), torch.int32, device, "verify_drafts lens")
     accepted = torch.empty(seqs, dtype=torch.int32, device=device)
     tokens = torch.empty((seqs, rows), dtype=torch.int32, device=device)
-    need = ctypes.c_size_t(0)
-    _check(lib.w4a16_verify_drafts_workspace(seqs, steps, vocab, ctypes.byref(need)), "verify_drafts")
+    size = ctypes.c_size_t(0)
+    _check(lib.w4a16_verify_drafts_workspace(seqs, steps, vocab, ctypes.byref(size)), "verify_drafts")
+    need = size.value
     if workspace is None:
-        workspace = torch.empty(need.value, dtype=torch.uint8, device=device)
-    wp = _dev(workspace, need.value, 1, "verify_drafts workspace", device)
-    _check(lib.w4a16_verify_drafts_f32(tp, t_seq, t_row, dp, d_seq, d_row, ip, lp, up, accepted.data_ptr(),
-                                       tokens.data_ptr(), seqs, steps, vocab, wp, need.value, _stream(stream)),
-           "verify_drafts")
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+        wp = workspace.data_ptr()
+    else:
+        wp = _dev(workspace, need, 1, "verify_drafts workspace", device)
+    st = lib.w4a16_verify_drafts_f32(tp, t_seq, t_row, dp, d_seq, d_row, ip, lp, up, accepted.data_ptr(),
+                                     tokens.data_ptr(), seqs, steps, vocab, wp, need, _raw_stream(stream, index))
+    if st:
+        _check(st, "verify_drafts")
     return accepted, tokens
