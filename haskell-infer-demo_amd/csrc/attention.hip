@@ -89,6 +89,18 @@ __device__ __forceinline__ int wave_upto(int v) {
     return v;
 }
 
+/* The largest of v >= 0 over the lanes. */
+__device__ __forceinline__ int wave_most(int v) {
+    auto with = [&](int o) { v = o > v ? o : v; };
+    with(dpp_or_zero<0x111, 0xF>(v));
+    with(dpp_or_zero<0x112, 0xF>(v));
+    with(dpp_or_zero<0x114, 0xF>(v));
+    with(dpp_or_zero<0x118, 0xF>(v));
+    with(dpp_or_zero<0x142, 0xA>(v));
+    with(dpp_or_zero<0x143, 0xC>(v));
+    return __builtin_amdgcn_readlane(v, 63);
+}
+
 /* Finds the `item`th tile of RM rows: the sequences' tiles are counted 64 sequences at a time.
  * Sequences whose rows do not lie in the call's tensors have none. */
 template <int RM>
@@ -728,7 +740,7 @@ struct Chunk {
     /* LDS: [2]{K, V}, then scales [2][2][BN], pages [3][BN], flags */
     static constexpr int kTile = BN * D * 2;
     static constexpr int kScales = 4 * kTile, kPages = kScales + (kCoded ? 4 * BN * 4 : 0);
-    static constexpr int kFlags = kPages + 3 * BN * 4, kBytes = kFlags + 16;
+    static constexpr int kFlags = kPages + 3 * BN * 4, kBytes = kFlags + 32; /* bad[3], exponents[2] */
 };
 
 /* 16 bytes a lane from memory to LDS, lane after lane from `to` (the same on every lane). */
@@ -750,6 +762,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_chunk_kernel(AttnA
     float *scales = reinterpret_cast<float *>(smem + C::kScales); /* [buffer][k, v][BN] */
     int *pages = reinterpret_cast<int *>(smem + C::kPages);       /* [step % 3][BN] */
     int *bad = reinterpret_cast<int *>(smem + C::kFlags);         /* [step % 3]: a token without a page */
+    int *exponents = bad + 3;                                      /* [step % 2]: V's scales are over 2 to this, biased */
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 31, half = lane >> 5;
     const int head = blockIdx.x % a.kv.heads, split = blockIdx.y;
     /* the last tiles of a sequence see the most keys: those first */
@@ -778,6 +791,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_chunk_kernel(AttnA
      * a time; a lane fetches the piece that belongs where it writes. */
     u4 kr[C::kLoads], vr[C::kLoads];
     float scale_r = 0.0f;
+    int v_run = 1;
     bool there_r[C::kLoads];
     constexpr int kLanes = D * (kCoded ? 1 : 2) / 16; /* a token's 16-byte loads */
     auto slot_of = [&](int step, int at, int page) -> long long {
@@ -828,6 +842,16 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_chunk_kernel(AttnA
                 const u4 v1 = {widen_f16<FMT, 0>(vx.z), widen_f16<FMT, 1>(vx.z), widen_f16<FMT, 0>(vx.w), widen_f16<FMT, 1>(vx.w)};
                 *reinterpret_cast<u4 *>(v + at * 2 * D + ((2 * part) ^ vs) * 16) = v0;
                 *reinterpret_cast<u4 *>(v + at * 2 * D + ((2 * part + 1) ^ vs) * 16) = v1;
+            }
+            /* V's scales over a power of two that holds the largest so far in [1, 2), as in
+             * attn_rows_kernel; the wave that has them keeps it for the block. Infinities and NaN are
+             * no measure of the others. */
+            if (wave == BN / 64) {
+                const int e = (int)(__builtin_bit_cast(uint32_t, scale_r) >> 23);
+                const int most = wave_most(tid >= BN && e <= 253 ? e : 0);
+                v_run = most > v_run ? most : v_run;
+                if (tid >= BN) scale_r *= power_of_two(254 - v_run);
+                if (lane == 0) exponents[step & 1] = v_run;
             }
             if (tid < 2 * BN) scales[(step & 1) * 2 * BN + tid] = scale_r;
         } else {
@@ -937,26 +961,14 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_chunk_kernel(AttnA
             for (int d = 0; d < DB; ++d) acc[d] *= grow;
         }
         const float base = m == -__builtin_inff() ? 0.0f : m;
-        float v_by = 1.0f;
         if constexpr (kCoded) {
-            /* V's largest scale of the step, as in attn_rows_kernel */
-            float top = lane < BN ? sc[BN + lane] : 0.0f;
-            int exp = (int)(__builtin_bit_cast(uint32_t, top) >> 23);
-            exp = exp > 253 ? 1 : exp;
-#pragma unroll
-            for (int x = 1; x < 64; x *= 2) {
-                const int o = __shfl_xor(exp, x);
-                exp = exp > o ? exp : o;
-            }
-            exp = __builtin_amdgcn_readfirstlane(exp);
-            if (exp > v_exp) {
-                const int fall = exp - v_exp > 126 ? 126 : exp - v_exp;
-                const float by = power_of_two(127 - fall);
+            const int now = __builtin_amdgcn_readfirstlane(exponents[step & 1]);
+            if (now != v_exp) {
+                const float by = power_of_two(now - v_exp > 126 ? 1 : 127 - (now - v_exp));
 #pragma unroll
                 for (int d = 0; d < DB; ++d) acc[d] *= by;
-                v_exp = exp;
+                v_exp = now;
             }
-            v_by = power_of_two(254 - v_exp);
         }
         uint32_t p[kHalves][8];
 #pragma unroll
@@ -972,7 +984,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_chunk_kernel(AttnA
                     w[i] = __builtin_amdgcn_exp2f(kCoded ? score - base : fmaf(score, a.scale, -base));
                     l += w[i];
                     if constexpr (kCoded) {
-                        w[i] *= x[i] * v_by;
+                        w[i] *= x[i];
                         if (cut && score == -__builtin_inff()) w[i] = 0.0f;
                     }
                 }

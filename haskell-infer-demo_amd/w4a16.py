@@ -15,6 +15,7 @@ and streams. There is no CPU fallback: if the library is missing the import fail
 """
 
 import ctypes
+import functools
 import os
 
 import numpy as np
@@ -841,6 +842,13 @@ def _floats3(t, what, device):
     return t.data_ptr(), t.stride(0), t.stride(1)
 
 
+@functools.lru_cache(maxsize=64)
+def _drafts_workspace(seqs, steps, vocab):
+    size = ctypes.c_size_t(0)
+    _check(lib.w4a16_verify_drafts_workspace(seqs, steps, vocab, ctypes.byref(size)), "verify_drafts")
+    return size.value
+
+
 def _exactly(t, shape, dtype, device, what):
     """Address of a contiguous tensor of this shape and type."""
     if not hasattr(t, "is_cuda") or t.shape != shape or t.dtype != dtype or t.device != device or not t.is_contiguous():
@@ -873,9 +881,7 @@ def verify_drafts(target, draft_tokens, uniforms, draft=None, lens=None, workspa
     lp = None if lens is None else _exactly(lens, (seqs,), torch.int32, device, "verify_drafts lens")
     accepted = torch.empty(seqs, dtype=torch.int32, device=device)
     tokens = torch.empty((seqs, rows), dtype=torch.int32, device=device)
-    size = ctypes.c_size_t(0)
-    _check(lib.w4a16_verify_drafts_workspace(seqs, steps, vocab, ctypes.byref(size)), "verify_drafts")
-    need = size.value
+    need = _drafts_workspace(seqs, steps, vocab)
     if workspace is None:
         workspace = torch.empty(need, dtype=torch.uint8, device=device)
         wp = workspace.data_ptr()
