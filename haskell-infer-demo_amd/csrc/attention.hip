@@ -261,7 +261,7 @@ __device__ __forceinline__ bf8 as_bf8(uint32_t a, uint32_t b, uint32_t c, uint32
 }
 
 __device__ __forceinline__ bool nonfinite2(uint32_t pair) {
-    return (pair & 0x7F80u) == 0x7F80u || (pair & 0x7F800000u) == 0x7F800000u;
+    return ((pair & 0x7F80u) == 0x7F80u) | ((pair & 0x7F800000u) == 0x7F800000u);
 }
 
 /* A partial result in the workspace: RM rows of D values, then RM pairs (m, l). */
@@ -348,27 +348,31 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
 
     const int32_t *table = a.kv.table + (long long)t.seq * a.kv.table_stride;
     /* Pages of this lane's K tokens and V tokens (page sizes are multiples of 8, so four
-     * neighbours from a multiple of 4 share one). Tokens that are not there read token 0 of page 0
-     * and are masked. */
+     * neighbours from a multiple of 4 share one). Tokens that are not there read page 0 and are
+     * masked. */
     int kpage[2], vpage[2];
     auto load_pages = [&](int t0) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             const int kt = t0 + 16 * c + n, vt = t0 + 16 * c + 4 * g;
-            kpage[c] = kt < t.length ? table[kt >> a.kv.shift] : -1;
-            vpage[c] = vt < t.length ? table[vt >> a.kv.shift] : -1;
+            kpage[c] = table[(kt < t.length ? kt : 0) >> a.kv.shift];
+            vpage[c] = table[(vt < t.length ? vt : 0) >> a.kv.shift];
+            kpage[c] = kt < t.length ? kpage[c] : -1;
+            vpage[c] = vt < t.length ? vpage[c] : -1;
         }
     };
-    auto slot_of = [&](int page, int token) -> long long {
-        return (unsigned)page < (unsigned)a.kv.pages ? (((long long)page * a.kv.heads + head) << a.kv.shift) + (token & mask) : 0;
+    auto offset_of = [&](int page, int token, uint32_t row) -> unsigned long long { /* rows of that many bytes */
+        const uint32_t safe = (unsigned)page < (unsigned)a.kv.pages ? page : 0;
+        return (unsigned long long)safe * (a.kv.page_tokens * row) + (uint32_t)((head << a.kv.shift) + (token & mask)) * row;
     };
+    constexpr uint32_t kRow = D * (kCoded ? 1 : 2);
     u4 kraw[2][kKLoads];
     uint32_t v[8][kVWords];
     f4 ks[2], vs[2];
     auto load_k = [&](int t0) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-            const uint8_t *p = static_cast<const uint8_t *>(a.kv.k) + slot_of(kpage[c], t0 + 16 * c + n) * (kCoded ? D : 2 * D) + 16 * g;
+            const uint8_t *p = static_cast<const uint8_t *>(a.kv.k) + offset_of(kpage[c], t0 + 16 * c + n, kRow) + 16 * g;
 #pragma unroll
             for (int s = 0; s < kKLoads; ++s) kraw[c][s] = *reinterpret_cast<const u4 *>(p + 64 * s);
         }
@@ -376,10 +380,10 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
     auto load_v = [&](int t0) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-            const long long slot = slot_of(vpage[c], t0 + 16 * c + 4 * g);
+            const uint8_t *first = static_cast<const uint8_t *>(a.kv.v) + offset_of(vpage[c], t0 + 16 * c + 4 * g, kRow) + n * (4 * kVWords);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const uint8_t *p = static_cast<const uint8_t *>(a.kv.v) + (slot + i) * (kCoded ? D : 2 * D) + n * (4 * kVWords);
+                const uint8_t *p = first + i * kRow;
                 if constexpr (kVWords == 1) {
                     v[4 * c + i][0] = *reinterpret_cast<const uint32_t *>(p);
                 } else if constexpr (kVWords == 2) {
@@ -403,9 +407,9 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
         if constexpr (kCoded) {
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                const long long slot = slot_of(vpage[c], t0 + 16 * c + 4 * g);
-                k_of[c] = *reinterpret_cast<const f4 *>(a.kv.k_scale + slot);
-                v_of[c] = *reinterpret_cast<const f4 *>(a.kv.v_scale + slot);
+                const unsigned long long from = offset_of(vpage[c], t0 + 16 * c + 4 * g, 1);
+                k_of[c] = *reinterpret_cast<const f4 *>(a.kv.k_scale + from);
+                v_of[c] = *reinterpret_cast<const f4 *>(a.kv.v_scale + from);
             }
         }
     };
@@ -425,14 +429,14 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
         const int i = r * 16 + n, token = (t.start + i) / a.group, h = head * a.group + (t.start + i) % a.group;
         const bool real = i < t.rows;
         const int place = t.length - t.news + token;
+        const uint16_t *row = a.q + (t.first_row + (real ? token : 0)) * a.q_row + h * a.q_head;
         hi[r] = !real ? 0 : a.causal ? place + 1 : t.length;
         lo[r] = t.window ? place - t.window + 1 : 0;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             const int d = kCoded ? 64 * (s / 2) + 16 * g + 8 * (s % 2) : 32 * s + 8 * g;
-            uint4 x = make_uint4(0u, 0u, 0u, 0u);
-            if (real) x = *reinterpret_cast<const uint4 *>(a.q + (t.first_row + token) * a.q_row + h * a.q_head + d);
-            q[r][s] = as_bf8(x.x ^ a.flip, x.y ^ a.flip, x.z ^ a.flip, x.w ^ a.flip);
+            const u4 x = *reinterpret_cast<const u4 *>(row + d);
+            q[r][s] = as_bf8(real ? x.x ^ a.flip : 0u, real ? x.y ^ a.flip : 0u, real ? x.z ^ a.flip : 0u, real ? x.w ^ a.flip : 0u);
         }
     }
 
@@ -488,7 +492,7 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
 #pragma unroll
                 for (int w = 0; w < kVWords; ++w) asm volatile("" : "+v"(v[i][w]));
         /* tokens that some row does not see, or that are not there: their V is not multiplied */
-        const bool cut = t0 < t.all_lo || t0 + 32 > t.all_hi || __any(!there[0] || !there[1]);
+        const bool cut = (t0 < t.all_lo) | (t0 + 32 > t.all_hi) | (__any(!there[0] | !there[1]) != 0);
         bool odd = false;
         if (cut) {
 #pragma unroll
@@ -496,14 +500,13 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int at = t0 + 16 * c + 4 * g + i;
-                    if (!there[c] || at < t.lo || at >= t.hi) {
+                    const bool none = !there[c] | (at < t.lo) | (at >= t.hi);
 #pragma unroll
-                        for (int w = 0; w < kVWords; ++w) v[4 * c + i][w] = 0u;
-                        if constexpr (kCoded) vs[c][i] = 0.0f;
-                    }
+                    for (int w = 0; w < kVWords; ++w) v[4 * c + i][w] = none ? 0u : v[4 * c + i][w];
+                    if constexpr (kCoded) vs[c][i] = none ? 0.0f : vs[c][i];
                     if constexpr (!kCoded)
 #pragma unroll
-                        for (int w = 0; w < kVWords; ++w) odd = odd || nonfinite2(v[4 * c + i][w]);
+                        for (int w = 0; w < kVWords; ++w) odd = odd | nonfinite2(v[4 * c + i][w]);
                 }
             odd = __any(odd);
         }
@@ -527,7 +530,10 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
                 v_exp = exp;
             }
 #pragma unroll
-            for (int c = 0; c < 2; ++c) vs[c] *= power_of_two(254 - v_exp);
+            for (int c = 0; c < 2; ++c) {
+                vs[c] *= power_of_two(254 - v_exp);
+                ks[c] *= a.scale;
+            }
         }
         uint32_t p[RT][4];
 #pragma unroll
@@ -535,12 +541,13 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 if constexpr (kCoded) s[r][c] *= ks[c];
-                s[r][c] *= a.scale;
+                else s[r][c] *= a.scale;
                 if (cut)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int at = t0 + 16 * c + 4 * g + i;
-                        if (!there[c] || at < lo[r] || at >= hi[r]) s[r][c][i] = -__builtin_inff();
+                        const bool hidden = !there[c] | (at < lo[r]) | (at >= hi[r]);
+                        s[r][c][i] = hidden ? -__builtin_inff() : s[r][c][i];
                     }
             }
             float most = fmaxf(fmaxf(fmaxf(s[r][0][0], s[r][0][1]), fmaxf(s[r][0][2], s[r][0][3])),
@@ -564,7 +571,7 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
                     l[r] += w[i];
                     if constexpr (kCoded) {
                         w[i] *= vs[c][i];
-                        if (cut && s[r][c][i] == -__builtin_inff()) w[i] = 0.0f;
+                        w[i] = (cut & (s[r][c][i] == -__builtin_inff())) ? 0.0f : w[i];
                     }
                 }
                 p[r][2 * c] = kCoded ? pack_f16(w[0], w[1]) : kv_pack_bf16(w[0], w[1]);
@@ -752,11 +759,28 @@ __device__ __forceinline__ void load_to_lds(const uint8_t *from, uint8_t *to) {
 /* Before the barrier behind which other waves read what load_to_lds wrote. */
 __device__ __forceinline__ void wait_for_lds_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
+/* Asks the scheduler for the LDS reads (READS for each of COUNT products) FAR products before their
+ * use. 4096 rows over 16384 tokens, without and with FAR = 2: BF16 D = 256 1774 and 1661 us, D = 128 1024
+ * and 997, D = 64 720 and 697; FP8 D = 256 2265 and 2469 (not taken there), D = 128 1241 and 1221. */
+template <int COUNT, int READS, int FAR>
+__device__ __forceinline__ void interleave() {
+    if constexpr (FAR > 0) {
+        __builtin_amdgcn_sched_group_barrier(0x100, READS * FAR, 0);
+#pragma unroll
+        for (int i = 0; i < COUNT - FAR; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x8, FAR, 0);
+    }
+}
+
 template <int D, int FMT>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_chunk_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attn_chunk_kernel(AttnArgs a) {
     using C = Chunk<D, FMT>;
     constexpr bool kCoded = C::kCoded;
     constexpr int BN = C::BN, RM = C::kRows, kHalves = BN / 32, KS = D / 16, DB = D / 32;
+    constexpr int kFar = kCoded && D == 256 ? 0 : 2;
     extern __shared__ uint4 smem4[];
     uint8_t *smem = reinterpret_cast<uint8_t *>(smem4);
     float *scales = reinterpret_cast<float *>(smem + C::kScales); /* [buffer][k, v][BN] */
@@ -794,8 +818,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_chunk_kernel(AttnA
     int v_run = 1;
     bool there_r[C::kLoads];
     constexpr int kLanes = D * (kCoded ? 1 : 2) / 16; /* a token's 16-byte loads */
-    auto slot_of = [&](int step, int at, int page) -> long long {
-        return page >= 0 ? (((long long)page * a.kv.heads + head) << a.kv.shift) + ((t.begin + step * BN + at) & mask) : 0;
+    /* the place in its page and head of token `at` of a step; rows of it that many bytes apart */
+    auto inside = [&](int step, int at) { return (uint32_t)((head << a.kv.shift) + ((t.begin + step * BN + at) & mask)); };
+    constexpr uint32_t kRow = D * (kCoded ? 1 : 2);
+    auto offset_of = [&](int step, int at, int page, uint32_t row) -> unsigned long long {
+        return (unsigned long long)(uint32_t)(page >= 0 ? page : 0) * (a.kv.page_tokens * row) + inside(step, at) * row;
     };
     auto load_tile = [&](int step) {
         const uint8_t *k = static_cast<const uint8_t *>(a.kv.k), *v = static_cast<const uint8_t *>(a.kv.v);
@@ -805,14 +832,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_chunk_kernel(AttnA
                 const int at = (x * 256 + tid) / kLanes, part = (x * 256 + tid) % kLanes;
                 const int page = pages[(step % 3) * BN + at];
                 there_r[x] = page >= 0;
-                const long long slot = slot_of(step, at, page);
-                kr[x] = *reinterpret_cast<const u4 *>(k + slot * D + part * 16);
-                vr[x] = *reinterpret_cast<const u4 *>(v + slot * D + part * 16);
+                const unsigned long long from = offset_of(step, at, page, kRow) + part * 16;
+                kr[x] = *reinterpret_cast<const u4 *>(k + from);
+                vr[x] = *reinterpret_cast<const u4 *>(v + from);
             }
             if (tid < 2 * BN) {
                 const int at = tid % BN, page = pages[(step % 3) * BN + at];
-                const long long slot = slot_of(step, at, page);
-                scale_r = page < 0 ? 0.0f : tid < BN ? a.kv.k_scale[slot] * a.scale : a.kv.v_scale[slot];
+                const unsigned long long from = offset_of(step, at, page, 1);
+                const float scale = (tid < BN ? a.kv.k_scale : a.kv.v_scale)[from];
+                scale_r = page < 0 ? 0.0f : tid < BN ? scale * a.scale : scale;
             }
         } else {
             const int wave_u = __builtin_amdgcn_readfirstlane(wave);
@@ -820,9 +848,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_chunk_kernel(AttnA
 #pragma unroll
             for (int x = 0; x < C::kLoads; ++x) {
                 const int at = (x * 256 + tid) / kLanes, part = (x * 256 + tid) % kLanes;
-                const long long slot = slot_of(step, at, pages[(step % 3) * BN + at]);
-                load_to_lds(k + slot * (2 * D) + (part ^ (at & C::kSwizzle)) * 16, to + x * 4096);
-                load_to_lds(v + slot * (2 * D) + (part ^ ((2 * at) & C::kSwizzle)) * 16, to + C::kTile + x * 4096);
+                const unsigned long long from = offset_of(step, at, pages[(step % 3) * BN + at], kRow);
+                load_to_lds(k + from + (part ^ (at & C::kSwizzle)) * 16, to + x * 4096);
+                load_to_lds(v + from + (part ^ ((2 * at) & C::kSwizzle)) * 16, to + C::kTile + x * 4096);
             }
         }
     };
@@ -876,16 +904,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_chunk_kernel(AttnA
     bf8 q[KS];
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-        uint4 x = make_uint4(0u, 0u, 0u, 0u);
-        if (real) x = *reinterpret_cast<const uint4 *>(a.q + (t.first_row + token) * a.q_row + h * a.q_head + 16 * s + 8 * half);
-        q[s] = as_bf8(x.x ^ a.flip, x.y ^ a.flip, x.z ^ a.flip, x.w ^ a.flip);
+        const u4 x = *reinterpret_cast<const u4 *>(a.q + (t.first_row + (real ? token : 0)) * a.q_row + h * a.q_head + 16 * s + 8 * half);
+        q[s] = as_bf8(real ? x.x ^ a.flip : 0u, real ? x.y ^ a.flip : 0u, real ? x.z ^ a.flip : 0u, real ? x.w ^ a.flip : 0u);
     }
     f16v acc[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[d][i] = 0.0f;
-    float m = -__builtin_inff(), l = 0.0f;
+    float m = real ? -__builtin_inff() : 0.0f, l = 0.0f;
     int v_exp = 1;
     if (steps > 0) {
         store_tile(0);
@@ -912,23 +939,24 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_chunk_kernel(AttnA
         for (int c = 0; c < kHalves; ++c) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[c][i] = 0.0f;
-            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int j = 0; j < KS; ++j) {
                 const bf8 k = *reinterpret_cast<const bf8 *>(kt + (k_at ^ (32 * j)) + 32 * c * 2 * D);
                 s[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, q[j], s[c], 0, 0, 0);
             }
         }
-        if constexpr (kCoded) {
+        interleave<kHalves * KS, 1, kFar>();
+        /* scores over the maximum that the sums stand at: the exponents of the weights */
+        float base = m == -__builtin_inff() ? 0.0f : m;
 #pragma unroll
-            for (int c = 0; c < kHalves; ++c)
+        for (int c = 0; c < kHalves; ++c)
 #pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    const f4 x = *reinterpret_cast<const f4 *>(sc + 32 * c + 8 * b + 4 * half);
+            for (int b = 0; b < 4; ++b) {
+                f4 x = {a.scale, a.scale, a.scale, a.scale};
+                if constexpr (kCoded) x = *reinterpret_cast<const f4 *>(sc + 32 * c + 8 * b + 4 * half);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) s[c][4 * b + i] *= x[i];
-                }
-        }
+                for (int i = 0; i < 4; ++i) s[c][4 * b + i] = fmaf(s[c][4 * b + i], x[i], -base);
+            }
         const bool cut = (t0 < t.all_lo) | (t0 + BN > t.all_hi) | (__builtin_amdgcn_readfirstlane(bad[step % 3]) != 0);
         if (cut) {
 #pragma unroll
@@ -950,17 +978,21 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_chunk_kernel(AttnA
         for (int c = 0; c < kHalves; ++c)
 #pragma unroll
             for (int i = 0; i < 16; ++i) most = fmaxf(most, s[c][i]);
-        most = lane_max32(most);
-        if constexpr (!kCoded) most *= a.scale;
-        if (__any(most > m + 8.0f)) {
-            const float upto = fmaxf(m, most);
-            const float grow = __builtin_amdgcn_exp2f(m - (upto == -__builtin_inff() ? 0.0f : upto));
-            m = upto;
+        if (__any((most > 8.0f) | (m == -__builtin_inff()))) {
+            /* a new maximum: for rows that have none yet, or whose weights would pass 2^8 */
+            most = lane_max32(most);
+            const bool none = m == -__builtin_inff();
+            const float rise = most > (none ? -__builtin_inff() : 8.0f) ? most : 0.0f;
+            const float grow = none ? 0.0f : __builtin_amdgcn_exp2f(-rise);
+            m = none && rise == 0.0f && most != 0.0f ? m : base + rise;
             l *= grow;
 #pragma unroll
             for (int d = 0; d < DB; ++d) acc[d] *= grow;
+#pragma unroll
+            for (int c = 0; c < kHalves; ++c)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[c][i] -= rise;
         }
-        const float base = m == -__builtin_inff() ? 0.0f : m;
         if constexpr (kCoded) {
             const int now = __builtin_amdgcn_readfirstlane(exponents[step & 1]);
             if (now != v_exp) {
@@ -980,12 +1012,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_chunk_kernel(AttnA
                 if constexpr (kCoded) x = *reinterpret_cast<const f4 *>(sc + BN + 32 * c + 8 * b + 4 * half);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float score = s[c][4 * b + i];
-                    w[i] = __builtin_amdgcn_exp2f(kCoded ? score - base : fmaf(score, a.scale, -base));
+                    const float over = s[c][4 * b + i];
+                    w[i] = __builtin_amdgcn_exp2f(over);
                     l += w[i];
                     if constexpr (kCoded) {
                         w[i] *= x[i];
-                        if (cut && score == -__builtin_inff()) w[i] = 0.0f;
+                        w[i] = (cut & (over == -__builtin_inff())) ? 0.0f : w[i];
                     }
                 }
                 p[c][2 * b] = kCoded ? pack_f16(w[0], w[1]) : kv_pack_bf16(w[0], w[1]);
@@ -1001,7 +1033,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_chunk_kernel(AttnA
                 bool odd = false;
                 for (int x = tid; x < C::kTile / 4; x += 256) {
                     if (pages[(step % 3) * BN + x / (D / 2)] < 0) tile[x] = 0u;
-                    else odd = odd || nonfinite2(tile[x]);
+                    else odd = odd | nonfinite2(tile[x]);
                 }
                 if (__syncthreads_or(odd)) {
                     for (int in = 0; in < BN; ++in) {
@@ -1012,10 +1044,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_chunk_kernel(AttnA
                             for (int b = 0; b < 4; ++b) {
                                 __builtin_amdgcn_sched_barrier(0); /* one piece at a time: registers */
                                 const uint2 x = *reinterpret_cast<const uint2 *>(vt + in * 2 * D + ((4 * d + b) ^ ((2 * in) & C::kSwizzle)) * 16 + 8 * half);
+                                if (!__any((int)nonfinite2(x.x) | (int)nonfinite2(x.y))) continue;
                                 const uint32_t f[4] = {x.x << 16, x.x & 0xFFFF0000u, x.y << 16, x.y & 0xFFFF0000u};
 #pragma unroll
-                                for (int i = 0; i < 4; ++i)
-                                    if (sees && (f[i] & 0x7F800000u) == 0x7F800000u) acc[d][4 * b + i] += __builtin_bit_cast(float, f[i]);
+                                for (int i = 0; i < 4; ++i) {
+                                    const bool adds = sees & ((f[i] & 0x7F800000u) == 0x7F800000u);
+                                    acc[d][4 * b + i] += adds ? __builtin_bit_cast(float, f[i]) : 0.0f;
+                                }
                             }
                     }
                     __syncthreads();
@@ -1031,7 +1066,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_chunk_kernel(AttnA
 #pragma unroll
         for (int u = 0; u < BN / 16; ++u) {
             const uint32_t *w = &p[u / 2][4 * (u % 2)];
-            if (u % 2 == 0) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int d = 0; d < DB; ++d) {
                 uint32_t v[4];
@@ -1050,6 +1084,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_chunk_kernel(AttnA
                 }
             }
         }
+        interleave<BN / 16 * DB, 2, kFar>();
         if (more) store_tile(step + 1);
         if (look) put_page(step + 2, page);
         __syncthreads();

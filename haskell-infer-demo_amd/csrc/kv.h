@@ -14,6 +14,7 @@ struct KvView {
     float *k_scale, *v_scale;
     const int32_t *table, *kv_lens, *starts;
     int heads, pages, shift; /* page_size = 1 << shift */
+    uint32_t page_tokens;    /* heads << shift: rows of a page, under 2^31 bytes of them */
     int seqs, rows, table_pages, table_stride;
 };
 

@@ -196,6 +196,9 @@ int kv_check(const W4A16KvCache *c, const W4A16KvBatch *b, const char *what, KvV
         (long long)c->num_pages * c->page_size > INT32_MAX)
         return set_error(W4A16_ERR_CONFIG, "%s: bad extents num_pages=%d page_size=%d kv_heads=%d", what,
                          c->num_pages, c->page_size, c->kv_heads);
+    if ((long long)c->kv_heads * c->page_size * c->head_dim * 2 > INT32_MAX)
+        return set_error(W4A16_ERR_CONFIG, "%s: a page of kv_heads=%d page_size=%d passes 2 GiB", what, c->kv_heads,
+                         c->page_size);
     if (!c->k || !c->v) return set_error(W4A16_ERR_CONFIG, "%s: null cache buffer", what);
     const bool coded = c->format != W4A16_KV_BF16;
     if (coded && (!c->k_scale || !c->v_scale))
@@ -216,7 +219,7 @@ int kv_check(const W4A16KvCache *c, const W4A16KvBatch *b, const char *what, KvV
     int shift = 0;
     while ((1 << shift) < c->page_size) ++shift;
     *view = {c->k, c->v, coded ? c->k_scale : nullptr, coded ? c->v_scale : nullptr, table, b->kv_lens, b->starts,
-             c->kv_heads, c->num_pages, shift, b->seqs, b->rows, b->table_pages, b->table_stride};
+             c->kv_heads, c->num_pages, shift, (uint32_t)(c->kv_heads * c->page_size), b->seqs, b->rows, b->table_pages, b->table_stride};
     /* positions are 32-bit in the kernels, and so are the tiles' ends behind them */
     if (view->table_pages > (1 << 30) >> shift) view->table_pages = (1 << 30) >> shift;
     return W4A16_OK;

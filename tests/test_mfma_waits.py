@@ -26,8 +26,8 @@ def registers(operand):
 
 
 def slots_needed(op):
-    """Passes of the instruction and three more, before another kind of instruction may touch its result."""
-    return 11 if "32x32x16" in op else 7 if "16x16x32" in op else 19
+    """Passes of the instruction (8, 4, 16) and four more, before another kind of instruction may touch its result."""
+    return 12 if "32x32x16" in op else 8 if "16x16x32" in op else 20
 
 
 def early_uses(asm):
@@ -106,7 +106,7 @@ def test_the_check_follows_branches():
 _Zok:
     v_mfma_f32_16x16x32_bf16 v[0:3], v[8:11], v[4:7], v[0:3]
     v_mfma_f32_16x16x32_bf16 v[0:3], v[12:15], v[4:7], v[0:3]
-    s_nop 6
+    s_nop 7
     v_mul_f32_e32 v0, v1, v2
     s_endpgm
 .Lfunc_end1:

@@ -58,6 +58,9 @@ CASES = [
     ([150] * 66, [1] * 66, 2, 1, 64, 32, 0),          # more sequences than a wave has lanes
     ([640, 1, 300], [257, 1, 129], 7, 1, 128, 64, 0),
     ([640, 300], [200, 129], 4, 2, 256, 64, 150),
+    ([70, 500], [3, 4], 4, 1, 256, 32, 37),           # windows that begin at every place of four tokens
+    ([333, 90], [9, 2], 3, 1, 64, 8, 10),
+    ([333, 90], [60, 2], 5, 1, 128, 8, 10),
 ]
 
 
@@ -109,11 +112,12 @@ def test_rows_that_see_nothing(cuda, fmt, many):
 
 
 @pytest.mark.parametrize("fmt", ["bf16", "int8", "fp8"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
 @pytest.mark.parametrize("news,window", [([6], 0), ([6], 20), ([100], 0), ([100], 20)])
-def test_nonfinite_values_stay_with_the_rows_that_see_them(cuda, fmt, news, window):
+def test_nonfinite_values_stay_with_the_rows_that_see_them(cuda, fmt, news, window, dim):
     """Keys and values with infinities and NaN behind the last token, outside the window and at later positions change
     nothing; a row that sees one is not a number where the value is not."""
-    page, pages, heads, dim, n = 32, 8, 2, 128, 170
+    page, pages, heads, n = 32, 8, 2, 170
     batch, table = make_batch([n], news, page, pages, cuda)
     clean = filled(pages, page, heads, dim, fmt, cuda, seed=8)
     q = torch.randn(news[0], 4, dim, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16).to(cuda)
@@ -141,16 +145,16 @@ def test_nonfinite_values_stay_with_the_rows_that_see_them(cuda, fmt, news, wind
 
 def test_an_infinite_value_reaches_its_rows_alone(cuda):
     """One value column of one BF16 token at infinity: the rows that see the token get it there and nowhere else."""
-    for news in (4, 70):
+    for news, dim in ((4, 64), (70, 64), (4, 256), (70, 256), (70, 128)):
         batch, table = make_batch([100], [news], 16, 8, cuda)
-        cache = filled(8, 16, 1, 64, "bf16", cuda, seed=2)
-        q = torch.randn(news, 2, 64, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16).to(cuda)
+        cache = filled(8, 16, 1, dim, "bf16", cuda, seed=2)
+        q = torch.randn(news, 2, dim, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16).to(cuda)
         want = w4a16.paged_attention(q, cache, batch)
         cache.v[table[0][98 // 16], 0, 98 % 16, 5] = float("inf")
         out = w4a16.paged_attention(q, cache, batch)
         assert torch.equal(out[:-2], want[:-2])
         assert (out[-2:, :, 5] == float("inf")).all()
-        rest = [d for d in range(64) if d != 5]
+        rest = [d for d in range(dim) if d != 5]
         assert torch.equal(out[-2:, :, rest], want[-2:, :, rest])
 
 
