@@ -799,22 +799,24 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attn_chu
     const int mask = (1 << a.kv.shift) - 1;
     const int steps = t.end > t.begin ? (t.end - t.begin + BN - 1) / BN : 0;
 
-    /* the page of token tid of a step, -1 where there is none */
-    auto page_of = [&](int step) {
-        const int at = t.begin + step * BN + tid;
-        int page = -1;
-        if (at >= t.lo && at < t.hi) page = table[at >> a.kv.shift];
-        return (unsigned)page < (unsigned)a.kv.pages ? page : -1;
+    /* Token tid % BN of a step: its entry of the page table, unread until put_page, so that nothing waits
+     * for it (and, loads arriving in order, for the tile's before it) at the start of a step. */
+    auto entry_of = [&](int step) {
+        const int at = t.begin + step * BN + tid % BN;
+        return table[(at >= t.lo && at < t.hi ? at : t.lo) >> a.kv.shift];
     };
-    auto put_page = [&](int step, int page) {
-        if (tid < BN) pages[(step % 3) * BN + tid] = page;
-        const bool none = __any(tid < BN && page < 0);
+    auto put_page = [&](int step, int entry) { /* by the first wave: -1 where there is no token */
+        const int at = t.begin + step * BN + tid % BN;
+        const bool ok = (at >= t.lo) & (at < t.hi) & ((unsigned)entry < (unsigned)a.kv.pages);
+        if (tid < BN) pages[(step % 3) * BN + tid] = ok ? entry : -1;
+        const bool none = __any(!ok);
         if (lane == 0) bad[step % 3] = none;
     };
     /* 8-bit: through registers, widened on the way into LDS. BF16: straight into LDS, a wave's 1 KiB at
      * a time; a lane fetches the piece that belongs where it writes. */
     u4 kr[C::kLoads], vr[C::kLoads];
     float scale_r = 0.0f;
+    bool scale_there = false;
     int v_run = 1;
     bool there_r[C::kLoads];
     constexpr int kLanes = D * (kCoded ? 1 : 2) / 16; /* a token's 16-byte loads */
@@ -836,12 +838,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attn_chu
                 kr[x] = *reinterpret_cast<const u4 *>(k + from);
                 vr[x] = *reinterpret_cast<const u4 *>(v + from);
             }
-            if (tid < 2 * BN) {
-                const int at = tid % BN, page = pages[(step % 3) * BN + at];
-                const unsigned long long from = offset_of(step, at, page, 1);
-                const float scale = (tid < BN ? a.kv.k_scale : a.kv.v_scale)[from];
-                scale_r = page < 0 ? 0.0f : tid < BN ? scale * a.scale : scale;
-            }
+            /* K's scales by threads 0 .. BN - 1 of each 2 BN, V's by the others; unread here, as entries are */
+            const int at = tid % BN, page = pages[(step % 3) * BN + at];
+            scale_there = page >= 0;
+            scale_r = (tid % (2 * BN) < BN ? a.kv.k_scale : a.kv.v_scale)[offset_of(step, at, page, 1)];
         } else {
             const int wave_u = __builtin_amdgcn_readfirstlane(wave);
             uint8_t *to = smem + (step & 1) * 2 * C::kTile + wave_u * 1024;
@@ -860,6 +860,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attn_chu
 #pragma unroll
             for (int x = 0; x < C::kLoads; ++x) {
                 const int at = (x * 256 + tid) / kLanes, part = (x * 256 + tid) % kLanes;
+                asm volatile("" : "+v"(kr[x]), "+v"(vr[x])); /* or the bytes are carried apart from the load on */
                 const u4 vx = there_r[x] ? vr[x] : u4{0u, 0u, 0u, 0u};
                 const int ks = at & C::kSwizzle, vs = (2 * at) & C::kSwizzle;
                 const u4 k0 = {kv_widen<FMT, 0>(kr[x].x), kv_widen<FMT, 1>(kr[x].x), kv_widen<FMT, 0>(kr[x].y), kv_widen<FMT, 1>(kr[x].y)};
@@ -874,6 +875,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attn_chu
             /* V's scales over a power of two that holds the largest so far in [1, 2), as in
              * attn_rows_kernel; the wave that has them keeps it for the block. Infinities and NaN are
              * no measure of the others. */
+            scale_r = !scale_there ? 0.0f : tid % (2 * BN) < BN ? scale_r * a.scale : scale_r;
             if (wave == BN / 64) {
                 const int e = (int)(__builtin_bit_cast(uint32_t, scale_r) >> 23);
                 const int most = wave_most(tid >= BN && e <= 253 ? e : 0);
@@ -889,8 +891,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attn_chu
 
     if (steps > 0) {
         if (tid < 64) {
-            put_page(0, tid < BN ? page_of(0) : 0);
-            if (steps > 1) put_page(1, tid < BN ? page_of(1) : 0);
+            const int first = entry_of(0), second = entry_of(steps > 1 ? 1 : 0);
+            put_page(0, first);
+            if (steps > 1) put_page(1, second);
         }
         __syncthreads();
         load_tile(0);
@@ -927,10 +930,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attn_chu
     const int v_at = v_row * 2 * D + ((v_piece ^ ((2 * v_row) & C::kSwizzle)) * 16) + 8 * (lane & 1);
     for (int step = 0; step < steps; ++step) {
         const bool more = step + 1 < steps;
-        int page = 0;
+        const bool look = step + 2 < steps;
         if (more) load_tile(step + 1);
-        const bool look = tid < 64 && step + 2 < steps;
-        if (look && tid < BN) page = page_of(step + 2);
+        const int entry = entry_of(look ? step + 2 : step);
         const int t0 = t.begin + step * BN;
         const uint8_t *kt = smem + (step & 1) * 2 * C::kTile, *vt = kt + C::kTile;
         const float *sc = scales + (step & 1) * 2 * BN;
@@ -1086,7 +1088,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attn_chu
         }
         interleave<BN / 16 * DB, 2, kFar>();
         if (more) store_tile(step + 1);
-        if (look) put_page(step + 2, page);
+        if (look && tid < 64) put_page(step + 2, entry);
         __syncthreads();
     }
 
