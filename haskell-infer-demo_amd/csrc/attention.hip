@@ -1252,9 +1252,20 @@ Plan plan_of(const W4A16KvCache *c, const W4A16KvBatch *b, int q_heads) {
         p.ws_bytes = (size_t)p.few.blocks * rm * (dim + 2) * 4;
     }
     if (p.many.items) {
-        const long long blocks = (long long)p.many.items * c->kv_heads, wanted = 2LL * device_cus();
+        /* Two blocks a CU, by the tiles there are if max_new holds (`items` can be up to twice as many);
+         * one, or parts of `least` tokens, where two would make those shorter, since a part's results
+         * are 66 KB at 128 values a head. 16 sequences of 4096 tokens with 32 new ones, FP8: 1024 tokens
+         * 80 us, 1536 91; one of 32768 with 64, BF16: 85 and 69. */
+        const int least = c->format == W4A16_KV_BF16 ? 1536 : 1024;
+        const long long blocks = (long long)p.many.items * c->kv_heads, cus = device_cus();
+        const long long likely = seqs * ((longest + kChunkRows - 1) / kChunkRows);
+        const long long tiles = (likely < p.many.items ? likely : p.many.items) * c->kv_heads;
         const long long most = (tokens + kFewestTokens - 1) / kFewestTokens;
-        long long splits = (wanted + blocks - 1) / blocks;
+        long long splits = (2 * cus + tiles - 1) / tiles;
+        if (tokens < least * splits) {
+            const long long one = (cus + tiles - 1) / tiles, parts = (tokens + least - 1) / least;
+            splits = one > parts ? one : parts;
+        }
         if (splits > most) splits = most;
         if (splits > 256) splits = 256;
         p.many.splits = splits < 1 ? 1 : (int)splits;
