@@ -13,8 +13,8 @@
  * between the lane groups that hold its other tokens. The order of the tokens inside a product is
  * free as long as both operands keep it, which is what makes the two layouts meet.
  *
- * An 8-bit cache's codes are BF16 values; their scales multiply the scores (K) and the weights (V)
- * in FP32.
+ * An 8-bit cache's codes are BF16 and FP16 values; their scales multiply the scores (K) and the weights
+ * (V) in FP32.
  */
 #include <cmath>
 
@@ -36,6 +36,7 @@ struct AttnArgs {
     long long q_row, q_head, out_row, out_head;
     int group, q_heads, causal, window;
     int splits, items;
+    int blocks;       /* few rows: as many parts have a place in the workspace */
     int over, upto;   /* only sequences of over < rows <= upto (token, head) rows */
     float scale;      /* |scale| log2(e) */
     uint32_t flip;    /* sign bits of a BF16 pair of q: a negative scale turns its sign over */
@@ -73,6 +74,8 @@ __device__ __forceinline__ void fill_tile(const AttnArgs &a, Tile *t) {
     if (t->lo < 0) t->lo = 0;
     if (t->hi < t->lo) t->hi = t->lo;
 }
+
+constexpr int kMostUnits = 1 << 23; /* of 2^30 tokens */
 
 template <int CTRL, int ROWS>
 __device__ __forceinline__ int dpp_or_zero(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false); }
@@ -179,6 +182,7 @@ __device__ __forceinline__ Seqs load_seqs(const AttnArgs &a, int base) {
 template <int RM>
 __device__ __forceinline__ int part_units(const AttnArgs &a, Seqs *q) {
     *q = load_seqs<RM>(a, 0);
+    if (a.splits == 0) return kMostUnits; /* pairs are whole */
     /* n < 2^47 in two pieces, whose sums over 64 lanes fit 32 bits */
     unsigned long long total = 0;
     long long pairs = 0;
@@ -194,7 +198,7 @@ __device__ __forceinline__ int part_units(const AttnArgs &a, Seqs *q) {
     }
     const unsigned long long wanted = pairs < a.splits ? a.splits - pairs / 2 : a.splits;
     const unsigned long long each = (total + wanted - 1) / wanted;
-    return each < 1 ? 1 : each > 1 << 23 ? 1 << 23 : (int)each;
+    return each < 1 ? 1 : each > kMostUnits ? kMostUnits : (int)each;
 }
 
 /* The part of this block (PAIR false) or the (tile, head) pair of number `index` (true): the tile, its head, its number of
@@ -308,6 +312,15 @@ __device__ __forceinline__ f4 mfma_v(const uint32_t *v, const uint32_t *w, f4 ac
 
 __device__ __forceinline__ float power_of_two(int biased) { return __builtin_bit_cast(float, (uint32_t)biased << 23); }
 
+/* The weights of an 8-bit cache carry V's scale, so they are FP16 (in which codes are exact), over a
+ * power of two that holds the largest scale so far in [1, 2), and times 2^kLift: at most 2^8 (a weight
+ * over the last maximum) * 2 * 2^kLift, half of what FP16 holds. A weight's rounding is 2^-11 of
+ * itself, or 2^-31 of the largest weight times the largest scale where that is more; BF16 would be 2^-8.
+ * Biased exponents below kLift + 1 are raised to it, for the factor to be a number. */
+constexpr int kLift = 6;
+__device__ __forceinline__ float over_power(int biased) { return power_of_two(254 + kLift - biased); }
+__device__ __forceinline__ float times_power(int biased) { return power_of_two(biased - kLift); }
+
 /* Blocks of attn_rows_kernel that a CU is to hold: as many as its registers allow without spilling.
  * More waves are what hides the latency of its loads: RT = 2, D = 128, FP8, 96 sequences' worth
  * of verify rows: 40.0 us at one block, 29.0 at two; D = 256, 2 x 100003 tokens: 107 and 82. */
@@ -330,10 +343,8 @@ constexpr int rows_blocks(int dim, int format, int rt) {
  * columns; a transposition of 8 tokens x 2 values at a time by byte permutations makes them the
  * operand of value e's product.
  *
- * A BF16 cache's weights are rounded to BF16, whose largest, 1, is exact. Those of an 8-bit cache
- * carry V's scale, so they are FP16 (codes are exact in it), scaled by a power of two that
- * holds the largest scale so far in [1, 2): eight times less rounding than BF16, and for INT8
- * fewer instructions to widen.
+ * A BF16 cache's weights are rounded to BF16, half a step of 2^-8 each; those of an 8-bit cache to
+ * FP16 (kLift), which also takes fewer instructions to widen INT8.
  */
 template <int D, int FMT, int RT>
 __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel(AttnArgs a) {
@@ -451,7 +462,7 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
 
     f4 acc[RT][E];
     float m[RT], l[RT];
-    int v_exp = 1; /* biased exponent that the weights are scaled by (8-bit caches) */
+    int v_exp = kLift + 1; /* biased exponent of the power of two that the weights are over (8-bit caches) */
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
         m[r] = -__builtin_inff();
@@ -546,7 +557,7 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
             }
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                vs[c] *= power_of_two(254 - v_exp);
+                vs[c] *= over_power(v_exp);
                 ks[c] *= a.scale;
             }
         }
@@ -647,7 +658,7 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
         }
     }
     if constexpr (kCoded) {
-        const float by = power_of_two(v_exp);
+        const float by = times_power(v_exp);
 #pragma unroll
         for (int r = 0; r < RT; ++r)
 #pragma unroll
@@ -832,7 +843,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attn_chu
     u4 kr[C::kLoads], vr[C::kLoads];
     float scale_r = 0.0f;
     bool scale_there = false;
-    int v_run = 1;
+    int v_run = kLift + 1;
     bool there_r[C::kLoads];
     constexpr int kLanes = D * (kCoded ? 1 : 2) / 16; /* a token's 16-byte loads */
     /* the place in its page and head of token `at` of a step; rows of it that many bytes apart */
@@ -895,7 +906,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attn_chu
                 const int e = (int)(__builtin_bit_cast(uint32_t, scale_r) >> 23);
                 const int most = wave_most(tid >= BN && e <= 253 ? e : 0);
                 v_run = most > v_run ? most : v_run;
-                if (tid >= BN) scale_r *= power_of_two(254 - v_run);
+                if (tid >= BN) scale_r *= over_power(v_run);
                 if (lane == 0) exponents[step & 1] = v_run;
             }
             if (tid < 2 * BN) scales[(step & 1) * 2 * BN + tid] = scale_r;
@@ -931,7 +942,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attn_chu
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[d][i] = 0.0f;
     float m = real ? -__builtin_inff() : 0.0f, l = 0.0f;
-    int v_exp = 1;
+    int v_exp = kLift + 1;
     if (steps > 0) {
         store_tile(0);
         __syncthreads();
@@ -1110,7 +1121,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attn_chu
     /* a lane has values 32 d + 8 b + 4 half .. + 3 of its row; so does lane ^ 32 the four between */
     const float total = lane_sum32(l);
     if (!real) return;
-    float by = kCoded ? power_of_two(v_exp) : 1.0f;
+    float by = kCoded ? times_power(v_exp) : 1.0f;
     float *partial = t.active > 1 ? partial_at<D, RM>(a, ((long long)item * a.kv.heads + head) * a.splits + split) : nullptr;
     if (partial) {
 #pragma unroll
@@ -1149,6 +1160,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     int head, first_part = 0;
     if constexpr (EVEN) {
         if (!find_part<RM, true>(a, blockIdx.x, &t, &head, &first_part)) return;
+        if (first_part + t.active > a.blocks) return; /* sequences that overlap: not all parts were worked on */
     } else {
         head = blockIdx.x % a.kv.heads;
         if (!find_tile<RM>(a, blockIdx.x / a.kv.heads, 0, &t)) return;
@@ -1248,8 +1260,13 @@ Plan plan_of(const W4A16KvCache *c, const W4A16KvBatch *b, int q_heads) {
         const long long blocks = (long long)rows_blocks(dim, c->format, p.rt) * device_cus();
         const long long pairs = (long long)p.few.items * c->kv_heads, units = pairs * ((tokens + kUnit - 1) / kUnit);
         p.few.splits = (int)(units < 1 ? 1 : units < blocks ? units : blocks);
+        /* Short sequences are not cut at all: no partial results and no second launch. One sequence,
+         * 8 key heads of 128, BF16, cut and whole, in a graph: 512 tokens 10.5 and 9.2 us, 768 10.6 and 11.6;
+         * sixteen sequences: 768 16.9 and 14.9, 1024 18.6 and 18.1, 1536 22.9 and 24.8. */
+        if (tokens <= (pairs >= device_cus() / 2 ? 1024 : 512)) p.few.splits = 0;
+        if (pairs > 65536) p.few.splits = 0; /* places for their parts would take gigabytes */
         p.few.blocks = p.few.splits + pairs;
-        p.ws_bytes = (size_t)p.few.blocks * rm * (dim + 2) * 4;
+        if (p.few.splits) p.ws_bytes = (size_t)p.few.blocks * rm * (dim + 2) * 4;
     }
     if (p.many.items) {
         /* Two blocks a CU, by the tiles there are if max_new holds (`items` can be up to twice as many);
@@ -1287,6 +1304,7 @@ AttnArgs part_args(const AttnArgs &all, const Part &p) {
     AttnArgs a = all;
     a.items = p.items;
     a.splits = p.splits;
+    a.blocks = (int)p.blocks;
     a.over = p.over;
     a.upto = p.upto;
     a.ws += p.ws_at / 4;
@@ -1306,10 +1324,11 @@ void launch_format(const Plan &p, const AttnArgs &all, hipStream_t s) {
         if constexpr (D <= 128)
             if (p.rt == 2) {
                 launch_k(attn_rows_kernel<D, FMT, 2>, dim3((unsigned)p.few.blocks), dim3(256), 0, s, a);
-                return launch_join<D, 32, true>(parts, a, s);
+                if (a.splits) launch_join<D, 32, true>(parts, a, s);
+                return;
             }
         launch_k(attn_rows_kernel<D, FMT, 1>, dim3((unsigned)p.few.blocks), dim3(256), 0, s, a);
-        launch_join<D, 16, true>(parts, a, s);
+        if (a.splits) launch_join<D, 16, true>(parts, a, s);
     }
 }
 
@@ -1405,7 +1424,7 @@ extern "C" int w4a16_paged_attention_bf16(const W4A16KvCache *cache, const W4A16
     a.q_heads = q_heads;
     a.causal = causal != 0;
     a.window = window;
-    a.splits = a.items = a.over = a.upto = 0; /* part_args */
+    a.splits = a.items = a.blocks = a.over = a.upto = 0; /* part_args */
     a.scale = fabsf(scale) * 1.4426950408889634f;
     a.flip = scale < 0.0f ? 0x80008000u : 0u;
     hipStream_t s = static_cast<hipStream_t>(stream);

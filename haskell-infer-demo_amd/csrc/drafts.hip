@@ -5,7 +5,8 @@
  * replaced by a draw from max(p - q, 0), after which the sequence's tokens are distributed as if
  * drawn from p. The random numbers are given, so the whole call is a function of its arguments.
  *
- * Two launches. drafts_sum_kernel: every block finds its sequence's first refused token (a few
+ * Up to kSmall words: one launch of one block a sequence that holds the row's weights in registers.
+ * More: two launches. drafts_sum_kernel: every block finds its sequence's first refused token (a few
  * gathers, the same in all of them) and sums one piece of that one row's weights in FP64.
  * drafts_draw_kernel: one block a sequence runs over the pieces' sums to the one in which the
  * running sum passes the drawn threshold, and through that piece alone. Bound by memory for many
@@ -22,6 +23,9 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kQuads = 4;                     /* of neighbouring weights, a thread's: quad j of thread t is at 4 (256 j + t) */
 constexpr int kPiece = kThreads * kQuads * 4; /* weights a block sums */
+
+constexpr int kSmallThreads = 1024, kSmallQuads = 4;
+constexpr int kSmall = kSmallThreads * kSmallQuads * 4;
 
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float f4_loose __attribute__((ext_vector_type(4), aligned(4))); /* rows start anywhere */
@@ -43,22 +47,25 @@ constexpr int kNone = INT32_MIN;
  * by one wave, 64 tokens at a time. */
 __device__ __forceinline__ int taken_of(const DraftArgs &a, int seq, int *refused) {
     const int lane = threadIdx.x & 63;
-    int n = a.lens ? a.lens[seq] : a.steps;
-    n = n < 0 ? 0 : n > a.steps ? a.steps : n;
+    /* the first 64 tokens are fetched beside their number, not after it */
+    const int asked = a.lens ? a.lens[seq] : a.steps;
+    int n = a.steps;
     for (int base = 0; base < n; base += 64) {
         const int i = base + lane;
         bool take = true;
         int x = 0;
         if (i < n) {
             x = a.draft_tokens[(long long)seq * a.steps + i];
-            take = false;
-            if ((unsigned)x < (unsigned)a.vocab) {
-                const double p = a.target[seq * a.target_seq + i * a.target_row + x];
-                const double q = a.draft ? a.draft[seq * a.draft_seq + i * a.draft_row + x] : 1.0f;
-                take = (double)a.uniforms[(long long)seq * (a.steps + 1) + i] * q < p;
-            }
+            const float u = a.uniforms[(long long)seq * (a.steps + 1) + i];
+            const bool inside = (unsigned)x < (unsigned)a.vocab;
+            const int at = inside ? x : 0;
+            const double p = a.target[seq * a.target_seq + i * a.target_row + at];
+            const double q = a.draft ? a.draft[seq * a.draft_seq + i * a.draft_row + at] : 1.0f;
+            take = inside && (double)u * q < p;
             x = x == kNone ? -1 : x; /* outside the vocabulary either way */
         }
+        if (base == 0) n = asked < 0 ? 0 : asked > a.steps ? a.steps : asked;
+        take = take || i >= n;
         const unsigned long long no = __ballot(!take);
         if (no) {
             const int l = __ffsll((long long)no) - 1;
@@ -128,6 +135,28 @@ __device__ __forceinline__ double lane_f64(double v, int lane) {
     const uint2 b = __builtin_bit_cast(uint2, v);
     return __builtin_bit_cast(double, make_uint2((uint32_t)__builtin_amdgcn_readlane((int)b.x, lane),
                                                  (uint32_t)__builtin_amdgcn_readlane((int)b.y, lane)));
+}
+
+/* The largest of v >= 0 over the lanes. */
+__device__ __forceinline__ int wave_most(int v) {
+#define W4A16_MOST(CTRL, ROWS) v = max(v, __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false))
+    W4A16_MOST(0x111, 0xF);
+    W4A16_MOST(0x112, 0xF);
+    W4A16_MOST(0x114, 0xF);
+    W4A16_MOST(0x118, 0xF);
+    W4A16_MOST(0x142, 0xA);
+    W4A16_MOST(0x143, 0xC);
+#undef W4A16_MOST
+    return __builtin_amdgcn_readlane(v, 63);
+}
+
+/* The block's smallest `mine` and largest `behind`, a wave's first: 64 lanes at one LDS word take turns. */
+__device__ __forceinline__ void join_found(int mine, int behind, int *found, int *last) {
+    const int first = INT32_MAX - wave_most(INT32_MAX - mine), end = wave_most(behind + 1) - 1;
+    if ((threadIdx.x & 63) == 0) {
+        if (first != INT32_MAX) atomicMin(found, first);
+        if (end >= 0) atomicMax(last, end);
+    }
 }
 
 __device__ __forceinline__ double wave_sum(double v) { return lane_f64(wave_scan(v), 63); }
@@ -272,10 +301,117 @@ __global__ __launch_bounds__(kThreads) void drafts_draw_kernel(DraftArgs a) {
             }
         }
     }
-    if (mine != INT32_MAX) atomicMin(&found, mine);
-    if (behind >= 0) atomicMax(&last, behind);
+    join_found(mine, behind, &found, &last);
     __syncthreads();
     if (tid == 0) *out = found != INT32_MAX ? found : last;
+}
+
+/* Everything in one block. A quad's place in the order is (round, wave, lane), as above; one wave sums
+ * the (round, wave) pairs. */
+template <int QUADS>
+__global__ __launch_bounds__(kSmallThreads) void drafts_small_kernel(DraftArgs a) {
+    constexpr int kWaves = kSmallThreads / 64, kPairs = QUADS * kWaves;
+    const int seq = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    __shared__ double sums[2][kWaves], before_of[kPairs];
+    __shared__ int found, last;
+    int refused;
+    const int taken = taken_of(a, seq, &refused);
+    const float uniform = a.uniforms[(long long)seq * (a.steps + 1) + a.steps];
+    int32_t *out = a.tokens + (long long)seq * (a.steps + 1);
+    for (int i = tid; i <= a.steps; i += kSmallThreads)
+        if (i != taken) out[i] = i < taken ? a.draft_tokens[(long long)seq * a.steps + i] : -1;
+    if (tid == 0) {
+        a.accepted[seq] = taken;
+        found = INT32_MAX;
+        last = -1;
+    }
+    const Row r = row_of(a, seq, taken, refused);
+    f4 own[QUADS];
+    double rest = 0.0, all = 0.0;
+#pragma unroll
+    for (int half = 0; half < QUADS; half += 2) { /* as many rows' loads at a time as there are registers for */
+        f4 p[2], q[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int i = ((half + j) * kSmallThreads + tid) * 4;
+            p[j] = load_quad(r.p, i, a.vocab);
+            q[j] = r.q ? load_quad(r.q, i, a.vocab) : f4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int i = ((half + j) * kSmallThreads + tid) * 4 + c;
+                own[half + j][c] = rest_of(p[j][c], q[j][c], r.q != nullptr, i, r.chosen);
+                rest += (double)own[half + j][c];
+                all += (double)weight(p[j][c]);
+            }
+    }
+    rest = wave_sum(rest);
+    all = wave_sum(all);
+    if (lane == 0) {
+        sums[0][wave] = rest;
+        sums[1][wave] = all;
+    }
+    __syncthreads();
+    rest = all = 0.0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        rest += sums[0][w];
+        all += sums[1][w];
+    }
+    const bool which = !(rest > 0.0); /* from the target's own weights */
+    const double total = which ? all : rest, pass = (double)uniform * total;
+    if (!(total > 0.0)) {
+        if (tid == 0) out[taken] = -1;
+        return;
+    }
+    if (which) {
+#pragma unroll
+        for (int j = 0; j < QUADS; ++j) {
+            const f4 p = load_quad(r.p, (j * kSmallThreads + tid) * 4, a.vocab);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) own[j][c] = weight(p[c]);
+        }
+    }
+    double upto[QUADS];
+#pragma unroll
+    for (int j = 0; j < QUADS; ++j) {
+        double sum = 0.0;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) sum += (double)own[j][c];
+        upto[j] = wave_scan(sum);
+        if (lane == 63) before_of[j * kWaves + wave] = upto[j];
+        upto[j] -= sum; /* before this quad */
+    }
+    __syncthreads();
+    if (wave == 0) {
+        double before = 0.0;
+        for (int base = 0; base < kPairs; base += 64) {
+            const double v = base + lane < kPairs ? before_of[base + lane] : 0.0;
+            const double to = before + wave_scan(v);
+            before = lane_f64(to, 63);
+            if (base + lane < kPairs) before_of[base + lane] = to - v;
+        }
+    }
+    __syncthreads();
+    int mine = INT32_MAX, behind = -1;
+#pragma unroll
+    for (int j = 0; j < QUADS; ++j) {
+        double run = before_of[j * kWaves + wave] + upto[j];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const int i = (j * kSmallThreads + tid) * 4 + c;
+            run += (double)own[j][c];
+            if (own[j][c] > 0.0f) {
+                behind = i;
+                if (run > pass && mine == INT32_MAX) mine = i;
+            }
+        }
+    }
+    join_found(mine, behind, &found, &last);
+    __syncthreads();
+    if (tid == 0) out[taken] = found != INT32_MAX ? found : last;
 }
 
 } // namespace
@@ -285,7 +421,7 @@ extern "C" int w4a16_verify_drafts_workspace(int seqs, int steps, int vocab, siz
     if (seqs < 0 || seqs > 65535 || steps < 0 || steps > 65535 || vocab < 1 || vocab > (1 << 28))
         return set_error(W4A16_ERR_CONFIG, "w4a16_verify_drafts: bad extents seqs=%d steps=%d vocab=%d (seqs and steps "
                          "up to 65535, vocab 1 to 2^28)", seqs, steps, vocab);
-    *bytes = (size_t)seqs * ((size_t)((vocab + kPiece - 1) / kPiece) * 16 + 16);
+    *bytes = vocab <= kSmall ? 0 : (size_t)seqs * ((size_t)((vocab + kPiece - 1) / kPiece) * 16 + 16);
     return W4A16_OK;
 }
 
@@ -299,7 +435,7 @@ extern "C" int w4a16_verify_drafts_f32(const float *target, long long target_seq
     int st = w4a16_verify_drafts_workspace(seqs, steps, vocab, &need);
     if (st) return st;
     if (seqs == 0) return W4A16_OK;
-    if (!target || !uniforms || !accepted || !tokens || !ws || (steps > 0 && !draft_tokens))
+    if (!target || !uniforms || !accepted || !tokens || (need && !ws) || (steps > 0 && !draft_tokens))
         return set_error(W4A16_ERR_CONFIG, "%s: null buffer", what);
     if (((uintptr_t)target | (uintptr_t)draft | (uintptr_t)draft_tokens | (uintptr_t)lens | (uintptr_t)uniforms |
          (uintptr_t)accepted | (uintptr_t)tokens) & 3)
@@ -328,10 +464,18 @@ extern "C" int w4a16_verify_drafts_f32(const float *target, long long target_seq
                 return set_error(W4A16_ERR_CONFIG, "%s: the outputs and the workspace overlap", what);
     }
     const int pieces = (vocab + kPiece - 1) / kPiece;
+    double *const sums = static_cast<double *>(ws);
     const DraftArgs a = {target, steps > 0 ? draft : nullptr, target_seq_stride, target_row_stride, draft_seq_stride,
-                         draft_row_stride, draft_tokens, lens, uniforms, accepted, tokens, static_cast<double *>(ws),
-                         reinterpret_cast<int2 *>(static_cast<double *>(ws) + (size_t)seqs * pieces * 2), steps, vocab, pieces};
+                         draft_row_stride, draft_tokens, lens, uniforms, accepted, tokens, sums,
+                         need ? reinterpret_cast<int2 *>(sums + (size_t)seqs * pieces * 2) : nullptr, steps, vocab, pieces};
     hipStream_t s = static_cast<hipStream_t>(stream);
+    /* 8000 words: 5.2 us in one launch, as many as a 1000; 16000: 7.0, and 7.6 for two (32000: 7.7),
+     * whose second call costs the host 2 more. */
+    if (vocab <= kSmall) {
+        const auto kernel = vocab <= kSmall / 2 ? drafts_small_kernel<kSmallQuads / 2> : drafts_small_kernel<kSmallQuads>;
+        launch_k(kernel, dim3(seqs), dim3(kSmallThreads), 0, s, a);
+        return hip_status(hipGetLastError(), "verify drafts launch");
+    }
     launch_k(drafts_sum_kernel, dim3(pieces, seqs), dim3(kThreads), 0, s, a);
     launch_k(drafts_draw_kernel, dim3(seqs), dim3(kThreads), 0, s, a);
     return hip_status(hipGetLastError(), "verify drafts launch");

@@ -664,10 +664,30 @@ def _torch_c():
     return torch._C
 
 
+def _under(stream, device):
+    """The context of a stream that a call names: what the call allocates is then that stream's, so that the allocator
+    gives it to nobody else before the call has run."""
+    import torch
+
+    if device.type != "cuda":
+        _refuse(f"expected tensors on a GPU, not on {device}")
+    if isinstance(stream, int):
+        stream = torch.cuda.ExternalStream(stream, device=device) if stream else torch.cuda.default_stream(device)
+    return torch.cuda.stream(stream)
+
+
+@functools.lru_cache(maxsize=None)
+def _bits16():
+    """What passes as BF16 values: their type, or their bits."""
+    import torch
+
+    return {torch.bfloat16, torch.int16, torch.uint16}
+
+
 def _rows3(t, shape, device, what):
     """Address and strides of a [rows, heads, dim] tensor of BF16 values whose last axis is dense."""
     try:
-        if t.shape == shape and t.device == device and t.element_size() == 2:
+        if t.shape == shape and t.device == device and t.dtype in _bits16():
             row, head, one = t.stride()
             if one == 1:
                 return t.data_ptr(), row, head
@@ -677,7 +697,7 @@ def _rows3(t, shape, device, what):
         _refuse(f"{what}: expected a tensor on {device}")
     if t.shape != shape:
         _refuse(f"{what}: shape {tuple(t.shape)}, the call needs {shape}")
-    if t.element_size() != 2:
+    if t.dtype not in _bits16():
         _refuse(f"{what}: {t.dtype} is not BF16 (or its bits)")
     _refuse(f"{what}: the last axis is strided")
 
@@ -737,14 +757,20 @@ class KvCache:
         `out` rows of no sequence are zeros; with it they are left as they were."""
         import torch
 
+        if stream is not None and out is None:
+            with _under(stream, self.device):
+                return self.read(batch)
         index = _on_current(self.device, "KvCache.read")
         batch.check(self.device, "KvCache.read")
-        shape = (batch.rows, self.kv_heads, self.head_dim)
+        size = batch.rows * self.kv_heads * self.head_dim * 2
         if out is None:
             make = torch.zeros if batch.padded else torch.empty
-            out = tuple(make(shape, dtype=torch.bfloat16, device=self.device) for _ in range(2))
-        size = batch.rows * self.kv_heads * self.head_dim * 2
-        k, v = (_dev(t, size, 2, "KvCache.read out", self.device) for t in out)
+            both = make((2, batch.rows, self.kv_heads, self.head_dim), dtype=torch.bfloat16, device=self.device)
+            out = both.unbind(0)
+            k = both.data_ptr()
+            v = k + size
+        else:
+            k, v = (_dev(t, size, 2, "KvCache.read out", self.device) for t in out)
         _check(lib.w4a16_kv_read_bf16(self._ref, batch._ref, k, v, _raw_stream(stream, index)), "KvCache.read")
         return out
 
@@ -788,10 +814,14 @@ def paged_attention(q, cache, batch, scale=None, causal=True, window=0, out=None
     """Attention of the batch's rows of q [rows, q_heads, head_dim] (BF16; strided views are fine)
     over the cache, their own keys and values written already. scale: 1 / sqrt(head_dim) unless it
     is given. Returns out [rows, q_heads, head_dim], or (out, lse [rows, q_heads]). `workspace`: a
-    uint8 tensor to use instead of a new one, not shared with a call that may still run."""
+    uint8 tensor to use instead of a new one, not shared with a call that may still run. With a
+    `stream`, what the call allocates is allocated under it."""
     import torch
 
     device = cache.device
+    if stream is not None:
+        with _under(stream, device):
+            return paged_attention(q, cache, batch, scale, causal, window, out, return_lse, workspace)
     index = _on_current(device, "paged_attention")
     batch.check(device, "paged_attention")
     rows, dim = batch.rows, cache.head_dim
@@ -825,8 +855,7 @@ def paged_attention(q, cache, batch, scale=None, causal=True, window=0, out=None
             wp = _dev(workspace, need, 1, "paged_attention workspace", device)
     st = lib.w4a16_paged_attention_bf16(cache._ref, batch._ref, qp, q_row, q_head, q_heads,
                                         dim ** -0.5 if scale is None else scale, 1 if causal else 0, window, op, o_row,
-                                        o_head, None if lse is None else lse.data_ptr(), wp, need,
-                                        _raw_stream(stream, index))
+                                        o_head, None if lse is None else lse.data_ptr(), wp, need, _raw_stream(None, index))
     if st:
         _check(st, "paged_attention")
     return (out, lse) if return_lse else out
@@ -865,6 +894,9 @@ def verify_drafts(target, draft_tokens, uniforms, draft=None, lens=None, workspa
     import torch
 
     device = target.device
+    if stream is not None:
+        with _under(stream, device):
+            return verify_drafts(target, draft_tokens, uniforms, draft, lens, workspace)
     index = _on_current(device, "verify_drafts")
     tp, t_seq, t_row = _floats3(target, "verify_drafts target", device)
     seqs, rows, vocab = target.shape
@@ -882,13 +914,16 @@ def verify_drafts(target, draft_tokens, uniforms, draft=None, lens=None, workspa
     accepted = torch.empty(seqs, dtype=torch.int32, device=device)
     tokens = torch.empty((seqs, rows), dtype=torch.int32, device=device)
     need = _drafts_workspace(seqs, steps, vocab)
-    if workspace is None:
+    wp = None
+    if need == 0:
+        pass
+    elif workspace is None:
         workspace = torch.empty(need, dtype=torch.uint8, device=device)
         wp = workspace.data_ptr()
     else:
         wp = _dev(workspace, need, 1, "verify_drafts workspace", device)
     st = lib.w4a16_verify_drafts_f32(tp, t_seq, t_row, dp, d_seq, d_row, ip, lp, up, accepted.data_ptr(),
-                                     tokens.data_ptr(), seqs, steps, vocab, wp, need, _raw_stream(stream, index))
+                                     tokens.data_ptr(), seqs, steps, vocab, wp, need, _raw_stream(None, index))
     if st:
         _check(st, "verify_drafts")
     return accepted, tokens

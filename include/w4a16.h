@@ -350,7 +350,9 @@ int engine_ffn_forward_residual_norm(W4A16Store *store, int layer, uint16_t *res
  *   scale = a / top, code = round to nearest even(x * (top / a)), the two quotients and the
  *   product rounded to FP32;
  * a row with a < 2^-117 is held as zeros (scale 0), one with an infinity or a NaN as zero codes
- * with a NaN scale, so it reads back as NaN and no attention masks that out by accident.
+ * with a NaN scale: it reads back as NaN, and in the attention spoils the rows that see it and no
+ * others. Codes are finite; a caller that writes NaN codes of its own (FP8 0x7F, 0xFF) spoils the
+ * rows beside those that see them too.
  *
  * The batch. page_table[s * table_stride + i] is the page of tokens i * page_size .. of sequence
  * s (i < table_pages), kv_lens[s] the tokens it has in the cache, the call's own among them.
@@ -359,10 +361,10 @@ int engine_ffn_forward_residual_norm(W4A16Store *store, int layer, uint16_t *res
  * decrease; rows outside starts[0] .. starts[seqs] - 1 are left as they were. These arrays are
  * read on the device at run time (a captured graph sees their values of each replay); they start
  * on a 4-byte boundary. max_new and max_kv bound the new tokens and kv_lens of any sequence
- * (0: rows, and what the table holds); they only plan the launch, so a loose bound costs speed and a wrong one is no fault. Tokens
- * past the table (or past 2^30) and pages outside the cache are seen as tokens that are not there: not written,
- * read as zeros, masked in the attention. A page that one call writes through two sequences
- * holds either's rows.
+ * (0: rows, and what the table holds); they only plan the launch, so a loose bound costs speed and
+ * a wrong one is no fault. Tokens past the table (or past 2^30) and pages outside the cache are seen
+ * as tokens that are not there: not written, read as zeros, masked in the attention. Sequences may
+ * share pages; one that a call writes through two of them holds either's rows.
  *
  * Strides are in elements; a token's heads and a head's values stand apart by multiples of 8
  * elements, values next to each other. Tensors that are read and written by one call must not
@@ -409,10 +411,11 @@ int w4a16_kv_read_bf16(const W4A16KvCache *cache, const W4A16KvBatch *batch, uin
 /* Attention of the batch's rows of q [rows][q_heads][head_dim] over the cache, to which the rows'
  * own keys and values have been written: out_i = sum_j softmax_j(scale * <q_i, k_j>) v_j. Query
  * head h reads key head h / (q_heads / kv_heads). causal: a row sees positions up to its own;
- * window > 0: only its last `window` ones of them (its own included). Scores, statistics and
- * sums are FP32; the weights are rounded to BF16 before the product with V (and after a V
- * scale's multiplication), the output once. A row that sees nothing gets zeros, and -infinity as
- * lse. lse (optional): [rows][q_heads], log of the sum of exp of the scaled scores.
+ * window > 0: none that is `window` or more before its own. Scores, statistics and sums are FP32.
+ * The weights are rounded before the product with V: to BF16, or with an 8-bit cache, where they
+ * carry V's scales, to FP16 (2^-11 of each, or 2^-31 of the largest weight times the largest of the
+ * sequence's scales for that head, whichever is more). The output is rounded once. A row that sees
+ * nothing gets zeros, and -infinity as lse. lse (optional): [rows][q_heads], log of the sum of exp of the scaled scores.
  * ws: device memory of at least the bytes w4a16_paged_attention_workspace gives for the same
  * arguments (on the same device), for this call alone until it has run; NULL if that is 0.
  * out may be q itself (the same strides). */
@@ -440,7 +443,7 @@ int w4a16_paged_attention_bf16(const W4A16KvCache *cache, const W4A16KvBatch *ba
  * accepted[s]: the tokens taken. tokens [seqs][steps + 1]: those, the drawn one (-1 if no weight
  * is positive), and -1 behind it. Every float row starts on a 4-byte boundary.
  * ws: w4a16_verify_drafts_workspace bytes of device memory, for this call alone until it has
- * run. */
+ * run; NULL if that is 0. */
 int w4a16_verify_drafts_workspace(int seqs, int steps, int vocab, size_t *bytes);
 int w4a16_verify_drafts_f32(const float *target, long long target_seq_stride,
                             long long target_row_stride, const float *draft,

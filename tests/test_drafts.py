@@ -34,7 +34,7 @@ def random_case(seqs, steps, vocab, seed, noise=0.5, drawn=True):
 
 @pytest.mark.parametrize("drawn", [True, False])
 @pytest.mark.parametrize("seqs,steps,vocab", [(1, 1, 1), (1, 0, 17), (3, 4, 2), (5, 3, 1000), (2, 1, 4095), (2, 2, 4097),
-                                              (3, 16, 8193), (2, 70, 513), (4, 5, 50257), (1, 4, 151936), (200, 2, 301)])
+                                              (3, 16, 8192), (3, 16, 8193), (2, 70, 513), (6, 4, 32000), (2, 3, 32768), (2, 3, 32769), (4, 5, 50257), (1, 4, 151936), (200, 2, 301)])
 def test_against_the_definition(cuda, seqs, steps, vocab, drawn):
     print(f"drafts seqs={seqs} steps={steps} vocab={vocab} drawn={drawn}", flush=True)
     for seed in range(3):
@@ -60,10 +60,10 @@ def test_borders(cuda):
     assert out[:, 0].tolist() == [1, 3, 6, 1, 3, 6] and out[1, 1] == 3 and out[4, 1] == 6
 
 
-def test_weights_that_are_none(cuda):
+@pytest.mark.parametrize("vocab", [5000, 9000, 40000])
+def test_weights_that_are_none(cuda, vocab):
     """Nothing left of the target where the draft refused: the target itself. Rows of zeros, NaN and infinities: no token.
     Tokens outside the vocabulary are refused; NaN uniforms refuse, and draw the last token that weighs anything."""
-    vocab = 9000
     target, draft, tokens, uniforms = random_case(8, 2, vocab, 1)
     draft[0, 0] = target[0, 0] * 2          # nothing left
     uniforms[0, 0] = 0.9
@@ -96,7 +96,7 @@ def test_strided_rows(cuda):
 
 def test_captured(cuda):
     """In a graph, replayed with other inputs and eager work between."""
-    shape = (5, 3, 10007)
+    shape = (5, 3, 40007)
     dev = [t.to(cuda) for t in random_case(*shape, 1)]
     call = lambda: w4a16.verify_drafts(dev[0], dev[2], dev[3], draft=dev[1])  # noqa: E731
     call()

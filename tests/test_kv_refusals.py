@@ -40,8 +40,8 @@ def attend(c=None, b=None, q=A * 256, qs=(256, 64), heads=4, scale=0.125, window
                                                 ws, ws_bytes, None)
 
 
-def verify(target=A * 256, ts=(400, 100), draft=A * 320, ds=(300, 100), tokens_in=A, lens=None, uniforms=A * 2, accepted=A * 3,
-           tokens=A * 4, seqs=2, steps=3, vocab=100, ws=A * 5, ws_bytes=1 << 20):
+def verify(target=A * 256, ts=(400000, 100000), draft=A * 320, ds=(300000, 100000), tokens_in=A, lens=None, uniforms=A * 2, accepted=A * 3,
+           tokens=A * 4, seqs=2, steps=3, vocab=100000, ws=A * 5, ws_bytes=1 << 20):
     return w4a16.lib.w4a16_verify_drafts_f32(target, *ts, draft, *ds, tokens_in, lens, uniforms, accepted, tokens, seqs, steps,
                                              vocab, ws, ws_bytes, None)
 
@@ -89,7 +89,7 @@ def test_batches(fields, why):
     (verify, dict(vocab=0), "extents"), (verify, dict(vocab=(1 << 28) + 1), "extents"), (verify, dict(target=None), "null"),
     (verify, dict(tokens_in=None), "null"), (verify, dict(uniforms=None), "null"), (verify, dict(accepted=None), "null"),
     (verify, dict(tokens=None), "null"), (verify, dict(ws=None), "null"), (verify, dict(draft=A * 320 + 2), "aligned"),
-    (verify, dict(ws=A * 5 + 8), "aligned"), (verify, dict(ws_bytes=16), "workspace"), (verify, dict(ts=(-1, 100)), "stride"),
+    (verify, dict(ws=A * 5 + 8), "aligned"), (verify, dict(ws_bytes=16), "workspace"), (verify, dict(ts=(-1, 100000)), "stride"),
     (verify, dict(accepted=A * 256), "overlap"), (verify, dict(tokens=A), "overlap"), (verify, dict(tokens=A * 3), "overlap"),
     (verify, dict(ws=A * 4), "overlap"),
 ])
@@ -109,10 +109,10 @@ def test_workspaces():
     one = cache(num_pages=1 << 20)
     lib = w4a16.lib
     sizes = []
-    for most in (100, 50000):
+    for most in (100, 2000, 50000):
         assert lib.w4a16_paged_attention_workspace(ctypes.byref(one), ctypes.byref(batch(max_kv=most)), 4, ctypes.byref(need)) == 0
         sizes.append(need.value)
-    assert 0 < sizes[0] < sizes[1]
+    assert 0 == sizes[0] < sizes[1] < sizes[2]  # short sequences are not cut
     # many rows in many tiles: nothing to join
     many = batch(rows=1 << 16, seqs=1, max_new=1 << 16)
     assert lib.w4a16_paged_attention_workspace(ctypes.byref(one), ctypes.byref(many), 4, ctypes.byref(need)) == 0
@@ -120,6 +120,7 @@ def test_workspaces():
     assert lib.w4a16_paged_attention_workspace(ctypes.byref(one), ctypes.byref(batch()), 4, None) == CONFIG
     assert lib.w4a16_paged_attention_workspace(None, ctypes.byref(batch()), 4, ctypes.byref(need)) == CONFIG
     assert lib.w4a16_verify_drafts_workspace(3, 2, 100000, ctypes.byref(need)) == 0 and need.value >= 3 * 16
+    assert lib.w4a16_verify_drafts_workspace(3, 2, 1000, ctypes.byref(need)) == 0 and need.value == 0
     assert lib.w4a16_verify_drafts_workspace(3, 2, 100, None) == CONFIG
 
 

@@ -78,15 +78,39 @@ def test_against_fp64(cuda, kv_lens, news, q_heads, heads, dim, page, window, fm
 
 
 @pytest.mark.parametrize("fmt", ["bf16", "fp8"])
+@pytest.mark.parametrize("window", [0, 50])
+@pytest.mark.parametrize("scale", [0.2, -0.1, 0.0])
 @pytest.mark.parametrize("news", [[3, 2], [80, 70]])
-def test_every_row_sees_all(cuda, fmt, news):
-    """causal=False, and a scale of the caller's."""
+def test_every_row_sees_all(cuda, fmt, news, scale, window):
+    """causal=False, and a scale of the caller's, of either sign or none."""
     kv_lens, page, pages = [333, 200], 16, 40
     cache = filled(pages, page, 2, 128, fmt, cuda, seed=9)
     batch, table = make_batch(kv_lens, news, page, pages, cuda)
     q = torch.randn(sum(news), 6, 128, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
-    out, lse = w4a16.paged_attention(q.to(cuda), cache, batch, scale=0.2, causal=False, return_lse=True)
-    check(out, lse, cache, table, q, kv_lens, news, page, pages, 0.2, causal=False)
+    out, lse = w4a16.paged_attention(q.to(cuda), cache, batch, scale=scale, causal=False, window=window, return_lse=True)
+    check(out, lse, cache, table, q, kv_lens, news, page, pages, scale, causal=False, window=window)
+
+
+def test_sequences_that_decrease_or_overlap(cuda):
+    """Starts that no caller should give: every access stays where it belongs, and the sequences that are whole and
+    alone are right."""
+    page, pages, dim = 8, 300, 64
+    cache = filled(pages, page, 2, dim, "fp8", cuda, seed=4)
+    order = torch.randperm(pages, generator=torch.Generator().manual_seed(0)).to(torch.int32)
+    table = order[:4 * 70].reshape(4, 70).to(cuda)
+    lens = torch.tensor([550, 560, 40, 555], dtype=torch.int32, device=cuda)
+    q = torch.randn(40, 4, dim, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16).to(cuda)
+    alone = w4a16.KvBatch(table[:1], lens[:1], torch.tensor([0, 3], dtype=torch.int32, device=cuda), 40, max_new=3, padded=True)
+    want = w4a16.paged_attention(q, cache, alone)
+    for starts in ([0, 3, 1, 9, 5], [0, 3, 60, 2, 40], [0, 3, -5, 20, 41], [0, 3, 3, 3, 3]):
+        batch = w4a16.KvBatch(table, lens, torch.tensor(starts, dtype=torch.int32, device=cuda), 40, max_new=3, padded=True)
+        out = w4a16.paged_attention(q, cache, batch)
+        if starts[2] >= 3:
+            assert torch.equal(out[:2], want[:2])
+        cache.write(q[:, :2], q[:, 2:], batch)
+        cache.read(batch)
+        torch.cuda.synchronize()
+        cache = filled(pages, page, 2, dim, "fp8", cuda, seed=4)
 
 
 @pytest.mark.parametrize("fmt", ["bf16", "int8", "fp8"])
@@ -241,6 +265,74 @@ def test_on_a_stream_of_its_own(cuda):
                           workspace=torch.empty(1 << 24, dtype=torch.uint8, device=cuda))
     stream.synchronize()
     assert torch.equal(got, want) and torch.equal(explicit, want)
+
+
+@pytest.mark.parametrize("raw", [False, True])
+def test_memory_of_a_call_on_another_stream(cuda, raw):
+    """What a call allocates for a stream that is not the current one, and lets go of when it returns, is not given to
+    the current stream while the call still runs."""
+    heads, q_heads, dim, page, pages = 2, 8, 128, 16, 700
+    cache = filled(pages, page, heads, dim, "fp8", cuda, seed=1)
+    batch, _ = make_batch([5000, 4000], [60, 3], page, pages, cuda, padded=True)
+    q = torch.randn(63, q_heads, dim, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16).to(cuda)
+    want, want_lse = w4a16.paged_attention(q, cache, batch, return_lse=True)
+    want_k, _ = cache.read(batch)
+    gen = torch.Generator().manual_seed(5)
+    probs = torch.rand(2, 3, 40000, generator=gen).to(cuda)
+    ids = torch.randint(0, 40000, (2, 2), generator=gen, dtype=torch.int32).to(cuda)
+    uniforms = torch.rand(2, 3, generator=gen).to(cuda)
+    want_ids = w4a16.verify_drafts(probs, ids, uniforms)[1]
+    stream, busy = torch.cuda.Stream(), torch.randn(4096, 4096, device=cuda)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        for _ in range(20):
+            busy @ busy
+    where = stream.cuda_stream if raw else stream
+    got, lse = w4a16.paged_attention(q, cache, batch, return_lse=True, stream=where)
+    got_k, _ = cache.read(batch, stream=where)
+    got_ids = w4a16.verify_drafts(probs, ids, uniforms, stream=where)[1]
+    others = [torch.full((1 << n,), 77, dtype=torch.uint8, device=cuda) for n in range(9, 28) for _ in range(2)]
+    stream.synchronize()
+    assert torch.equal(got, want) and torch.equal(lse, want_lse) and torch.equal(got_k, want_k) and torch.equal(got_ids, want_ids)
+    assert all((t == 77).all() for t in others)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("dim", [64, 256])
+@pytest.mark.parametrize("news", [3, 60])
+@pytest.mark.parametrize("at", [0, 100, 230])
+def test_scales_far_apart(cuda, fmt, dim, news, at):
+    """A token that weighs nothing, but whose values are 2^20 times the others', takes nothing from their weights."""
+    page, pages, n = 16, 20, 300
+    gen = torch.Generator().manual_seed(at)
+    k, v = torch.zeros(n, 2, dim), torch.rand(n, 2, dim, generator=gen) * 2 - 1
+    k[:, :, 1] = torch.randn(n, 2, generator=gen) / 8
+    k[at, :, 0] = -64.0
+    v[at] *= 2.0**20
+    q = torch.zeros(news, 4, dim)
+    q[:, :, :2] = 1.0
+    k, v, q = (t.to(torch.bfloat16) for t in (k, v, q))
+    cache = w4a16.KvCache.empty(pages, page, 2, dim, fmt, device=cuda)
+    every, table = make_batch([n], [n], page, pages, cuda)
+    cache.write(k.to(cuda), v.to(cuda), every)
+    batch = w4a16.KvBatch(every.page_table, every.kv_lens, torch.tensor([0, news], dtype=torch.int32, device=cuda), news)
+    out, lse = w4a16.paged_attention(q.to(cuda), cache, batch, scale=1.0, return_lse=True)
+    check(out, lse, cache, table, q, [n], [news], page, pages, 1.0)
+
+
+def test_refusals_of_tensors(cuda):
+    """FP16 is not BF16, and neither are strided values or other shapes."""
+    cache = filled(8, 16, 2, 64, "bf16", cuda, seed=1)
+    batch, _ = make_batch([20], [2], 16, 8, cuda)
+    q = torch.zeros(2, 4, 64, dtype=torch.bfloat16, device=cuda)
+    for bad in (q.half(), q[:1], q[:, :, :32], q.transpose(1, 2), q.cpu(), q.float()):
+        with pytest.raises(w4a16.W4A16Error):
+            w4a16.paged_attention(bad, cache, batch)
+        with pytest.raises(w4a16.W4A16Error):
+            w4a16.paged_attention(q, cache, batch, out=bad)
+        with pytest.raises(w4a16.W4A16Error):
+            cache.write(bad[:, :2], q[:, :2], batch)
+    assert torch.equal(w4a16.paged_attention(q.view(torch.int16), cache, batch), w4a16.paged_attention(q, cache, batch))
 
 
 def test_a_step_of_speculative_decoding(cuda):
