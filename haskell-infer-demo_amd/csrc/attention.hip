@@ -462,6 +462,7 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
 
     f4 acc[RT][E];
     float m[RT], l[RT];
+    float spoiled[RT] = {}; /* 1: this lane's row has seen a scale that is no number */
     int v_exp = kLift + 1; /* biased exponent of the power of two that the weights are over (8-bit caches) */
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
@@ -477,6 +478,39 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
         for (int c = 0; c < 2; ++c) there[c] = is_there(vnext[c], t0 + 16 * c + 4 * g);
         const int next = t0 + 128;
         const bool more = next < t.end;
+        const bool cut = (t0 < t.all_lo) | (t0 + 32 > t.all_hi) | (__any(!there[0] | !there[1]) != 0);
+        if constexpr (kCoded)
+            if (cut) {
+                bool odd_scale = false;
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int at = t0 + 16 * c + 4 * g + i;
+                        vs[c][i] = !there[c] | (at < t.lo) | (at >= t.hi) ? 0.0f : vs[c][i];
+                        odd_scale = odd_scale | !(vs[c][i] < __builtin_inff());
+                    }
+                if (__any(odd_scale)) {
+                    /* a scale that is no number, at a token that not every row sees: 0 times it would
+                     * reach the rows that do not. Those that do are noted, and the product goes
+                     * without it. */
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) {
+#pragma unroll
+                        for (int c = 0; c < 2; ++c)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const int at = t0 + 16 * c + 4 * g + i;
+                                const bool sees = (at >= lo[r]) & (at < hi[r]) & !(vs[c][i] < __builtin_inff());
+                                spoiled[r] = sees ? 1.0f : spoiled[r];
+                            }
+                    }
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) vs[c][i] = vs[c][i] < __builtin_inff() ? vs[c][i] : 0.0f;
+                }
+            }
         if constexpr (!kAhead)
             if (more) load_pages(next);
         f4 s[RT][2];
@@ -518,7 +552,6 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
 #pragma unroll
                 for (int w = 0; w < kVWords; ++w) asm volatile("" : "+v"(v[i][w]));
         /* tokens that some row does not see, or that are not there: their V is not multiplied */
-        const bool cut = (t0 < t.all_lo) | (t0 + 32 > t.all_hi) | (__any(!there[0] | !there[1]) != 0);
         bool odd = false;
         if (cut) {
 #pragma unroll
@@ -529,7 +562,6 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
                     const bool none = !there[c] | (at < t.lo) | (at >= t.hi);
 #pragma unroll
                     for (int w = 0; w < kVWords; ++w) v[4 * c + i][w] = none ? 0u : v[4 * c + i][w];
-                    if constexpr (kCoded) vs[c][i] = none ? 0.0f : vs[c][i];
                     if constexpr (!kCoded)
 #pragma unroll
                         for (int w = 0; w < kVWords; ++w) odd = odd | nonfinite2(v[4 * c + i][w]);
@@ -595,16 +627,13 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
                 for (int i = 0; i < 4; ++i) {
                     w[i] = __builtin_amdgcn_exp2f(s[r][c][i] - base);
                     l[r] += w[i];
-                    if constexpr (kCoded) {
-                        w[i] *= vs[c][i];
-                        w[i] = (cut & (s[r][c][i] == -__builtin_inff())) ? 0.0f : w[i];
-                    }
+                    if constexpr (kCoded) w[i] *= vs[c][i];
                 }
                 p[r][2 * c] = kCoded ? pack_f16(w[0], w[1]) : kv_pack_bf16(w[0], w[1]);
                 p[r][2 * c + 1] = kCoded ? pack_f16(w[2], w[3]) : kv_pack_bf16(w[2], w[3]);
             }
         }
-        if (!odd) {
+        if (kCoded || !odd) {
 #pragma unroll
             for (int e = 0; e < E; e += 2) {
                 uint32_t even[4], odds[4];
@@ -658,11 +687,12 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
         }
     }
     if constexpr (kCoded) {
-        const float by = times_power(v_exp);
 #pragma unroll
-        for (int r = 0; r < RT; ++r)
+        for (int r = 0; r < RT; ++r) {
+            const float by = lane_max32(lane_max16(spoiled[r])) > 0.0f ? __builtin_nanf("") : times_power(v_exp);
 #pragma unroll
             for (int e = 0; e < E; ++e) acc[r][e] *= by;
+        }
     }
 
     /* the four waves together: 128 values of 16 rows at a time */
@@ -812,7 +842,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attn_chu
     float *scales = reinterpret_cast<float *>(smem + C::kScales); /* [buffer][k, v][BN] */
     int *pages = reinterpret_cast<int *>(smem + C::kPages);       /* [step % 3][BN] */
     int *bad = reinterpret_cast<int *>(smem + C::kFlags);         /* [step % 3]: a token without a page */
-    int *exponents = bad + 3;                                      /* [step % 2]: V's scales are over 2 to this, biased */
+    int *exponents = bad + 3;                                      /* [step % 2]: V's scales are over 2 to this, biased; + 256: one is not finite */
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 31, half = lane >> 5;
     const int head = blockIdx.x % a.kv.heads, split = blockIdx.y;
     /* the last tiles of a sequence see the most keys: those first */
@@ -907,7 +937,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attn_chu
                 const int most = wave_most(tid >= BN && e <= 253 ? e : 0);
                 v_run = most > v_run ? most : v_run;
                 if (tid >= BN) scale_r *= over_power(v_run);
-                if (lane == 0) exponents[step & 1] = v_run;
+                const bool odd = __any((tid >= BN) & ((e & 255) == 255));
+                if (lane == 0) exponents[step & 1] = v_run + (odd ? 256 : 0);
             }
             if (tid < 2 * BN) scales[(step & 1) * 2 * BN + tid] = scale_r;
         } else {
@@ -943,6 +974,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attn_chu
         for (int i = 0; i < 16; ++i) acc[d][i] = 0.0f;
     float m = real ? -__builtin_inff() : 0.0f, l = 0.0f;
     int v_exp = kLift + 1;
+    bool spoiled = false; /* this lane's row has seen a scale that is no number */
     if (steps > 0) {
         store_tile(0);
         __syncthreads();
@@ -957,9 +989,21 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attn_chu
     for (int step = 0; step < steps; ++step) {
         const bool more = step + 1 < steps;
         const bool look = step + 2 < steps;
+        const int t0 = t.begin + step * BN;
+        const bool cut = (t0 < t.all_lo) | (t0 + BN > t.all_hi) | (__builtin_amdgcn_readfirstlane(bad[step % 3]) != 0);
+        if constexpr (kCoded) {
+            if (cut & (__builtin_amdgcn_readfirstlane(exponents[step & 1]) > 255)) {
+                /* a scale that is no number, at a token that not every row sees: as in attn_rows_kernel */
+                float *of = scales + (step & 1) * 2 * BN + BN;
+#pragma unroll 1
+                for (int in = 0; in < BN; ++in) spoiled |= (t0 + in >= lo) & (t0 + in < hi) & !(of[in] < __builtin_inff());
+                __syncthreads();
+                if (tid < BN) of[tid] = of[tid] < __builtin_inff() ? of[tid] : 0.0f;
+                __syncthreads();
+            }
+        }
         if (more) load_tile(step + 1);
         const int entry = entry_of(look ? step + 2 : step);
-        const int t0 = t.begin + step * BN;
         const uint8_t *kt = smem + (step & 1) * 2 * C::kTile, *vt = kt + C::kTile;
         const float *sc = scales + (step & 1) * 2 * BN;
         f16v s[kHalves];
@@ -985,7 +1029,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attn_chu
 #pragma unroll
                 for (int i = 0; i < 4; ++i) s[c][4 * b + i] = fmaf(s[c][4 * b + i], x[i], -base);
             }
-        const bool cut = (t0 < t.all_lo) | (t0 + BN > t.all_hi) | (__builtin_amdgcn_readfirstlane(bad[step % 3]) != 0);
         if (cut) {
 #pragma unroll
             for (int c = 0; c < kHalves; ++c)
@@ -1022,7 +1065,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attn_chu
                 for (int i = 0; i < 16; ++i) s[c][i] -= rise;
         }
         if constexpr (kCoded) {
-            const int now = __builtin_amdgcn_readfirstlane(exponents[step & 1]);
+            const int now = __builtin_amdgcn_readfirstlane(exponents[step & 1]) & 255;
             if (now != v_exp) {
                 const float by = power_of_two(now - v_exp > 126 ? 1 : 127 - (now - v_exp));
 #pragma unroll
@@ -1040,13 +1083,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attn_chu
                 if constexpr (kCoded) x = *reinterpret_cast<const f4 *>(sc + BN + 32 * c + 8 * b + 4 * half);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float over = s[c][4 * b + i];
-                    w[i] = __builtin_amdgcn_exp2f(over);
+                    w[i] = __builtin_amdgcn_exp2f(s[c][4 * b + i]);
                     l += w[i];
-                    if constexpr (kCoded) {
-                        w[i] *= x[i];
-                        w[i] = (cut & (over == -__builtin_inff())) ? 0.0f : w[i];
-                    }
+                    if constexpr (kCoded) w[i] *= x[i];
                 }
                 p[c][2 * b] = kCoded ? pack_f16(w[0], w[1]) : kv_pack_bf16(w[0], w[1]);
                 p[c][2 * b + 1] = kCoded ? pack_f16(w[2], w[3]) : kv_pack_bf16(w[2], w[3]);
@@ -1121,7 +1160,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attn_chu
     /* a lane has values 32 d + 8 b + 4 half .. + 3 of its row; so does lane ^ 32 the four between */
     const float total = lane_sum32(l);
     if (!real) return;
-    float by = kCoded ? times_power(v_exp) : 1.0f;
+    float by = !kCoded ? 1.0f : spoiled ? __builtin_nanf("") : times_power(v_exp);
     float *partial = t.active > 1 ? partial_at<D, RM>(a, ((long long)item * a.kv.heads + head) * a.splits + split) : nullptr;
     if (partial) {
 #pragma unroll
