@@ -487,7 +487,8 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int at = t0 + 16 * c + 4 * g + i;
-                        vs[c][i] = !there[c] | (at < t.lo) | (at >= t.hi) ? 0.0f : vs[c][i];
+                        const bool none = !there[c] | (at < t.lo) | (at >= t.hi);
+                        vs[c][i] = none ? 0.0f : vs[c][i];
                         odd_scale = odd_scale | !(vs[c][i] < __builtin_inff());
                     }
                 if (__any(odd_scale)) {
@@ -803,7 +804,10 @@ struct Chunk {
     /* LDS: [2]{K, V}, then scales [2][2][BN], pages [3][BN], flags */
     static constexpr int kTile = BN * D * 2;
     static constexpr int kScales = 4 * kTile, kPages = kScales + (kCoded ? 4 * BN * 4 : 0);
-    static constexpr int kFlags = kPages + 3 * BN * 4, kBytes = kFlags + 32; /* bad[3], exponents[2] */
+    static constexpr int kFlags = kPages + 3 * BN * 4, kQueries = kFlags + 32; /* bad[3], exponents[2] */
+    /* the last steps' queries of a K product that stand in LDS, [step][half][row]: the registers of 8-bit
+     * codes on their way leave no room for all of 256 values */
+    static constexpr int kStored = kCoded && D == 256 ? 3 : 0, kBytes = kQueries + kStored * 2 * kRows * 16;
 };
 
 /* 16 bytes a lane from memory to LDS, lane after lane from `to` (the same on every lane). */
@@ -816,8 +820,9 @@ __device__ __forceinline__ void load_to_lds(const uint8_t *from, uint8_t *to) {
 __device__ __forceinline__ void wait_for_lds_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 /* Asks the scheduler for the LDS reads (READS for each of COUNT products) FAR products before their
- * use. 4096 rows over 16384 tokens, without and with FAR = 2: BF16 D = 256 1774 and 1661 us, D = 128 1024
- * and 997, D = 64 720 and 697; FP8 D = 256 2265 and 2469 (not taken there), D = 128 1241 and 1221. */
+ * use. 4096 rows over 16384 tokens, without and with FAR = 2: BF16 D = 128 1024 and 997 us, D = 64 720 and 697,
+ * FP8 D = 128 1241 and 1221; at D = 256, where the registers are for FAR = 1: BF16 1099 and 1086, FP8 1296 and
+ * 1259. */
 template <int COUNT, int READS, int FAR>
 __device__ __forceinline__ void interleave() {
     if constexpr (FAR > 0) {
@@ -831,12 +836,20 @@ __device__ __forceinline__ void interleave() {
     }
 }
 
-template <int D, int FMT>
-__global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attn_chunk_kernel(AttnArgs a) {
+/* Blocks of attn_chunk_kernel that a CU is to hold, without spilling: the waves of one multiply while those
+ * of another find their weights. TIGHT: addresses are worked out at every step, for one block more. At D =
+ * 256 that is two instead of one, and 4096 rows over 16384 tokens take BF16 1022 us instead of 1610, FP8
+ * 1260 instead of 2074. 64 values of 8 bits: four instead of three, INT8 856 instead of 917 us, but 624 tiles
+ * of ragged sequences, for which three have room, 85 instead of 78, so those go without (BF16 needs the
+ * registers, and gains nothing: 680 and 685). */
+constexpr int chunk_blocks(int dim, bool tight) { return dim > 64 ? 2 : tight ? 4 : 3; }
+
+template <int D, int FMT, bool TIGHT>
+__global__ __launch_bounds__(256, chunk_blocks(D, TIGHT)) void attn_chunk_kernel(AttnArgs a) {
     using C = Chunk<D, FMT>;
     constexpr bool kCoded = C::kCoded;
     constexpr int BN = C::BN, RM = C::kRows, kHalves = BN / 32, KS = D / 16, DB = D / 32;
-    constexpr int kFar = kCoded && D == 256 ? 0 : 2;
+    constexpr int kFar = D == 256 ? 1 : 2;
     extern __shared__ uint4 smem4[];
     uint8_t *smem = reinterpret_cast<uint8_t *>(smem4);
     float *scales = reinterpret_cast<float *>(smem + C::kScales); /* [buffer][k, v][BN] */
@@ -883,6 +896,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attn_chu
         return (unsigned long long)(uint32_t)(page >= 0 ? page : 0) * (a.kv.page_tokens * row) + inside(step, at) * row;
     };
     auto load_tile = [&](int step) {
+        int tid = threadIdx.x;
+        if constexpr (TIGHT) asm volatile("" : "+v"(tid)); /* or what follows from it is kept over the loop */
         const uint8_t *k = static_cast<const uint8_t *>(a.kv.k), *v = static_cast<const uint8_t *>(a.kv.v);
         if constexpr (kCoded) {
 #pragma unroll
@@ -912,6 +927,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attn_chu
     };
     auto store_tile = [&](int step) {
         if constexpr (kCoded) {
+            int tid = threadIdx.x;
+            if constexpr (TIGHT) asm volatile("" : "+v"(tid));
             uint8_t *k = smem + (step & 1) * 2 * C::kTile, *v = k + C::kTile;
 #pragma unroll
             for (int x = 0; x < C::kLoads; ++x) {
@@ -961,11 +978,14 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attn_chu
     const bool real = i_row < t.rows;
     const int place = t.length - t.news + token;
     const int hi = !real ? 0 : a.causal ? place + 1 : t.length, lo = t.window ? place - t.window + 1 : 0;
-    bf8 q[KS];
+    constexpr int kHeld = KS - C::kStored;
+    bf8 q[kHeld], *const q_stored = reinterpret_cast<bf8 *>(smem + C::kQueries) + half * RM + i_row;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
         const u4 x = *reinterpret_cast<const u4 *>(a.q + (t.first_row + (real ? token : 0)) * a.q_row + h * a.q_head + 16 * s + 8 * half);
-        q[s] = as_bf8(real ? x.x ^ a.flip : 0u, real ? x.y ^ a.flip : 0u, real ? x.z ^ a.flip : 0u, real ? x.w ^ a.flip : 0u);
+        const bf8 y = as_bf8(real ? x.x ^ a.flip : 0u, real ? x.y ^ a.flip : 0u, real ? x.z ^ a.flip : 0u, real ? x.w ^ a.flip : 0u);
+        if (s < kHeld) q[s < kHeld ? s : 0] = y;
+        else q_stored[(s - kHeld) * 2 * RM] = y;
     }
     f16v acc[DB];
 #pragma unroll
@@ -983,9 +1003,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attn_chu
     /* This lane's places in a tile of K: piece `half` of token n (that of step j, 2 j + half, is an XOR
      * away); and in one of V, for the transposing read: row (lane % 16) / 4 of four tokens, four of
      * 16 columns. */
-    const int k_at = n * 2 * D + ((half ^ (n & C::kSwizzle)) * 16);
+    int k_at = n * 2 * D + ((half ^ (n & C::kSwizzle)) * 16);
     const int v_row = 4 * half + ((lane >> 2) & 3), v_piece = 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
-    const int v_at = v_row * 2 * D + ((v_piece ^ ((2 * v_row) & C::kSwizzle)) * 16) + 8 * (lane & 1);
+    int v_at = v_row * 2 * D + ((v_piece ^ ((2 * v_row) & C::kSwizzle)) * 16) + 8 * (lane & 1);
     for (int step = 0; step < steps; ++step) {
         const bool more = step + 1 < steps;
         const bool look = step + 2 < steps;
@@ -1004,6 +1024,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attn_chu
         }
         if (more) load_tile(step + 1);
         const int entry = entry_of(look ? step + 2 : step);
+        if constexpr (TIGHT) asm volatile("" : "+v"(k_at), "+v"(v_at));
         const uint8_t *kt = smem + (step & 1) * 2 * C::kTile, *vt = kt + C::kTile;
         const float *sc = scales + (step & 1) * 2 * BN;
         f16v s[kHalves];
@@ -1014,7 +1035,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void attn_chu
 #pragma unroll
             for (int j = 0; j < KS; ++j) {
                 const bf8 k = *reinterpret_cast<const bf8 *>(kt + (k_at ^ (32 * j)) + 32 * c * 2 * D);
-                s[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, q[j], s[c], 0, 0, 0);
+                const bf8 y = j < kHeld ? q[j < kHeld ? j : 0] : q_stored[(j - kHeld) * 2 * RM];
+                s[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, y, s[c], 0, 0, 0);
             }
         }
         interleave<kHalves * KS, 1, kFar>();
@@ -1354,7 +1376,10 @@ template <int D, int FMT>
 void launch_format(const Plan &p, const AttnArgs &all, hipStream_t s) {
     if (p.many.items) {
         const AttnArgs a = part_args(all, p.many);
-        launch_k(attn_chunk_kernel<D, FMT>, dim3(a.kv.heads * a.items, a.splits), dim3(256), Chunk<D, FMT>::kBytes, s, a);
+        auto kernel = attn_chunk_kernel<D, FMT, D == 256>;
+        if constexpr (D == 64 && FMT != W4A16_KV_BF16)
+            if ((long long)a.kv.heads * a.items * a.splits > chunk_blocks(D, false) * device_cus()) kernel = attn_chunk_kernel<D, FMT, true>;
+        launch_k(kernel, dim3(a.kv.heads * a.items, a.splits), dim3(256), Chunk<D, FMT>::kBytes, s, a);
         launch_join<D, kChunkRows, false>(a.splits, a, s);
     }
     if (p.few.items) {

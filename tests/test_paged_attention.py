@@ -61,6 +61,8 @@ CASES = [
     ([70, 500], [3, 4], 4, 1, 256, 32, 37),           # windows that begin at every place of four tokens
     ([333, 90], [9, 2], 3, 1, 64, 8, 10),
     ([333, 90], [60, 2], 5, 1, 128, 8, 10),
+    ([3 + 37 * i % 300 for i in range(50)], [1 + i % 3 for i in range(50)], 528, 16, 64, 32, 0),   # more tiles than
+    ([3 + 37 * i % 300 for i in range(50)], [1 + i % 3 for i in range(50)], 528, 16, 64, 32, 70),  # there is room for
 ]
 
 
