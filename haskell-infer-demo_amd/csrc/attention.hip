@@ -322,8 +322,9 @@ __device__ __forceinline__ float over_power(int biased) { return power_of_two(25
 __device__ __forceinline__ float times_power(int biased) { return power_of_two(biased - kLift); }
 
 /* Blocks of attn_rows_kernel that a CU is to hold: as many as its registers allow without spilling.
- * More waves are what hides the latency of its loads: RT = 2, D = 128, FP8, 96 sequences' worth
- * of verify rows: 40.0 us at one block, 29.0 at two; D = 256, 2 x 100003 tokens: 107 and 82. */
+ * More waves are what hides the latency of its loads. At one block and at these (the join included): 48
+ * ragged sequences of up to 8192 tokens, D = 128, INT8, 129 and 93.5 us; 16 of 4096 with five rows each, FP8,
+ * RT = 2, 31.0 and 25.4; 64 of 8192, D = 256, FP8, 152 and 109, though 2 of 100003 take 91 and 94. */
 constexpr int rows_blocks(int dim, int format, int rt) {
     return dim == 256 ? (format == W4A16_KV_BF16 ? 1 : 2) : dim == 128 ? (rt == 1 ? 3 : 2) : rt == 1 ? 4 : 3;
 }
@@ -345,6 +346,10 @@ constexpr int rows_blocks(int dim, int format, int rt) {
  *
  * A BF16 cache's weights are rounded to BF16, half a step of 2^-8 each; those of an 8-bit cache to
  * FP16 (kLift), which also takes fewer instructions to widen INT8.
+ *
+ * Bound by memory: 32 sequences of 8192 tokens, one row of 32 heads each (16 of 256 values), the join included:
+ * BF16 D = 64 102 us (5.2 TB/s), D = 128 192 (5.6), D = 256 200 (5.4); FP8 66 (4.4), 108 (5.1), 107 (5.1); INT8
+ * 70, 110, 109.
  */
 template <int D, int FMT, int RT>
 __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel(AttnArgs a) {
@@ -793,6 +798,11 @@ __device__ __forceinline__ uint32_t widen_f16(uint32_t codes) {
  *
  * 16-byte pieces of a token's K are exchanged by its number (XOR), pairs of pieces of its V by
  * the same, so that the eight lanes of a step of a read fall on different banks.
+ *
+ * Every wave reads the whole tile, so the LDS reads of 32 rows take as long as their products; above
+ * that it is bound by the weights' VALU work (five instructions each, and for 8-bit caches the widening
+ * of a tile over 128 rows). 4096 rows over 16384 tokens, 32 heads (16 of 256 values): BF16 D = 64 671 us, 717
+ * TFLOP/s; D = 128 979, 983; D = 256 1017, 946; INT8 859, 1193, 1308; FP8 748, 1134, 1269.
  */
 template <int D, int FMT>
 struct Chunk {
@@ -1230,6 +1240,20 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     const int lane = threadIdx.x & 15, unit = threadIdx.x >> 4, sub = unit / kRows, i = blockIdx.y * kRows + unit % kRows;
     const int row = i < t.rows ? i : t.rows - 1;
     auto part_of = [&](int s) { return partial_at<D, RM>(a, (EVEN ? first_part : (long long)blockIdx.x * a.splits) + s); };
+    /* Of many parts the first ones' values are on their way beside the maxima: 64 parts of 256 values 8.6
+     * and 7.4 us; of few that costs more than it gives. */
+    constexpr int kFirst = SUB == 16 ? 2 : 0;
+    f4 x[kFirst + 1][kPer / 4];
+    float m[kFirst + 1], l[kFirst + 1];
+#pragma unroll
+    for (int k = 0; k < kFirst; ++k) {
+        const int s = sub + k * SUB;
+        const float *from = part_of(s < t.active ? s : 0), *ml = from + RM * D + 2 * row, *values = from + row * D + lane * kPer;
+        m[k] = ml[0];
+        l[k] = ml[1];
+#pragma unroll
+        for (int j = 0; j < kPer / 4; ++j) x[k][j] = *reinterpret_cast<const f4 *>(values + 4 * j);
+    }
     float top = -__builtin_inff();
     for (int s = lane; s < t.active; s += 16) top = fmaxf(top, part_of(s)[RM * D + 2 * row]);
 #pragma unroll
@@ -1238,8 +1262,16 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     float total = 0.0f, o[kPer];
 #pragma unroll
     for (int j = 0; j < kPer; ++j) o[j] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kFirst; ++k)
+        if (sub + k * SUB < t.active) {
+            const float f = __builtin_amdgcn_exp2f(m[k] - base);
+            total += f * l[k];
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) o[j] += f * x[k][j / 4][j % 4];
+        }
 #pragma unroll 4
-    for (int s = sub; s < t.active; s += SUB) {
+    for (int s = sub + kFirst * SUB; s < t.active; s += SUB) {
         const float *from = part_of(s), *ml = from + RM * D + 2 * row, *values = from + row * D + lane * kPer;
         const float f = __builtin_amdgcn_exp2f(ml[0] - base);
         total += f * ml[1];

@@ -11,7 +11,8 @@
  * drafts_draw_kernel: one block a sequence runs over the pieces' sums to the one in which the
  * running sum passes the drawn threshold, and through that piece alone. Bound by memory for many
  * sequences (two rows of the vocabulary each), by the two launches and their few dependent round
- * trips for few. FP64 sums put the threshold within 2^-52 of its exact place, so that the drawn
+ * trips for few: 64 sequences of 128257 words 17.2 us (66 MB, 3.8 TB/s), one of 151936 7.6 in a
+ * graph. FP64 sums put the threshold within 2^-52 of its exact place, so that the drawn
  * index does not hang on the order in which a vocabulary's many small weights are added.
  */
 #include "launch.h"
