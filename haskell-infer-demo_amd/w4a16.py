@@ -9,6 +9,9 @@ This module mirrors the reference's operator interface for the path:
   csrc/kernels/silu.cu:78-95.
 * ``mlp_int4`` - the INT4 branch of ``mlp_from_normed`` (reference csrc/kernels/layers.cu:126-145).
 * ``test_gemm_int4`` - the reference bridge symbol (tests/kernels/kernel_bridge.cu:83-95).
+* ``KvCache``, ``KvBatch``, ``paged_attention``, ``verify_drafts`` - a paged KV cache, attention over
+  it and the verification of drafted tokens, around the FFN in a decode or verify step (no
+  counterpart in the reference's C interface).
 
 Device tensors are torch CUDA tensors (on ROCm, HIP memory); torch is used only for device memory
 and streams. There is no CPU fallback: if the library is missing the import fails.
