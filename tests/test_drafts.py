@@ -44,6 +44,26 @@ def test_against_the_definition(cuda, seqs, steps, vocab, drawn):
         same(cuda, target, draft, tokens, lens, uniforms)
 
 
+@pytest.mark.parametrize("drawn", [True, False])
+@pytest.mark.parametrize("vocab", [300, 10000, 20000])
+def test_many_taken(cuda, vocab, drawn):
+    """More drafted tokens than a wave has lanes, of which 0, 63, 64, 65, 128, 149 and all are taken."""
+    taken, steps = [0, 63, 64, 65, 128, 149, 150], 150
+    gen = torch.Generator().manual_seed(7)
+    target = torch.rand(len(taken), steps + 1, vocab, generator=gen) / vocab
+    draft = torch.rand(len(taken), steps, vocab, generator=gen) / vocab
+    tokens = torch.randint(0, vocab, (len(taken), steps), generator=gen).to(torch.int32)
+    uniforms = torch.rand(len(taken), steps + 1, generator=gen)
+    at = tokens.long()[..., None]
+    target[:, :steps].scatter_(2, at, 1.0)
+    draft.scatter_(2, at, 0.5)
+    for s, n in enumerate(taken):
+        if n < steps:
+            target[s, n, tokens[s, n]] = 0.0
+    accepted, _ = same(cuda, target, draft if drawn else None, tokens, None, uniforms)
+    assert accepted.tolist() == taken
+
+
 def test_borders(cuda):
     """Exact ties: dyadic weights whose sums are exact in any order. The threshold is passed, not reached; a uniform of 0
     takes the first token that weighs anything; a product equal to the target's probability refuses."""
