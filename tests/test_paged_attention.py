@@ -63,6 +63,10 @@ CASES = [
     ([333, 90], [60, 2], 5, 1, 128, 8, 10),
     ([3 + 37 * i % 300 for i in range(50)], [1 + i % 3 for i in range(50)], 528, 16, 64, 32, 0),   # more tiles than
     ([3 + 37 * i % 300 for i in range(50)], [1 + i % 3 for i in range(50)], 528, 16, 64, 32, 70),  # there is room for
+    ([500, 40, 700, 16], [16, 9, 16, 16], 8, 2, 64, 16, 0),   # 64 rows
+    ([500, 40, 700, 16], [16, 9, 13, 16], 8, 2, 128, 16, 75),
+    ([5000, 3000], [16, 12], 8, 2, 128, 64, 0),
+    ([4100], [21], 6, 2, 64, 32, 3500),
 ]
 
 
@@ -139,7 +143,7 @@ def test_rows_that_see_nothing(cuda, fmt, many):
 
 @pytest.mark.parametrize("fmt", ["bf16", "int8", "fp8"])
 @pytest.mark.parametrize("dim", [64, 128, 256])
-@pytest.mark.parametrize("news,window", [([6], 0), ([6], 20), ([100], 0), ([100], 20)])
+@pytest.mark.parametrize("news,window", [([6], 0), ([6], 20), ([20], 0), ([20], 20), ([100], 0), ([100], 20)])
 def test_nonfinite_values_stay_with_the_rows_that_see_them(cuda, fmt, news, window, dim):
     """Keys and values with infinities and NaN behind the last token, outside the window and at later positions change
     nothing; a row that sees one is not a number where the value is not."""
