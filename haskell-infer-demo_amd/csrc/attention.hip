@@ -816,8 +816,8 @@ struct Chunk {
     static constexpr int kScales = 4 * kTile, kPages = kScales + (kCoded ? 4 * BN * 4 : 0);
     static constexpr int kFlags = kPages + 3 * BN * 4, kQueries = kFlags + 32; /* bad[3], exponents[2] */
     /* the last steps' queries of a K product that stand in LDS, [step][half][row]: the registers of 8-bit
-     * codes on their way leave no room for all of 256 values */
-    static constexpr int kStored = kCoded && D == 256 ? 3 : 0, kBytes = kQueries + kStored * 2 * kRows * 16;
+     * codes on their way leave no room for all of 256 values, or of 64 where four blocks are to fit */
+    static constexpr int kStored = !kCoded ? 0 : D == 256 ? 3 : D == 64 ? 1 : 0, kBytes = kQueries + kStored * 2 * kRows * 16;
 };
 
 /* 16 bytes a lane from memory to LDS, lane after lane from `to` (the same on every lane). */
@@ -988,7 +988,8 @@ __global__ __launch_bounds__(256, chunk_blocks(D, TIGHT)) void attn_chunk_kernel
     const bool real = i_row < t.rows;
     const int place = t.length - t.news + token;
     const int hi = !real ? 0 : a.causal ? place + 1 : t.length, lo = t.window ? place - t.window + 1 : 0;
-    constexpr int kHeld = KS - C::kStored;
+    const uint32_t seen = hi > lo ? hi - lo : 0; /* this row sees a key where its place less lo, unsigned, is below this */
+    constexpr int kHeld = KS - (TIGHT ? C::kStored : 0);
     bf8 q[kHeld], *const q_stored = reinterpret_cast<bf8 *>(smem + C::kQueries) + half * RM + i_row;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
@@ -1026,7 +1027,7 @@ __global__ __launch_bounds__(256, chunk_blocks(D, TIGHT)) void attn_chunk_kernel
                 /* a scale that is no number, at a token that not every row sees: as in attn_rows_kernel */
                 float *of = scales + (step & 1) * 2 * BN + BN;
 #pragma unroll 1
-                for (int in = 0; in < BN; ++in) spoiled |= (t0 + in >= lo) & (t0 + in < hi) & !(of[in] < __builtin_inff());
+                for (int in = 0; in < BN; ++in) spoiled |= ((uint32_t)(t0 + in - lo) < seen) & !(of[in] < __builtin_inff());
                 __syncthreads();
                 if (tid < BN) of[tid] = of[tid] < __builtin_inff() ? of[tid] : 0.0f;
                 __syncthreads();
@@ -1062,6 +1063,7 @@ __global__ __launch_bounds__(256, chunk_blocks(D, TIGHT)) void attn_chunk_kernel
                 for (int i = 0; i < 4; ++i) s[c][4 * b + i] = fmaf(s[c][4 * b + i], x[i], -base);
             }
         if (cut) {
+            const uint32_t at = t0 - lo;
 #pragma unroll
             for (int c = 0; c < kHalves; ++c)
 #pragma unroll
@@ -1071,7 +1073,7 @@ __global__ __launch_bounds__(256, chunk_blocks(D, TIGHT)) void attn_chunk_kernel
                     const int each[4] = {page.x, page.y, page.z, page.w};
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const bool hidden = (t0 + in + i < lo) | (t0 + in + i >= hi) | (each[i] < 0);
+                        const bool hidden = ((at + in + i) | (each[i] & 0x80000000u)) >= seen; /* a page of -1 as well */
                         s[c][4 * b + i] = hidden ? -__builtin_inff() : s[c][4 * b + i];
                     }
                 }
@@ -1136,7 +1138,7 @@ __global__ __launch_bounds__(256, chunk_blocks(D, TIGHT)) void attn_chunk_kernel
                 }
                 if (__syncthreads_or(odd)) {
                     for (int in = 0; in < BN; ++in) {
-                        const bool sees = t0 + in >= lo && t0 + in < hi;
+                        const bool sees = (uint32_t)(t0 + in - lo) < seen;
 #pragma unroll
                         for (int d = 0; d < DB; ++d)
 #pragma unroll
