@@ -273,6 +273,27 @@ def test_on_a_stream_of_its_own(cuda):
     assert torch.equal(got, want) and torch.equal(explicit, want)
 
 
+@pytest.mark.parametrize("fmt", ["bf16", "int8"])
+@pytest.mark.parametrize("news", [[1, 2, 1], [50, 2, 70]])
+def test_shared_pages(cuda, fmt, news):
+    """Sequences that begin with the same pages, and one that holds a page twice, as against copies of the pages."""
+    page, heads, dim = 16, 2, 128
+    table = [[3, 1, 4, 5, 9], [3, 1, 4, 2, 6], [3, 3, 7, 8, 0]]
+    flat = torch.tensor(table).flatten()
+    cache = filled(10, page, heads, dim, fmt, cuda, seed=2)
+    apart = w4a16.KvCache.empty(15, page, heads, dim, fmt, device=cuda)
+    for name in ("k", "v", "k_scale", "v_scale"):
+        if getattr(cache, name) is not None:
+            bits = [getattr(c, name).view(torch.int16 if fmt == "bf16" else getattr(c, name).dtype) for c in (apart, cache)]
+            bits[0].copy_(bits[1][flat.to(cuda)])
+    lens = torch.tensor([78, 70, 80], dtype=torch.int32, device=cuda)
+    starts = torch.tensor([0, news[0], news[0] + news[1], sum(news)], dtype=torch.int32, device=cuda)
+    q = torch.randn(sum(news), 4, dim, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16).to(cuda)
+    out = [w4a16.paged_attention(q, c, w4a16.KvBatch(t.to(torch.int32).to(cuda), lens, starts, sum(news)))
+           for c, t in ((cache, torch.tensor(table)), (apart, torch.arange(15).reshape(3, 5)))]
+    assert torch.equal(out[0], out[1])
+
+
 @pytest.mark.parametrize("raw", [False, True])
 def test_memory_of_a_call_on_another_stream(cuda, raw):
     """What a call allocates for a stream that is not the current one, and lets go of when it returns, is not given to
