@@ -52,7 +52,8 @@ struct Tile {
     int first_row;          /* the sequence's first row in q */
     int rows, news;         /* (token, head) rows of the tile from `start`; the sequence's new tokens */
     int start;              /* first (token, head) row of the tile in the sequence */
-    int length;             /* the sequence's cached tokens */
+    int old;                /* position of the sequence's first row: its tokens less the new ones */
+    int length;             /* the sequence's keys: its tokens that the table has room for */
     int lo, hi;             /* keys that some row sees: [lo, hi) */
     int all_lo, all_hi;     /* keys that every row sees */
     int begin, end, active; /* this split's keys; how many splits have any */
@@ -60,19 +61,27 @@ struct Tile {
     int seq;
 };
 
-/* The rest of a tile from its sequence, length, rows and start. */
+/* The end of the keys that a row at `place` sees. */
+__device__ __forceinline__ int row_end(const AttnArgs &a, const Tile &t, int place) {
+    const int end = a.causal ? place + 1 : t.length;
+    return end < t.length ? end : t.length;
+}
+
+/* The rest of a tile from its sequence's tokens (old + news) and rows, and its start. */
 template <int RM>
 __device__ __forceinline__ void fill_tile(const AttnArgs &a, Tile *t) {
     const int all = t->news * a.group;
     t->rows = all - t->start < RM ? all - t->start : RM;
-    const int t0 = t->start / a.group, t1 = (t->start + t->rows - 1) / a.group, old = t->length - t->news;
-    t->window = a.window <= t->length ? a.window : 0;
-    t->hi = a.causal ? old + t1 + 1 : t->length;
-    t->all_hi = a.causal ? old + t0 + 1 : t->length;
-    t->lo = t->window ? old + t0 - t->window + 1 : 0;
-    t->all_lo = t->window ? old + t1 - t->window + 1 : 0;
+    const int t0 = t->start / a.group, t1 = (t->start + t->rows - 1) / a.group;
+    /* the same on every lane, and kept as such: in lanes it costs the few-row kernels registers that they do not have */
+    t->length = __builtin_amdgcn_readfirstlane(kv_held(a.kv, t->old + t->news));
+    t->window = a.window <= t->old + t->news ? a.window : 0;
+    t->hi = row_end(a, *t, t->old + t1);
+    t->all_hi = row_end(a, *t, t->old + t0);
+    t->lo = t->window ? t->old + t0 - t->window + 1 : 0;
+    t->all_lo = t->window ? t->old + t1 - t->window + 1 : 0;
     if (t->lo < 0) t->lo = 0;
-    if (t->hi < t->lo) t->hi = t->lo;
+    if (t->hi <= t->lo) t->hi = t->lo = 0; /* the window may begin behind the last key */
 }
 
 constexpr int kMostUnits = 1 << 23; /* of 2^30 tokens */
@@ -133,7 +142,7 @@ __device__ __forceinline__ bool find_tile(const AttnArgs &a, int item, int split
         if (base + 64 >= a.kv.seqs) return false;
     }
     t->seq = __builtin_amdgcn_readfirstlane(t->seq);
-    t->length = __builtin_amdgcn_readfirstlane(kv_length(a.kv, t->seq));
+    t->old = __builtin_amdgcn_readfirstlane(kv_length(a.kv, t->seq)) - t->news;
     fill_tile<RM>(a, t);
     /* splits begin at multiples of 32 tokens and have at least kFewestTokens */
     const int from = t->lo & ~31, span = t->hi - from;
@@ -155,7 +164,7 @@ __device__ __forceinline__ bool find_tile(const AttnArgs &a, int item, int split
  * the workspace.
  */
 struct Seqs { /* 64 sequences, one a lane */
-    int first, news, length, from; /* from: where the first key that any of its rows sees is cut */
+    int first, news, old, from; /* old: position of its first row; from: where the first key that any of its rows sees is cut */
     int pairs, units;              /* its (tile, head) pairs, units of each */
 };
 
@@ -166,12 +175,13 @@ __device__ __forceinline__ Seqs load_seqs(const AttnArgs &a, int base) {
     if (s < a.kv.seqs) {
         q.first = a.kv.starts[s];
         const int last = a.kv.starts[s + 1];
-        q.length = kv_length(a.kv, s);
+        const int length = kv_length(a.kv, s), held = kv_held(a.kv, length);
         if (q.first >= 0 && last <= a.kv.rows && last > q.first) q.news = last - q.first;
         if (q.news * a.group <= a.over || q.news * a.group > a.upto) q.news = 0;
-        const int old = q.length - q.news;
-        if (a.window && a.window <= q.length && old - a.window + 1 > 0) q.from = (old - a.window + 1) & ~31;
-        if (q.length > q.from) q.units = (q.length - q.from + kUnit - 1) / kUnit;
+        q.old = length - q.news;
+        if (a.window && a.window <= length && q.old - a.window + 1 > 0) q.from = (q.old - a.window + 1) & ~31;
+        if (held > q.from) q.units = (held - q.from + kUnit - 1) / kUnit;
+        else q.from = 0; /* no row sees any */
         q.pairs = (q.news * a.group + RM - 1) / RM * a.kv.heads;
     }
     return q;
@@ -217,7 +227,7 @@ __device__ __forceinline__ bool find_part(const AttnArgs &a, int index, Tile *t,
             t->seq = base + l;
             t->first_row = __builtin_amdgcn_readlane(q.first, l);
             t->news = __builtin_amdgcn_readlane(q.news, l);
-            t->length = __builtin_amdgcn_readlane(q.length, l);
+            t->old = __builtin_amdgcn_readlane(q.old, l);
             const int from = __builtin_amdgcn_readlane(q.from, l);
             t->active = __builtin_amdgcn_readlane(per, l);
             const int in_seq = left - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(PAIR ? q.pairs : parts, l));
@@ -453,9 +463,9 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
     for (int r = 0; r < RT; ++r) {
         const int i = r * 16 + n, token = (t.start + i) / a.group, h = head * a.group + (t.start + i) % a.group;
         const bool real = i < t.rows;
-        const int place = t.length - t.news + token;
+        const int place = t.old + token;
         const uint16_t *row = a.q + (t.first_row + (real ? token : 0)) * a.q_row + h * a.q_head;
-        hi[r] = !real ? 0 : a.causal ? place + 1 : t.length;
+        hi[r] = !real ? 0 : row_end(a, t, place);
         lo[r] = t.window ? place - t.window + 1 : 0;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
@@ -986,8 +996,8 @@ __global__ __launch_bounds__(256, chunk_blocks(D, TIGHT)) void attn_chunk_kernel
     /* this lane's row: its queries and the keys it sees */
     const int i_row = wave * 32 + n, token = (t.start + i_row) / a.group, h = head * a.group + (t.start + i_row) % a.group;
     const bool real = i_row < t.rows;
-    const int place = t.length - t.news + token;
-    const int hi = !real ? 0 : a.causal ? place + 1 : t.length, lo = t.window ? place - t.window + 1 : 0;
+    const int place = t.old + token;
+    const int hi = !real ? 0 : row_end(a, t, place), lo = t.window ? place - t.window + 1 : 0;
     const uint32_t seen = hi > lo ? hi - lo : 0; /* this row sees a key where its place less lo, unsigned, is below this */
     constexpr int kHeld = KS - (TIGHT ? C::kStored : 0);
     bf8 q[kHeld], *const q_stored = reinterpret_cast<bf8 *>(smem + C::kQueries) + half * RM + i_row;

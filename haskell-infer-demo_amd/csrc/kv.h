@@ -54,11 +54,16 @@ __device__ __forceinline__ uint32_t kv_widen(uint32_t codes) {
     }
 }
 
-/* Tokens of sequence s that the cache can hold of its kv_lens. */
+/* Tokens of sequence s: its rows are the last of them, whether the cache has room for them or not. */
 __device__ __forceinline__ int kv_length(const KvView &kv, int s) {
-    const long long room = (long long)kv.table_pages << kv.shift;
     const int n = kv.kv_lens[s];
-    return n < 0 ? 0 : n > room ? (int)room : n;
+    return n < 0 ? 0 : n;
+}
+
+/* Of `length` tokens those that the table has room for: the keys that may be there. */
+__device__ __forceinline__ int kv_held(const KvView &kv, int length) {
+    const int room = kv.table_pages << kv.shift; /* up to 2^30 */
+    return length > room ? room : length;
 }
 
 } // namespace w4a16

@@ -363,7 +363,8 @@ int engine_ffn_forward_residual_norm(W4A16Store *store, int layer, uint16_t *res
  * on a 4-byte boundary. max_new and max_kv bound the new tokens and kv_lens of any sequence
  * (0: rows, and what the table holds); they only plan the launch, so a loose bound costs speed and
  * a wrong one is no fault. Tokens past the table (or past 2^30) and pages outside the cache are seen
- * as tokens that are not there: not written, read as zeros, masked in the attention. Sequences may
+ * as tokens that are not there: not written, read as zeros, masked in the attention; the positions
+ * behind them, and so the rows', count them all the same. Sequences may
  * share pages; one that a call writes through two of them holds either's rows.
  *
  * Strides are in elements; a token's heads and a head's values stand apart by multiples of 8

@@ -17,6 +17,22 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs an MI355X (runs the HIP library on cuda:0)")
 
 
+# Tests that hold a wrong value: what it is, and where the right one is tested.
+HOLD_WRONG_VALUES = {
+    "test_paged_attention.py::test_rows_that_see_nothing":
+        "places the rows of a sequence whose kv_lens pass its table by the table's end (kv_lens 40 of 32 places: 29 to 31 for "
+        "three rows) where the interface, the write and the read have them at kv_lens (37 to 39): "
+        "test_lengths_past_the_table.py has the right places, and everything else that this test looks at",
+}
+
+
+def pytest_collection_modifyitems(items):
+    for item in items:
+        for name, why in HOLD_WRONG_VALUES.items():
+            if f"{item.path.name}::{getattr(item, 'originalname', item.name)}" == name:
+                item.add_marker(pytest.mark.xfail(reason=why, strict=True))
+
+
 @pytest.fixture(scope="session")
 def cuda():
     import torch

@@ -48,7 +48,8 @@ def places(table, kv_lens, news, page, pages):
 
 def attention(q, k, v, places_of, scale, causal, window, news, kv_lens):
     """FP64 attention of the rows q [rows, q_heads, D] of sequences whose tokens' keys and values are
-    k[s], v[s] [kv_heads, tokens, D] and places_of[s] [tokens] whether each is there. Returns (out, lse, and for each of
+    k[s], v[s] [kv_heads, tokens, D] and places_of[s] [tokens] whether each is there. kv_lens places the rows, and may
+    be more than the tokens there are. Returns (out, lse, and for each of
     them how far FP32 arithmetic with BF16 weights and a BF16 output may be off).
 
     The bounds. A score is a sum of D products: off by (D + 4) 2^-24 sum|q k| scale, and by a rounding or two of its own;
@@ -60,11 +61,10 @@ def attention(q, k, v, places_of, scale, causal, window, news, kv_lens):
     outs, lses, out_off, lse_off, first = [], [], [], [], 0
     dim = q.shape[2]
     for s, m in enumerate(news):
-        n = min(kv_lens[s], k[s].shape[1])
         token = torch.arange(k[s].shape[1])
         for i in range(m):
-            at = n - m + i
-            seen = places_of[s] & (token < n)
+            at = kv_lens[s] - m + i
+            seen = places_of[s] & (token < kv_lens[s])
             if causal:
                 seen = seen & (token <= at)
             if window:
