@@ -705,6 +705,14 @@ def _rows3(t, shape, device, what):
     _refuse(f"{what}: the last axis is strided")
 
 
+def _rows3_dense(t, shape, device, what):
+    """Address of a contiguous tensor that _rows3 takes."""
+    address = _rows3(t, shape, device, what)[0]
+    if not t.is_contiguous():
+        _refuse(f"{what}: tensor is not contiguous")
+    return address
+
+
 class KvCache:
     """A paged cache over tensors of the caller: k, v [pages, kv_heads, page_size, head_dim] of
     torch.bfloat16, int8 or float8_e4m3fn, with FP32 scales [pages, kv_heads, page_size] for the
@@ -757,7 +765,7 @@ class KvCache:
 
     def read(self, batch, out=None, stream=None):
         """The batch's rows out of the cache: (k, v) as BF16 [rows, kv_heads, head_dim]. Without
-        `out` rows of no sequence are zeros; with it they are left as they were."""
+        `out` rows of no sequence are zeros; with it (two such tensors, contiguous) they are left as they were."""
         import torch
 
         if stream is not None and out is None:
@@ -773,7 +781,7 @@ class KvCache:
             k = both.data_ptr()
             v = k + size
         else:
-            k, v = (_dev(t, size, 2, "KvCache.read out", self.device) for t in out)
+            k, v = (_rows3_dense(t, (batch.rows, self.kv_heads, self.head_dim), self.device, "KvCache.read out") for t in out)
         _check(lib.w4a16_kv_read_bf16(self._ref, batch._ref, k, v, _raw_stream(stream, index)), "KvCache.read")
         return out
 
