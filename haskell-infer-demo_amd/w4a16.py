@@ -730,8 +730,8 @@ class KvCache:
         size = k.numel() * k.element_size()
         scales = [None, None]
         if formats[k.dtype]:
-            if any(s is None or s.dtype != torch.float32 for s in (k_scale, v_scale)):
-                _refuse("KvCache: an 8-bit cache has FP32 scales for keys and values")
+            if any(s is None or s.dtype != torch.float32 or s.shape != k.shape[:3] for s in (k_scale, v_scale)):
+                _refuse(f"KvCache: an 8-bit cache has FP32 scales {tuple(k.shape[:3])} for keys and values")
             scales = [_dev(s, k.numel() // self.head_dim * 4, 4, "KvCache scales", k.device) for s in (k_scale, v_scale)]
         self._c = _KvCacheStruct(_dev(k, size, k.element_size(), "KvCache k"),
                                  _dev(v, size, v.element_size(), "KvCache v", k.device), scales[0], scales[1],
