@@ -251,8 +251,11 @@ extern "C" int w4a16_kv_write_bf16(const W4A16KvCache *cache, const W4A16KvBatch
     for (const void *dst : {(const void *)kv.k_scale, (const void *)kv.v_scale})
         if (overlap(dst, sb, k, kb) || overlap(dst, sb, v, vb))
             return set_error(W4A16_ERR_CONFIG, "%s: the rows overlap the cache's scales", what);
-    if (overlap(cache->k, cb, cache->v, cb))
-        return set_error(W4A16_ERR_CONFIG, "%s: the cache's keys and values overlap", what);
+    const struct { const void *p; size_t n; } parts[] = {{cache->k, cb}, {cache->v, cb}, {kv.k_scale, sb}, {kv.v_scale, sb}};
+    for (int i = 0; i < 4; ++i)
+        for (int j = 0; j < i; ++j)
+            if (overlap(parts[i].p, parts[i].n, parts[j].p, parts[j].n))
+                return set_error(W4A16_ERR_CONFIG, "%s: the cache's keys, values and scales overlap", what);
     hipStream_t s = static_cast<hipStream_t>(stream);
     auto launch = cache->head_dim == 64 ? launch_write<64> : cache->head_dim == 128 ? launch_write<128> : launch_write<256>;
     launch(cache->format, kv, k, k_row_stride, k_head_stride, v, v_row_stride, v_head_stride, s);
