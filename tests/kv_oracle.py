@@ -46,17 +46,25 @@ def places(table, kv_lens, news, page, pages):
     return out
 
 
-def attention(q, k, v, places_of, scale, causal, window, news, kv_lens):
+def attention(q, k, v, places_of, scale, causal, window, news, kv_lens, coded=None):
     """FP64 attention of the rows q [rows, q_heads, D] of sequences whose tokens' keys and values are
     k[s], v[s] [kv_heads, tokens, D] and places_of[s] [tokens] whether each is there. kv_lens places the rows, and may
     be more than the tokens there are. Returns (out, lse, and for each of
-    them how far FP32 arithmetic with BF16 weights and a BF16 output may be off).
+    them how far FP32 arithmetic with BF16 weights and a BF16 output may be off). `coded`: of an 8-bit cache, whose weights are
+    FP16, the sizes of each sequence's V codes [kv_heads, tokens, D] and of their scales [kv_heads, tokens].
 
     The bounds. A score is a sum of D products: off by (D + 4) 2^-24 sum|q k| scale, and by a rounding or two of its own;
     a weight exp(s - m) by as much relatively, and 2^-21 for the exponential; both a weight and the sum of weights can
     be off by that, so an output by twice that of sum p|v|. Weights are rounded to BF16 (half a step, 2^-8, of
-    sum p|v|), the output once more (2^-8 of itself); sums of n terms add n 2^-24."""
-    half = torch.finfo(torch.bfloat16).eps / 2
+    sum p|v|), the output once more (2^-8 of itself); sums of n terms add n 2^-24.
+
+    FP16 weights carry V's scales: what is rounded is exp(s - m) scale 2^6 / 2^e, where m is no more than the row's maximum
+    and 2^e no more than the largest scale of the sequence's tokens for that head, 2^-120 at least (or the kernel's tile
+    has not come across it yet, and both are less). Half a step of FP16 is 2^-11 of the value, or 2^-25 under 2^-14. The
+    first is 2^-11 of sum p|v|. The second, less 2^6 / 2^e, is 2^-31 2^e of an exp(s - m); over the sum of weights
+    exp(m) is at most the largest weight p: 2^-31 max p, max scale for each |code|."""
+    bf16 = torch.finfo(torch.bfloat16).eps / 2
+    half = bf16 if coded is None else torch.finfo(torch.float16).eps / 2
     group = q.shape[1] // k[0].shape[0]
     outs, lses, out_off, lse_off, first = [], [], [], [], 0
     dim = q.shape[2]
@@ -86,8 +94,13 @@ def attention(q, k, v, places_of, scale, causal, window, news, kv_lens):
             out = torch.matmul(p, vals)
             weight = torch.matmul(p, vals.abs())
             rel = 2 * (score_off + 2.0**-21) + (keys.shape[1] + 16) * 2.0**-24
+            least = 0.0
+            if coded is not None:
+                codes, scales = coded[s]
+                most = scales[:, places_of[s]].amax(-1).clamp(min=2.0**-120)
+                least = 2.0**-31 * p.amax(-1)[..., None] * most[:, None, None] * codes[:, seen].sum(1)[:, None]
             outs.append(out.reshape(-1, dim))
-            out_off.append((weight * (half + rel[..., None]) * (1 + half) + out.abs() * half).reshape(-1, dim))
+            out_off.append(((weight * (half + rel[..., None]) + least) * (1 + bf16) + out.abs() * bf16).reshape(-1, dim))
             lses.append(lse.reshape(-1))
             lse_off.append((score_off + 2.0**-20 + (keys.shape[1] + 16) * 2.0**-24
                             + (lse.abs() + score.abs().amax(-1)) * 2.0**-22).reshape(-1))

@@ -7,7 +7,7 @@ import torch
 import kv_oracle
 import w4a16
 from test_kv_cache import filled
-from test_paged_attention import check
+from kv_check import check
 
 pytestmark = pytest.mark.gpu
 
