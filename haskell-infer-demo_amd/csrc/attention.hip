@@ -504,7 +504,7 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
                         const int at = t0 + 16 * c + 4 * g + i;
                         const bool none = !there[c] | (at < t.lo) | (at >= t.hi);
                         vs[c][i] = none ? 0.0f : vs[c][i];
-                        odd_scale = odd_scale | !(vs[c][i] < __builtin_inff());
+                        odd_scale = odd_scale | !(fabsf(vs[c][i]) < __builtin_inff());
                     }
                 if (__any(odd_scale)) {
                     /* a scale that is no number, at a token that not every row sees: 0 times it would
@@ -517,14 +517,14 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
                                 const int at = t0 + 16 * c + 4 * g + i;
-                                const bool sees = (at >= lo[r]) & (at < hi[r]) & !(vs[c][i] < __builtin_inff());
+                                const bool sees = (at >= lo[r]) & (at < hi[r]) & !(fabsf(vs[c][i]) < __builtin_inff());
                                 spoiled[r] = sees ? 1.0f : spoiled[r];
                             }
                     }
 #pragma unroll
                     for (int c = 0; c < 2; ++c)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) vs[c][i] = vs[c][i] < __builtin_inff() ? vs[c][i] : 0.0f;
+                        for (int i = 0; i < 4; ++i) vs[c][i] = fabsf(vs[c][i]) < __builtin_inff() ? vs[c][i] : 0.0f;
                 }
             }
         if constexpr (!kAhead)
@@ -585,12 +585,12 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
             odd = __any(odd);
         }
         if constexpr (kCoded) {
-            /* the scales are positive, or not numbers: those are no measure of the others */
+            /* the largest scale's size; infinities and NaN are no measure of the others */
             float most = 0.0f;
 #pragma unroll
             for (int c = 0; c < 2; ++c)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) most = fmaxf(most, vs[c][i] < __builtin_inff() ? vs[c][i] : 0.0f);
+                for (int i = 0; i < 4; ++i) most = fmaxf(most, fabsf(vs[c][i]) < __builtin_inff() ? fabsf(vs[c][i]) : 0.0f);
             most = lane_max32(lane_max16(most));
             int exp = (int)(__builtin_bit_cast(uint32_t, most) >> 23);
             exp = __builtin_amdgcn_readfirstlane(exp > 253 ? 1 : exp);
@@ -970,11 +970,11 @@ __global__ __launch_bounds__(256, chunk_blocks(D, TIGHT)) void attn_chunk_kernel
              * no measure of the others. */
             scale_r = !scale_there ? 0.0f : tid % (2 * BN) < BN ? scale_r * a.scale : scale_r;
             if (wave == BN / 64) {
-                const int e = (int)(__builtin_bit_cast(uint32_t, scale_r) >> 23);
+                const int e = (int)(__builtin_bit_cast(uint32_t, scale_r) >> 23) & 255;
                 const int most = wave_most(tid >= BN && e <= 253 ? e : 0);
                 v_run = most > v_run ? most : v_run;
                 if (tid >= BN) scale_r *= over_power(v_run);
-                const bool odd = __any((tid >= BN) & ((e & 255) == 255));
+                const bool odd = __any((tid >= BN) & (e == 255));
                 if (lane == 0) exponents[step & 1] = v_run + (odd ? 256 : 0);
             }
             if (tid < 2 * BN) scales[(step & 1) * 2 * BN + tid] = scale_r;
@@ -1037,9 +1037,9 @@ __global__ __launch_bounds__(256, chunk_blocks(D, TIGHT)) void attn_chunk_kernel
                 /* a scale that is no number, at a token that not every row sees: as in attn_rows_kernel */
                 float *of = scales + (step & 1) * 2 * BN + BN;
 #pragma unroll 1
-                for (int in = 0; in < BN; ++in) spoiled |= ((uint32_t)(t0 + in - lo) < seen) & !(of[in] < __builtin_inff());
+                for (int in = 0; in < BN; ++in) spoiled |= ((uint32_t)(t0 + in - lo) < seen) & !(fabsf(of[in]) < __builtin_inff());
                 __syncthreads();
-                if (tid < BN) of[tid] = of[tid] < __builtin_inff() ? of[tid] : 0.0f;
+                if (tid < BN) of[tid] = fabsf(of[tid]) < __builtin_inff() ? of[tid] : 0.0f;
                 __syncthreads();
             }
         }

@@ -351,7 +351,8 @@ int engine_ffn_forward_residual_norm(W4A16Store *store, int layer, uint16_t *res
  *   product rounded to FP32;
  * a row with a < 2^-117 is held as zeros (scale 0), one with an infinity or a NaN as zero codes
  * with a NaN scale: it reads back as NaN, and in the attention spoils the rows that see it and no
- * others. Codes are finite; a caller that writes NaN codes of its own (FP8 0x7F, 0xFF) spoils the
+ * others. Scales that a caller fills in itself may be of either sign; infinite ones spoil as NaN
+ * does. Codes are finite; a caller that writes NaN codes of its own (FP8 0x7F, 0xFF) spoils the
  * rows beside those that see them too.
  *
  * The batch. page_table[s * table_stride + i] is the page of tokens i * page_size .. of sequence
