@@ -1485,6 +1485,8 @@ extern "C" int w4a16_paged_attention_bf16(const W4A16KvCache *cache, const W4A16
     if (misaligned(q) || misaligned(out) || misaligned(ws) || ((uintptr_t)lse & 3))
         return set_error(W4A16_ERR_CONFIG, "%s: buffers must be 16-byte aligned (lse: 4)", what);
     const int dim = cache->head_dim;
+    drop_strides_of_one(kv.rows, &q_row_stride, q_heads, &q_head_stride);
+    drop_strides_of_one(kv.rows, &out_row_stride, q_heads, &out_head_stride);
     const size_t qb = strided_bytes(kv.rows, q_row_stride, q_heads, q_head_stride, dim);
     const size_t ob = strided_bytes(kv.rows, out_row_stride, q_heads, out_head_stride, dim);
     if (!qb || !ob) return set_error(W4A16_ERR_CONFIG, "%s: strides must be multiples of 8 elements from 0", what);

@@ -27,6 +27,12 @@ int kv_check(const W4A16KvCache *cache, const W4A16KvBatch *batch, const char *w
 size_t strided_bytes(long long rows, long long row_stride, long long heads, long long head_stride,
                      int dim);
 
+/* An axis of one has no stride: whatever its caller's says is 0 from here on. */
+inline void drop_strides_of_one(int rows, long long *row_stride, int heads, long long *head_stride) {
+    if (rows == 1) *row_stride = 0;
+    if (heads == 1) *head_stride = 0;
+}
+
 /* Bytes of one of the cache's code and scale buffers. */
 size_t kv_bytes(const W4A16KvCache *cache);
 size_t kv_scale_bytes(const W4A16KvCache *cache);

@@ -240,6 +240,8 @@ extern "C" int w4a16_kv_write_bf16(const W4A16KvCache *cache, const W4A16KvBatch
     if (!k || !v) return set_error(W4A16_ERR_CONFIG, "%s: null buffer", what);
     if (misaligned(k) || misaligned(v))
         return set_error(W4A16_ERR_CONFIG, "%s: buffers must be 16-byte aligned", what);
+    drop_strides_of_one(kv.rows, &k_row_stride, kv.heads, &k_head_stride);
+    drop_strides_of_one(kv.rows, &v_row_stride, kv.heads, &v_head_stride);
     const size_t kb = strided_bytes(kv.rows, k_row_stride, kv.heads, k_head_stride, cache->head_dim);
     const size_t vb = strided_bytes(kv.rows, v_row_stride, kv.heads, v_head_stride, cache->head_dim);
     if (!kb || !vb)

@@ -369,7 +369,7 @@ int engine_ffn_forward_residual_norm(W4A16Store *store, int layer, uint16_t *res
  * share pages; one that a call writes through two of them holds either's rows.
  *
  * Strides are in elements; a token's heads and a head's values stand apart by multiples of 8
- * elements, values next to each other. Tensors that are read and written by one call must not
+ * elements, values next to each other; the stride of an axis of one is not looked at. Tensors that are read and written by one call must not
  * share memory unless it says so.
  * ------------------------------------------------------------------------------------- */
 #define W4A16_KV_BF16 0
