@@ -320,6 +320,17 @@ __device__ __forceinline__ f4 mfma_v(const uint32_t *v, const uint32_t *w, f4 ac
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf8(v[0], v[1], v[2], v[3]), as_bf8(w[0], w[1], w[2], w[3]), acc, 0, 0, 0);
 }
 
+/* A pair of BF16 weights and a pair of what they leave of a and b: a weight is then off by 2^-15 of itself
+ * (cut to 8 bits, and the rest rounded to 8), not 2^-8. The rest is positive, as the weight is, and not
+ * zero: an infinity among V's values stays one, it meets no product of the other sign or of zero. A last bit
+ * set beforehand (2^-23) sees to that, for weights from 2^-100 of the largest. */
+__device__ __forceinline__ void split_weights(float a, float b, uint32_t *first, uint32_t *rest) {
+    const uint32_t x = __builtin_bit_cast(uint32_t, a), y = __builtin_bit_cast(uint32_t, b);
+    *first = __builtin_amdgcn_perm(y, x, 0x07060302u);
+    *rest = kv_pack_bf16(__builtin_bit_cast(float, x | 1u) - __builtin_bit_cast(float, x & 0xFFFF0000u),
+                         __builtin_bit_cast(float, y | 1u) - __builtin_bit_cast(float, y & 0xFFFF0000u));
+}
+
 __device__ __forceinline__ float power_of_two(int biased) { return __builtin_bit_cast(float, (uint32_t)biased << 23); }
 
 /* The weights of an 8-bit cache carry V's scale, so they are FP16 (in which codes are exact), over a
@@ -354,8 +365,10 @@ constexpr int rows_blocks(int dim, int format, int rt) {
  * columns; a transposition of 8 tokens x 2 values at a time by byte permutations makes them the
  * operand of value e's product.
  *
- * A BF16 cache's weights are rounded to BF16, half a step of 2^-8 each; those of an 8-bit cache to
- * FP16 (kLift), which also takes fewer instructions to widen INT8.
+ * A BF16 cache's weights are two BF16 numbers each (split_weights), 2^-15: the second product takes 0 to 0.3 % (16
+ * sequences of 4096 with five rows each, D = 128 39.5 and 39.9 us, D = 64 24.4 and 25.3), and one user's output of 1337 tokens is off
+ * by 1.7e-3, its own rounding, where it was by 1.8e-3 to 2.2e-3. Those of an 8-bit cache are rounded to FP16
+ * (kLift), which also takes fewer instructions to widen INT8.
  *
  * Bound by memory: 32 sequences of 8192 tokens, one row of 32 heads each (16 of 256 values), the join included:
  * BF16 D = 64 102 us (5.2 TB/s), D = 128 192 (5.6), D = 256 200 (5.4); FP8 66 (4.4), 108 (5.1), 107 (5.1); INT8
@@ -609,7 +622,7 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
                 ks[c] *= a.scale;
             }
         }
-        uint32_t p[RT][4];
+        uint32_t p[RT][4], p_rest[kCoded ? 1 : RT][4];
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
 #pragma unroll
@@ -645,53 +658,75 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
                     l[r] += w[i];
                     if constexpr (kCoded) w[i] *= vs[c][i];
                 }
-                p[r][2 * c] = kCoded ? pack_f16(w[0], w[1]) : kv_pack_bf16(w[0], w[1]);
-                p[r][2 * c + 1] = kCoded ? pack_f16(w[2], w[3]) : kv_pack_bf16(w[2], w[3]);
+                if constexpr (kCoded) {
+                    p[r][2 * c] = pack_f16(w[0], w[1]);
+                    p[r][2 * c + 1] = pack_f16(w[2], w[3]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; i += 2) split_weights(w[i], w[i + 1], &p[r][2 * c + i / 2], &p_rest[r][2 * c + i / 2]);
+                }
             }
         }
-        if (kCoded || !odd) {
+        if constexpr (!kCoded)
+            if (odd) {
+                /* An infinity or a NaN among values that not every row sees: 0 times it would reach the
+                 * rows that do not. Those that do have it added as it is, and the products go without it.
+                 * Value E (4 g + i) + e of a token, which is acc[][e][i], is lane 4 g + i's of its 16. */
 #pragma unroll
-            for (int e = 0; e < E; e += 2) {
-                uint32_t even[4], odds[4];
+                for (int x = 0; x < 8; ++x) {
+                    bool some = false;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) { /* values e, e + 1 of tokens 2 j and 2 j + 1 */
-                    if constexpr (kCoded) {
-                        if (e % 4) code_pairs<FMT, 1>(v[2 * j][e / 4], v[2 * j + 1][e / 4], &even[j], &odds[j]);
-                        else code_pairs<FMT, 0>(v[2 * j][e / 4], v[2 * j + 1][e / 4], &even[j], &odds[j]);
-                    } else {
-                        even[j] = __builtin_amdgcn_perm(v[2 * j + 1][e / 2], v[2 * j][e / 2], 0x05040100u);
-                        odds[j] = __builtin_amdgcn_perm(v[2 * j + 1][e / 2], v[2 * j][e / 2], 0x07060302u);
+                    for (int w = 0; w < kVWords; ++w) some = some | nonfinite2(v[x][w]);
+                    const unsigned long long where = __ballot(some);
+                    if (where == 0) continue;
+#pragma unroll 1
+                    for (int of = 0; of < 4; ++of) {
+                        if ((where >> (16 * of) & 0xFFFF) == 0) continue;
+                        const int at = t0 + 16 * (x / 4) + 4 * of + x % 4;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+#pragma unroll
+                            for (int w = 0; w < kVWords; ++w) {
+                                const uint32_t pair = __shfl(v[x][w], 16 * of + 4 * g + i);
+                                const uint32_t f[2] = {pair << 16, pair & 0xFFFF0000u};
+#pragma unroll
+                                for (int r = 0; r < RT; ++r)
+#pragma unroll
+                                    for (int half = 0; half < 2; ++half) {
+                                        const bool adds = (at >= lo[r]) & (at < hi[r]) & ((f[half] & 0x7F800000u) == 0x7F800000u);
+                                        acc[r][2 * w + half][i] += adds ? __builtin_bit_cast(float, f[half]) : 0.0f;
+                                    }
+                            }
                     }
-                }
 #pragma unroll
-                for (int r = 0; r < RT; ++r) {
-                    acc[r][e] = mfma_v<kCoded>(even, p[r], acc[r][e]);
-                    acc[r][e + 1] = mfma_v<kCoded>(odds, p[r], acc[r][e + 1]);
+                    for (int w = 0; w < kVWords; ++w) {
+                        const uint32_t pair = v[x][w];
+                        v[x][w] = ((pair & 0x7F80u) == 0x7F80u ? 0u : pair & 0xFFFFu) | ((pair & 0x7F800000u) == 0x7F800000u ? 0u : pair & 0xFFFF0000u);
+                    }
                 }
             }
-        } else if constexpr (!kCoded) {
-            /* an infinity or a NaN among values that not every row sees: 0 times it would
-             * reach the rows that do not, so each row's product is formed apart, without
-             * the tokens that it does not see */
 #pragma unroll
-            for (int r = 0; r < RT; ++r)
-                for (int one = 0; one < 16; ++one) {
-                    const int o_lo = __shfl(lo[r], one), o_hi = __shfl(hi[r], one);
+        for (int e = 0; e < E; e += 2) {
+            uint32_t even[4], odds[4];
 #pragma unroll
-                    for (int e = 0; e < E; ++e) {
-                        uint32_t pair[4];
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const int at = t0 + 16 * (j / 2) + 4 * g + 2 * (j % 2);
-                            const uint32_t x = at >= o_lo && at < o_hi ? v[2 * j][e / 2] : 0u;
-                            const uint32_t y = at + 1 >= o_lo && at + 1 < o_hi ? v[2 * j + 1][e / 2] : 0u;
-                            pair[j] = __builtin_amdgcn_perm(y, x, e % 2 ? 0x07060302u : 0x05040100u);
-                        }
-                        const f4 got = mfma_v<kCoded>(pair, p[r], acc[r][e]);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) acc[r][e][i] = n == one ? got[i] : acc[r][e][i];
-                    }
+            for (int j = 0; j < 4; ++j) { /* values e, e + 1 of tokens 2 j and 2 j + 1 */
+                if constexpr (kCoded) {
+                    if (e % 4) code_pairs<FMT, 1>(v[2 * j][e / 4], v[2 * j + 1][e / 4], &even[j], &odds[j]);
+                    else code_pairs<FMT, 0>(v[2 * j][e / 4], v[2 * j + 1][e / 4], &even[j], &odds[j]);
+                } else {
+                    even[j] = __builtin_amdgcn_perm(v[2 * j + 1][e / 2], v[2 * j][e / 2], 0x05040100u);
+                    odds[j] = __builtin_amdgcn_perm(v[2 * j + 1][e / 2], v[2 * j][e / 2], 0x07060302u);
                 }
+            }
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                acc[r][e] = mfma_v<kCoded>(even, p[r], acc[r][e]);
+                acc[r][e + 1] = mfma_v<kCoded>(odds, p[r], acc[r][e + 1]);
+                if constexpr (!kCoded) {
+                    acc[r][e] = mfma_v<kCoded>(even, p_rest[r], acc[r][e]);
+                    acc[r][e + 1] = mfma_v<kCoded>(odds, p_rest[r], acc[r][e + 1]);
+                }
+            }
         }
         if (more) load_v(next);
         if constexpr (kCoded) {

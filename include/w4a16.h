@@ -414,10 +414,12 @@ int w4a16_kv_read_bf16(const W4A16KvCache *cache, const W4A16KvBatch *batch, uin
  * own keys and values have been written: out_i = sum_j softmax_j(scale * <q_i, k_j>) v_j. Query
  * head h reads key head h / (q_heads / kv_heads). causal: a row sees positions up to its own;
  * window > 0: none that is `window` or more before its own. Scores, statistics and sums are FP32.
- * The weights are rounded before the product with V: to BF16, or with an 8-bit cache, where they
- * carry V's scales, to FP16 (2^-11 of each, or 2^-31 of the largest weight times the largest of the
- * sequence's scales for that head, whichever is more). The output is rounded once. A row that sees
- * nothing gets zeros, and -infinity as lse. lse (optional): [rows][q_heads], log of the sum of exp of the scaled scores.
+ * The weights are rounded before the product with V: with a BF16 cache to 2^-15 of each in sequences of
+ * few rows (new tokens times the query heads of a key head up to 32, or 16 of 256 values), to BF16 (2^-8)
+ * in chunks; with an 8-bit cache, where they carry V's scales, to FP16 (2^-11 of each, or 2^-31 of the
+ * largest weight times the largest of the sequence's scales for that head, whichever is more). The output
+ * is rounded once. A row that sees nothing gets zeros, and -infinity as lse.
+ * lse (optional): [rows][q_heads], log of the sum of exp of the scaled scores.
  * ws: device memory of at least the bytes w4a16_paged_attention_workspace gives for the same
  * arguments (on the same device), for this call alone until it has run; NULL if that is 0.
  * out may be q itself (the same strides). */

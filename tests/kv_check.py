@@ -22,10 +22,10 @@ def sizes(cache, table, kv_lens, page, pages):
     return out
 
 
-def check(out, lse, cache, table, q, kv_lens, news, page, pages, scale, causal=True, window=0):
+def check(out, lse, cache, table, q, kv_lens, news, page, pages, scale, causal=True, window=0, half=None):
     k, v, there = whole(cache, table, kv_lens, page, pages)
     coded = sizes(cache, table, kv_lens, page, pages)
-    want, want_lse, off, lse_off = kv_oracle.attention(q, k, v, there, scale, causal, window, news, kv_lens, coded)
+    want, want_lse, off, lse_off = kv_oracle.attention(q, k, v, there, scale, causal, window, news, kv_lens, coded, half)
     got, got_lse = out.cpu().double(), lse.cpu().double()
     empty = want_lse == float("-inf")
     assert torch.equal(got_lse == float("-inf"), empty)

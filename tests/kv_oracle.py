@@ -46,12 +46,13 @@ def places(table, kv_lens, news, page, pages):
     return out
 
 
-def attention(q, k, v, places_of, scale, causal, window, news, kv_lens, coded=None):
+def attention(q, k, v, places_of, scale, causal, window, news, kv_lens, coded=None, half=None):
     """FP64 attention of the rows q [rows, q_heads, D] of sequences whose tokens' keys and values are
     k[s], v[s] [kv_heads, tokens, D] and places_of[s] [tokens] whether each is there. kv_lens places the rows, and may
     be more than the tokens there are. Returns (out, lse, and for each of
     them how far FP32 arithmetic with BF16 weights and a BF16 output may be off). `coded`: of an 8-bit cache, whose weights are
-    FP16, the sizes of each sequence's V codes [kv_heads, tokens, D] and of their scales [kv_heads, tokens].
+    FP16, the sizes of each sequence's V codes [kv_heads, tokens, D] and of their scales [kv_heads, tokens]. `half`: how far
+    a weight may be off instead, relatively.
 
     The bounds. A score is a sum of D products: off by (D + 4) 2^-24 sum|q k| scale, and by a rounding or two of its own;
     a weight exp(s - m) by as much relatively, and 2^-21 for the exponential; both a weight and the sum of weights can
@@ -64,7 +65,8 @@ def attention(q, k, v, places_of, scale, causal, window, news, kv_lens, coded=No
     first is 2^-11 of sum p|v|. The second, less 2^6 / 2^e, is 2^-31 2^e of an exp(s - m); over the sum of weights
     exp(m) is at most the largest weight p: 2^-31 max p, max scale for each |code|."""
     bf16 = torch.finfo(torch.bfloat16).eps / 2
-    half = bf16 if coded is None else torch.finfo(torch.float16).eps / 2
+    if half is None:
+        half = bf16 if coded is None else torch.finfo(torch.float16).eps / 2
     group = q.shape[1] // k[0].shape[0]
     outs, lses, out_off, lse_off, first = [], [], [], [], 0
     dim = q.shape[2]
