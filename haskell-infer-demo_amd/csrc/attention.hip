@@ -1394,9 +1394,12 @@ Plan plan_of(const W4A16KvCache *c, const W4A16KvBatch *b, int q_heads) {
     }
     const long long tokens = b->max_kv ? b->max_kv : (long long)b->table_pages * c->page_size;
     if (p.few.items) {
-        /* One round of blocks (48 ragged sequences of up to 8192 tokens, INT8: 91.0 us; one and a
-         * half: 100.5, two: 85.8; 16 with verify rows, FP8: 22.0 / 25.8 / 24.0; 2 of 100003 tokens,
-         * D = 256: 77.8 / 89.7 / 82.8), and no more than there are units. */
+        /* One round of blocks, and no more than there are units. Two rounds are better for batches of many
+         * sequences and worse for few or short ones; the host knows bounds, not lengths, and one round loses least
+         * where it loses. One, one and a half, two rounds, the join included, us: 48 ragged sequences of up to 8192
+         * tokens, D = 128, INT8 100.7 / 106.4 / 95.5, BF16 142 / 152 / 138; 32 of 8192, BF16, D = 128 201 / 210 / 206,
+         * D = 256 217 / 245 / 203; 16 of up to 4096 with five rows, FP8 31.0 / 35.5 / 33.5; 100003 tokens, one
+         * sequence, BF16 91.7 / 99.8 / 96.0, two, D = 256, FP8 93.7 / 99.4 / 100.6. */
         const long long blocks = (long long)rows_blocks(dim, c->format, p.rt) * device_cus();
         const long long pairs = (long long)p.few.items * c->kv_heads, units = pairs * ((tokens + kUnit - 1) / kUnit);
         p.few.splits = (int)(units < 1 ? 1 : units < blocks ? units : blocks);
