@@ -21,6 +21,7 @@
  * where a running sum lies within 2^-46 of the total from the threshold.
  */
 #include "launch.h"
+#include "wave.h"
 
 using namespace w4a16;
 
@@ -141,19 +142,6 @@ __device__ __forceinline__ double lane_f64(double v, int lane) {
     const uint2 b = __builtin_bit_cast(uint2, v);
     return __builtin_bit_cast(double, make_uint2((uint32_t)__builtin_amdgcn_readlane((int)b.x, lane),
                                                  (uint32_t)__builtin_amdgcn_readlane((int)b.y, lane)));
-}
-
-/* The largest of v >= 0 over the lanes. */
-__device__ __forceinline__ int wave_most(int v) {
-#define W4A16_MOST(CTRL, ROWS) v = max(v, __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false))
-    W4A16_MOST(0x111, 0xF);
-    W4A16_MOST(0x112, 0xF);
-    W4A16_MOST(0x114, 0xF);
-    W4A16_MOST(0x118, 0xF);
-    W4A16_MOST(0x142, 0xA);
-    W4A16_MOST(0x143, 0xC);
-#undef W4A16_MOST
-    return __builtin_amdgcn_readlane(v, 63);
 }
 
 /* The block's smallest `mine` and largest `behind`, a wave's first: 64 lanes at one LDS word take turns. */
