@@ -1502,24 +1502,14 @@ extern "C" int w4a16_paged_attention_bf16(const W4A16KvCache *cache, const W4A16
     const size_t qb = strided_bytes(kv.rows, q_row_stride, q_heads, q_head_stride, dim);
     const size_t ob = strided_bytes(kv.rows, out_row_stride, q_heads, out_head_stride, dim);
     if (!qb || !ob) return set_error(W4A16_ERR_CONFIG, "%s: strides must be multiples of 8 elements from 0", what);
-    const long long by_row = (long long)(q_heads - 1) * out_head_stride + dim;
-    const long long by_head = (long long)(kv.rows - 1) * out_row_stride + dim;
-    const bool apart = ((q_heads == 1 || out_head_stride >= dim) && (kv.rows == 1 || out_row_stride >= by_row)) ||
-                       ((kv.rows == 1 || out_row_stride >= dim) && (q_heads == 1 || out_head_stride >= by_head));
-    if (!apart) return set_error(W4A16_ERR_CONFIG, "%s: output rows overlap each other", what);
+    const RowsView qr = {q, qb, q_row_stride, q_head_stride, q_heads}, outs = {out, ob, out_row_stride, out_head_stride, q_heads};
+    if (!rows_apart(kv.rows, outs, dim)) return set_error(W4A16_ERR_CONFIG, "%s: output rows overlap each other", what);
     const Plan p = plan_of(cache, batch, q_heads);
     if (p.ws_bytes > 0 && (!ws || ws_bytes < p.ws_bytes))
         return set_error(W4A16_ERR_CONFIG, "%s: a workspace of %zu bytes, the call needs %zu", what, ws ? ws_bytes : 0,
                          p.ws_bytes);
     /* q and out may be the same tensor, or heads of the same rows side by side */
-    bool clash = overlap(q, qb, out, ob);
-    if (clash && q_row_stride == out_row_stride && kv.rows > 0) {
-        const long long q_wide = (long long)(q_heads - 1) * q_head_stride + dim, o_wide = by_row;
-        const long long off = ((const uint8_t *)out - (const uint8_t *)q) / 2;
-        if (off == 0 && q_head_stride == out_head_stride) clash = false;
-        else if (off > 0) clash = !(off >= q_wide && off + o_wide <= q_row_stride);
-        else clash = !(-off >= o_wide && -off + q_wide <= q_row_stride);
-    }
+    bool clash = !rows_same(qr, outs) && !rows_beside(kv.rows, outs, qr, dim);
     const size_t lb = lse ? (size_t)kv.rows * q_heads * 4 : 0, cb = kv_bytes(cache), sb = kv_scale_bytes(cache);
     const struct { const void *p; size_t n; } writes[] = {{out, ob}, {lse, lb}, {ws, p.ws_bytes}};
     const struct { const void *p; size_t n; } reads[] = {{cache->k, cb}, {cache->v, cb}, {kv.k_scale, sb}, {kv.v_scale, sb}};

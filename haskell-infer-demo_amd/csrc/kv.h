@@ -33,6 +33,23 @@ inline void drop_strides_of_one(int rows, long long *row_stride, int heads, long
     if (heads == 1) *head_stride = 0;
 }
 
+/* A [rows][heads][dim] tensor of 2-byte elements, checked by strided_bytes, as others are compared with it. */
+struct RowsView {
+    const void *p;
+    size_t bytes;
+    long long row, head;
+    int heads;
+};
+
+/* Whether no two of its (row, head)s share memory. */
+bool rows_apart(int rows, const RowsView &x, int dim);
+
+/* Whether x and y share no element: memory of their own, or columns of the same rows side by side. */
+bool rows_beside(int rows, const RowsView &x, const RowsView &y, int dim);
+
+/* Whether they are one tensor. */
+inline bool rows_same(const RowsView &x, const RowsView &y) { return x.p == y.p && x.row == y.row && x.head == y.head && x.heads == y.heads; }
+
 /* Bytes of one of the cache's code and scale buffers. */
 size_t kv_bytes(const W4A16KvCache *cache);
 size_t kv_scale_bytes(const W4A16KvCache *cache);

@@ -1,6 +1,6 @@
 /*
- * kv_cache.hip - Writing rows of keys and values into the paged cache, quantised on the way, and
- * reading them back; the checks of a cache and a batch.
+ * kv_cache.hip - Writing rows of keys and values into the paged cache, turned by their positions and
+ * quantised on the way, and reading them back; the checks of a cache and a batch.
  */
 #include "kv.h"
 
@@ -14,6 +14,7 @@ constexpr float kSmallest = 0x1p-117f; /* 448 / kSmallest is still finite in FP3
  * The sequences whose rows end at or before `row` are counted 64 at a time. */
 struct Place {
     int seq, page, inside; /* seq < 0: no sequence's row; page < 0: a row without a place */
+    int at;                /* the row's token in its sequence */
 };
 
 __device__ __forceinline__ Place find_place(const KvView &kv, int row) {
@@ -26,15 +27,15 @@ __device__ __forceinline__ Place find_place(const KvView &kv, int row) {
         before += n;
         if (n < 64) break;
     }
-    if (before >= kv.seqs) return {-1, -1, 0};
+    if (before >= kv.seqs) return {-1, -1, 0, 0};
     const int first = kv.starts[before], last = kv.starts[before + 1];
-    if (row < first || row >= last) return {-1, -1, 0};
+    if (row < first || row >= last) return {-1, -1, 0, 0};
     /* kv_lens and the number of rows may be anything up to 2^31: the difference in 64 bits */
     const long long at = (long long)kv.kv_lens[before] - last + row;
-    if (at < 0 || (at >> kv.shift) >= kv.table_pages) return {before, -1, 0};
+    if (at < 0 || (at >> kv.shift) >= kv.table_pages) return {before, -1, 0, (int)at};
     const int page = kv.table[(long long)before * kv.table_stride + (at >> kv.shift)];
-    if ((unsigned)page >= (unsigned)kv.pages) return {before, -1, 0};
-    return {before, page, (int)(at & ((1 << kv.shift) - 1))};
+    if ((unsigned)page >= (unsigned)kv.pages) return {before, -1, 0, (int)at};
+    return {before, page, (int)(at & ((1 << kv.shift) - 1)), (int)at};
 }
 
 /* The largest of v over groups of N lanes (8, 16 or 32). */
@@ -45,10 +46,37 @@ __device__ __forceinline__ float group_max(float v) {
     return v;
 }
 
+/* A lane's eight of a row's values as codes, and the row's scale. `most`: the largest of them in size, infinity if one is
+ * none that is finite. The scale and its inverse are each one division a row, and a value costs a product
+ * and a conversion. */
+template <int FMT, int LANES>
+__device__ __forceinline__ float encode(float (&f)[8], float most, uint32_t (&out)[2]) {
+    constexpr float kTop = FMT == W4A16_KV_INT8 ? 127.0f : 448.0f;
+    most = group_max<LANES>(most);
+    const bool held = most >= kSmallest && most < __builtin_inff();
+    const float inverse = held ? kTop / most : 0.0f;
+    out[0] = out[1] = 0u;
+    if (held) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = __builtin_amdgcn_fmed3f(f[i] * inverse, -kTop, kTop);
+        if constexpr (FMT == W4A16_KV_FP8) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                int word = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i], f[4 * i + 1], 0, false);
+                out[i] = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i + 2], f[4 * i + 3], word, true);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                out[i / 4] |= ((uint32_t)(int)__builtin_rintf(f[i]) & 0xFFu) << (8 * (i % 4));
+        }
+    }
+    return held ? most / kTop : most < kSmallest ? 0.0f : __builtin_nanf("");
+}
+
 /* One wave a row of K (blockIdx.y = 0) or V (1): D / 8 lanes a head, eight values a lane. Bound by
  * memory: a row is read once with 16 bytes a lane and its codes are written once. The row's
- * largest value is found over the head's lanes by shuffles; the scale and its inverse are each
- * one division a row, and a value costs a product and a conversion. 8198 rows of 8 heads of 128 to FP8:
+ * largest value is found over the head's lanes by shuffles. 8198 rows of 8 heads of 128 to FP8:
  * 12.6 us, 51 MB at 4.0 TB/s (a large copy: 4.9); four rows: 3.4, a launch and three round trips. */
 template <int D, int FMT>
 __global__ __launch_bounds__(256) void kv_write_kernel(KvView kv, const uint16_t *k, long long k_row,
@@ -71,7 +99,6 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvView kv, const uint16_t
         if constexpr (FMT == W4A16_KV_BF16) {
             *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(codes) + slot * D + part) = x;
         } else {
-            constexpr float kTop = FMT == W4A16_KV_INT8 ? 127.0f : 448.0f;
             const uint32_t w[4] = {x.x, x.y, x.z, x.w};
             float f[8], most = 0.0f;
             bool finite = true;
@@ -82,29 +109,11 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvView kv, const uint16_t
                 finite = finite && (w[i] & 0x7F800000u) != 0x7F800000u && (w[i] & 0x7F80u) != 0x7F80u;
                 most = fmaxf(most, fmaxf(fabsf(f[2 * i]), fabsf(f[2 * i + 1])));
             }
-            most = group_max<kLanes>(finite ? most : __builtin_inff());
-            const bool held = most >= kSmallest && most < __builtin_inff();
-            const float inverse = held ? kTop / most : 0.0f;
-            uint32_t out[2] = {0u, 0u};
-            if (held) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) f[i] = __builtin_amdgcn_fmed3f(f[i] * inverse, -kTop, kTop);
-                if constexpr (FMT == W4A16_KV_FP8) {
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        int word = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i], f[4 * i + 1], 0, false);
-                        out[i] = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i + 2], f[4 * i + 3], word, true);
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        out[i / 4] |= ((uint32_t)(int)__builtin_rintf(f[i]) & 0xFFu) << (8 * (i % 4));
-                }
-            }
+            uint32_t out[2];
+            const float scale = encode<FMT, kLanes>(f, finite ? most : __builtin_inff(), out);
             *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(codes) + slot * D + part) =
                 make_uint2(out[0], out[1]);
-            if (lane % kLanes == 0)
-                scales[slot] = held ? most / kTop : most < kSmallest ? 0.0f : __builtin_nanf("");
+            if (lane % kLanes == 0) scales[slot] = scale;
         }
     }
 }
@@ -146,6 +155,135 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvView kv, uint16_t *k, ui
     }
 }
 
+/*
+ * Keys turned by their positions and quantised, values quantised, queries turned: y = R(position * inv_freq) x.
+ *
+ * One wave a row and part of its heads. The row's angles are worked out first, one or two pairs a lane, into
+ * a table of the wave's own in LDS, from which a lane takes the four pairs that it turns in
+ * every head: the sines of a row cost 1 / heads of what they would beside each value. An angle is
+ * reduced in FP64 to a part of a turn (position * inv_freq is exact to 2^-53, so at 2^30 to 2^-23), and
+ * from there FP32 is enough. A head has D / 8 lanes of eight values; in halves a lane has four values of the one and
+ * their partners of the other, so that a turn stays in its registers and q_out may be q.
+ *
+ * Work beyond the row's place comes in steps of 64 lanes (1 KiB): heads of K, of V, of q, in this order, kAhead of them on
+ * their way at a time.
+ */
+struct AppendArgs {
+    const uint16_t *k, *v, *q;
+    uint16_t *q_out;
+    long long k_row, k_head, v_row, v_head, q_row, q_head, o_row, o_head;
+    const float *inv_freq;
+    const int32_t *positions;
+    int q_heads, pairs, interleaved;
+};
+
+constexpr double kTurns = 0.15915494309189535; /* 1 / (2 pi) */
+
+template <int D, int FMT>
+__global__ __launch_bounds__(256) void kv_append_kernel(KvView kv, AppendArgs a) {
+    constexpr int kLanes = D / 8, kHeads = 64 / kLanes, kAhead = 4;
+    __shared__ float2 turns[4][D / 2];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, row = blockIdx.x * 4 + wave, sub = lane % kLanes;
+    if (row >= kv.rows) return;
+    const Place at = find_place(kv, row);
+    if (at.seq < 0) return;
+    const double position = a.positions ? a.positions[row] : at.at;
+    for (int i = lane; i < a.pairs; i += 64) {
+        const double turn = position * (double)a.inv_freq[i] * kTurns;
+        float s, c;
+        sincospif(2.0f * (float)(turn - __builtin_rint(turn)), &s, &c);
+        turns[wave][i] = make_float2(c, s);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); /* the wave's own table: no other reads it */
+    const bool turned = 4 * sub < a.pairs;
+    float c[4], s[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 t = turns[wave][turned ? 4 * sub + i : 0];
+        c[i] = t.x;
+        s[i] = t.y;
+    }
+    /* this lane's values of a head: four from `first` and four from `second` */
+    const int first = a.interleaved ? 8 * sub : turned ? 4 * sub : 2 * a.pairs + 8 * (sub - a.pairs / 4);
+    const int second = a.interleaved || !turned ? first + 4 : first + a.pairs;
+    const int of_kv = (kv.heads + kHeads - 1) / kHeads, of_q = (a.q_heads + kHeads - 1) / kHeads, steps = 2 * of_kv + of_q;
+    for (int step0 = blockIdx.y; step0 < steps; step0 += kAhead * gridDim.y) {
+        uint2 x[kAhead][2];
+#pragma unroll
+        for (int n = 0; n < kAhead; ++n) {
+            const int step = step0 + n * gridDim.y;
+            const int which = step < of_kv ? 0 : step < 2 * of_kv ? 1 : 2;
+            const int h = (step - which * of_kv) * kHeads + lane / kLanes;
+            x[n][0] = x[n][1] = make_uint2(0u, 0u);
+            if (step < steps && h < (which == 2 ? a.q_heads : kv.heads)) {
+                const uint16_t *from = which == 0   ? a.k + row * a.k_row + h * a.k_head
+                                       : which == 1 ? a.v + row * a.v_row + h * a.v_head
+                                                    : a.q + row * a.q_row + h * a.q_head;
+                x[n][0] = *reinterpret_cast<const uint2 *>(from + first);
+                x[n][1] = *reinterpret_cast<const uint2 *>(from + second);
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < kAhead; ++n) {
+            const int step = step0 + n * gridDim.y;
+            if (step >= steps) break;
+            const int which = step < of_kv ? 0 : step < 2 * of_kv ? 1 : 2;
+            const int h = (step - which * of_kv) * kHeads + lane / kLanes;
+            const bool is_v = which == 1;
+            if (which < 2 && at.page < 0) continue;
+            const uint32_t w[4] = {x[n][0].x, x[n][0].y, x[n][1].x, x[n][1].y};
+            float f[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                f[2 * i] = __builtin_bit_cast(float, w[i] << 16);
+                f[2 * i + 1] = __builtin_bit_cast(float, w[i] & 0xFFFF0000u);
+            }
+            if (!is_v) {
+                float y[8];
+                if (a.interleaved) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        y[2 * i] = f[2 * i] * c[i] - f[2 * i + 1] * s[i];
+                        y[2 * i + 1] = f[2 * i + 1] * c[i] + f[2 * i] * s[i];
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        y[i] = f[i] * c[i] - f[4 + i] * s[i];
+                        y[4 + i] = f[4 + i] * c[i] + f[i] * s[i];
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) f[i] = turned ? y[i] : f[i];
+            }
+            if (which == 2 || FMT == W4A16_KV_BF16) {
+                if (h >= (which == 2 ? a.q_heads : kv.heads)) continue;
+                const long long slot = (((long long)at.page * kv.heads + h) << kv.shift) + at.inside;
+                uint16_t *to = which == 2 ? a.q_out + row * a.o_row + h * a.o_head
+                                          : static_cast<uint16_t *>(is_v ? kv.v : kv.k) + slot * D;
+                *reinterpret_cast<uint2 *>(to + first) = make_uint2(kv_pack_bf16(f[0], f[1]), kv_pack_bf16(f[2], f[3]));
+                *reinterpret_cast<uint2 *>(to + second) = make_uint2(kv_pack_bf16(f[4], f[5]), kv_pack_bf16(f[6], f[7]));
+            } else {
+                float most = 0.0f;
+                bool finite = true;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    finite = finite && fabsf(f[i]) < __builtin_inff();
+                    most = fmaxf(most, fabsf(f[i]));
+                }
+                uint32_t out[2];
+                const float scale = encode<FMT, kLanes>(f, finite ? most : __builtin_inff(), out);
+                if (h >= kv.heads) continue;
+                const long long slot = (((long long)at.page * kv.heads + h) << kv.shift) + at.inside;
+                uint8_t *to = static_cast<uint8_t *>(is_v ? kv.v : kv.k) + slot * D;
+                *reinterpret_cast<uint32_t *>(to + first) = out[0];
+                *reinterpret_cast<uint32_t *>(to + second) = out[1];
+                if (sub == 0) (is_v ? kv.v_scale : kv.k_scale)[slot] = scale;
+            }
+        }
+    }
+}
+
 template <int D>
 void launch_write(int format, const KvView &kv, const uint16_t *k, long long k_row, long long k_head,
                   const uint16_t *v, long long v_row, long long v_head, hipStream_t s) {
@@ -154,6 +292,19 @@ void launch_write(int format, const KvView &kv, const uint16_t *k, long long k_r
                   : format == W4A16_KV_INT8 ? kv_write_kernel<D, W4A16_KV_INT8>
                                             : kv_write_kernel<D, W4A16_KV_FP8>;
     launch_k(kernel, grid, block, 0, s, kv, k, k_row, k_head, v, v_row, v_head);
+}
+
+template <int D>
+void launch_append(int format, const KvView &kv, const AppendArgs &a, hipStream_t s) {
+    constexpr int kHeads = 512 / D;
+    const int steps = 2 * ((kv.heads + kHeads - 1) / kHeads) + (a.q_heads + kHeads - 1) / kHeads;
+    /* every step a wave of its own where there are few rows; a wave's angles serve all of its steps */
+    const int blocks = (kv.rows + 3) / 4, most = (8 * device_cus() + blocks - 1) / blocks;
+    const dim3 grid(blocks, steps < most ? steps : most), block(256);
+    auto kernel = format == W4A16_KV_BF16   ? kv_append_kernel<D, W4A16_KV_BF16>
+                  : format == W4A16_KV_INT8 ? kv_append_kernel<D, W4A16_KV_INT8>
+                                            : kv_append_kernel<D, W4A16_KV_FP8>;
+    launch_k(kernel, grid, block, 0, s, kv, a);
 }
 
 template <int D>
@@ -183,6 +334,20 @@ size_t strided_bytes(long long rows, long long row_stride, long long heads, long
     if (rows > 1 && row_stride > kMost / (rows - 1)) return 0;
     if (heads > 1 && head_stride > kMost / (heads - 1)) return 0;
     return ((size_t)(rows - 1) * row_stride + (size_t)(heads - 1) * head_stride + dim) * 2;
+}
+
+bool rows_apart(int rows, const RowsView &x, int dim) {
+    const long long by_row = (long long)(x.heads - 1) * x.head + dim, by_head = (long long)(rows - 1) * x.row + dim;
+    return ((x.heads == 1 || x.head >= dim) && (rows == 1 || x.row >= by_row)) ||
+           ((rows == 1 || x.row >= dim) && (x.heads == 1 || x.head >= by_head));
+}
+
+bool rows_beside(int rows, const RowsView &x, const RowsView &y, int dim) {
+    if (!overlap(x.p, x.bytes, y.p, y.bytes)) return true;
+    if (x.row != y.row || rows == 1) return false;
+    const long long off = ((const uint8_t *)x.p - (const uint8_t *)y.p) / 2;
+    const long long x_wide = (long long)(x.heads - 1) * x.head + dim, y_wide = (long long)(y.heads - 1) * y.head + dim;
+    return off > 0 ? off >= y_wide && off + x_wide <= x.row : off < 0 && -off >= x_wide && -off + y_wide <= x.row;
 }
 
 int kv_check(const W4A16KvCache *c, const W4A16KvBatch *b, const char *what, KvView *view) {
@@ -229,6 +394,27 @@ int kv_check(const W4A16KvCache *c, const W4A16KvBatch *b, const char *what, KvV
 
 } // namespace w4a16
 
+namespace {
+
+/* Rows that are read share no memory with the cache, nor its parts with each other. */
+int check_apart(const W4A16KvCache *cache, const KvView &kv, const void *k, size_t kb, const void *v, size_t vb, const char *what) {
+    const size_t cb = kv_bytes(cache), sb = kv_scale_bytes(cache);
+    for (const void *dst : {(const void *)cache->k, (const void *)cache->v})
+        if (overlap(dst, cb, k, kb) || overlap(dst, cb, v, vb))
+            return set_error(W4A16_ERR_CONFIG, "%s: the rows overlap the cache", what);
+    for (const void *dst : {(const void *)kv.k_scale, (const void *)kv.v_scale})
+        if (overlap(dst, sb, k, kb) || overlap(dst, sb, v, vb))
+            return set_error(W4A16_ERR_CONFIG, "%s: the rows overlap the cache's scales", what);
+    const struct { const void *p; size_t n; } parts[] = {{cache->k, cb}, {cache->v, cb}, {kv.k_scale, sb}, {kv.v_scale, sb}};
+    for (int i = 0; i < 4; ++i)
+        for (int j = 0; j < i; ++j)
+            if (overlap(parts[i].p, parts[i].n, parts[j].p, parts[j].n))
+                return set_error(W4A16_ERR_CONFIG, "%s: the cache's keys, values and scales overlap", what);
+    return W4A16_OK;
+}
+
+} // namespace
+
 extern "C" int w4a16_kv_write_bf16(const W4A16KvCache *cache, const W4A16KvBatch *batch, const uint16_t *k,
                                    long long k_row_stride, long long k_head_stride, const uint16_t *v,
                                    long long v_row_stride, long long v_head_stride, void *stream) {
@@ -246,18 +432,8 @@ extern "C" int w4a16_kv_write_bf16(const W4A16KvCache *cache, const W4A16KvBatch
     const size_t vb = strided_bytes(kv.rows, v_row_stride, kv.heads, v_head_stride, cache->head_dim);
     if (!kb || !vb)
         return set_error(W4A16_ERR_CONFIG, "%s: strides must be multiples of 8 elements from 0", what);
-    const size_t cb = kv_bytes(cache), sb = kv_scale_bytes(cache);
-    for (const void *dst : {(const void *)cache->k, (const void *)cache->v})
-        if (overlap(dst, cb, k, kb) || overlap(dst, cb, v, vb))
-            return set_error(W4A16_ERR_CONFIG, "%s: the rows overlap the cache", what);
-    for (const void *dst : {(const void *)kv.k_scale, (const void *)kv.v_scale})
-        if (overlap(dst, sb, k, kb) || overlap(dst, sb, v, vb))
-            return set_error(W4A16_ERR_CONFIG, "%s: the rows overlap the cache's scales", what);
-    const struct { const void *p; size_t n; } parts[] = {{cache->k, cb}, {cache->v, cb}, {kv.k_scale, sb}, {kv.v_scale, sb}};
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < i; ++j)
-            if (overlap(parts[i].p, parts[i].n, parts[j].p, parts[j].n))
-                return set_error(W4A16_ERR_CONFIG, "%s: the cache's keys, values and scales overlap", what);
+    st = check_apart(cache, kv, k, kb, v, vb, what);
+    if (st) return st;
     hipStream_t s = static_cast<hipStream_t>(stream);
     auto launch = cache->head_dim == 64 ? launch_write<64> : cache->head_dim == 128 ? launch_write<128> : launch_write<256>;
     launch(cache->format, kv, k, k_row_stride, k_head_stride, v, v_row_stride, v_head_stride, s);
@@ -285,4 +461,67 @@ extern "C" int w4a16_kv_read_bf16(const W4A16KvCache *cache, const W4A16KvBatch 
     auto launch = cache->head_dim == 64 ? launch_read<64> : cache->head_dim == 128 ? launch_read<128> : launch_read<256>;
     launch(cache->format, kv, k, v, s);
     return hip_status(hipGetLastError(), "kv read launch");
+}
+
+extern "C" int w4a16_kv_append_rope_bf16(const W4A16KvCache *cache, const W4A16KvBatch *batch, const uint16_t *k,
+                                         long long k_row_stride, long long k_head_stride, const uint16_t *v,
+                                         long long v_row_stride, long long v_head_stride, const uint16_t *q,
+                                         long long q_row_stride, long long q_head_stride, int q_heads, uint16_t *q_out,
+                                         long long q_out_row_stride, long long q_out_head_stride,
+                                         const float *inv_freq, int rotary_dim, int interleaved,
+                                         const int32_t *positions, void *stream) {
+    const char *what = "w4a16_kv_append_rope_bf16";
+    KvView kv;
+    int st = kv_check(cache, batch, what, &kv);
+    if (st) return st;
+    const int dim = cache->head_dim;
+    if (rotary_dim < 8 || rotary_dim > dim || rotary_dim % 8)
+        return set_error(W4A16_ERR_CONFIG, "%s: rotary_dim=%d is no multiple of 8 from 8 to head_dim=%d", what, rotary_dim, dim);
+    if (q_heads < 0 || q_heads > 65535 || (q == nullptr) != (q_heads == 0) || (q == nullptr) != (q_out == nullptr))
+        return set_error(W4A16_ERR_CONFIG, "%s: q_heads=%d (0 to 65535) for queries that are %s and %s", what, q_heads,
+                         q ? "given" : "null", q_out ? "wanted" : "not");
+    if (kv.rows == 0 || kv.seqs == 0) return W4A16_OK;
+    if (!k || !v || !inv_freq) return set_error(W4A16_ERR_CONFIG, "%s: null buffer", what);
+    if (misaligned(k) || misaligned(v) || misaligned(q) || misaligned(q_out))
+        return set_error(W4A16_ERR_CONFIG, "%s: buffers must be 16-byte aligned", what);
+    if (((uintptr_t)inv_freq | (uintptr_t)positions) & 3)
+        return set_error(W4A16_ERR_CONFIG, "%s: inv_freq and positions must be 4-byte aligned", what);
+    drop_strides_of_one(kv.rows, &k_row_stride, kv.heads, &k_head_stride);
+    drop_strides_of_one(kv.rows, &v_row_stride, kv.heads, &v_head_stride);
+    const size_t kb = strided_bytes(kv.rows, k_row_stride, kv.heads, k_head_stride, dim);
+    const size_t vb = strided_bytes(kv.rows, v_row_stride, kv.heads, v_head_stride, dim);
+    size_t qb = 0, ob = 0;
+    if (q) {
+        drop_strides_of_one(kv.rows, &q_row_stride, q_heads, &q_head_stride);
+        drop_strides_of_one(kv.rows, &q_out_row_stride, q_heads, &q_out_head_stride);
+        qb = strided_bytes(kv.rows, q_row_stride, q_heads, q_head_stride, dim);
+        ob = strided_bytes(kv.rows, q_out_row_stride, q_heads, q_out_head_stride, dim);
+    }
+    if (!kb || !vb || (q && (!qb || !ob)))
+        return set_error(W4A16_ERR_CONFIG, "%s: strides must be multiples of 8 elements from 0", what);
+    st = check_apart(cache, kv, k, kb, v, vb, what);
+    if (st) return st;
+    const size_t cb = kv_bytes(cache), sb = kv_scale_bytes(cache), fb = (size_t)rotary_dim * 2,
+                 pb = positions ? (size_t)kv.rows * 4 : 0;
+    const struct { const void *p; size_t n; } held[] = {{cache->k, cb}, {cache->v, cb}, {kv.k_scale, sb}, {kv.v_scale, sb}},
+        others[] = {{q, qb}, {inv_freq, fb}, {positions, pb}, {q_out, ob}};
+    for (const auto &h : held)
+        for (const auto &o : others)
+            if (overlap(h.p, h.n, o.p, o.n))
+                return set_error(W4A16_ERR_CONFIG, "%s: queries, frequencies or positions overlap the cache", what);
+    if (q) {
+        const RowsView kr = {k, kb, k_row_stride, k_head_stride, kv.heads}, vr = {v, vb, v_row_stride, v_head_stride, kv.heads},
+                       qr = {q, qb, q_row_stride, q_head_stride, q_heads},
+                       out = {q_out, ob, q_out_row_stride, q_out_head_stride, q_heads};
+        if (!rows_apart(kv.rows, out, dim)) return set_error(W4A16_ERR_CONFIG, "%s: output rows overlap each other", what);
+        if ((!rows_same(out, qr) && !rows_beside(kv.rows, out, qr, dim)) || !rows_beside(kv.rows, out, kr, dim) ||
+            !rows_beside(kv.rows, out, vr, dim) || overlap(q_out, ob, inv_freq, fb) || overlap(q_out, ob, positions, pb))
+            return set_error(W4A16_ERR_CONFIG, "%s: q_out overlaps another tensor of the call", what);
+    }
+    const AppendArgs a = {k, v, q, q_out, k_row_stride, k_head_stride, v_row_stride, v_head_stride, q_row_stride, q_head_stride,
+                          q_out_row_stride, q_out_head_stride, inv_freq, positions, q_heads, rotary_dim / 2, interleaved != 0};
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    auto launch = dim == 64 ? launch_append<64> : dim == 128 ? launch_append<128> : launch_append<256>;
+    launch(cache->format, kv, a, s);
+    return hip_status(hipGetLastError(), "kv append launch");
 }

@@ -101,6 +101,8 @@ _SIGNATURES = {
     "test_gemm_int4": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i]),
     "test_silu_mul_packed": (_i, [_vp, _vp, _i, _i]),
     "w4a16_kv_write_bf16": (_i, [_vp, _vp, _vp, _ll, _ll, _vp, _ll, _ll, _vp]),
+    "w4a16_kv_append_rope_bf16": (_i, [_vp, _vp, _vp, _ll, _ll, _vp, _ll, _ll, _vp, _ll, _ll, _i, _vp, _ll, _ll, _vp, _i, _i, _vp,
+                                       _vp]),
     "w4a16_kv_read_bf16": (_i, [_vp, _vp, _vp, _vp, _vp]),
     "w4a16_paged_attention_workspace": (_i, [_vp, _vp, _i, ctypes.POINTER(ctypes.c_size_t)]),
     "w4a16_paged_attention_bf16": (_i, [_vp, _vp, _vp, _ll, _ll, _i, ctypes.c_float, _i, _i, _vp, _ll, _ll, _vp, _vp,
@@ -763,6 +765,48 @@ class KvCache:
         if st:
             _check(st, "KvCache.write")
 
+    def append(self, k, v, batch, rope, q=None, positions=None, out=None, stream=None):
+        """Writes the batch's rows of k and v [rows, kv_heads, head_dim], k turned by `rope` (a Rope). `q` [rows, q_heads,
+        head_dim]: queries to be turned beside them; returns them as a new tensor, or in `out` (which may be q itself), and None without
+        any. positions: int32 [rows], where they are not the rows' places in their sequences. Strided views are fine."""
+        import torch
+
+        if stream is not None and q is not None and out is None:
+            with _under(stream, self.device):
+                return self.append(k, v, batch, rope, q, positions)
+        what = "KvCache.append"
+        index = _on_current(self.device, what)
+        batch.check(self.device, what)
+        rows, dim = batch.rows, self.head_dim
+        shape = (rows, self.kv_heads, dim)
+        kp, k_row, k_head = _rows3(k, shape, self.device, "KvCache.append k")
+        vp, v_row, v_head = _rows3(v, shape, self.device, "KvCache.append v")
+        if rope.inv_freq.device != self.device:
+            _refuse(f"{what}: the frequencies are on {rope.inv_freq.device}")
+        pp = None if positions is None else _exactly(positions, (rows,), torch.int32, self.device, "KvCache.append positions")
+        qp, q_row, q_head, q_heads, op, o_row, o_head = None, 0, 0, 0, None, 0, 0
+        if q is not None:
+            q_heads = q.shape[1] if len(q.shape) == 3 else 0
+            shape = (rows, q_heads, dim)
+            qp, q_row, q_head = _rows3(q, shape, self.device, "KvCache.append q")
+            if out is None:
+                make = torch.zeros if batch.padded else torch.empty
+                out = make(shape, dtype=q.dtype, device=self.device)
+                op, o_row, o_head = out.data_ptr(), q_heads * dim, dim
+            else:
+                op, o_row, o_head = _rows3(out, shape, self.device, "KvCache.append out")
+            if q_heads == 0 or rows == 0:
+                qp = op = None  # nothing to turn
+                q_heads = 0
+        elif out is not None:
+            _refuse(f"{what}: out without q")
+        st = lib.w4a16_kv_append_rope_bf16(self._ref, batch._ref, kp, k_row, k_head, vp, v_row, v_head, qp, q_row, q_head, q_heads, op,
+                                           o_row, o_head, rope._pointer, rope.rotary_dim, rope.interleaved, pp,
+                                           _raw_stream(stream, index))
+        if st:
+            _check(st, what)
+        return out
+
     def read(self, batch, out=None, stream=None):
         """The batch's rows out of the cache: (k, v) as BF16 [rows, kv_heads, head_dim]. Without
         `out` rows of no sequence are zeros; with it (two such tensors, contiguous) they are left as they were."""
@@ -784,6 +828,32 @@ class KvCache:
             k, v = (_rows3_dense(t, (batch.rows, self.kv_heads, self.head_dim), self.device, "KvCache.read out") for t in out)
         _check(lib.w4a16_kv_read_bf16(self._ref, batch._ref, k, v, _raw_stream(stream, index)), "KvCache.read")
         return out
+
+
+class Rope:
+    """How positions turn keys and queries: inv_freq, FP32 on the device, are the angles a position adds to each of the first
+    inv_freq.numel() pairs of a head's values; pair i is values (i, i + pairs), or (2 i, 2 i + 1) if interleaved. The handle keeps the
+    tensor, whose values are read at run time."""
+
+    def __init__(self, inv_freq, interleaved=False):
+        import torch
+
+        if not hasattr(inv_freq, "is_cuda") or not inv_freq.is_cuda or inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or \
+                not inv_freq.is_contiguous() or inv_freq.numel() % 4 or not inv_freq.numel():
+            _refuse("Rope: inv_freq is no dense FP32 CUDA tensor of a multiple of four angles")
+        self.inv_freq, self.interleaved = inv_freq, 1 if interleaved else 0
+        self.rotary_dim = 2 * inv_freq.numel()
+        self._pointer = inv_freq.data_ptr()
+
+    @classmethod
+    def of(cls, rotary_dim, base=10000.0, interleaved=False, device="cuda"):
+        """Angles base ** (-2 i / rotary_dim)."""
+        import torch
+
+        if rotary_dim < 8 or rotary_dim % 8:
+            _refuse(f"Rope: rotary_dim={rotary_dim} is no multiple of 8")
+        exponent = torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim
+        return cls((float(base) ** -exponent).to(torch.float32).to(device), interleaved)
 
 
 class KvBatch:

@@ -405,6 +405,22 @@ int w4a16_kv_write_bf16(const W4A16KvCache *cache, const W4A16KvBatch *batch, co
                         long long k_row_stride, long long k_head_stride, const uint16_t *v,
                         long long v_row_stride, long long v_head_stride, void *stream);
 
+/* The same for keys that are still to be turned by their positions, with the rows of q beside them. Of every head of k and
+ * q the first rotary_dim values (a multiple of 8 from 8 to head_dim) are pairs i = 0 .. rotary_dim / 2 - 1, values (i, i + rotary_dim / 2),
+ * or (2 i, 2 i + 1) if interleaved; a pair (a, b) becomes (a cos - b sin, b cos + a sin) of the angle position *
+ * inv_freq[i]. The angle is reduced in FP64, cos, sin and the turn are FP32, and what they give is rounded once: to
+ * BF16, or to the cache's codes by its rule for the FP32 values (a row that a turn takes past FP32 is one with an infinity). Values from
+ * rotary_dim on and v are as they were.
+ * positions: [rows], or NULL for the rows' places (kv_lens less the rows from the row on). q [rows][q_heads][head_dim]
+ * is written to q_out (which may be q itself, with its strides), also where a row has no place in the cache; q NULL (and
+ * q_heads 0): no queries. Rows of no sequence are left as they were. inv_freq: [rotary_dim / 2] on the device, read at run time as positions are. */
+int w4a16_kv_append_rope_bf16(const W4A16KvCache *cache, const W4A16KvBatch *batch, const uint16_t *k,
+                              long long k_row_stride, long long k_head_stride, const uint16_t *v,
+                              long long v_row_stride, long long v_head_stride, const uint16_t *q,
+                              long long q_row_stride, long long q_head_stride, int q_heads, uint16_t *q_out,
+                              long long q_out_row_stride, long long q_out_head_stride, const float *inv_freq,
+                              int rotary_dim, int interleaved, const int32_t *positions, void *stream);
+
 /* Reads the batch's rows out of the cache as BF16: code * scale, rounded to nearest even once.
  * k, v: [rows][kv_heads][head_dim], contiguous. */
 int w4a16_kv_read_bf16(const W4A16KvCache *cache, const W4A16KvBatch *batch, uint16_t *k,
