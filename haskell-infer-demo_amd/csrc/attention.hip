@@ -15,6 +15,10 @@
  *
  * An 8-bit cache's codes are BF16 and FP16 values; their scales multiply the scores (K) and the weights
  * (V) in FP32.
+ *
+ * TREE: a sequence's last tokens are the nodes of a tree, and a row sees of them those that its bits name. The tokens before
+ * them and those that no row of a tile may see are found as without; a step that holds nodes is one that is
+ * cut, in which a lane has the bits of its row's next tokens in one word.
  */
 #include <cmath>
 
@@ -41,6 +45,7 @@ struct AttnArgs {
     int over, upto;   /* only sequences of over < rows <= upto (token, head) rows */
     float scale;      /* |scale| log2(e) */
     uint32_t flip;    /* sign bits of a BF16 pair of q: a negative scale turns its sign over */
+    W4A16KvTree tree; /* of the kernels with TREE */
 };
 
 constexpr int kFewestTokens = 256; /* of a split of the chunk kernel */
@@ -60,6 +65,7 @@ struct Tile {
     int begin, end, active; /* this split's keys; how many splits have any */
     int window;             /* 0 where it cuts nothing */
     int seq;
+    int base, nodes;        /* TREE: the tree's first token, and how many it has */
 };
 
 /* The end of the keys that a row at `place` sees. */
@@ -68,8 +74,14 @@ __device__ __forceinline__ int row_end(const AttnArgs &a, const Tile &t, int pla
     return end < t.length ? end : t.length;
 }
 
+/* Nodes that a sequence's tree has. */
+__device__ __forceinline__ int tree_nodes(const AttnArgs &a, int seq) {
+    const int n = a.tree.sizes ? a.tree.sizes[seq] : a.tree.nodes;
+    return n < 0 ? 0 : n > a.tree.nodes ? a.tree.nodes : n;
+}
+
 /* The rest of a tile from its sequence's tokens (old + news) and rows, and its start. */
-template <int RM>
+template <int RM, bool TREE>
 __device__ __forceinline__ void fill_tile(const AttnArgs &a, Tile *t) {
     const int all = t->news * a.group;
     t->rows = all - t->start < RM ? all - t->start : RM;
@@ -79,17 +91,51 @@ __device__ __forceinline__ void fill_tile(const AttnArgs &a, Tile *t) {
     t->window = a.window <= t->old + t->news ? a.window : 0;
     t->hi = row_end(a, *t, t->old + t1);
     t->all_hi = row_end(a, *t, t->old + t0);
-    t->lo = t->window ? t->old + t0 - t->window + 1 : 0;
+    int least = t->old + t0; /* position of any of the tile's rows */
+    if constexpr (TREE) {
+        t->base = t->old + t->news - t->nodes;
+        if (t->base < t->all_hi) t->all_hi = t->base;
+        if (t->base < least) least = t->base;
+    }
+    t->lo = t->window ? least - t->window + 1 : 0;
     t->all_lo = t->window ? t->old + t1 - t->window + 1 : 0;
     if (t->lo < 0) t->lo = 0;
     if (t->hi <= t->lo) t->hi = t->lo = 0; /* the window may begin behind the last key */
+}
+
+/* TREE: which of the 32 tokens from `at` on the sequence's row `token` sees (none: -1), bit k for token at + k. Everything that it
+ * follows from is found anew at each step that needs it: kept over a loop it would cost registers that there are not. */
+__device__ __forceinline__ uint32_t tree_sees(const AttnArgs &a, const Tile &t, int token, int at) {
+    if (token < 0) return 0u;
+    const int row = t.first_row + token, place = t.old + token;
+    /* [from, to) of the 32 */
+    const int to = row_end(a, t, place) - at;
+    int from = 0;
+    if (t.window) {
+        /* a node's position lies between its tree's first token and its place */
+        int position = place;
+        if (place >= t.base) {
+            const int p = a.tree.positions[row];
+            position = p < t.base ? t.base : p > place ? place : p;
+        }
+        from = position - t.window + 1 - at;
+    }
+    uint32_t sees = (to >= 32 ? 0xFFFFFFFFu : to > 0 ? (1u << to) - 1u : 0u) & (from <= 0 ? 0xFFFFFFFFu : from < 32 ? 0xFFFFFFFFu << from : 0u);
+    const int node = at - t.base; /* of the first of them; the tokens before node 0 are no nodes */
+    if (node > -32) {
+        const int words = (a.tree.nodes + 63) >> 6 << 1, w = node >> 5;
+        const uint32_t *bits = reinterpret_cast<const uint32_t *>(a.tree.seen) + (long long)row * words;
+        const uint32_t low = w < 0 ? 0xFFFFFFFFu : w < words ? bits[w] : 0u, high = w + 1 < words ? bits[w + 1] : 0u;
+        sees &= __builtin_amdgcn_alignbit(high, low, node & 31);
+    }
+    return sees;
 }
 
 constexpr int kMostUnits = 1 << 23; /* of 2^30 tokens */
 
 /* Finds the `item`th tile of RM rows: the sequences' tiles are counted 64 sequences at a time.
  * Sequences whose rows do not lie in the call's tensors have none. */
-template <int RM>
+template <int RM, bool TREE>
 __device__ __forceinline__ bool find_tile(const AttnArgs &a, int item, int split, Tile *t) {
     const int lane = threadIdx.x & 63;
     int left = item;
@@ -116,8 +162,9 @@ __device__ __forceinline__ bool find_tile(const AttnArgs &a, int item, int split
         if (base + 64 >= a.kv.seqs) return false;
     }
     t->seq = __builtin_amdgcn_readfirstlane(t->seq);
+    if constexpr (TREE) t->nodes = __builtin_amdgcn_readfirstlane(tree_nodes(a, t->seq));
     t->old = __builtin_amdgcn_readfirstlane(kv_length(a.kv, t->seq)) - t->news;
-    fill_tile<RM>(a, t);
+    fill_tile<RM, TREE>(a, t);
     /* splits begin at multiples of 32 tokens and have at least kFewestTokens */
     const int from = t->lo & ~31, span = t->hi - from;
     int per = (span + a.splits - 1) / a.splits;
@@ -140,12 +187,13 @@ __device__ __forceinline__ bool find_tile(const AttnArgs &a, int item, int split
 struct Seqs { /* 64 sequences, one a lane */
     int first, news, old, from; /* old: position of its first row; from: where the first key that any of its rows sees is cut */
     int pairs, units;              /* its (tile, head) pairs, units of each */
+    int nodes;                     /* TREE */
 };
 
-template <int RM>
+template <int RM, bool TREE>
 __device__ __forceinline__ Seqs load_seqs(const AttnArgs &a, int base) {
     const int s = base + (threadIdx.x & 63);
-    Seqs q = {0, 0, 0, 0, 0, 1};
+    Seqs q = {0, 0, 0, 0, 0, 1, 0};
     if (s < a.kv.seqs) {
         q.first = a.kv.starts[s];
         const int last = a.kv.starts[s + 1];
@@ -153,7 +201,12 @@ __device__ __forceinline__ Seqs load_seqs(const AttnArgs &a, int base) {
         if (q.first >= 0 && last <= a.kv.rows && last > q.first) q.news = last - q.first;
         if (q.news * a.group <= a.over || q.news * a.group > a.upto) q.news = 0;
         q.old = length - q.news;
-        if (a.window && a.window <= length && q.old - a.window + 1 > 0) q.from = (q.old - a.window + 1) & ~31;
+        int least = q.old;
+        if constexpr (TREE) {
+            q.nodes = tree_nodes(a, s);
+            if (length - q.nodes < least) least = length - q.nodes;
+        }
+        if (a.window && a.window <= length && least - a.window + 1 > 0) q.from = (least - a.window + 1) & ~31;
         if (held > q.from) q.units = (held - q.from + kUnit - 1) / kUnit;
         else q.from = 0; /* no row sees any */
         q.pairs = (q.news * a.group + RM - 1) / RM * a.kv.heads;
@@ -163,9 +216,9 @@ __device__ __forceinline__ Seqs load_seqs(const AttnArgs &a, int base) {
 
 /* Units of a part; *q is left with the first 64 sequences. N / (blocks wanted) where that makes no
  * more parts than blocks; each pair's last part is on average half as long. */
-template <int RM>
+template <int RM, bool TREE>
 __device__ __forceinline__ int part_units(const AttnArgs &a, Seqs *q) {
-    *q = load_seqs<RM>(a, 0);
+    *q = load_seqs<RM, TREE>(a, 0);
     if (a.splits == 0) return kMostUnits; /* pairs are whole */
     /* n < 2^47 in two pieces, whose sums over 64 lanes fit 32 bits */
     unsigned long long total = 0;
@@ -178,7 +231,7 @@ __device__ __forceinline__ int part_units(const AttnArgs &a, Seqs *q) {
         pairs += __builtin_amdgcn_readlane(wave_upto(s.pairs), 63);
         base += 64;
         if (base >= a.kv.seqs) break;
-        s = load_seqs<RM>(a, base);
+        s = load_seqs<RM, TREE>(a, base);
     }
     const unsigned long long wanted = pairs < a.splits ? a.splits - pairs / 2 : a.splits;
     const unsigned long long each = (total + wanted - 1) / wanted;
@@ -187,10 +240,10 @@ __device__ __forceinline__ int part_units(const AttnArgs &a, Seqs *q) {
 
 /* The part of this block (PAIR false) or the (tile, head) pair of number `index` (true): the tile, its head, its number of
  * parts, and the number of its first one. */
-template <int RM, bool PAIR>
+template <int RM, bool PAIR, bool TREE>
 __device__ __forceinline__ bool find_part(const AttnArgs &a, int index, Tile *t, int *head, int *first_part) {
     Seqs q;
-    const int each = part_units<RM>(a, &q);
+    const int each = part_units<RM, TREE>(a, &q);
     int left = index, before = 0; /* parts of the sequences before */
     for (int base = 0;;) {
         const int per = (q.units + each - 1) / each, parts = q.pairs * per;
@@ -202,6 +255,7 @@ __device__ __forceinline__ bool find_part(const AttnArgs &a, int index, Tile *t,
             t->first_row = __builtin_amdgcn_readlane(q.first, l);
             t->news = __builtin_amdgcn_readlane(q.news, l);
             t->old = __builtin_amdgcn_readlane(q.old, l);
+            if constexpr (TREE) t->nodes = __builtin_amdgcn_readlane(q.nodes, l);
             const int from = __builtin_amdgcn_readlane(q.from, l);
             t->active = __builtin_amdgcn_readlane(per, l);
             const int in_seq = left - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(PAIR ? q.pairs : parts, l));
@@ -209,7 +263,7 @@ __device__ __forceinline__ bool find_part(const AttnArgs &a, int index, Tile *t,
             *first_part = before + __builtin_amdgcn_readlane(upto_parts, l) - __builtin_amdgcn_readlane(parts, l) + pair * t->active;
             *head = pair % a.kv.heads;
             t->start = pair / a.kv.heads * RM;
-            fill_tile<RM>(a, t);
+            fill_tile<RM, TREE>(a, t);
             t->begin = from + part * each * kUnit;
             t->end = part + 1 < t->active && t->begin + each * kUnit < t->hi ? t->begin + each * kUnit : t->hi;
             return true;
@@ -218,7 +272,7 @@ __device__ __forceinline__ bool find_part(const AttnArgs &a, int index, Tile *t,
         before += __builtin_amdgcn_readlane(upto_parts, 63);
         base += 64;
         if (base >= a.kv.seqs) return false;
-        q = load_seqs<RM>(a, base);
+        q = load_seqs<RM, TREE>(a, base);
     }
 }
 
@@ -348,7 +402,7 @@ constexpr int rows_blocks(int dim, int format, int rt) {
  * BF16 D = 64 102 us (5.2 TB/s), D = 128 192 (5.6), D = 256 200 (5.4); FP8 66 (4.4), 108 (5.1), 107 (5.1); INT8
  * 70, 110, 109.
  */
-template <int D, int FMT, int RT>
+template <int D, int FMT, int RT, bool TREE>
 __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel(AttnArgs a) {
     constexpr int RM = 16 * RT, E = D / 16, KS = D / 32; /* values of V a lane has; steps of the K product */
     constexpr bool kCoded = FMT != W4A16_KV_BF16;
@@ -357,7 +411,7 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
     const int mask = (1 << a.kv.shift) - 1;
     Tile t;
     int head, first_part;
-    if (!find_part<RM, false>(a, blockIdx.x, &t, &head, &first_part)) return;
+    if (!find_part<RM, false, TREE>(a, blockIdx.x, &t, &head, &first_part)) return;
 
     const int32_t *table = a.kv.table + (long long)t.seq * a.kv.table_stride;
     /* Pages of this lane's K tokens and V tokens (page sizes are multiples of 8, so four
@@ -445,7 +499,7 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
 
     /* this lane's rows: their queries as the products' operand, and the keys they see */
     bf8 q[RT][KS];
-    int lo[RT], hi[RT];
+    int lo[RT], hi[RT]; /* TREE: unused, tree_sees instead */
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
         const int i = r * 16 + n, token = (t.start + i) / a.group, h = head * a.group + (t.start + i) % a.group;
@@ -464,6 +518,11 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
 
     f4 acc[RT][E];
     float m[RT], l[RT];
+    auto token_of = [&](int r) { /* TREE: of this lane's row */
+        int i = r * 16 + n;
+        asm volatile("" : "+v"(i)); /* or it is kept */
+        return i < t.rows ? (t.start + i) / a.group : -1;
+    };
     float spoiled[RT] = {}; /* 1: this lane's row has seen a scale that is no number */
     int v_exp = kLift + 1; /* biased exponent of the power of two that the weights are over (8-bit caches) */
 #pragma unroll
@@ -499,12 +558,15 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
                      * without it. */
 #pragma unroll
                     for (int r = 0; r < RT; ++r) {
+                        uint32_t row_sees = 0;
+                        if constexpr (TREE) row_sees = tree_sees(a, t, token_of(r), t0) >> (4 * g);
 #pragma unroll
                         for (int c = 0; c < 2; ++c)
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
                                 const int at = t0 + 16 * c + 4 * g + i;
-                                const bool sees = (at >= lo[r]) & (at < hi[r]) & !(fabsf(vs[c][i]) < __builtin_inff());
+                                const bool shown = TREE ? row_sees >> (16 * c + i) & 1u : (at >= lo[r]) & (at < hi[r]);
+                                const bool sees = shown & !(fabsf(vs[c][i]) < __builtin_inff());
                                 spoiled[r] = sees ? 1.0f : spoiled[r];
                             }
                     }
@@ -599,6 +661,9 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
         uint32_t p[RT][4], p_rest[kCoded ? 1 : RT][4];
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
+            uint32_t row_sees = 0;
+            if constexpr (TREE)
+                if (cut) row_sees = tree_sees(a, t, token_of(r), t0) >> (4 * g);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 if constexpr (kCoded) s[r][c] *= ks[c];
@@ -607,7 +672,7 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int at = t0 + 16 * c + 4 * g + i;
-                        const bool hidden = !there[c] | (at < lo[r]) | (at >= hi[r]);
+                        const bool hidden = TREE ? !there[c] | !(row_sees >> (16 * c + i) & 1u) : !there[c] | (at < lo[r]) | (at >= hi[r]);
                         s[r][c][i] = hidden ? -__builtin_inff() : s[r][c][i];
                     }
             }
@@ -646,6 +711,10 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
                 /* An infinity or a NaN among values that not every row sees: 0 times it would reach the
                  * rows that do not. Those that do have it added as it is, and the products go without it.
                  * Value E (4 g + i) + e of a token, which is acc[][e][i], is lane 4 g + i's of its 16. */
+                uint32_t row_sees[RT];
+                if constexpr (TREE)
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) row_sees[r] = tree_sees(a, t, token_of(r), t0);
 #pragma unroll
                 for (int x = 0; x < 8; ++x) {
                     bool some = false;
@@ -667,7 +736,8 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
                                 for (int r = 0; r < RT; ++r)
 #pragma unroll
                                     for (int half = 0; half < 2; ++half) {
-                                        const bool adds = (at >= lo[r]) & (at < hi[r]) & ((f[half] & 0x7F800000u) == 0x7F800000u);
+                                        const bool shown = TREE ? row_sees[r] >> (at - t0) & 1u : (at >= lo[r]) & (at < hi[r]);
+                                        const bool adds = shown & ((f[half] & 0x7F800000u) == 0x7F800000u);
                                         acc[r][2 * w + half][i] += adds ? __builtin_bit_cast(float, f[half]) : 0.0f;
                                     }
                             }
@@ -823,20 +893,21 @@ __device__ __forceinline__ uint32_t widen_f16(uint32_t codes) {
  * of a tile over 128 rows). 4096 rows over 16384 tokens, 32 heads (16 of 256 values): BF16 D = 64 671 us, 717
  * TFLOP/s; D = 128 979, 983; D = 256 1017, 946; INT8 859, 1193, 1308; FP8 748, 1134, 1269.
  */
-template <int D, int FMT>
+template <int D, int FMT, bool TIGHT, bool TREE>
 struct Chunk {
     static constexpr bool kCoded = FMT != W4A16_KV_BF16;
     static constexpr int kRows = 128, BN = D == 256 ? 32 : 64;
     static constexpr int kPieces = D / 8;                              /* of 8 values a token */
     static constexpr int kLoads = BN * D * (kCoded ? 1 : 2) / (256 * 16); /* 16-byte loads a thread and matrix */
     static constexpr int kSwizzle = kPieces < 16 ? kPieces - 1 : 15;
-    /* LDS: [2]{K, V}, then scales [2][2][BN], pages [3][BN], flags */
+    /* LDS: [2]{K, V}, then scales [2][2][BN], pages [3][BN], flags, queries, rows' tokens (TREE) */
     static constexpr int kTile = BN * D * 2;
     static constexpr int kScales = 4 * kTile, kPages = kScales + (kCoded ? 4 * BN * 4 : 0);
     static constexpr int kFlags = kPages + 3 * BN * 4, kQueries = kFlags + 32; /* bad[3], exponents[2] */
     /* the last steps' queries of a K product that stand in LDS, [step][half][row]: the registers of 8-bit
      * codes on their way leave no room for all of 256 values, or of 64 where four blocks are to fit */
-    static constexpr int kStored = !kCoded ? 0 : D == 256 ? 3 : D == 64 ? 1 : 0, kBytes = kQueries + kStored * 2 * kRows * 16;
+    static constexpr int kStored = !kCoded || (!TIGHT && !TREE) ? 0 : D == 256 ? 3 : D == 64 ? 1 : 0;
+    static constexpr int kTokens = kQueries + kStored * 2 * kRows * 16, kBytes = kTokens + (TREE ? kRows * 4 : 0);
 };
 
 /* 16 bytes a lane from memory to LDS, lane after lane from `to` (the same on every lane). */
@@ -873,9 +944,9 @@ __device__ __forceinline__ void interleave() {
  * registers, and gains nothing: 680 and 685). */
 constexpr int chunk_blocks(int dim, bool tight) { return dim > 64 ? 2 : tight ? 4 : 3; }
 
-template <int D, int FMT, bool TIGHT>
+template <int D, int FMT, bool TIGHT, bool TREE>
 __global__ __launch_bounds__(256, chunk_blocks(D, TIGHT)) void attn_chunk_kernel(AttnArgs a) {
-    using C = Chunk<D, FMT>;
+    using C = Chunk<D, FMT, TIGHT, TREE>;
     constexpr bool kCoded = C::kCoded;
     constexpr int BN = C::BN, RM = C::kRows, kHalves = BN / 32, KS = D / 16, DB = D / 32;
     constexpr int kFar = D == 256 ? 1 : 2;
@@ -890,7 +961,7 @@ __global__ __launch_bounds__(256, chunk_blocks(D, TIGHT)) void attn_chunk_kernel
     /* the last tiles of a sequence see the most keys: those first */
     const int item = a.items - 1 - (int)(blockIdx.x / a.kv.heads);
     Tile t;
-    if (!find_tile<RM>(a, item, split, &t)) return;
+    if (!find_tile<RM, TREE>(a, item, split, &t)) return;
     if (split >= t.active) return;
 
     const int32_t *table = a.kv.table + (long long)t.seq * a.kv.table_stride;
@@ -1003,12 +1074,22 @@ __global__ __launch_bounds__(256, chunk_blocks(D, TIGHT)) void attn_chunk_kernel
     }
 
     /* this lane's row: its queries and the keys it sees */
-    const int i_row = wave * 32 + n, token = (t.start + i_row) / a.group, h = head * a.group + (t.start + i_row) % a.group;
-    const bool real = i_row < t.rows;
+    int i_row = wave * 32 + n, token = (t.start + i_row) / a.group, h = head * a.group + (t.start + i_row) % a.group;
+    bool real = i_row < t.rows;
     const int place = t.old + token;
+    /* TREE: unused, tree_sees instead */
     const int hi = !real ? 0 : row_end(a, t, place), lo = t.window ? place - t.window + 1 : 0;
     const uint32_t seen = hi > lo ? hi - lo : 0; /* this row sees a key where its place less lo, unsigned, is below this */
-    constexpr int kHeld = KS - (TIGHT ? C::kStored : 0);
+    /* TREE: rows' tokens, -1 where there is none; read by the waves that wrote them */
+    int *tokens = reinterpret_cast<int *>(smem + C::kTokens);
+    if constexpr (TREE) tokens[i_row] = real ? token : -1;
+    auto row_of = [&] {
+        int tid = threadIdx.x;
+        asm volatile("" : "+v"(tid)); /* or it is kept over the loop, and what follows from it */
+        return (tid >> 6) * 32 + (tid & 31);
+    };
+    auto token_of = [&] { return tokens[row_of()]; };
+    constexpr int kHeld = KS - C::kStored;
     bf8 q[kHeld], *const q_stored = reinterpret_cast<bf8 *>(smem + C::kQueries) + half * RM + i_row;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
@@ -1046,7 +1127,10 @@ __global__ __launch_bounds__(256, chunk_blocks(D, TIGHT)) void attn_chunk_kernel
                 /* a scale that is no number, at a token that not every row sees: as in attn_rows_kernel */
                 float *of = scales + (step & 1) * 2 * BN + BN;
 #pragma unroll 1
-                for (int in = 0; in < BN; ++in) spoiled |= ((uint32_t)(t0 + in - lo) < seen) & !(fabsf(of[in]) < __builtin_inff());
+                for (int in = 0; in < BN; ++in) {
+                    const bool shown = TREE ? tree_sees(a, t, token_of(), t0 + in) & 1u : (uint32_t)(t0 + in - lo) < seen;
+                    spoiled |= shown & !(fabsf(of[in]) < __builtin_inff());
+                }
                 __syncthreads();
                 if (tid < BN) of[tid] = fabsf(of[tid]) < __builtin_inff() ? of[tid] : 0.0f;
                 __syncthreads();
@@ -1084,7 +1168,9 @@ __global__ __launch_bounds__(256, chunk_blocks(D, TIGHT)) void attn_chunk_kernel
         if (cut) {
             const uint32_t at = t0 - lo;
 #pragma unroll
-            for (int c = 0; c < kHalves; ++c)
+            for (int c = 0; c < kHalves; ++c) {
+                uint32_t row_sees = 0;
+                if constexpr (TREE) row_sees = tree_sees(a, t, token_of(), t0 + 32 * c) >> (4 * half);
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
                     const int in = 32 * c + 8 * b + 4 * half;
@@ -1092,10 +1178,12 @@ __global__ __launch_bounds__(256, chunk_blocks(D, TIGHT)) void attn_chunk_kernel
                     const int each[4] = {page.x, page.y, page.z, page.w};
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const bool hidden = ((at + in + i) | (each[i] & 0x80000000u)) >= seen; /* a page of -1 as well */
+                        const bool hidden = TREE ? (each[i] < 0) | !(row_sees >> (8 * b + i) & 1u)
+                                                 : ((at + in + i) | (each[i] & 0x80000000u)) >= seen; /* a page of -1 as well */
                         s[c][4 * b + i] = hidden ? -__builtin_inff() : s[c][4 * b + i];
                     }
                 }
+            }
         }
         float most = s[0][0];
 #pragma unroll
@@ -1157,7 +1245,7 @@ __global__ __launch_bounds__(256, chunk_blocks(D, TIGHT)) void attn_chunk_kernel
                 }
                 if (__syncthreads_or(odd)) {
                     for (int in = 0; in < BN; ++in) {
-                        const bool sees = (uint32_t)(t0 + in - lo) < seen;
+                        const bool sees = TREE ? tree_sees(a, t, token_of(), t0 + in) & 1u : (uint32_t)(t0 + in - lo) < seen;
 #pragma unroll
                         for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -1212,6 +1300,12 @@ __global__ __launch_bounds__(256, chunk_blocks(D, TIGHT)) void attn_chunk_kernel
 
     /* a lane has values 32 d + 8 b + 4 half .. + 3 of its row; so does lane ^ 32 the four between */
     const float total = lane_sum32(l);
+    if constexpr (TREE) {
+        i_row = row_of();
+        token = (t.start + i_row) / a.group;
+        h = head * a.group + (t.start + i_row) % a.group;
+        real = i_row < t.rows;
+    }
     if (!real) return;
     float by = !kCoded ? 1.0f : spoiled ? __builtin_nanf("") : times_power(v_exp);
     float *partial = t.active > 1 ? partial_at<D, RM>(a, ((long long)item * a.kv.heads + head) * a.splits + split) : nullptr;
@@ -1245,17 +1339,17 @@ __global__ __launch_bounds__(256, chunk_blocks(D, TIGHT)) void attn_chunk_kernel
  * parts of the few-row kernel (EVEN). A block has 16 / SUB rows (blockIdx.y of
  * them), 16 lanes a row and part of its splits: with many splits the sum over them is what takes
  * time, so SUB parts of it run side by side and meet in LDS. */
-template <int D, int RM, int SUB, bool EVEN>
+template <int D, int RM, int SUB, bool EVEN, bool TREE>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     constexpr int kPer = D / 16, kRows = 16 / SUB;
     Tile t;
     int head, first_part = 0;
     if constexpr (EVEN) {
-        if (!find_part<RM, true>(a, blockIdx.x, &t, &head, &first_part)) return;
+        if (!find_part<RM, true, TREE>(a, blockIdx.x, &t, &head, &first_part)) return;
         if (first_part + t.active > a.blocks) return; /* sequences that overlap: not all parts were worked on */
     } else {
         head = blockIdx.x % a.kv.heads;
-        if (!find_tile<RM>(a, blockIdx.x / a.kv.heads, 0, &t)) return;
+        if (!find_tile<RM, TREE>(a, blockIdx.x / a.kv.heads, 0, &t)) return;
     }
     if (t.active < 2 || (int)blockIdx.y * kRows >= t.rows) return;
     const int lane = threadIdx.x & 15, unit = threadIdx.x >> 4, sub = unit / kRows, i = blockIdx.y * kRows + unit % kRows;
@@ -1409,12 +1503,12 @@ Plan plan_of(const W4A16KvCache *c, const W4A16KvBatch *b, int q_heads) {
     return p;
 }
 
-template <int D, int RM, bool EVEN>
+template <int D, int RM, bool EVEN, bool TREE>
 void launch_join(int parts, const AttnArgs &a, hipStream_t s) {
     const unsigned x = a.kv.heads * a.items;
-    if (parts > 16) launch_k(attn_join_kernel<D, RM, 16, EVEN>, dim3(x, RM), dim3(256), 0, s, a);
-    else if (parts > 4) launch_k(attn_join_kernel<D, RM, 4, EVEN>, dim3(x, RM / 4), dim3(256), 0, s, a);
-    else if (parts > 1) launch_k(attn_join_kernel<D, RM, 1, EVEN>, dim3(x, RM / 16), dim3(256), 0, s, a);
+    if (parts > 16) launch_k(attn_join_kernel<D, RM, 16, EVEN, TREE>, dim3(x, RM), dim3(256), 0, s, a);
+    else if (parts > 4) launch_k(attn_join_kernel<D, RM, 4, EVEN, TREE>, dim3(x, RM / 4), dim3(256), 0, s, a);
+    else if (parts > 1) launch_k(attn_join_kernel<D, RM, 1, EVEN, TREE>, dim3(x, RM / 16), dim3(256), 0, s, a);
 }
 
 AttnArgs part_args(const AttnArgs &all, const Part &p) {
@@ -1428,35 +1522,46 @@ AttnArgs part_args(const AttnArgs &all, const Part &p) {
     return a;
 }
 
-template <int D, int FMT>
+template <int D, int FMT, bool TREE>
 void launch_format(const Plan &p, const AttnArgs &all, hipStream_t s) {
     if (p.many.items) {
         const AttnArgs a = part_args(all, p.many);
-        auto kernel = attn_chunk_kernel<D, FMT, D == 256>;
-        if constexpr (D == 64 && FMT != W4A16_KV_BF16)
-            if ((long long)a.kv.heads * a.items * a.splits > chunk_blocks(D, false) * device_cus()) kernel = attn_chunk_kernel<D, FMT, true>;
-        launch_k(kernel, dim3(a.kv.heads * a.items, a.splits), dim3(256), Chunk<D, FMT>::kBytes, s, a);
-        launch_join<D, kChunkRows, false>(a.splits, a, s);
+        auto kernel = attn_chunk_kernel<D, FMT, D == 256, TREE>;
+        size_t lds = Chunk<D, FMT, D == 256, TREE>::kBytes;
+        if constexpr (D == 64 && FMT != W4A16_KV_BF16 && !TREE) /* with trees it would spill */
+            if ((long long)a.kv.heads * a.items * a.splits > chunk_blocks(D, false) * device_cus()) {
+                kernel = attn_chunk_kernel<D, FMT, true, TREE>;
+                lds = Chunk<D, FMT, true, TREE>::kBytes;
+            }
+        launch_k(kernel, dim3(a.kv.heads * a.items, a.splits), dim3(256), lds, s, a);
+        launch_join<D, kChunkRows, false, TREE>(a.splits, a, s);
     }
     if (p.few.items) {
         const AttnArgs a = part_args(all, p.few);
         const int parts = (a.splits + a.items * a.kv.heads - 1) / (a.items * a.kv.heads) + 1; /* of each, about */
         if constexpr (D <= 128)
             if (p.rt == 2) {
-                launch_k(attn_rows_kernel<D, FMT, 2>, dim3((unsigned)p.few.blocks), dim3(256), 0, s, a);
-                if (a.splits) launch_join<D, 32, true>(parts, a, s);
+                launch_k(attn_rows_kernel<D, FMT, 2, TREE>, dim3((unsigned)p.few.blocks), dim3(256), 0, s, a);
+                if (a.splits) launch_join<D, 32, true, TREE>(parts, a, s);
                 return;
             }
-        launch_k(attn_rows_kernel<D, FMT, 1>, dim3((unsigned)p.few.blocks), dim3(256), 0, s, a);
-        if (a.splits) launch_join<D, 16, true>(parts, a, s);
+        launch_k(attn_rows_kernel<D, FMT, 1, TREE>, dim3((unsigned)p.few.blocks), dim3(256), 0, s, a);
+        if (a.splits) launch_join<D, 16, true, TREE>(parts, a, s);
     }
 }
 
-template <int D>
+template <int D, bool TREE>
 void launch_dim(int format, const Plan &p, const AttnArgs &a, hipStream_t s) {
-    if (format == W4A16_KV_BF16) launch_format<D, W4A16_KV_BF16>(p, a, s);
-    else if (format == W4A16_KV_INT8) launch_format<D, W4A16_KV_INT8>(p, a, s);
-    else launch_format<D, W4A16_KV_FP8>(p, a, s);
+    if (format == W4A16_KV_BF16) launch_format<D, W4A16_KV_BF16, TREE>(p, a, s);
+    else if (format == W4A16_KV_INT8) launch_format<D, W4A16_KV_INT8, TREE>(p, a, s);
+    else launch_format<D, W4A16_KV_FP8, TREE>(p, a, s);
+}
+
+template <bool TREE>
+void launch_all(int dim, int format, const Plan &p, const AttnArgs &a, hipStream_t s) {
+    if (dim == 64) launch_dim<64, TREE>(format, p, a, s);
+    else if (dim == 128) launch_dim<128, TREE>(format, p, a, s);
+    else launch_dim<256, TREE>(format, p, a, s);
 }
 
 int check_heads(const KvView &kv, int q_heads, const char *what) {
@@ -1480,18 +1585,23 @@ extern "C" int w4a16_paged_attention_workspace(const W4A16KvCache *cache, const 
     return W4A16_OK;
 }
 
-extern "C" int w4a16_paged_attention_bf16(const W4A16KvCache *cache, const W4A16KvBatch *batch, const uint16_t *q,
-                                          long long q_row_stride, long long q_head_stride, int q_heads, float scale,
-                                          int causal, int window, uint16_t *out, long long out_row_stride,
-                                          long long out_head_stride, float *lse, void *ws, size_t ws_bytes,
-                                          void *stream) {
-    const char *what = "w4a16_paged_attention_bf16";
+namespace {
+
+int attend(const char *what, const W4A16KvCache *cache, const W4A16KvBatch *batch, const W4A16KvTree *tree, const uint16_t *q,
+           long long q_row_stride, long long q_head_stride, int q_heads, float scale, int causal, int window, uint16_t *out,
+           long long out_row_stride, long long out_head_stride, float *lse, void *ws, size_t ws_bytes, void *stream) {
     KvView kv;
     int st = kv_check(cache, batch, what, &kv);
     if (!st) st = check_heads(kv, q_heads, what);
     if (st) return st;
     if (!(scale - scale == 0.0f)) return set_error(W4A16_ERR_CONFIG, "%s: the scale is not finite", what);
     if (window < 0) return set_error(W4A16_ERR_CONFIG, "%s: window=%d is negative", what, window);
+    if (tree) {
+        if (tree->nodes < 1 || tree->nodes > 256)
+            return set_error(W4A16_ERR_CONFIG, "%s: trees of nodes=%d are not of 1 to 256", what, tree->nodes);
+        if (window && window < tree->nodes) /* a row's window would end inside its tree, by depths that the bits do not have */
+            return set_error(W4A16_ERR_CONFIG, "%s: window=%d is smaller than trees of %d nodes", what, window, tree->nodes);
+    }
     if (kv.rows == 0 || kv.seqs == 0) return W4A16_OK;
     if (!q || !out) return set_error(W4A16_ERR_CONFIG, "%s: null buffer", what);
     if (misaligned(q) || misaligned(out) || misaligned(ws) || ((uintptr_t)lse & 3))
@@ -1510,9 +1620,20 @@ extern "C" int w4a16_paged_attention_bf16(const W4A16KvCache *cache, const W4A16
                          p.ws_bytes);
     /* q and out may be the same tensor, or heads of the same rows side by side */
     bool clash = !rows_same(qr, outs) && !rows_beside(kv.rows, outs, qr, dim);
+    size_t tb = 0, pb = 0, nb = 0;
+    if (tree) {
+        if (!tree->seen || !tree->positions) return set_error(W4A16_ERR_CONFIG, "%s: null tree", what);
+        if (((uintptr_t)tree->seen & 7) || (((uintptr_t)tree->positions | (uintptr_t)tree->sizes) & 3))
+            return set_error(W4A16_ERR_CONFIG, "%s: the tree's bits must be 8-byte aligned, positions and sizes 4-byte", what);
+        tb = (size_t)kv.rows * ((tree->nodes + 63) / 64) * 8;
+        pb = (size_t)kv.rows * 4;
+        nb = tree->sizes ? (size_t)kv.seqs * 4 : 0;
+    }
     const size_t lb = lse ? (size_t)kv.rows * q_heads * 4 : 0, cb = kv_bytes(cache), sb = kv_scale_bytes(cache);
     const struct { const void *p; size_t n; } writes[] = {{out, ob}, {lse, lb}, {ws, p.ws_bytes}};
-    const struct { const void *p; size_t n; } reads[] = {{cache->k, cb}, {cache->v, cb}, {kv.k_scale, sb}, {kv.v_scale, sb}};
+    const struct { const void *p; size_t n; } reads[] = {{cache->k, cb}, {cache->v, cb}, {kv.k_scale, sb}, {kv.v_scale, sb},
+                                                         {tree ? tree->seen : nullptr, tb}, {tree ? tree->positions : nullptr, pb},
+                                                         {tree ? tree->sizes : nullptr, nb}};
     for (int i = 0; i < 3; ++i) {
         for (const auto &r : reads) clash = clash || overlap(writes[i].p, writes[i].n, r.p, r.n);
         if (i) clash = clash || overlap(writes[i].p, writes[i].n, q, qb);
@@ -1539,9 +1660,30 @@ extern "C" int w4a16_paged_attention_bf16(const W4A16KvCache *cache, const W4A16
     a.splits = a.items = a.blocks = a.over = a.upto = 0; /* part_args */
     a.scale = fabsf(scale) * 1.4426950408889634f;
     a.flip = scale < 0.0f ? 0x80008000u : 0u;
+    a.tree = tree ? *tree : W4A16KvTree{};
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (dim == 64) launch_dim<64>(cache->format, p, a, s);
-    else if (dim == 128) launch_dim<128>(cache->format, p, a, s);
-    else launch_dim<256>(cache->format, p, a, s);
+    (tree ? launch_all<true> : launch_all<false>)(dim, cache->format, p, a, s);
     return hip_status(hipGetLastError(), "paged attention launch");
+}
+
+} // namespace
+
+extern "C" int w4a16_paged_attention_bf16(const W4A16KvCache *cache, const W4A16KvBatch *batch, const uint16_t *q,
+                                          long long q_row_stride, long long q_head_stride, int q_heads, float scale,
+                                          int causal, int window, uint16_t *out, long long out_row_stride,
+                                          long long out_head_stride, float *lse, void *ws, size_t ws_bytes,
+                                          void *stream) {
+    return attend("w4a16_paged_attention_bf16", cache, batch, nullptr, q, q_row_stride, q_head_stride, q_heads, scale, causal,
+                  window, out, out_row_stride, out_head_stride, lse, ws, ws_bytes, stream);
+}
+
+extern "C" int w4a16_paged_tree_attention_bf16(const W4A16KvCache *cache, const W4A16KvBatch *batch, const W4A16KvTree *tree,
+                                               const uint16_t *q, long long q_row_stride, long long q_head_stride,
+                                               int q_heads, float scale, int window, uint16_t *out,
+                                               long long out_row_stride, long long out_head_stride, float *lse, void *ws,
+                                               size_t ws_bytes, void *stream) {
+    const char *what = "w4a16_paged_tree_attention_bf16";
+    if (!tree) return set_error(W4A16_ERR_CONFIG, "%s: null tree", what);
+    return attend(what, cache, batch, tree, q, q_row_stride, q_head_stride, q_heads, scale, 1, window, out, out_row_stride,
+                  out_head_stride, lse, ws, ws_bytes, stream);
 }

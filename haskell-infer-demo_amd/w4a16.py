@@ -17,6 +17,7 @@ Device tensors are torch CUDA tensors (on ROCm, HIP memory); torch is used only 
 and streams. There is no CPU fallback: if the library is missing the import fails.
 """
 
+import contextlib
 import ctypes
 import functools
 import os
@@ -107,6 +108,9 @@ _SIGNATURES = {
     "w4a16_paged_attention_workspace": (_i, [_vp, _vp, _i, ctypes.POINTER(ctypes.c_size_t)]),
     "w4a16_paged_attention_bf16": (_i, [_vp, _vp, _vp, _ll, _ll, _i, ctypes.c_float, _i, _i, _vp, _ll, _ll, _vp, _vp,
                                         ctypes.c_size_t, _vp]),
+    "w4a16_kv_tree_plan": (_i, [_vp, _vp, _i, _vp, _i, _vp, _vp, _vp]),
+    "w4a16_paged_tree_attention_bf16": (_i, [_vp, _vp, _vp, _vp, _ll, _ll, _i, ctypes.c_float, _i, _vp, _ll, _ll, _vp, _vp,
+                                             ctypes.c_size_t, _vp]),
     "w4a16_verify_drafts_workspace": (_i, [_i, _i, _i, ctypes.POINTER(ctypes.c_size_t)]),
     "w4a16_verify_drafts_f32": (_i, [_vp, _ll, _ll, _vp, _ll, _ll, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp,
                                      ctypes.c_size_t, _vp]),
@@ -640,6 +644,10 @@ class _KvBatchStruct(ctypes.Structure):
                 ("table_stride", _i), ("max_new", _i), ("max_kv", _i)]
 
 
+class _KvTreeStruct(ctypes.Structure):
+    _fields_ = [("seen", _vp), ("positions", _vp), ("sizes", _vp), ("nodes", _i)]
+
+
 def _refuse(what):
     raise W4A16Error(W4A16_ERR_CONFIG, what)
 
@@ -890,19 +898,56 @@ class KvBatch:
             _refuse(f"{what}: the batch is on {self.device}, the call on {device}")
 
 
+class KvTree:
+    """Trees of drafted tokens: the last sizes[s] tokens (all `nodes` without `sizes`) of every sequence of a batch. parents [seqs,
+    nodes] int32: the node above each one, one before it; a root's is -1. Made once a step, for all its layers: `seen` (int64 [rows,
+    (nodes + 63) // 64], the bits of a row's node and of those above it) and `positions` (int32 [rows]: the tokens before the tree and the
+    links above), of the batch's rows. update() finds them anew, in the same tensors, for what parents, sizes and the
+    batch's arrays hold then. The tensors may also be filled by hand, with bits of one's own."""
+
+    def __init__(self, parents, batch, sizes=None, stream=None):
+        import torch
+
+        if not hasattr(parents, "is_cuda") or not parents.is_cuda or parents.dtype != torch.int32 or parents.dim() != 2 or \
+                (parents.shape[1] > 1 and parents.stride(1) != 1):
+            _refuse("KvTree: parents is no int32 CUDA tensor [seqs, nodes] with a dense last axis")
+        seqs, nodes = parents.shape
+        batch.check(parents.device, "KvTree")
+        if seqs != batch.kv_lens.shape[0] or not 1 <= nodes <= 256:
+            _refuse(f"KvTree: parents {tuple(parents.shape)} for {batch.kv_lens.shape[0]} sequences of 1 to 256 nodes")
+        self._sizes = None if sizes is None else _exactly(sizes, (seqs,), torch.int32, parents.device, "KvTree sizes")
+        self.parents, self.sizes, self.batch, self.nodes = parents, sizes, batch, nodes
+        with _under(stream, parents.device) if stream is not None else contextlib.nullcontext():
+            # rows of no sequence see nothing
+            self.seen = torch.zeros(batch.rows, (nodes + 63) // 64, dtype=torch.int64, device=parents.device)
+            self.positions = torch.zeros(batch.rows, dtype=torch.int32, device=parents.device)
+        self._c = _KvTreeStruct(self.seen.data_ptr(), self.positions.data_ptr(), self._sizes, nodes)
+        self._ref = ctypes.addressof(self._c)
+        self._stride = parents.stride(0) if seqs > 1 else nodes
+        self.update(stream)
+
+    def update(self, stream=None):
+        index = _on_current(self.parents.device, "KvTree")
+        st = lib.w4a16_kv_tree_plan(self.batch._ref, self.parents.data_ptr(), self._stride, self._sizes, self.nodes, self._c.seen,
+                                    self._c.positions, _raw_stream(stream, index))
+        if st:
+            _check(st, "KvTree")
+
+
 def paged_attention(q, cache, batch, scale=None, causal=True, window=0, out=None, return_lse=False, workspace=None,
-                    stream=None):
+                    stream=None, tree=None):
     """Attention of the batch's rows of q [rows, q_heads, head_dim] (BF16; strided views are fine)
     over the cache, their own keys and values written already. scale: 1 / sqrt(head_dim) unless it
     is given. Returns out [rows, q_heads, head_dim], or (out, lse [rows, q_heads]). `workspace`: a
     uint8 tensor to use instead of a new one, not shared with a call that may still run. With a
-    `stream`, what the call allocates is allocated under it."""
+    `stream`, what the call allocates is allocated under it. `tree`: a KvTree of this batch; its rows see what stands before
+    their tree, and of the tree what its bits name."""
     import torch
 
     device = cache.device
     if stream is not None:
         with _under(stream, device):
-            return paged_attention(q, cache, batch, scale, causal, window, out, return_lse, workspace)
+            return paged_attention(q, cache, batch, scale, causal, window, out, return_lse, workspace, None, tree)
     index = _on_current(device, "paged_attention")
     batch.check(device, "paged_attention")
     rows, dim = batch.rows, cache.head_dim
@@ -934,9 +979,15 @@ def paged_attention(q, cache, batch, scale=None, causal=True, window=0, out=None
             wp = workspace.data_ptr()
         else:
             wp = _dev(workspace, need, 1, "paged_attention workspace", device)
-    st = lib.w4a16_paged_attention_bf16(cache._ref, batch._ref, qp, q_row, q_head, q_heads,
-                                        dim ** -0.5 if scale is None else scale, 1 if causal else 0, window, op, o_row,
-                                        o_head, None if lse is None else lse.data_ptr(), wp, need, _raw_stream(None, index))
+    scale, lp = dim ** -0.5 if scale is None else scale, None if lse is None else lse.data_ptr()
+    if tree is None:
+        st = lib.w4a16_paged_attention_bf16(cache._ref, batch._ref, qp, q_row, q_head, q_heads, scale, 1 if causal else 0, window, op,
+                                            o_row, o_head, lp, wp, need, _raw_stream(None, index))
+    else:
+        if tree.batch is not batch or not causal:
+            _refuse("paged_attention: the tree is another batch's, or its rows are to see what stands behind them")
+        st = lib.w4a16_paged_tree_attention_bf16(cache._ref, batch._ref, tree._ref, qp, q_row, q_head, q_heads, scale, window, op,
+                                                 o_row, o_head, lp, wp, need, _raw_stream(None, index))
     if st:
         _check(st, "paged_attention")
     return (out, lse) if return_lse else out

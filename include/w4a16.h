@@ -447,6 +447,34 @@ int w4a16_paged_attention_bf16(const W4A16KvCache *cache, const W4A16KvBatch *ba
                                long long out_row_stride, long long out_head_stride, float *lse,
                                void *ws, size_t ws_bytes, void *stream);
 
+/* Trees of drafted tokens. The last sizes[s] tokens of sequence s (kv_lens counts them; sizes NULL: `nodes`; clipped to 0 ..
+ * nodes) are the nodes of a tree, a node behind its parent; its rows may be all of them, or the last ones of a tree that is being grown,
+ * or begin before it. What a row sees of the tree is in its bits: bit j % 64 of seen[row][j / 64] for node j, of nodes up to the
+ * row's own place. The positions are the rows' own (the tokens before the tree, and the links above it), as
+ * w4a16_kv_append_rope_bf16 takes them. A sequence without nodes is an ordinary one. All three are read on the device at run time. */
+typedef struct W4A16KvTree {
+    const uint64_t *seen;     /* [rows][(nodes + 63) / 64] */
+    const int32_t *positions; /* [rows] */
+    const int32_t *sizes;     /* [seqs], or NULL */
+    int nodes;                /* 1 to 256 */
+} W4A16KvTree;
+
+/* The bits and positions of trees by their links: parents[s * parents_stride + j] is the node above node j, one
+ * before it; anything else says that it is a root. A node sees itself and those above it. Rows before the tree see
+ * no node, and stand at their place; rows of no sequence are left as they were. */
+int w4a16_kv_tree_plan(const W4A16KvBatch *batch, const int32_t *parents, int parents_stride, const int32_t *sizes,
+                       int nodes, uint64_t *seen, int32_t *positions, void *stream);
+
+/* w4a16_paged_attention_bf16 for such rows: a row sees the tokens before its sequence's tree, and of the tree the nodes that
+ * its bits name, none behind its own place. window > 0 (at least `nodes`): none of the tokens before the tree whose position is
+ * `window` or more before the row's (positions outside base .. the row's place count as the nearer of the two, base being the
+ * tokens before the tree). The workspace is that of w4a16_paged_attention_workspace. */
+int w4a16_paged_tree_attention_bf16(const W4A16KvCache *cache, const W4A16KvBatch *batch, const W4A16KvTree *tree,
+                                    const uint16_t *q, long long q_row_stride, long long q_head_stride,
+                                    int q_heads, float scale, int window, uint16_t *out,
+                                    long long out_row_stride, long long out_head_stride, float *lse, void *ws,
+                                    size_t ws_bytes, void *stream);
+
 /* Verification of drafted tokens against the target's probabilities, from given random numbers.
  * Sequence s has lens[s] drafted tokens (lens NULL: `steps` each; clipped to 0..steps) in
  * draft_tokens[s * steps + i]. Its target row i (i = 0..steps) of `vocab` probabilities is at
