@@ -1,0 +1,393 @@
+/*
+ * beams.hip - Beam search's step: the best continuations over a group's beams and the vocabulary, and where the beams' caches go on.
+ *
+ *   candidate (b, v) scores  score_b + x_bv - log sum_w exp(x_bw)
+ *
+ * beams_scan_kernel reads the logits once: it leaves the sum of each wave's piece of a row and the largest value of every
+ * chunk (what a wave loads at once: 256 FP32 values or 512 BF16 ones). beams_pick_kernel, one block a group, has then little to read: the `take`
+ * best candidates lie in the `take` best chunks, by their largest values and, where those are equal, their numbers: a
+ * candidate outside of them stands behind the largest of each, all of which are better or equal with a lower number. So it
+ * picks chunks by their largest values, and candidates out of those.
+ *
+ * Either pick is of a few out of many: each wave gives a lower bound of the last one that is picked (with 16 waves, the least of their
+ * ceil(take / 16)th largest: there are `take` values at or above it), what reaches the bound is collected (not many more than
+ * are picked, if the values are not alike), and each of these counts those before it, which is its place. Scores are FP64
+ * and numbers unique, so the order is too. Where more are collected than there is room for, which takes rows of equal values, the
+ * picks are made one after another instead.
+ *
+ * Exponentials are FP32 with the rounding of their arguments made good (2^-23), their sums FP64.
+ */
+#include "launch.h"
+#include "wave.h"
+
+using namespace w4a16;
+
+namespace {
+
+typedef float f4_loose __attribute__((ext_vector_type(4), aligned(4)));       /* rows start anywhere */
+typedef uint32_t u4_loose __attribute__((ext_vector_type(4), aligned(2)));
+
+constexpr int kMostTake = 128, kMostBeams = 1024;
+constexpr int kScanThreads = 256, kLoads = 4;   /* 16-byte loads of a scanning wave's piece: chunks of it */
+constexpr int kPickThreads = 1024, kPickWaves = kPickThreads / 64, kRoom = 512;
+
+constexpr int values_a_load(bool bf16) { return bf16 ? 8 : 4; }
+constexpr int chunk_values(bool bf16) { return 64 * values_a_load(bf16); }
+
+struct SelectArgs {
+    const void *logits;
+    long long group_stride, beam_stride;
+    const float *scores;
+    int beams, vocab, take, chunks, pieces; /* of a row */
+    float *tops;                            /* [groups][beams][chunks] */
+    double *sums;                           /* [groups][beams][pieces]: of exp(x - the piece's largest) */
+    float *mosts;                           /* [groups][beams][pieces] */
+    float *out_scores;
+    int32_t *out_parents, *out_tokens;
+};
+
+/* The values of lane l's load at element i of a row of n; -infinity behind it. */
+template <bool BF16>
+__device__ __forceinline__ void load_values(const void *row, int i, int n, float (&x)[values_a_load(BF16)]) {
+    constexpr int kValues = values_a_load(BF16);
+    if (i + kValues <= n) {
+        if constexpr (BF16) {
+            const u4_loose v = *reinterpret_cast<const u4_loose *>(static_cast<const uint16_t *>(row) + i);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                x[2 * j] = __builtin_bit_cast(float, v[j] << 16);
+                x[2 * j + 1] = __builtin_bit_cast(float, v[j] & 0xFFFF0000u);
+            }
+        } else {
+            const f4_loose v = *reinterpret_cast<const f4_loose *>(static_cast<const float *>(row) + i);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = v[j];
+        }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < kValues; ++j) {
+        x[j] = -__builtin_inff();
+        if (i + j < n) {
+            if constexpr (BF16) x[j] = __builtin_bit_cast(float, (uint32_t)static_cast<const uint16_t *>(row)[i + j] << 16);
+            else x[j] = static_cast<const float *>(row)[i + j];
+        }
+    }
+}
+
+template <bool BF16>
+__device__ __forceinline__ const void *row_of(const SelectArgs &a, int group, int beam) {
+    return static_cast<const uint8_t *>(a.logits) + (group * a.group_stride + beam * a.beam_stride) * (BF16 ? 2 : 4);
+}
+
+/* exp(x - most) for x <= most: the product with log2(e) in two parts, the second for what the first rounds off. */
+__device__ __forceinline__ float exp_below(float x, float most) {
+    constexpr float kHigh = 1.44269502162933349609375f, kLow = 1.92596299112661746887e-8f;
+    const float d = x - most, high = d * kHigh, low = fmaf(d, kHigh, -high) + d * kLow;
+    const float e = __builtin_amdgcn_exp2f(high);
+    return high < -126.0f ? 0.0f : fmaf(e, low * 0.693147182464599609375f, e); /* 2^-126: nothing, beside 1 */
+}
+
+__device__ __forceinline__ float wave_largest(float v) {
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) v = fmaxf(v, __shfl_xor(v, m));
+    return v;
+}
+
+/* One wave a piece of kLoads chunks. */
+template <bool BF16>
+__global__ __launch_bounds__(kScanThreads) void beams_scan_kernel(SelectArgs a) {
+    constexpr int kValues = values_a_load(BF16), kChunk = chunk_values(BF16);
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, beam = blockIdx.y, group = blockIdx.z;
+    const int piece = blockIdx.x * (kScanThreads / 64) + wave;
+    if (piece >= a.pieces) return;
+    const void *row = row_of<BF16>(a, group, beam);
+    const long long which = (long long)group * a.beams + beam;
+    float x[kLoads][kValues], top[kLoads], most = -__builtin_inff();
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) load_values<BF16>(row, (piece * kLoads + j) * kChunk + lane * kValues, a.vocab, x[j]);
+    bool odd = false; /* a NaN, which no maximum sees */
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+        top[j] = x[j][0];
+#pragma unroll
+        for (int i = 0; i < kValues; ++i) {
+            top[j] = fmaxf(top[j], x[j][i]);
+            odd = odd | (x[j][i] != x[j][i]);
+        }
+        top[j] = wave_largest(top[j]);
+        most = fmaxf(most, top[j]);
+    }
+    const float base = most == -__builtin_inff() ? 0.0f : most;
+    double sum = 0.0;
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j)
+#pragma unroll
+        for (int i = 0; i < kValues; ++i) sum += (double)exp_below(x[j][i], base);
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) sum += __shfl_xor(sum, m);
+    if (__any(odd) || most == __builtin_inff()) sum = __builtin_nan("");
+    if (lane == 0) {
+        a.sums[which * a.pieces + piece] = sum;
+        a.mosts[which * a.pieces + piece] = base;
+    }
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j)
+        if (lane == j && piece * kLoads + j < a.chunks) a.tops[which * a.chunks + piece * kLoads + j] = top[j];
+}
+
+/* What is picked from: a score and its number, among all of a group. The one is before the other if it scores more, or the
+ * same with a lower number. Scores of -infinity and NaN are none. */
+struct Entry {
+    double score;
+    int index;
+};
+
+__device__ __forceinline__ bool before(double score, int index, const Entry &than) {
+    return score > than.score || (score == than.score && index < than.index);
+}
+
+__device__ __forceinline__ double wave_most(double v) {
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) {
+        const double o = __shfl_xor(v, m);
+        v = o > v ? o : v;
+    }
+    return v;
+}
+
+struct PickShared {
+    Entry list[kRoom], picked[kMostTake], wave_best[kPickWaves];
+    double bounds[kPickWaves], offsets[kMostBeams];
+    int count, waves;
+};
+
+/* The bound of this wave for a pick of `take`: its `rank`th largest of the lanes' largest values. */
+__device__ __forceinline__ double wave_bound(double mine, int rank) {
+    double bound = -__builtin_inf();
+    for (int r = 0; r < rank; ++r) {
+        bound = wave_most(mine);
+        if (!(bound > -__builtin_inf())) break;
+        /* one lane of those that have it */
+        const unsigned long long have = __ballot(mine == bound);
+        if ((int)(threadIdx.x & 63) == __ffsll((long long)have) - 1) mine = -__builtin_inf();
+    }
+    return bound;
+}
+
+/*
+ * Picks the `take` first of the entries that each(f) gives to f(score, index), in whatever order and on whatever thread, the same
+ * ones each time, into shared.picked in their order; returns how many there are. `least`: a bound that is known.
+ * Called by the whole block.
+ */
+template <typename EACH>
+__device__ __forceinline__ int pick(PickShared &s, int take, double least, EACH each) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    double mine = -__builtin_inf();
+    each([&](double score, int) { mine = score > mine ? score : mine; });
+    /* waves that hold anything share the ranks */
+    const bool some = __any(mine > -__builtin_inf());
+    __syncthreads();
+    if (tid == 0) s.count = s.waves = 0;
+    __syncthreads();
+    if (lane == 0 && some) atomicAdd(&s.waves, 1);
+    __syncthreads();
+    const int waves = s.waves, rank = waves ? (take + waves - 1) / waves : 1;
+    if (rank <= 64 && some) {
+        const double bound = wave_bound(mine, rank);
+        if (lane == 0) s.bounds[wave] = bound;
+    } else if (lane == 0) {
+        s.bounds[wave] = some ? -__builtin_inf() : __builtin_inf();
+    }
+    __syncthreads();
+    double bound = __builtin_inf();
+    for (int w = 0; w < kPickWaves; ++w) bound = s.bounds[w] < bound ? s.bounds[w] : bound;
+    bound = bound > least ? bound : least;
+    each([&](double score, int index) {
+        if (score >= bound && score > -__builtin_inf()) {
+            const int at = atomicAdd(&s.count, 1);
+            if (at < kRoom) s.list[at] = {score, index};
+        }
+    });
+    __syncthreads();
+    const int count = s.count;
+    if (count <= kRoom) {
+        for (int i = tid; i < count; i += kPickThreads) {
+            const Entry own = s.list[i];
+            int place = 0;
+            for (int j = 0; j < count; ++j) {
+                const Entry other = s.list[j];
+                place += before(other.score, other.index, own);
+            }
+            if (place < take) s.picked[place] = own;
+        }
+        __syncthreads();
+        return count < take ? count : take;
+    }
+    /* more than there is room for: one after another */
+    Entry last = {__builtin_inf(), -1};
+    for (int n = 0; n < take; ++n) {
+        Entry best = {-__builtin_inf(), INT32_MAX};
+        each([&](double score, int index) {
+            if (before(last.score, last.index, Entry{score, index}) && before(score, index, best)) best = {score, index};
+        });
+        for (int m = 1; m < 64; m *= 2) {
+            const Entry o = {__shfl_xor(best.score, m), __shfl_xor(best.index, m)};
+            if (before(o.score, o.index, best)) best = o;
+        }
+        if (lane == 0) s.wave_best[wave] = best;
+        __syncthreads();
+        best = s.wave_best[0];
+        for (int w = 1; w < kPickWaves; ++w)
+            if (before(s.wave_best[w].score, s.wave_best[w].index, best)) best = s.wave_best[w];
+        if (tid == 0) s.picked[n] = best;
+        last = best;
+        __syncthreads();
+        if (!(best.score > -__builtin_inf())) return n;
+    }
+    return take;
+}
+
+template <bool BF16>
+__global__ __launch_bounds__(kPickThreads) void beams_pick_kernel(SelectArgs a) {
+    constexpr int kValues = values_a_load(BF16), kChunk = chunk_values(BF16);
+    __shared__ PickShared s;
+    const int group = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    /* what a beam's logits are moved by: its score less the logarithm of its sum; NaN, which no comparison passes, where it has none */
+    for (int b = wave; b < a.beams; b += kPickWaves) {
+        const long long which = (long long)group * a.beams + b;
+        float most = -__builtin_inff();
+        for (int p = lane; p < a.pieces; p += 64) {
+            const double sum = a.sums[which * a.pieces + p];
+            const float m = a.mosts[which * a.pieces + p];
+            if (!(sum == 0.0)) most = fmaxf(most, m);
+        }
+        most = wave_largest(most);
+        double sum = 0.0;
+        for (int p = lane; p < a.pieces; p += 64) {
+            const double part = a.sums[which * a.pieces + p];
+            if (!(part == 0.0)) sum += part * exp((double)a.mosts[which * a.pieces + p] - (double)most);
+        }
+#pragma unroll
+        for (int m = 1; m < 64; m *= 2) sum += __shfl_xor(sum, m);
+        const double offset = (double)a.scores[which] - ((double)most + log(sum));
+        if (lane == 0) s.offsets[b] = fabs(offset) < __builtin_inf() ? offset : __builtin_nan("");
+    }
+    __syncthreads();
+    /* chunks, by their numbers in the group; few of them are spread over the waves, whose bounds are then of use */
+    const float *tops = a.tops + (long long)group * a.beams * a.chunks;
+    const int all = a.beams * a.chunks, first = all < 4 * kPickThreads ? wave + kPickWaves * lane : tid;
+    const int chunks = pick(s, a.take, -__builtin_inf(), [&](auto &&f) {
+        for (int e = first; e < all; e += kPickThreads) f(s.offsets[e / a.chunks] + (double)tops[e], e);
+    });
+    /* their values: a wave's load is a chunk. The last of `take` chunks' largest value is a bound. */
+    const double least = chunks == a.take ? s.picked[chunks - 1].score : -__builtin_inf();
+    __shared__ int chosen[kMostTake];
+    if (tid < chunks) chosen[tid] = s.picked[tid].index;
+    __syncthreads();
+    const int found = pick(s, a.take, least, [&](auto &&f) {
+        for (int c = wave; c < chunks; c += kPickWaves) {
+            const int e = chosen[c], beam = e / a.chunks, at = (e - beam * a.chunks) * kChunk + lane * kValues;
+            float x[kValues];
+            load_values<BF16>(row_of<BF16>(a, group, beam), at, a.vocab, x);
+#pragma unroll
+            for (int i = 0; i < kValues; ++i)
+                if (at + i < a.vocab) f(s.offsets[beam] + (double)x[i], beam * a.vocab + at + i);
+        }
+    });
+    for (int i = tid; i < a.take; i += kPickThreads) {
+        const bool real = i < found;
+        const Entry own = s.picked[real ? i : 0];
+        const int parent = own.index / a.vocab;
+        const long long to = (long long)group * a.take + i;
+        a.out_scores[to] = real ? (float)own.score : -__builtin_inff();
+        a.out_parents[to] = real ? parent : -1;
+        a.out_tokens[to] = real ? own.index - parent * a.vocab : -1;
+    }
+}
+
+template <bool BF16>
+void launch_select(const SelectArgs &a, int groups, hipStream_t s) {
+    constexpr int kWaves = kScanThreads / 64;
+    launch_k(beams_scan_kernel<BF16>, dim3((a.pieces + kWaves - 1) / kWaves, a.beams, groups), dim3(kScanThreads), 0, s, a);
+    launch_k(beams_pick_kernel<BF16>, dim3(groups), dim3(kPickThreads), 0, s, a);
+}
+
+} // namespace
+
+namespace {
+
+int select(const char *what, bool bf16, const void *logits, long long group_stride, long long beam_stride, const float *scores, int groups,
+           int beams, int vocab, int take, float *out_scores, int32_t *parents, int32_t *tokens, void *ws, size_t ws_bytes, void *stream) {
+    size_t need = 0;
+    int st = w4a16_beam_select_workspace(groups, beams, vocab, &need);
+    if (st) return st;
+    if (take < 1 || take > kMostTake) return set_error(W4A16_ERR_CONFIG, "%s: take=%d is not 1 to %d", what, take, kMostTake);
+    if (groups == 0) return W4A16_OK;
+    if (!logits || !scores || !out_scores || !parents || !tokens || !ws) return set_error(W4A16_ERR_CONFIG, "%s: null buffer", what);
+    if (((uintptr_t)logits & (bf16 ? 1 : 3)) ||
+        (((uintptr_t)scores | (uintptr_t)out_scores | (uintptr_t)parents | (uintptr_t)tokens) & 3))
+        return set_error(W4A16_ERR_CONFIG, "%s: buffers must be 4-byte aligned (BF16 logits: 2)", what);
+    if (misaligned(ws)) return set_error(W4A16_ERR_CONFIG, "%s: the workspace must be 16-byte aligned", what);
+    if (ws_bytes < need)
+        return set_error(W4A16_ERR_CONFIG, "%s: a workspace of %zu bytes, the call needs %zu", what, ws_bytes, need);
+    constexpr long long kMost = 1LL << 43;
+    for (long long x : {group_stride, beam_stride})
+        if (x < 0 || x > kMost) return set_error(W4A16_ERR_CONFIG, "%s: stride %lld outside 0 to 2^43", what, x);
+    const size_t size = bf16 ? 2 : 4, out = (size_t)groups * take * 4;
+    const struct { const void *p; size_t n; } reads[] = {
+        {logits, ((size_t)(groups - 1) * group_stride + (size_t)(beams - 1) * beam_stride + vocab) * size},
+        {scores, (size_t)groups * beams * 4}}, writes[] = {{out_scores, out}, {parents, out}, {tokens, out}, {ws, need}};
+    bool clash = false;
+    for (int i = 0; i < 4; ++i) {
+        for (const auto &r : reads) clash = clash || overlap(writes[i].p, writes[i].n, r.p, r.n);
+        for (int j = 0; j < i; ++j) clash = clash || overlap(writes[i].p, writes[i].n, writes[j].p, writes[j].n);
+    }
+    if (clash) return set_error(W4A16_ERR_CONFIG, "%s: an output or the workspace overlaps another buffer", what);
+    SelectArgs a;
+    a.logits = logits;
+    a.group_stride = group_stride;
+    a.beam_stride = beam_stride;
+    a.scores = scores;
+    a.beams = beams;
+    a.vocab = vocab;
+    a.take = take;
+    a.chunks = (vocab + chunk_values(bf16) - 1) / chunk_values(bf16);
+    a.pieces = (a.chunks + kLoads - 1) / kLoads;
+    const size_t rows = (size_t)groups * beams;
+    a.sums = static_cast<double *>(ws);
+    a.mosts = reinterpret_cast<float *>(a.sums + rows * a.pieces);
+    a.tops = a.mosts + rows * a.pieces;
+    a.out_scores = out_scores;
+    a.out_parents = parents;
+    a.out_tokens = tokens;
+    (bf16 ? launch_select<true> : launch_select<false>)(a, groups, static_cast<hipStream_t>(stream));
+    return hip_status(hipGetLastError(), "beam select launch");
+}
+
+} // namespace
+
+extern "C" int w4a16_beam_select_workspace(int groups, int beams, int vocab, size_t *bytes) {
+    if (!bytes) return set_error(W4A16_ERR_CONFIG, "w4a16_beam_select_workspace: null result");
+    if (groups < 0 || groups > 65535 || beams < 1 || beams > kMostBeams || vocab < 1 || (long long)beams * vocab > INT32_MAX)
+        return set_error(W4A16_ERR_CONFIG, "w4a16_beam_select: bad extents groups=%d beams=%d vocab=%d (groups up to 65535, beams 1 to "
+                         "%d, beams * vocab up to 2^31 - 1)", groups, beams, vocab, kMostBeams);
+    /* of FP32 logits, whose chunks are the smaller */
+    const size_t chunks = ((size_t)vocab + chunk_values(false) - 1) / chunk_values(false), pieces = (chunks + kLoads - 1) / kLoads;
+    *bytes = (size_t)groups * beams * (pieces * 12 + chunks * 4);
+    return W4A16_OK;
+}
+
+extern "C" int w4a16_beam_select_f32(const float *logits, long long group_stride, long long beam_stride, const float *scores, int groups,
+                                     int beams, int vocab, int take, float *out_scores, int32_t *parents, int32_t *tokens,
+                                     void *ws, size_t ws_bytes, void *stream) {
+    return select("w4a16_beam_select_f32", false, logits, group_stride, beam_stride, scores, groups, beams, vocab, take, out_scores, parents,
+                  tokens, ws, ws_bytes, stream);
+}
+
+extern "C" int w4a16_beam_select_bf16(const uint16_t *logits, long long group_stride, long long beam_stride, const float *scores,
+                                      int groups, int beams, int vocab, int take, float *out_scores, int32_t *parents,
+                                      int32_t *tokens, void *ws, size_t ws_bytes, void *stream) {
+    return select("w4a16_beam_select_bf16", true, logits, group_stride, beam_stride, scores, groups, beams, vocab, take, out_scores, parents,
+                  tokens, ws, ws_bytes, stream);
+}

@@ -111,6 +111,12 @@ _SIGNATURES = {
     "w4a16_kv_tree_plan": (_i, [_vp, _vp, _i, _vp, _i, _vp, _vp, _vp]),
     "w4a16_paged_tree_attention_bf16": (_i, [_vp, _vp, _vp, _vp, _ll, _ll, _i, ctypes.c_float, _i, _vp, _ll, _ll, _vp, _vp,
                                              ctypes.c_size_t, _vp]),
+    "w4a16_kv_keep_path": (_i, [_vp, _vp, _vp, _i, _vp]),
+    "w4a16_beam_select_workspace": (_i, [_i, _i, _i, ctypes.POINTER(ctypes.c_size_t)]),
+    "w4a16_beam_select_f32": (_i, [_vp, _ll, _ll, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "w4a16_beam_select_bf16": (_i, [_vp, _ll, _ll, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "w4a16_beam_tables": (_i, [_vp, _i, _i, _vp, _vp, _i, _i, _i, _vp, _i, _vp, _vp]),
+    "w4a16_kv_copy_tails": (_i, [_vp, _vp, _i, _i, _vp, _vp, _i, _vp]),
     "w4a16_verify_drafts_workspace": (_i, [_i, _i, _i, ctypes.POINTER(ctypes.c_size_t)]),
     "w4a16_verify_drafts_f32": (_i, [_vp, _ll, _ll, _vp, _ll, _ll, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp,
                                      ctypes.c_size_t, _vp]),
@@ -838,6 +844,30 @@ class KvCache:
         return out
 
 
+    def keep_path(self, batch, path, stream=None):
+        """Token j of each sequence's rows takes what its token path[s, j] (int32, more than j) holds: verify_tree's path goes to the
+        front of its tree. Entries that are not more than their place leave it as it is."""
+        import torch
+
+        index = _on_current(self.device, "KvCache.keep_path")
+        batch.check(self.device, "KvCache.keep_path")
+        width = path.shape[1] if len(path.shape) == 2 else 0
+        pp = _exactly(path, (batch.kv_lens.shape[0], width), torch.int32, self.device, "KvCache.keep_path path")
+        st = lib.w4a16_kv_keep_path(self._ref, batch._ref, pp, width, _raw_stream(stream, index))
+        if st:
+            _check(st, "KvCache.keep_path")
+
+    def copy_tails(self, page_table, kv_lens, source, stream=None):
+        """Sequence s takes the tokens of its last page, where that is not full, from sequence source[s]'s (int32; none: -1), whose length is
+        the same: what beam_tables leaves to be copied in each layer's cache. page_table [seqs, pages] (its rows may be strided) and kv_lens
+        [seqs] are int32."""
+        index = _on_current(self.device, "KvCache.copy_tails")
+        tp, stride, pages, lp, sp = _tables(page_table, kv_lens, source, self.device, "KvCache.copy_tails")
+        st = lib.w4a16_kv_copy_tails(self._ref, tp, stride, pages, lp, sp, page_table.shape[0], _raw_stream(stream, index))
+        if st:
+            _check(st, "KvCache.copy_tails")
+
+
 class Rope:
     """How positions turn keys and queries: inv_freq, FP32 on the device, are the angles a position adds to each of the first
     inv_freq.numel() pairs of a head's values; pair i is values (i, i + pairs), or (2 i, 2 i + 1) if interleaved. The handle keeps the
@@ -991,6 +1021,89 @@ def paged_attention(q, cache, batch, scale=None, causal=True, window=0, out=None
     if st:
         _check(st, "paged_attention")
     return (out, lse) if return_lse else out
+
+
+def _tables(page_table, kv_lens, third, device, what):
+    """Addresses of a table [seqs, pages] of int32, its lengths and a third array of one entry a sequence, and the table's stride and
+    pages."""
+    import torch
+
+    if not hasattr(page_table, "is_cuda") or page_table.device != device or page_table.dtype != torch.int32 or page_table.dim() != 2 or \
+            (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+        _refuse(f"{what}: the table is no int32 tensor [seqs, pages] on {device} with a dense last axis")
+    seqs, pages = page_table.shape
+    return (page_table.data_ptr(), page_table.stride(0) if seqs > 1 else pages, pages,
+            _exactly(kv_lens, (seqs,), torch.int32, device, f"{what} kv_lens"),
+            _exactly(third, tuple(third.shape) if third.dim() == 2 and third.numel() == seqs else (seqs,), torch.int32, device, what))
+
+
+@functools.lru_cache(maxsize=64)
+def _select_workspace(groups, beams, vocab):
+    size = ctypes.c_size_t(0)
+    _check(lib.w4a16_beam_select_workspace(groups, beams, vocab, ctypes.byref(size)), "beam_select")
+    return size.value
+
+
+def beam_select(logits, scores, take, workspace=None, stream=None):
+    """The `take` best continuations of every group of beams (see include/w4a16.h): logits [groups, beams, vocab], FP32 or BF16
+    (rows may be strided), scores [groups, beams] FP32, what each beam has come to. Returns (scores [groups, take], parents, tokens), the best
+    first; where there are fewer candidates, -infinity, -1 and -1."""
+    import torch
+
+    device = logits.device
+    if stream is not None:
+        with _under(stream, device):
+            return beam_select(logits, scores, take, workspace)
+    index = _on_current(device, "beam_select")
+    if logits.dim() != 3 or logits.dtype not in (torch.float32, torch.bfloat16) or (logits.shape[-1] > 1 and logits.stride(-1) != 1):
+        _refuse(f"beam_select: expected FP32 or BF16 [groups, beams, vocab] with a dense last axis, got {logits.dtype} {tuple(logits.shape)}")
+    groups, beams, vocab = logits.shape
+    sp = _exactly(scores, (groups, beams), torch.float32, device, "beam_select scores")
+    need = _select_workspace(groups, beams, vocab)
+    if not 1 <= take <= 128:
+        _refuse(f"beam_select: take={take} is not 1 to 128")
+    # one allocation for the three
+    out = torch.empty((3, groups, take), dtype=torch.float32, device=device)
+    whole = out.view(torch.int32)
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+        wp = workspace.data_ptr()
+    else:
+        wp = _dev(workspace, need, 1, "beam_select workspace", device)
+    call = lib.w4a16_beam_select_f32 if logits.dtype == torch.float32 else lib.w4a16_beam_select_bf16
+    at, size = out.data_ptr(), groups * take * 4
+    st = call(logits.data_ptr(), logits.stride(0), logits.stride(1), sp, groups, beams, vocab, take, at, at + size, at + 2 * size, wp, need,
+              _raw_stream(None, index))
+    if st:
+        _check(st, "beam_select")
+    return out[0], whole[1], whole[2]
+
+
+def beam_tables(page_table, kv_lens, parents, page_size, out=None, stream=None):
+    """Tables of beams that go on from their parents [groups, beams] (see include/w4a16.h): beam b of group g is sequence g * beams +
+    b of page_table [seqs, pages] and kv_lens [seqs], all int32. Returns (table, source [seqs]): the new table (or `out`), and for
+    KvCache.copy_tails, which each layer's cache then does with them, whose last page a sequence lacks."""
+    import torch
+
+    device = page_table.device
+    if stream is not None:
+        with _under(stream, device):
+            return beam_tables(page_table, kv_lens, parents, page_size, out)
+    index = _on_current(device, "beam_tables")
+    if parents.dim() != 2 or parents.numel() != page_table.shape[0]:
+        _refuse(f"beam_tables: parents {tuple(parents.shape)} for {page_table.shape[0]} sequences")
+    tp, stride, pages, lp, pp = _tables(page_table, kv_lens, parents, device, "beam_tables")
+    groups, beams = parents.shape
+    if out is None:
+        out = torch.empty((groups * beams, pages), dtype=torch.int32, device=device)
+    elif out.shape != page_table.shape or out.dtype != torch.int32 or out.device != device or (pages > 1 and out.stride(1) != 1):
+        _refuse(f"beam_tables: out is no int32 tensor {tuple(page_table.shape)} on {device} with a dense last axis")
+    source = torch.empty(groups * beams, dtype=torch.int32, device=device)
+    st = lib.w4a16_beam_tables(tp, stride, pages, lp, pp, groups, beams, page_size, out.data_ptr(),
+                               out.stride(0) if groups * beams > 1 else pages, source.data_ptr(), _raw_stream(None, index))
+    if st:
+        _check(st, "beam_tables")
+    return out, source
 
 
 def _floats3(t, what, device):

@@ -475,6 +475,40 @@ int w4a16_paged_tree_attention_bf16(const W4A16KvCache *cache, const W4A16KvBatc
                                     long long out_row_stride, long long out_head_stride, float *lse, void *ws,
                                     size_t ws_bytes, void *stream);
 
+/* Moves the tokens of a tree's path to its front: token j of sequence s's new ones (rows of the batch; j < width) takes what its token
+ * path[s * width + j] holds, for entries of more than j; the others (-1 among them) leave their tokens as they are. What is
+ * moved are codes and scales as they stand. The lengths are the caller's to cut back behind the path. */
+int w4a16_kv_keep_path(const W4A16KvCache *cache, const W4A16KvBatch *batch, const int32_t *path, int width, void *stream);
+
+/* Beam search. The `take` best continuations of each of `groups` groups of `beams` beams: of all (b, v) the largest
+ *   scores[b] + logits[b][v] - log(sum over w of exp(logits[b][w])),
+ * the best first, and of equal ones those of the lowest b * vocab + v. The sum of exponentials is exact to 2^-22, everything behind it FP64;
+ * scores are rounded to FP32 at the end. Logits of -infinity are no candidates, nor is any of a beam
+ * whose score is not finite (a beam that is not to go on: -infinity) or that has an infinite or NaN logit: where there are fewer than
+ * `take`, the rest have a score of -infinity and -1 for parent and token. logits [groups][beams][vocab], rows on any
+ * element's boundary; scores [groups][beams]; out_scores, parents (b), tokens (v): [groups][take]. take is 1 to 128, beams 1 to
+ * 1024, beams * vocab under 2^31. ws: w4a16_beam_select_workspace bytes of device memory, for this call alone until it has run. */
+int w4a16_beam_select_workspace(int groups, int beams, int vocab, size_t *bytes);
+int w4a16_beam_select_f32(const float *logits, long long group_stride, long long beam_stride, const float *scores, int groups,
+                          int beams, int vocab, int take, float *out_scores, int32_t *parents, int32_t *tokens,
+                          void *ws, size_t ws_bytes, void *stream);
+int w4a16_beam_select_bf16(const uint16_t *logits, long long group_stride, long long beam_stride, const float *scores, int groups,
+                           int beams, int vocab, int take, float *out_scores, int32_t *parents, int32_t *tokens,
+                           void *ws, size_t ws_bytes, void *stream);
+
+/* The beams' caches go on from their parents: beam b of group g, sequence g * beams + b, from sequence g * beams + parents[g][b]
+ * (one outside 0 .. beams - 1: from its own). The beams of a group have one length, kv_lens of its first. new_table has the
+ * parent's entries for the pages that are full; from the first page that is not on a beam's pages are its own: a parent's first
+ * child has the parent's, the others those of the beams without children. source[sequence] is then the sequence
+ * (in the new table) whose tokens in that page the beam lacks, -1 if it lacks none: w4a16_kv_copy_tails copies them, for each layer's
+ * cache. It does so for any source [seqs] (none: outside 0 .. seqs - 1) of sequences of equal lengths; a sequence that is
+ * copied from must not be copied to. What pages are still in use is the caller's to know. */
+int w4a16_beam_tables(const int32_t *page_table, int table_stride, int table_pages, const int32_t *kv_lens,
+                      const int32_t *parents, int groups, int beams, int page_size, int32_t *new_table, int new_stride,
+                      int32_t *source, void *stream);
+int w4a16_kv_copy_tails(const W4A16KvCache *cache, const int32_t *page_table, int table_stride, int table_pages,
+                        const int32_t *kv_lens, const int32_t *source, int seqs, void *stream);
+
 /* Verification of drafted tokens against the target's probabilities, from given random numbers.
  * Sequence s has lens[s] drafted tokens (lens NULL: `steps` each; clipped to 0..steps) in
  * draft_tokens[s * steps + i]. Its target row i (i = 0..steps) of `vocab` probabilities is at
