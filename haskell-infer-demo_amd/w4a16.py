@@ -111,6 +111,8 @@ _SIGNATURES = {
     "w4a16_kv_tree_plan": (_i, [_vp, _vp, _i, _vp, _i, _vp, _vp, _vp]),
     "w4a16_paged_tree_attention_bf16": (_i, [_vp, _vp, _vp, _vp, _ll, _ll, _i, ctypes.c_float, _i, _vp, _ll, _ll, _vp, _vp,
                                              ctypes.c_size_t, _vp]),
+    "w4a16_verify_tree_workspace": (_i, [_i, _i, _i, ctypes.POINTER(ctypes.c_size_t)]),
+    "w4a16_verify_tree_f32": (_i, [_vp, _ll, _ll, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, ctypes.c_size_t, _vp]),
     "w4a16_kv_keep_path": (_i, [_vp, _vp, _vp, _i, _vp]),
     "w4a16_beam_select_workspace": (_i, [_i, _i, _i, ctypes.POINTER(ctypes.c_size_t)]),
     "w4a16_beam_select_f32": (_i, [_vp, _ll, _ll, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
@@ -1172,3 +1174,49 @@ def verify_drafts(target, draft_tokens, uniforms, draft=None, lens=None, workspa
     if st:
         _check(st, "verify_drafts")
     return accepted, tokens
+
+
+@functools.lru_cache(maxsize=64)
+def _tree_workspace(seqs, nodes, vocab):
+    size = ctypes.c_size_t(0)
+    _check(lib.w4a16_verify_tree_workspace(seqs, nodes, vocab, ctypes.byref(size)), "verify_tree")
+    return size.value
+
+
+def verify_tree(target, node_tokens, parents, uniforms, sizes=None, workspace=None, stream=None):
+    """Verification of trees of drafted tokens that were chosen, not drawn (see include/w4a16.h): target [seqs, nodes, vocab]
+    probabilities in FP32, row i behind node i; node_tokens and parents [seqs, nodes] int32, node 0 being the last token that stands;
+    uniforms [seqs, nodes] FP32; sizes [seqs] int32 or None. Returns (accepted [seqs], path [seqs, nodes], tokens [seqs, nodes]), int32:
+    tokens[s, :accepted[s] + 1] are new. KvCache.keep_path takes the path."""
+    import torch
+
+    device = target.device
+    if stream is not None:
+        with _under(stream, device):
+            return verify_tree(target, node_tokens, parents, uniforms, sizes, workspace)
+    index = _on_current(device, "verify_tree")
+    tp, t_seq, t_row = _floats3(target, "verify_tree target", device)
+    seqs, nodes, vocab = target.shape
+    shape = (seqs, nodes)
+    ip = _exactly(node_tokens, shape, torch.int32, device, "verify_tree node_tokens")
+    pp = _exactly(parents, shape, torch.int32, device, "verify_tree parents")
+    up = _exactly(uniforms, shape, torch.float32, device, "verify_tree uniforms")
+    sp = None if sizes is None else _exactly(sizes, (seqs,), torch.int32, device, "verify_tree sizes")
+    need = _tree_workspace(seqs, nodes, vocab)
+    # one allocation for the three
+    out = torch.empty(seqs * (2 * nodes + 1), dtype=torch.int32, device=device)
+    path, tokens, accepted = out[:seqs * nodes].view(shape), out[seqs * nodes:2 * seqs * nodes].view(shape), out[2 * seqs * nodes:]
+    wp = None
+    if need == 0:
+        pass
+    elif workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+        wp = workspace.data_ptr()
+    else:
+        wp = _dev(workspace, need, 1, "verify_tree workspace", device)
+    at, size = out.data_ptr(), 4 * seqs * nodes
+    st = lib.w4a16_verify_tree_f32(tp, t_seq, t_row, ip, pp, sp, up, at + 2 * size, at, at + size, seqs, nodes, vocab, wp, need,
+                                   _raw_stream(None, index))
+    if st:
+        _check(st, "verify_tree")
+    return accepted, path, tokens

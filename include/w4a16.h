@@ -534,6 +534,27 @@ int w4a16_verify_drafts_f32(const float *target, long long target_seq_stride,
                             const float *uniforms, int32_t *accepted, int32_t *tokens, int seqs,
                             int steps, int vocab, void *ws, size_t ws_bytes, void *stream);
 
+/* Verification of a tree of drafted tokens that were chosen, not drawn (the likeliest ones, say), from given random numbers.
+ * Sequence s has sizes[s] nodes (sizes NULL: `nodes` each; clipped to 1 .. nodes). Node 0 is the last token that stands already; node i has
+ * the token node_tokens[s * nodes + i] and stands behind node parents[s * nodes + i], one before it (a node with any other parent
+ * is never reached). The target's row behind node i, of `vocab` probabilities, is at target + s * target_seq_stride + i *
+ * target_row_stride. uniforms: [seqs][nodes]. From node 0 on, a node's children are asked in their order; child i is taken if
+ *   uniforms[s][i] * left < p,   left = max(0, 1 - the p of the siblings that were refused before it),
+ * p being its token's probability in its parent's row (in FP64, left one subtraction after the other); it is the next
+ * node then. A child whose token a sibling before it had, or one outside the vocabulary, is refused and takes nothing off. Behind the last
+ * taken node one token is drawn from its row without its children's tokens (with them, if that leaves nothing), as verify_drafts
+ * draws, by uniforms[s][0]. What comes out is distributed as if drawn from the target. Probabilities that are not positive and finite count as
+ * zero.
+ * accepted[s]: the nodes taken behind the root. path [seqs][nodes]: 0, those nodes, and -1 behind them. tokens [seqs][nodes]: their tokens,
+ * the drawn one (-1 if no weight is positive), and -1 behind it. A chain gives what w4a16_verify_drafts_f32 gives without a
+ * draft, with its uniforms in another order. ws: w4a16_verify_tree_workspace bytes of device memory, for this call alone until it has
+ * run; NULL if that is 0. */
+int w4a16_verify_tree_workspace(int seqs, int nodes, int vocab, size_t *bytes);
+int w4a16_verify_tree_f32(const float *target, long long target_seq_stride, long long target_row_stride,
+                          const int32_t *node_tokens, const int32_t *parents, const int32_t *sizes, const float *uniforms,
+                          int32_t *accepted, int32_t *path, int32_t *tokens, int seqs, int nodes, int vocab,
+                          void *ws, size_t ws_bytes, void *stream);
+
 /* ---------------------------------------------------------------------------------------
  * Status of the split-K combines (no counterpart in the reference, whose kernels have no
  * cross-block waits).

@@ -105,3 +105,50 @@ def check(out, lse, wanted):
     if far.numel():
         print(f"  of what the roundings allow: out {far.max():.3f}, lse {lse_far.max():.3f}", flush=True)
         assert far.max() <= 1 and lse_far.max() <= 1
+
+
+def verify(target, tokens, parents, sizes, uniforms):
+    """The definition of the tree's verification, one sequence and one node after another, in FP64: (accepted, path, tokens)."""
+    seqs, nodes, vocab = target.shape
+    accepted, paths, out = [], np.full((seqs, nodes), -1, np.int64), np.full((seqs, nodes), -1, np.int64)
+
+    def weight(w):
+        return np.where((w > 0) & np.isfinite(w), w, np.float32(0)).astype(np.float32)
+
+    for s in range(seqs):
+        size = nodes if sizes is None else min(max(int(sizes[s]), 1), nodes)
+        node, path = 0, [0]
+        while True:
+            children = [i for i in range(size) if 0 <= int(parents[s, i]) < i and int(parents[s, i]) == node]
+            left, asked, following = np.float64(1), set(), None
+            for i in children:
+                x = int(tokens[s, i])
+                if x in asked:
+                    continue
+                asked.add(x)
+                p = np.float64(weight(target[s, node, x])) if 0 <= x < vocab else np.float64(0)
+                if np.float64(uniforms[s, i]) * left < p:
+                    following = i
+                    break
+                left = max(left - p, np.float64(0))
+            if following is None:
+                break
+            node = following
+            path.append(node)
+        row = weight(target[s, node])
+        rest = row.copy()
+        for x in asked:
+            if 0 <= x < vocab:
+                rest[x] = 0
+        if not rest.any():
+            rest = row
+        taken = len(path) - 1
+        paths[s, :taken + 1] = path
+        out[s, :taken] = [tokens[s, i] for i in path[1:]]
+        if rest.any():
+            run = np.cumsum(rest.astype(np.float64))
+            with np.errstate(invalid="ignore"):
+                past = np.nonzero((run > np.float64(uniforms[s, 0]) * run[-1]) & (rest > 0))[0]
+            out[s, taken] = past[0] if len(past) else np.nonzero(rest)[0][-1]
+        accepted.append(taken)
+    return np.array(accepted), paths, out
