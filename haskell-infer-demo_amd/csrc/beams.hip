@@ -24,8 +24,8 @@ using namespace w4a16;
 
 namespace {
 
-typedef float f4_loose __attribute__((ext_vector_type(4), aligned(4)));       /* rows start anywhere */
-typedef uint32_t u4_loose __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u4_loose __attribute__((ext_vector_type(4), aligned(2))); /* rows start anywhere */
 
 constexpr int kMostTake = 128, kMostBeams = 1024;
 constexpr int kScanThreads = 256, kLoads = 4;   /* 16-byte loads of a scanning wave's piece: chunks of it */
@@ -46,33 +46,30 @@ struct SelectArgs {
     int32_t *out_parents, *out_tokens;
 };
 
-/* The values of lane l's load at element i of a row of n; -infinity behind it. */
+/* 16 bytes of a row of n values from value i on; -infinity behind it. */
 template <bool BF16>
-__device__ __forceinline__ void load_values(const void *row, int i, int n, float (&x)[values_a_load(BF16)]) {
+__device__ __forceinline__ u4 load_raw(const void *row, int i, int n) {
     constexpr int kValues = values_a_load(BF16);
-    if (i + kValues <= n) {
-        if constexpr (BF16) {
-            const u4_loose v = *reinterpret_cast<const u4_loose *>(static_cast<const uint16_t *>(row) + i);
+    if (i + kValues <= n) return *reinterpret_cast<const u4_loose *>(static_cast<const uint8_t *>(row) + (long long)i * (BF16 ? 2 : 4));
+    constexpr uint32_t kLeast = BF16 ? 0xFF80FF80u : 0xFF800000u;
+    u4 v = {kLeast, kLeast, kLeast, kLeast};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                x[2 * j] = __builtin_bit_cast(float, v[j] << 16);
-                x[2 * j + 1] = __builtin_bit_cast(float, v[j] & 0xFFFF0000u);
-            }
-        } else {
-            const f4_loose v = *reinterpret_cast<const f4_loose *>(static_cast<const float *>(row) + i);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] = v[j];
-        }
-        return;
-    }
-#pragma unroll
-    for (int j = 0; j < kValues; ++j) {
-        x[j] = -__builtin_inff();
+    for (int j = 0; j < kValues; ++j)
         if (i + j < n) {
-            if constexpr (BF16) x[j] = __builtin_bit_cast(float, (uint32_t)static_cast<const uint16_t *>(row)[i + j] << 16);
-            else x[j] = static_cast<const float *>(row)[i + j];
+            if constexpr (BF16) {
+                const uint32_t x = static_cast<const uint16_t *>(row)[i + j];
+                v[j / 2] = j % 2 ? (v[j / 2] & 0xFFFFu) | x << 16 : (v[j / 2] & 0xFFFF0000u) | x;
+            } else {
+                v[j] = static_cast<const uint32_t *>(row)[i + j];
+            }
         }
-    }
+    return v;
+}
+
+template <bool BF16>
+__device__ __forceinline__ float value_of(u4 raw, int j) {
+    const uint32_t word = raw[BF16 ? j / 2 : j]; /* an element itself is no operand of a bit cast: it gives the first one */
+    return __builtin_bit_cast(float, !BF16 ? word : j % 2 ? word & 0xFFFF0000u : word << 16);
 }
 
 template <bool BF16>
@@ -88,12 +85,6 @@ __device__ __forceinline__ float exp_below(float x, float most) {
     return high < -126.0f ? 0.0f : fmaf(e, low * 0.693147182464599609375f, e); /* 2^-126: nothing, beside 1 */
 }
 
-__device__ __forceinline__ float wave_largest(float v) {
-#pragma unroll
-    for (int m = 1; m < 64; m *= 2) v = fmaxf(v, __shfl_xor(v, m));
-    return v;
-}
-
 /* One wave a piece of kLoads chunks. */
 template <bool BF16>
 __global__ __launch_bounds__(kScanThreads) void beams_scan_kernel(SelectArgs a) {
@@ -103,19 +94,21 @@ __global__ __launch_bounds__(kScanThreads) void beams_scan_kernel(SelectArgs a) 
     if (piece >= a.pieces) return;
     const void *row = row_of<BF16>(a, group, beam);
     const long long which = (long long)group * a.beams + beam;
-    float x[kLoads][kValues], top[kLoads], most = -__builtin_inff();
+    u4 raw[kLoads];
+    float top[kLoads], most = -__builtin_inff();
 #pragma unroll
-    for (int j = 0; j < kLoads; ++j) load_values<BF16>(row, (piece * kLoads + j) * kChunk + lane * kValues, a.vocab, x[j]);
+    for (int j = 0; j < kLoads; ++j) raw[j] = load_raw<BF16>(row, (piece * kLoads + j) * kChunk + lane * kValues, a.vocab);
     bool odd = false; /* a NaN, which no maximum sees */
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
-        top[j] = x[j][0];
+        top[j] = value_of<BF16>(raw[j], 0);
 #pragma unroll
         for (int i = 0; i < kValues; ++i) {
-            top[j] = fmaxf(top[j], x[j][i]);
-            odd = odd | (x[j][i] != x[j][i]);
+            const float x = value_of<BF16>(raw[j], i);
+            top[j] = fmaxf(top[j], x);
+            odd = odd | (x != x);
         }
-        top[j] = wave_largest(top[j]);
+        top[j] = wave_most(top[j]);
         most = fmaxf(most, top[j]);
     }
     const float base = most == -__builtin_inff() ? 0.0f : most;
@@ -123,9 +116,8 @@ __global__ __launch_bounds__(kScanThreads) void beams_scan_kernel(SelectArgs a) 
 #pragma unroll
     for (int j = 0; j < kLoads; ++j)
 #pragma unroll
-        for (int i = 0; i < kValues; ++i) sum += (double)exp_below(x[j][i], base);
-#pragma unroll
-    for (int m = 1; m < 64; m *= 2) sum += __shfl_xor(sum, m);
+        for (int i = 0; i < kValues; ++i) sum += (double)exp_below(value_of<BF16>(raw[j], i), base);
+    sum = wave_sum(sum);
     if (__any(odd) || most == __builtin_inff()) sum = __builtin_nan("");
     if (lane == 0) {
         a.sums[which * a.pieces + piece] = sum;
@@ -147,79 +139,77 @@ __device__ __forceinline__ bool before(double score, int index, const Entry &tha
     return score > than.score || (score == than.score && index < than.index);
 }
 
-__device__ __forceinline__ double wave_most(double v) {
-#pragma unroll
-    for (int m = 1; m < 64; m *= 2) {
-        const double o = __shfl_xor(v, m);
-        v = o > v ? o : v;
-    }
-    return v;
-}
-
 struct PickShared {
     Entry list[kRoom], picked[kMostTake], wave_best[kPickWaves];
-    double bounds[kPickWaves], offsets[kMostBeams];
-    int count, waves;
+    double offsets[kMostBeams];
+    float bounds[kPickWaves];
+    int count;
 };
 
-/* The bound of this wave for a pick of `take`: its `rank`th largest of the lanes' largest values. */
-__device__ __forceinline__ double wave_bound(double mine, int rank) {
-    double bound = -__builtin_inf();
+/* An FP32 number that is not above v: a bound may be less than it need be. */
+__device__ __forceinline__ float not_above(double v) {
+    const float f = (float)v;
+    return f - fabsf(f) * 0x1p-22f - 0x1p-140f;
+}
+
+/* The `rank`th largest of the lanes' values, -infinity where there are fewer. */
+__device__ __forceinline__ float wave_bound(float mine, int rank) {
+    float bound = -__builtin_inff();
     for (int r = 0; r < rank; ++r) {
         bound = wave_most(mine);
-        if (!(bound > -__builtin_inf())) break;
+        if (!(bound > -__builtin_inff())) break;
         /* one lane of those that have it */
         const unsigned long long have = __ballot(mine == bound);
-        if ((int)(threadIdx.x & 63) == __ffsll((long long)have) - 1) mine = -__builtin_inf();
+        if ((int)(threadIdx.x & 63) == __ffsll((long long)have) - 1) mine = -__builtin_inff();
     }
     return bound;
 }
 
 /*
  * Picks the `take` first of the entries that each(f) gives to f(score, index), in whatever order and on whatever thread, the same
- * ones each time, into shared.picked in their order; returns how many there are. `least`: a bound that is known.
- * Called by the whole block.
+ * ones each time, into s.picked in their order; returns how many there are. The first `waves` waves have all of them, evenly, and
+ * `least` is a bound that is known. Called by the whole block; s.picked is its own until the next call.
  */
 template <typename EACH>
-__device__ __forceinline__ int pick(PickShared &s, int take, double least, EACH each) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    double mine = -__builtin_inf();
-    each([&](double score, int) { mine = score > mine ? score : mine; });
-    /* waves that hold anything share the ranks */
-    const bool some = __any(mine > -__builtin_inf());
-    __syncthreads();
-    if (tid == 0) s.count = s.waves = 0;
-    __syncthreads();
-    if (lane == 0 && some) atomicAdd(&s.waves, 1);
-    __syncthreads();
-    const int waves = s.waves, rank = waves ? (take + waves - 1) / waves : 1;
-    if (rank <= 64 && some) {
-        const double bound = wave_bound(mine, rank);
-        if (lane == 0) s.bounds[wave] = bound;
-    } else if (lane == 0) {
-        s.bounds[wave] = some ? -__builtin_inf() : __builtin_inf();
+__device__ __forceinline__ int pick(PickShared &s, int take, int waves, double least, EACH each) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, rank = (take + waves - 1) / waves;
+    float bound = __builtin_inff();
+    if (wave < waves) {
+        double mine = -__builtin_inf();
+        each([&](double score, int) { mine = score > mine ? score : mine; });
+        bound = rank <= 64 ? wave_bound(not_above(mine), rank) : -__builtin_inff();
     }
+    if (lane == 0) s.bounds[wave] = bound;
+    if (tid == 0) s.count = 0;
     __syncthreads();
-    double bound = __builtin_inf();
-    for (int w = 0; w < kPickWaves; ++w) bound = s.bounds[w] < bound ? s.bounds[w] : bound;
-    bound = bound > least ? bound : least;
-    each([&](double score, int index) {
-        if (score >= bound && score > -__builtin_inf()) {
-            const int at = atomicAdd(&s.count, 1);
-            if (at < kRoom) s.list[at] = {score, index};
-        }
-    });
+    bound = s.bounds[lane % kPickWaves];
+    bound = -wave_most(-bound);
+    const double from = bound > least ? (double)bound : least;
+    if (wave < waves)
+        each([&](double score, int index) {
+            if (score >= from && score > -__builtin_inf()) {
+                const int at = atomicAdd(&s.count, 1);
+                if (at < kRoom) s.list[at] = {score, index};
+            }
+        });
     __syncthreads();
     const int count = s.count;
     if (count <= kRoom) {
-        for (int i = tid; i < count; i += kPickThreads) {
-            const Entry own = s.list[i];
+        /* eight threads an entry, each with an eighth of the others */
+        const int part = tid & 7;
+        for (int i0 = 0; i0 < count; i0 += kPickThreads / 8) {
+            const int i = i0 + (tid >> 3);
+            const Entry own = s.list[i < count ? i : 0];
             int place = 0;
-            for (int j = 0; j < count; ++j) {
+#pragma unroll 4
+            for (int j = part; j < count; j += 8) {
                 const Entry other = s.list[j];
                 place += before(other.score, other.index, own);
             }
-            if (place < take) s.picked[place] = own;
+            place += __shfl_xor(place, 1);
+            place += __shfl_xor(place, 2);
+            place += __shfl_xor(place, 4);
+            if (part == 0 && i < count && place < take) s.picked[place] = own;
         }
         __syncthreads();
         return count < take ? count : take;
@@ -228,9 +218,10 @@ __device__ __forceinline__ int pick(PickShared &s, int take, double least, EACH 
     Entry last = {__builtin_inf(), -1};
     for (int n = 0; n < take; ++n) {
         Entry best = {-__builtin_inf(), INT32_MAX};
-        each([&](double score, int index) {
-            if (before(last.score, last.index, Entry{score, index}) && before(score, index, best)) best = {score, index};
-        });
+        if (wave < waves)
+            each([&](double score, int index) {
+                if (before(last.score, last.index, Entry{score, index}) && before(score, index, best)) best = {score, index};
+            });
         for (int m = 1; m < 64; m *= 2) {
             const Entry o = {__shfl_xor(best.score, m), __shfl_xor(best.index, m)};
             if (before(o.score, o.index, best)) best = o;
@@ -250,50 +241,83 @@ __device__ __forceinline__ int pick(PickShared &s, int take, double least, EACH 
 
 template <bool BF16>
 __global__ __launch_bounds__(kPickThreads) void beams_pick_kernel(SelectArgs a) {
-    constexpr int kValues = values_a_load(BF16), kChunk = chunk_values(BF16);
+    constexpr int kValues = values_a_load(BF16), kChunk = chunk_values(BF16), kHeld = 8;
     __shared__ PickShared s;
     const int group = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    /* chunks, by their numbers in the group: neighbours, which are of one beam, go to different waves. A thread's first ones are on
+     * their way from the start. */
+    const float *tops = a.tops + (long long)group * a.beams * a.chunks;
+    const int all = a.beams * a.chunks, first = wave + kPickWaves * lane;
+    float top[kHeld];
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) top[i] = first + i * kPickThreads < all ? tops[first + i * kPickThreads] : -__builtin_inff();
     /* what a beam's logits are moved by: its score less the logarithm of its sum; NaN, which no comparison passes, where it has none */
     for (int b = wave; b < a.beams; b += kPickWaves) {
         const long long which = (long long)group * a.beams + b;
         float most = -__builtin_inff();
-        for (int p = lane; p < a.pieces; p += 64) {
-            const double sum = a.sums[which * a.pieces + p];
-            const float m = a.mosts[which * a.pieces + p];
-            if (!(sum == 0.0)) most = fmaxf(most, m);
-        }
-        most = wave_largest(most);
-        double sum = 0.0;
-        for (int p = lane; p < a.pieces; p += 64) {
-            const double part = a.sums[which * a.pieces + p];
-            if (!(part == 0.0)) sum += part * exp((double)a.mosts[which * a.pieces + p] - (double)most);
-        }
+        double sum = 0.0; /* of exp(x - most) */
+        const double score = a.scores[which];
+        for (int p0 = 0; p0 < a.pieces; p0 += 4 * 64) {
+            double part[4];
+            float of[4], next = most;
 #pragma unroll
-        for (int m = 1; m < 64; m *= 2) sum += __shfl_xor(sum, m);
-        const double offset = (double)a.scores[which] - ((double)most + log(sum));
+            for (int j = 0; j < 4; ++j) {
+                const int p = p0 + 64 * j + lane;
+                part[j] = p < a.pieces ? a.sums[which * a.pieces + p] : 0.0;
+                of[j] = p < a.pieces ? a.mosts[which * a.pieces + p] : 0.0f;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) next = part[j] == 0.0 ? next : fmaxf(next, of[j]);
+            next = wave_most(next);
+            sum = most == next ? sum : sum * exp((double)most - (double)next);
+            most = next;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sum += part[j] == 0.0 ? 0.0 : part[j] * exp((double)of[j] - (double)most);
+        }
+        sum = wave_sum(sum);
+        const double offset = score - ((double)most + log(sum));
         if (lane == 0) s.offsets[b] = fabs(offset) < __builtin_inf() ? offset : __builtin_nan("");
     }
     __syncthreads();
-    /* chunks, by their numbers in the group; few of them are spread over the waves, whose bounds are then of use */
-    const float *tops = a.tops + (long long)group * a.beams * a.chunks;
-    const int all = a.beams * a.chunks, first = all < 4 * kPickThreads ? wave + kPickWaves * lane : tid;
-    const int chunks = pick(s, a.take, -__builtin_inf(), [&](auto &&f) {
-        for (int e = first; e < all; e += kPickThreads) f(s.offsets[e / a.chunks] + (double)tops[e], e);
-    });
-    /* their values: a wave's load is a chunk. The last of `take` chunks' largest value is a bound. */
-    const double least = chunks == a.take ? s.picked[chunks - 1].score : -__builtin_inf();
-    __shared__ int chosen[kMostTake];
-    if (tid < chunks) chosen[tid] = s.picked[tid].index;
-    __syncthreads();
-    const int found = pick(s, a.take, least, [&](auto &&f) {
-        for (int c = wave; c < chunks; c += kPickWaves) {
-            const int e = chosen[c], beam = e / a.chunks, at = (e - beam * a.chunks) * kChunk + lane * kValues;
-            float x[kValues];
-            load_values<BF16>(row_of<BF16>(a, group, beam), at, a.vocab, x);
+    double held[kHeld];
 #pragma unroll
-            for (int i = 0; i < kValues; ++i)
-                if (at + i < a.vocab) f(s.offsets[beam] + (double)x[i], beam * a.vocab + at + i);
+    for (int i = 0; i < kHeld; ++i) {
+        const int e = first + i * kPickThreads;
+        held[i] = e < all ? s.offsets[e / a.chunks] + (double)top[i] : -__builtin_inf();
+    }
+    const int chunks = pick(s, a.take, kPickWaves, -__builtin_inf(), [&](auto &&f) {
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) f(held[i], first + i * kPickThreads);
+        for (int e = first + kHeld * kPickThreads; e < all; e += kPickThreads) f(s.offsets[e / a.chunks] + (double)tops[e], e);
+    });
+    /* Their values: a wave's load is a chunk, all of a wave's on their way at once. The last of `take` chunks' largest value is a bound. */
+    const double least = chunks == a.take ? s.picked[chunks - 1].score : -__builtin_inf();
+    constexpr int kMost = kMostTake / kPickWaves;
+    u4 raw[kMost];
+    int base[kMost]; /* number of the lane's first value; -1: none */
+    double offset[kMost];
+#pragma unroll
+    for (int i = 0; i < kMost; ++i) {
+        const int c = wave + i * kPickWaves;
+        base[i] = -1;
+        if (c < chunks) {
+            const int e = s.picked[c].index, beam = e / a.chunks, at = (e - beam * a.chunks) * kChunk + lane * kValues;
+            offset[i] = s.offsets[beam];
+            base[i] = beam * a.vocab + at;
+            raw[i] = load_raw<BF16>(row_of<BF16>(a, group, beam), at, a.vocab);
         }
+    }
+    /* values behind a row's end are -infinity: never picked, whatever their numbers */
+    __syncthreads();
+    const int found = pick(s, a.take, chunks < kPickWaves ? (chunks ? chunks : 1) : kPickWaves, least, [&](auto &&f) {
+#pragma unroll
+        for (int i = 0; i < kMost; ++i)
+            if (base[i] >= 0) {
+                u4 own = raw[i];
+                asm volatile("" : "+v"(own)); /* or every score is kept from one pass to the next, in more registers than there are */
+#pragma unroll
+                for (int j = 0; j < kValues; ++j) f(offset[i] + (double)value_of<BF16>(own, j), base[i] + j);
+            }
     });
     for (int i = tid; i < a.take; i += kPickThreads) {
         const bool real = i < found;

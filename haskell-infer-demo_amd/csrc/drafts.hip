@@ -236,31 +236,6 @@ __device__ __forceinline__ void take_out(f4 (&own)[QUADS], int first, int step, 
     }
 }
 
-template <int CTRL, int ROWS>
-__device__ __forceinline__ double dpp_or_zero(double v) {
-    const uint2 b = __builtin_bit_cast(uint2, v);
-    return __builtin_bit_cast(double, make_uint2((uint32_t)__builtin_amdgcn_update_dpp(0, (int)b.x, CTRL, ROWS, 0xF, false),
-                                                 (uint32_t)__builtin_amdgcn_update_dpp(0, (int)b.y, CTRL, ROWS, 0xF, false)));
-}
-
-/* Sum of v over the lanes up to and with this one, by VALU moves: row shifts within 16 lanes, then the
- * rows' last lanes carried to the rows behind. */
-__device__ __forceinline__ double wave_scan(double v) {
-    v += dpp_or_zero<0x111, 0xF>(v);
-    v += dpp_or_zero<0x112, 0xF>(v);
-    v += dpp_or_zero<0x114, 0xF>(v);
-    v += dpp_or_zero<0x118, 0xF>(v);
-    v += dpp_or_zero<0x142, 0xA>(v); /* row_bcast:15 into rows 1 and 3 */
-    v += dpp_or_zero<0x143, 0xC>(v); /* row_bcast:31 into rows 2 and 3 */
-    return v;
-}
-
-__device__ __forceinline__ double lane_f64(double v, int lane) {
-    const uint2 b = __builtin_bit_cast(uint2, v);
-    return __builtin_bit_cast(double, make_uint2((uint32_t)__builtin_amdgcn_readlane((int)b.x, lane),
-                                                 (uint32_t)__builtin_amdgcn_readlane((int)b.y, lane)));
-}
-
 /* The block's smallest `mine` and largest `behind`, a wave's first: 64 lanes at one LDS word take turns. */
 __device__ __forceinline__ void join_found(int mine, int behind, int *found, int *last) {
     const int first = INT32_MAX - wave_most(INT32_MAX - mine), end = wave_most(behind + 1) - 1;
@@ -269,8 +244,6 @@ __device__ __forceinline__ void join_found(int mine, int behind, int *found, int
         if (end >= 0) atomicMax(last, end);
     }
 }
-
-__device__ __forceinline__ double wave_sum(double v) { return lane_f64(wave_scan(v), 63); }
 
 /* The block's walk through a sequence's tree: the nodes taken and the last one's row; its children in the list. `writes`: this block
  * writes what is known then. */
