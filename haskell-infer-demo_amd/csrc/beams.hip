@@ -15,7 +15,8 @@
  * and numbers unique, so the order is too. Where more are collected than there is room for, which takes rows of equal values, the
  * picks are made one after another instead.
  *
- * Exponentials are FP32 with the rounding of their arguments made good (2^-23), their sums FP64.
+ * Exponentials are FP32 with the rounding of their arguments made good (2^-23), the sums of a load's four or eight too (2^-24 for each of two
+ * or three additions), the sums of those FP64: 2^-21 in all.
  */
 #include "launch.h"
 #include "wave.h"
@@ -41,7 +42,7 @@ struct SelectArgs {
     int beams, vocab, take, chunks, pieces; /* of a row */
     float *tops;                            /* [groups][beams][chunks] */
     double *sums;                           /* [groups][beams][pieces]: of exp(x - the piece's largest) */
-    float *mosts;                           /* [groups][beams][pieces] */
+    float *mosts;                           /* [groups][beams][pieces]: the piece's largest, -infinity where it is nothing else */
     float *out_scores;
     int32_t *out_parents, *out_tokens;
 };
@@ -80,9 +81,10 @@ __device__ __forceinline__ const void *row_of(const SelectArgs &a, int group, in
 /* exp(x - most) for x <= most: the product with log2(e) in two parts, the second for what the first rounds off. */
 __device__ __forceinline__ float exp_below(float x, float most) {
     constexpr float kHigh = 1.44269502162933349609375f, kLow = 1.92596299112661746887e-8f;
-    const float d = x - most, high = d * kHigh, low = fmaf(d, kHigh, -high) + d * kLow;
+    const float d = fmaxf(x - most, -128.0f); /* its exponential is nothing beside 1 */
+    const float high = d * kHigh, low = fmaf(d, kHigh, -high) + d * kLow;
     const float e = __builtin_amdgcn_exp2f(high);
-    return high < -126.0f ? 0.0f : fmaf(e, low * 0.693147182464599609375f, e); /* 2^-126: nothing, beside 1 */
+    return fmaf(e, low * 0.693147182464599609375f, e);
 }
 
 /* One wave a piece of kLoads chunks. */
@@ -111,17 +113,23 @@ __global__ __launch_bounds__(kScanThreads) void beams_scan_kernel(SelectArgs a) 
         top[j] = wave_most(top[j]);
         most = fmaxf(most, top[j]);
     }
-    const float base = most == -__builtin_inff() ? 0.0f : most;
     double sum = 0.0;
 #pragma unroll
-    for (int j = 0; j < kLoads; ++j)
+    for (int j = 0; j < kLoads; ++j) {
+        float part[kValues];
 #pragma unroll
-        for (int i = 0; i < kValues; ++i) sum += (double)exp_below(value_of<BF16>(raw[j], i), base);
-    sum = wave_sum(sum);
+        for (int i = 0; i < kValues; ++i) part[i] = exp_below(value_of<BF16>(raw[j], i), most);
+#pragma unroll
+        for (int n = kValues / 2; n > 0; n /= 2)
+#pragma unroll
+            for (int i = 0; i < n; ++i) part[i] += part[i + n];
+        sum += (double)part[0];
+    }
+    sum = most == -__builtin_inff() ? 0.0 : wave_sum(sum);
     if (__any(odd) || most == __builtin_inff()) sum = __builtin_nan("");
     if (lane == 0) {
         a.sums[which * a.pieces + piece] = sum;
-        a.mosts[which * a.pieces + piece] = base;
+        a.mosts[which * a.pieces + piece] = most;
     }
 #pragma unroll
     for (int j = 0; j < kLoads; ++j)
@@ -166,19 +174,16 @@ __device__ __forceinline__ float wave_bound(float mine, int rank) {
 }
 
 /*
- * Picks the `take` first of the entries that each(f) gives to f(score, index), in whatever order and on whatever thread, the same
- * ones each time, into s.picked in their order; returns how many there are. The first `waves` waves have all of them, evenly, and
- * `least` is a bound that is known. Called by the whole block; s.picked is its own until the next call.
+ * Picks the `take` first of the entries that each(from, f) gives to f(score, index): all whose score is at least `from`, and others if it
+ * likes, in whatever order and on whatever thread, the same ones each time. They come into s.picked in their order; returns how many
+ * there are. most(): the largest score of a thread's. The first `waves` waves have all of them, evenly, and `least` is a bound
+ * that is known. Called by the whole block; s.picked is its own until the next call.
  */
-template <typename EACH>
-__device__ __forceinline__ int pick(PickShared &s, int take, int waves, double least, EACH each) {
+template <typename MOST, typename EACH>
+__device__ __forceinline__ int pick(PickShared &s, int take, int waves, double least, MOST most, EACH each) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, rank = (take + waves - 1) / waves;
     float bound = __builtin_inff();
-    if (wave < waves) {
-        double mine = -__builtin_inf();
-        each([&](double score, int) { mine = score > mine ? score : mine; });
-        bound = rank <= 64 ? wave_bound(not_above(mine), rank) : -__builtin_inff();
-    }
+    if (wave < waves) bound = rank <= 64 ? wave_bound(not_above(most()), rank) : -__builtin_inff();
     if (lane == 0) s.bounds[wave] = bound;
     if (tid == 0) s.count = 0;
     __syncthreads();
@@ -186,7 +191,7 @@ __device__ __forceinline__ int pick(PickShared &s, int take, int waves, double l
     bound = -wave_most(-bound);
     const double from = bound > least ? (double)bound : least;
     if (wave < waves)
-        each([&](double score, int index) {
+        each(from, [&](double score, int index) {
             if (score >= from && score > -__builtin_inf()) {
                 const int at = atomicAdd(&s.count, 1);
                 if (at < kRoom) s.list[at] = {score, index};
@@ -219,7 +224,7 @@ __device__ __forceinline__ int pick(PickShared &s, int take, int waves, double l
     for (int n = 0; n < take; ++n) {
         Entry best = {-__builtin_inf(), INT32_MAX};
         if (wave < waves)
-            each([&](double score, int index) {
+            each(-__builtin_inf(), [&](double score, int index) {
                 if (before(last.score, last.index, Entry{score, index}) && before(score, index, best)) best = {score, index};
             });
         for (int m = 1; m < 64; m *= 2) {
@@ -244,13 +249,15 @@ __global__ __launch_bounds__(kPickThreads) void beams_pick_kernel(SelectArgs a) 
     constexpr int kValues = values_a_load(BF16), kChunk = chunk_values(BF16), kHeld = 8;
     __shared__ PickShared s;
     const int group = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    /* chunks, by their numbers in the group: neighbours, which are of one beam, go to different waves. A thread's first ones are on
-     * their way from the start. */
-    const float *tops = a.tops + (long long)group * a.beams * a.chunks;
-    const int all = a.beams * a.chunks, first = wave + kPickWaves * lane;
+    /* Chunks, by their numbers in the group: neighbours, which are of one beam, go to different waves. A thread's first ones are on
+     * their way from the start. More of them than that are looked at by pieces first, in the same way. */
+    const float *tops = a.tops + (long long)group * a.beams * a.chunks, *mosts = a.mosts + (long long)group * a.beams * a.pieces;
+    const bool by_pieces = a.beams * a.chunks > kHeld * kPickThreads;
+    const float *const of = by_pieces ? mosts : tops;
+    const int each_beam = by_pieces ? a.pieces : a.chunks, all = a.beams * each_beam, first = wave + kPickWaves * lane;
     float top[kHeld];
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) top[i] = first + i * kPickThreads < all ? tops[first + i * kPickThreads] : -__builtin_inff();
+    for (int i = 0; i < kHeld; ++i) top[i] = first + i * kPickThreads < all ? of[first + i * kPickThreads] : -__builtin_inff();
     /* what a beam's logits are moved by: its score less the logarithm of its sum; NaN, which no comparison passes, where it has none */
     for (int b = wave; b < a.beams; b += kPickWaves) {
         const long long which = (long long)group * a.beams + b;
@@ -272,7 +279,7 @@ __global__ __launch_bounds__(kPickThreads) void beams_pick_kernel(SelectArgs a) 
             sum = most == next ? sum : sum * exp((double)most - (double)next);
             most = next;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) sum += part[j] == 0.0 ? 0.0 : part[j] * exp((double)of[j] - (double)most);
+            for (int j = 0; j < 4; ++j) sum += part[j] == 0.0 ? 0.0 : part[j] * exp((double)of[j] - (double)most); /* 0: nothing but -infinity */
         }
         sum = wave_sum(sum);
         const double offset = score - ((double)most + log(sum));
@@ -283,13 +290,33 @@ __global__ __launch_bounds__(kPickThreads) void beams_pick_kernel(SelectArgs a) 
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) {
         const int e = first + i * kPickThreads;
-        held[i] = e < all ? s.offsets[e / a.chunks] + (double)top[i] : -__builtin_inf();
+        held[i] = e < all ? s.offsets[e / each_beam] + (double)top[i] : -__builtin_inf();
     }
-    const int chunks = pick(s, a.take, kPickWaves, -__builtin_inf(), [&](auto &&f) {
+    auto each = [&](double, auto &&f) {
 #pragma unroll
         for (int i = 0; i < kHeld; ++i) f(held[i], first + i * kPickThreads);
-        for (int e = first + kHeld * kPickThreads; e < all; e += kPickThreads) f(s.offsets[e / a.chunks] + (double)tops[e], e);
-    });
+        for (int e = first + kHeld * kPickThreads; e < all; e += kPickThreads) f(s.offsets[e / each_beam] + (double)of[e], e);
+    };
+    auto largest = [&] {
+        double most = -__builtin_inf();
+        each(0.0, [&](double score, int) { most = score > most ? score : most; });
+        return most;
+    };
+    int chunks = pick(s, a.take, kPickWaves, -__builtin_inf(), largest, each);
+    if (by_pieces) {
+        /* the chunks of `chunks` pieces, a thread each */
+        static_assert(kMostTake * kLoads <= kPickThreads, "one chunk a thread");
+        const double least = chunks == a.take ? s.picked[chunks - 1].score : -__builtin_inf();
+        double score = -__builtin_inf();
+        int number = 0;
+        if (first < chunks * kLoads) {
+            const int e = s.picked[first / kLoads].index, beam = e / a.pieces, chunk = (e - beam * a.pieces) * kLoads + first % kLoads;
+            number = beam * a.chunks + chunk;
+            if (chunk < a.chunks) score = s.offsets[beam] + (double)tops[number];
+        }
+        __syncthreads();
+        chunks = pick(s, a.take, kPickWaves, least, [&] { return score; }, [&](double, auto &&f) { f(score, number); });
+    }
     /* Their values: a wave's load is a chunk, all of a wave's on their way at once. The last of `take` chunks' largest value is a bound. */
     const double least = chunks == a.take ? s.picked[chunks - 1].score : -__builtin_inf();
     constexpr int kMost = kMostTake / kPickWaves;
@@ -307,18 +334,39 @@ __global__ __launch_bounds__(kPickThreads) void beams_pick_kernel(SelectArgs a) 
             raw[i] = load_raw<BF16>(row_of<BF16>(a, group, beam), at, a.vocab);
         }
     }
-    /* values behind a row's end are -infinity: never picked, whatever their numbers */
+    float most[kMost]; /* of the lane's values of a chunk; values behind a row's end are -infinity, and never picked */
+#pragma unroll
+    for (int i = 0; i < kMost; ++i) {
+        most[i] = -__builtin_inff();
+        if (base[i] >= 0)
+#pragma unroll
+            for (int j = 0; j < kValues; ++j) most[i] = fmaxf(most[i], value_of<BF16>(raw[i], j));
+    }
     __syncthreads();
-    const int found = pick(s, a.take, chunks < kPickWaves ? (chunks ? chunks : 1) : kPickWaves, least, [&](auto &&f) {
+    const int found = pick(
+        s, a.take, chunks < kPickWaves ? (chunks ? chunks : 1) : kPickWaves, least,
+        [&] {
+            double largest = -__builtin_inf();
 #pragma unroll
-        for (int i = 0; i < kMost; ++i)
-            if (base[i] >= 0) {
-                u4 own = raw[i];
-                asm volatile("" : "+v"(own)); /* or every score is kept from one pass to the next, in more registers than there are */
+            for (int i = 0; i < kMost; ++i)
+                if (base[i] >= 0) {
+                    const double score = offset[i] + (double)most[i];
+                    largest = score > largest ? score : largest;
+                }
+            return largest;
+        },
+        [&](double from, auto &&f) {
 #pragma unroll
-                for (int j = 0; j < kValues; ++j) f(offset[i] + (double)value_of<BF16>(own, j), base[i] + j);
-            }
-    });
+            for (int i = 0; i < kMost; ++i)
+                if (base[i] >= 0 && offset[i] + (double)most[i] >= from)
+#pragma unroll
+                    for (int j = 0; j < kValues; ++j) {
+                        u4 own = raw[i];
+                        asm volatile("" : "+v"(own)); /* or scores are kept for where they are needed again, in more registers than there are */
+                        const double score = offset[i] + (double)value_of<BF16>(own, j);
+                        if (score >= from) f(score, base[i] + j);
+                    }
+        });
     for (int i = tid; i < a.take; i += kPickThreads) {
         const bool real = i < found;
         const Entry own = s.picked[real ? i : 0];
