@@ -46,6 +46,7 @@ struct AttnArgs {
     float scale;      /* |scale| log2(e) */
     uint32_t flip;    /* sign bits of a BF16 pair of q: a negative scale turns its sign over */
     W4A16KvTree tree; /* of the kernels with TREE */
+    int least;        /* units of a part at least, where pairs are cut */
 };
 
 constexpr int kFewestTokens = 256; /* of a split of the chunk kernel */
@@ -135,7 +136,7 @@ constexpr int kMostUnits = 1 << 23; /* of 2^30 tokens */
 
 /* Finds the `item`th tile of RM rows: the sequences' tiles are counted 64 sequences at a time.
  * Sequences whose rows do not lie in the call's tensors have none. */
-template <int RM, bool TREE>
+template <int RM>
 __device__ __forceinline__ bool find_tile(const AttnArgs &a, int item, int split, Tile *t) {
     const int lane = threadIdx.x & 63;
     int left = item;
@@ -162,9 +163,8 @@ __device__ __forceinline__ bool find_tile(const AttnArgs &a, int item, int split
         if (base + 64 >= a.kv.seqs) return false;
     }
     t->seq = __builtin_amdgcn_readfirstlane(t->seq);
-    if constexpr (TREE) t->nodes = __builtin_amdgcn_readfirstlane(tree_nodes(a, t->seq));
     t->old = __builtin_amdgcn_readfirstlane(kv_length(a.kv, t->seq)) - t->news;
-    fill_tile<RM, TREE>(a, t);
+    fill_tile<RM, false>(a, t);
     /* splits begin at multiples of 32 tokens and have at least kFewestTokens */
     const int from = t->lo & ~31, span = t->hi - from;
     int per = (span + a.splits - 1) / a.splits;
@@ -178,7 +178,7 @@ __device__ __forceinline__ bool find_tile(const AttnArgs &a, int item, int split
 }
 
 /*
- * The few-row kernel's work is cut by the lengths that it finds: with N units of kUnit tokens over
+ * The few-row kernel's work, and with trees the chunk kernel's too, is cut by the lengths that it finds: with N units of kUnit tokens over
  * all (tile, head) pairs and a.splits blocks wanted, every pair is cut into parts of
  * ceil(N / a.splits) units, so that long sequences have many parts and none is much longer
  * than another. The parts are counted through the sequences; a part is a block's, and its place in
@@ -235,7 +235,8 @@ __device__ __forceinline__ int part_units(const AttnArgs &a, Seqs *q) {
     }
     const unsigned long long wanted = pairs < a.splits ? a.splits - pairs / 2 : a.splits;
     const unsigned long long each = (total + wanted - 1) / wanted;
-    return each < 1 ? 1 : each > kMostUnits ? kMostUnits : (int)each;
+    const int least = TREE ? a.least : 1;
+    return each < least ? least : each > kMostUnits ? kMostUnits : (int)each;
 }
 
 /* The part of this block (PAIR false) or the (tile, head) pair of number `index` (true): the tile, its head, its number of
@@ -375,7 +376,7 @@ __device__ __forceinline__ float times_power(int biased) { return power_of_two(b
  * ragged sequences of up to 8192 tokens, D = 128, INT8, 129 and 93.5 us; 16 of 4096 with five rows each, FP8,
  * RT = 2, 31.0 and 25.4; 64 of 8192, D = 256, FP8, 152 and 109, though 2 of 100003 take 91 and 94. */
 constexpr int rows_blocks(int dim, int format, int rt) {
-    return dim == 256 ? (format == W4A16_KV_BF16 ? 1 : 2) : dim == 128 ? (rt == 1 ? 3 : 2) : rt == 1 ? 4 : 3;
+    return dim == 256 && rt == 2 ? 1 : dim == 256 ? (format == W4A16_KV_BF16 ? 1 : 2) : dim == 128 ? (rt == 1 ? 3 : 2) : rt == 1 ? 4 : 3;
 }
 
 /*
@@ -498,7 +499,10 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
     }
 
     /* this lane's rows: their queries as the products' operand, and the keys they see */
-    bf8 q[RT][KS];
+    /* 32 rows of 256 values: in LDS, beside sums that take half of the registers */
+    constexpr bool kStored = D == 256 && RT == 2;
+    __shared__ bf8 q_stored[kStored ? RT * KS * 64 : 1];
+    bf8 q[RT][kStored ? 1 : KS];
     int lo[RT], hi[RT]; /* TREE: unused, tree_sees instead */
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
@@ -511,10 +515,14 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             const int d = kCoded ? 64 * (s / 2) + 16 * g + 8 * (s % 2) : 32 * s + 8 * g;
+            if (kStored && s % 4 != wave) continue;
             const u4 x = *reinterpret_cast<const u4 *>(row + d);
-            q[r][s] = as_bf8(real ? x.x ^ a.flip : 0u, real ? x.y ^ a.flip : 0u, real ? x.z ^ a.flip : 0u, real ? x.w ^ a.flip : 0u);
+            const bf8 y = as_bf8(real ? x.x ^ a.flip : 0u, real ? x.y ^ a.flip : 0u, real ? x.z ^ a.flip : 0u, real ? x.w ^ a.flip : 0u);
+            if constexpr (kStored) q_stored[(r * KS + s) * 64 + lane] = y;
+            else q[r][s] = y;
         }
     }
+    if constexpr (kStored) __syncthreads();
 
     f4 acc[RT][E];
     float m[RT], l[RT];
@@ -579,6 +587,12 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
         if constexpr (!kAhead)
             if (more) load_pages(next);
         f4 s[RT][2];
+        int q_lane = lane;
+        if constexpr (kStored) asm volatile("" : "+v"(q_lane)); /* or what is read is kept */
+        auto query = [&](int r, int step) {
+            if constexpr (kStored) return q_stored[(r * KS + step) * 64 + q_lane];
+            else return q[r][step];
+        };
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
 #pragma unroll
@@ -592,12 +606,12 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
                     const bf8 k1 = as_bf8(kv_widen<FMT, 0>(x.z), kv_widen<FMT, 1>(x.z), kv_widen<FMT, 0>(x.w), kv_widen<FMT, 1>(x.w));
 #pragma unroll
                     for (int r = 0; r < RT; ++r) {
-                        s[r][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, q[r][2 * j], s[r][c], 0, 0, 0);
-                        s[r][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, q[r][2 * j + 1], s[r][c], 0, 0, 0);
+                        s[r][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, query(r, 2 * j), s[r][c], 0, 0, 0);
+                        s[r][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, query(r, 2 * j + 1), s[r][c], 0, 0, 0);
                     }
                 } else {
 #pragma unroll
-                    for (int r = 0; r < RT; ++r) s[r][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, x), q[r][j], s[r][c], 0, 0, 0);
+                    for (int r = 0; r < RT; ++r) s[r][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, x), query(r, j), s[r][c], 0, 0, 0);
                 }
             }
         }
@@ -957,12 +971,15 @@ __global__ __launch_bounds__(256, chunk_blocks(D, TIGHT)) void attn_chunk_kernel
     int *bad = reinterpret_cast<int *>(smem + C::kFlags);         /* [step % 3]: a token without a page */
     int *exponents = bad + 3;                                      /* [step % 2]: V's scales are over 2 to this, biased; + 256: one is not finite */
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 31, half = lane >> 5;
-    const int head = blockIdx.x % a.kv.heads, split = blockIdx.y;
     /* the last tiles of a sequence see the most keys: those first */
-    const int item = a.items - 1 - (int)(blockIdx.x / a.kv.heads);
+    int head = blockIdx.x % a.kv.heads, split = blockIdx.y, item = a.items - 1 - (int)(blockIdx.x / a.kv.heads), first_part;
     Tile t;
-    if (!find_tile<RM, TREE>(a, item, split, &t)) return;
-    if (split >= t.active) return;
+    if constexpr (TREE) {
+        if (!find_part<RM, false, TREE>(a, blockIdx.x, &t, &head, &first_part)) return;
+    } else {
+        if (!find_tile<RM>(a, item, split, &t)) return;
+        if (split >= t.active) return;
+    }
 
     const int32_t *table = a.kv.table + (long long)t.seq * a.kv.table_stride;
     const int mask = (1 << a.kv.shift) - 1;
@@ -1308,7 +1325,7 @@ __global__ __launch_bounds__(256, chunk_blocks(D, TIGHT)) void attn_chunk_kernel
     }
     if (!real) return;
     float by = !kCoded ? 1.0f : spoiled ? __builtin_nanf("") : times_power(v_exp);
-    float *partial = t.active > 1 ? partial_at<D, RM>(a, ((long long)item * a.kv.heads + head) * a.splits + split) : nullptr;
+    float *partial = t.active > 1 ? partial_at<D, RM>(a, TREE ? blockIdx.x : ((long long)item * a.kv.heads + head) * a.splits + split) : nullptr;
     if (partial) {
 #pragma unroll
         for (int d = 0; d < DB; ++d)
@@ -1349,7 +1366,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
         if (first_part + t.active > a.blocks) return; /* sequences that overlap: not all parts were worked on */
     } else {
         head = blockIdx.x % a.kv.heads;
-        if (!find_tile<RM, TREE>(a, blockIdx.x / a.kv.heads, 0, &t)) return;
+        if (!find_tile<RM>(a, blockIdx.x / a.kv.heads, 0, &t)) return;
     }
     if (t.active < 2 || (int)blockIdx.y * kRows >= t.rows) return;
     const int lane = threadIdx.x & 15, unit = threadIdx.x >> 4, sub = unit / kRows, i = blockIdx.y * kRows + unit % kRows;
@@ -1428,7 +1445,8 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
 struct Part {
     int items, splits, over, upto;
     size_t ws_at;
-    long long blocks; /* few rows */
+    long long blocks; /* few rows, and with trees */
+    int least;
 };
 struct Plan {
     int rt;
@@ -1438,18 +1456,19 @@ struct Plan {
 
 constexpr int kChunkRows = 128;
 
-Plan plan_of(const W4A16KvCache *c, const W4A16KvBatch *b, int q_heads) {
+Plan plan_of(const W4A16KvCache *c, const W4A16KvBatch *b, int q_heads, bool tree) {
     Plan p = {};
     const int group = q_heads / c->kv_heads, dim = c->head_dim;
     const int max_new = b->max_new ? b->max_new : b->rows;
     const long long rows = (long long)b->rows * group, longest = (long long)max_new * group;
     const long long seqs = b->seqs < b->rows ? b->seqs : b->rows;
-    /* attn_rows_kernel has registers for 32 rows, or 16 of 256 values */
-    const int limit = dim == 256 ? 16 : 32;
-    p.rt = longest <= 16 || dim == 256 ? 1 : 2;
+    /* attn_rows_kernel has registers for 32 rows, or 16 of 256 values at two blocks a CU; trees have more than 16 more often
+     * than not, and one block is better than the chunk kernel there */
+    const int limit = dim == 256 && !tree ? 16 : 32;
+    p.rt = longest <= 16 || limit == 16 ? 1 : 2;
     const int rm = 16 * p.rt;
-    p.few = {0, 1, 0, INT32_MAX, 0, 0};
-    p.many = {0, 1, 0, INT32_MAX, 0, 0};
+    p.few = {0, 1, 0, INT32_MAX, 0, 0, 1};
+    p.many = {0, 1, 0, INT32_MAX, 0, 0, 1};
     if (longest <= limit) {
         p.few.items = (int)(rows / rm + seqs);
     } else if ((long long)b->seqs * max_new == b->rows || group > limit) {
@@ -1479,7 +1498,18 @@ Plan plan_of(const W4A16KvCache *c, const W4A16KvBatch *b, int q_heads) {
         p.few.blocks = p.few.splits + pairs;
         if (p.few.splits) p.ws_bytes = (size_t)p.few.blocks * rm * (dim + 2) * 4;
     }
-    if (p.many.items) {
+    if (p.many.items && tree) {
+        /* A tree's rows see all of what stands before them, and sequences are as long as they are: parts of equal size, one round
+         * of blocks. */
+        const long long blocks = (long long)chunk_blocks(dim, dim == 256) * device_cus();
+        const long long pairs = (long long)p.many.items * c->kv_heads, units = pairs * ((tokens + kUnit - 1) / kUnit);
+        p.many.splits = (int)(units < 1 ? 1 : units < blocks ? units : blocks);
+        if (pairs > 65536) p.many.splits = 0;
+        p.many.least = 2;
+        p.many.blocks = p.many.splits + pairs;
+        p.many.ws_at = p.ws_bytes;
+        if (p.many.splits) p.ws_bytes += (size_t)p.many.blocks * kChunkRows * (dim + 2) * 4;
+    } else if (p.many.items) {
         /* Two blocks a CU, by the tiles there are if max_new holds (`items` can be up to twice as many);
          * one, or parts of `least` tokens, where two would make those shorter, since a part's results
          * are 66 KB at 128 values a head. 16 sequences of 4096 tokens with 32 new ones, FP8: 1024 tokens
@@ -1511,6 +1541,9 @@ void launch_join(int parts, const AttnArgs &a, hipStream_t s) {
     else if (parts > 1) launch_k(attn_join_kernel<D, RM, 1, EVEN, TREE>, dim3(x, RM / 16), dim3(256), 0, s, a);
 }
 
+/* Parts of a (tile, head), about. */
+int parts_of(const AttnArgs &a) { return (a.splits + a.items * a.kv.heads - 1) / (a.items * a.kv.heads) + 1; }
+
 AttnArgs part_args(const AttnArgs &all, const Part &p) {
     AttnArgs a = all;
     a.items = p.items;
@@ -1518,6 +1551,7 @@ AttnArgs part_args(const AttnArgs &all, const Part &p) {
     a.blocks = (int)p.blocks;
     a.over = p.over;
     a.upto = p.upto;
+    a.least = p.least;
     a.ws += p.ws_at / 4;
     return a;
 }
@@ -1533,20 +1567,24 @@ void launch_format(const Plan &p, const AttnArgs &all, hipStream_t s) {
                 kernel = attn_chunk_kernel<D, FMT, true, TREE>;
                 lds = Chunk<D, FMT, true, TREE>::kBytes;
             }
-        launch_k(kernel, dim3(a.kv.heads * a.items, a.splits), dim3(256), lds, s, a);
-        launch_join<D, kChunkRows, false, TREE>(a.splits, a, s);
+        if constexpr (TREE) {
+            launch_k(kernel, dim3((unsigned)p.many.blocks), dim3(256), lds, s, a);
+            if (a.splits) launch_join<D, kChunkRows, true, TREE>(parts_of(a), a, s);
+        } else {
+            launch_k(kernel, dim3(a.kv.heads * a.items, a.splits), dim3(256), lds, s, a);
+            launch_join<D, kChunkRows, false, TREE>(a.splits, a, s);
+        }
     }
     if (p.few.items) {
         const AttnArgs a = part_args(all, p.few);
-        const int parts = (a.splits + a.items * a.kv.heads - 1) / (a.items * a.kv.heads) + 1; /* of each, about */
-        if constexpr (D <= 128)
+        if constexpr (D <= 128 || TREE)
             if (p.rt == 2) {
                 launch_k(attn_rows_kernel<D, FMT, 2, TREE>, dim3((unsigned)p.few.blocks), dim3(256), 0, s, a);
-                if (a.splits) launch_join<D, 32, true, TREE>(parts, a, s);
+                if (a.splits) launch_join<D, 32, true, TREE>(parts_of(a), a, s);
                 return;
             }
         launch_k(attn_rows_kernel<D, FMT, 1, TREE>, dim3((unsigned)p.few.blocks), dim3(256), 0, s, a);
-        if (a.splits) launch_join<D, 16, true, TREE>(parts, a, s);
+        if (a.splits) launch_join<D, 16, true, TREE>(parts_of(a), a, s);
     }
 }
 
@@ -1573,16 +1611,28 @@ int check_heads(const KvView &kv, int q_heads, const char *what) {
 
 } // namespace
 
-extern "C" int w4a16_paged_attention_workspace(const W4A16KvCache *cache, const W4A16KvBatch *batch, int q_heads,
-                                               size_t *bytes) {
-    const char *what = "w4a16_paged_attention_workspace";
+namespace {
+
+int workspace(const char *what, const W4A16KvCache *cache, const W4A16KvBatch *batch, int q_heads, bool tree, size_t *bytes) {
     if (!bytes) return set_error(W4A16_ERR_CONFIG, "%s: null result", what);
     KvView kv;
     int st = kv_check(cache, batch, what, &kv);
     if (!st) st = check_heads(kv, q_heads, what);
     if (st) return st;
-    *bytes = kv.rows && kv.seqs ? plan_of(cache, batch, q_heads).ws_bytes : 0;
+    *bytes = kv.rows && kv.seqs ? plan_of(cache, batch, q_heads, tree).ws_bytes : 0;
     return W4A16_OK;
+}
+
+} // namespace
+
+extern "C" int w4a16_paged_attention_workspace(const W4A16KvCache *cache, const W4A16KvBatch *batch, int q_heads,
+                                               size_t *bytes) {
+    return workspace("w4a16_paged_attention_workspace", cache, batch, q_heads, false, bytes);
+}
+
+extern "C" int w4a16_paged_tree_attention_workspace(const W4A16KvCache *cache, const W4A16KvBatch *batch, int q_heads,
+                                                    size_t *bytes) {
+    return workspace("w4a16_paged_tree_attention_workspace", cache, batch, q_heads, true, bytes);
 }
 
 namespace {
@@ -1614,7 +1664,7 @@ int attend(const char *what, const W4A16KvCache *cache, const W4A16KvBatch *batc
     if (!qb || !ob) return set_error(W4A16_ERR_CONFIG, "%s: strides must be multiples of 8 elements from 0", what);
     const RowsView qr = {q, qb, q_row_stride, q_head_stride, q_heads}, outs = {out, ob, out_row_stride, out_head_stride, q_heads};
     if (!rows_apart(kv.rows, outs, dim)) return set_error(W4A16_ERR_CONFIG, "%s: output rows overlap each other", what);
-    const Plan p = plan_of(cache, batch, q_heads);
+    const Plan p = plan_of(cache, batch, q_heads, tree != nullptr);
     if (p.ws_bytes > 0 && (!ws || ws_bytes < p.ws_bytes))
         return set_error(W4A16_ERR_CONFIG, "%s: a workspace of %zu bytes, the call needs %zu", what, ws ? ws_bytes : 0,
                          p.ws_bytes);
@@ -1657,7 +1707,7 @@ int attend(const char *what, const W4A16KvCache *cache, const W4A16KvBatch *batc
     a.q_heads = q_heads;
     a.causal = causal != 0;
     a.window = window;
-    a.splits = a.items = a.blocks = a.over = a.upto = 0; /* part_args */
+    a.splits = a.items = a.blocks = a.over = a.upto = a.least = 0; /* part_args */
     a.scale = fabsf(scale) * 1.4426950408889634f;
     a.flip = scale < 0.0f ? 0x80008000u : 0u;
     a.tree = tree ? *tree : W4A16KvTree{};

@@ -109,6 +109,7 @@ _SIGNATURES = {
     "w4a16_paged_attention_bf16": (_i, [_vp, _vp, _vp, _ll, _ll, _i, ctypes.c_float, _i, _i, _vp, _ll, _ll, _vp, _vp,
                                         ctypes.c_size_t, _vp]),
     "w4a16_kv_tree_plan": (_i, [_vp, _vp, _i, _vp, _i, _vp, _vp, _vp]),
+    "w4a16_paged_tree_attention_workspace": (_i, [_vp, _vp, _i, ctypes.POINTER(ctypes.c_size_t)]),
     "w4a16_paged_tree_attention_bf16": (_i, [_vp, _vp, _vp, _vp, _ll, _ll, _i, ctypes.c_float, _i, _vp, _ll, _ll, _vp, _vp,
                                              ctypes.c_size_t, _vp]),
     "w4a16_verify_tree_workspace": (_i, [_i, _i, _i, ctypes.POINTER(ctypes.c_size_t)]),
@@ -998,11 +999,12 @@ def paged_attention(q, cache, batch, scale=None, causal=True, window=0, out=None
     if return_lse:
         lse = torch.full((rows, q_heads), float("-inf"), device=device) if batch.padded else \
             torch.empty((rows, q_heads), dtype=torch.float32, device=device)
-    key = (cache._plan, q_heads)
+    key = (cache._plan, q_heads, tree is None)
     need = batch._workspaces.get(key)  # by the sizes alone
     if need is None:
         size = ctypes.c_size_t(0)
-        _check(lib.w4a16_paged_attention_workspace(cache._ref, batch._ref, q_heads, ctypes.byref(size)), "paged_attention")
+        ask = lib.w4a16_paged_attention_workspace if tree is None else lib.w4a16_paged_tree_attention_workspace
+        _check(ask(cache._ref, batch._ref, q_heads, ctypes.byref(size)), "paged_attention")
         need = batch._workspaces[key] = size.value
     wp = None
     if need:

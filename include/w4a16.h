@@ -468,7 +468,8 @@ int w4a16_kv_tree_plan(const W4A16KvBatch *batch, const int32_t *parents, int pa
 /* w4a16_paged_attention_bf16 for such rows: a row sees the tokens before its sequence's tree, and of the tree the nodes that
  * its bits name, none behind its own place. window > 0 (at least `nodes`): none of the tokens before the tree whose position is
  * `window` or more before the row's (positions outside base .. the row's place count as the nearer of the two, base being the
- * tokens before the tree). The workspace is that of w4a16_paged_attention_workspace. */
+ * tokens before the tree). The workspace is as w4a16_paged_attention_bf16's, of the bytes w4a16_paged_tree_attention_workspace gives. */
+int w4a16_paged_tree_attention_workspace(const W4A16KvCache *cache, const W4A16KvBatch *batch, int q_heads, size_t *bytes);
 int w4a16_paged_tree_attention_bf16(const W4A16KvCache *cache, const W4A16KvBatch *batch, const W4A16KvTree *tree,
                                     const uint16_t *q, long long q_row_stride, long long q_head_stride,
                                     int q_heads, float scale, int window, uint16_t *out,
