@@ -1091,7 +1091,10 @@ __global__ __launch_bounds__(256, chunk_blocks(D, TIGHT)) void attn_chunk_kernel
     }
 
     /* this lane's row: its queries and the keys it sees */
-    int i_row = wave * 32 + n, token = (t.start + i_row) / a.group, h = head * a.group + (t.start + i_row) % a.group;
+    /* TREE: a wave without any rows only helps with the tiles. Which waves have the rows goes round with the blocks, so that those of the
+     * blocks that share a CU are on different SIMDs. */
+    const int turn = TREE ? (blockIdx.x + 2 * (blockIdx.x >> 8)) & 3 : 0;
+    int i_row = ((wave + turn) & 3) * 32 + n, token = (t.start + i_row) / a.group, h = head * a.group + (t.start + i_row) % a.group;
     bool real = i_row < t.rows;
     const int place = t.old + token;
     /* TREE: unused, tree_sees instead */
@@ -1103,8 +1106,9 @@ __global__ __launch_bounds__(256, chunk_blocks(D, TIGHT)) void attn_chunk_kernel
     auto row_of = [&] {
         int tid = threadIdx.x;
         asm volatile("" : "+v"(tid)); /* or it is kept over the loop, and what follows from it */
-        return (tid >> 6) * 32 + (tid & 31);
+        return (((tid >> 6) + turn) & 3) * 32 + (tid & 31);
     };
+    const bool idle = TREE && __builtin_amdgcn_readfirstlane(i_row) >= t.rows;
     auto token_of = [&] { return tokens[row_of()]; };
     constexpr int kHeld = KS - C::kStored;
     bf8 q[kHeld], *const q_stored = reinterpret_cast<bf8 *>(smem + C::kQueries) + half * RM + i_row;
@@ -1158,6 +1162,8 @@ __global__ __launch_bounds__(256, chunk_blocks(D, TIGHT)) void attn_chunk_kernel
         if constexpr (TIGHT) asm volatile("" : "+v"(k_at), "+v"(v_at));
         const uint8_t *kt = smem + (step & 1) * 2 * C::kTile, *vt = kt + C::kTile;
         const float *sc = scales + (step & 1) * 2 * BN;
+        uint32_t p[kHalves][8];
+        if (!idle) {
         f16v s[kHalves];
 #pragma unroll
         for (int c = 0; c < kHalves; ++c) {
@@ -1231,7 +1237,6 @@ __global__ __launch_bounds__(256, chunk_blocks(D, TIGHT)) void attn_chunk_kernel
                 v_exp = now;
             }
         }
-        uint32_t p[kHalves][8];
 #pragma unroll
         for (int c = 0; c < kHalves; ++c)
 #pragma unroll
@@ -1248,6 +1253,7 @@ __global__ __launch_bounds__(256, chunk_blocks(D, TIGHT)) void attn_chunk_kernel
                 p[c][2 * b] = kCoded ? pack_f16(w[0], w[1]) : kv_pack_bf16(w[0], w[1]);
                 p[c][2 * b + 1] = kCoded ? pack_f16(w[2], w[3]) : kv_pack_bf16(w[2], w[3]);
             }
+        }
         if constexpr (!kCoded) {
             /* Tokens that are not there weigh nothing, and what memory holds for them is taken
              * out. An infinity or a NaN among values that not every row sees: 0 times it would
@@ -1288,6 +1294,7 @@ __global__ __launch_bounds__(256, chunk_blocks(D, TIGHT)) void attn_chunk_kernel
             }
         }
         /* O^T: 16 tokens and 32 values a product */
+        if (!idle) {
 #pragma unroll
         for (int u = 0; u < BN / 16; ++u) {
             const uint32_t *w = &p[u / 2][4 * (u % 2)];
@@ -1310,6 +1317,7 @@ __global__ __launch_bounds__(256, chunk_blocks(D, TIGHT)) void attn_chunk_kernel
             }
         }
         interleave<BN / 16 * DB, 2, kFar>();
+        }
         if (more) store_tile(step + 1);
         if (look && tid < 64) put_page(step + 2, entry);
         __syncthreads();
