@@ -1477,17 +1477,23 @@ Plan plan_of(const W4A16KvCache *c, const W4A16KvBatch *b, int q_heads, bool tre
     const int rm = 16 * p.rt;
     p.few = {0, 1, 0, INT32_MAX, 0, 0, 1};
     p.many = {0, 1, 0, INT32_MAX, 0, 0, 1};
-    if (longest <= limit) {
+    const long long most_tokens = b->max_kv ? b->max_kv : (long long)b->table_pages * c->page_size;
+    const long long short_units = (rows / rm + seqs) * c->kv_heads * ((most_tokens + kUnit - 1) / kUnit);
+    if (longest <= limit || (tree && short_units <= 4 * device_cus())) {
+        /* Trees over few tokens too: tiles of 128 rows would leave most of the CUs without any, and take longer to begin. One sequence of
+         * 1500 tokens, 8 key heads of 128, BF16: 36, 64, 128 rows 14.6, 14.1, 17.2 us, with the chunk kernel 18.1, 18.8,
+         * 23.6; of 20000: 31.5, 32.7, 44.8 and 30.0, 31.1, 40.9. */
         p.few.items = (int)(rows / rm + seqs);
-    } else if ((long long)b->seqs * max_new == b->rows || group > limit) {
-        /* all alike (whatever the bound says, this launch takes every sequence) */
+    } else if ((long long)b->seqs * max_new == b->rows || group > limit || (tree && rows > 32 * seqs)) {
+        /* all alike (whatever the bound says, this launch takes every sequence), or of trees that have more rows on average: two
+         * launches more cost more than a few idle waves */
         p.many.items = (int)(rows / kChunkRows + seqs);
     } else {
         p.few.items = (int)seqs;
         p.few.upto = p.many.over = rm;
         p.many.items = (int)(rows / kChunkRows + (rows / (rm + 1) < seqs ? rows / (rm + 1) : seqs));
     }
-    const long long tokens = b->max_kv ? b->max_kv : (long long)b->table_pages * c->page_size;
+    const long long tokens = most_tokens;
     if (p.few.items) {
         /* One round of blocks, and no more than there are units. Two rounds are better for batches of many
          * sequences and worse for few or short ones; the host knows bounds, not lengths, and one round loses least
