@@ -217,8 +217,9 @@ __device__ __forceinline__ Seqs load_seqs(const AttnArgs &a, int base) {
 /* Units of a part; *q is left with the first 64 sequences. N / (blocks wanted) where that makes no
  * more parts than blocks; each pair's last part is on average half as long. */
 template <int RM, bool TREE>
-__device__ __forceinline__ int part_units(const AttnArgs &a, Seqs *q) {
+__device__ __forceinline__ int part_units(const AttnArgs &a, Seqs *q, bool *equal) {
     *q = load_seqs<RM, TREE>(a, 0);
+    *equal = false;
     if (a.splits == 0) return kMostUnits; /* pairs are whole */
     /* n < 2^47 in two pieces, whose sums over 64 lanes fit 32 bits */
     unsigned long long total = 0;
@@ -235,8 +236,20 @@ __device__ __forceinline__ int part_units(const AttnArgs &a, Seqs *q) {
     }
     const unsigned long long wanted = pairs < a.splits ? a.splits - pairs / 2 : a.splits;
     const unsigned long long each = (total + wanted - 1) / wanted;
-    const int least = TREE ? a.least : 1;
-    return each < least ? least : each > kMostUnits ? kMostUnits : (int)each;
+    if constexpr (TREE) {
+        if (RM == 128 && a.kv.seqs <= 64 && pairs > 0 && pairs < a.splits) {
+            /* Sequences that are about as long as each other: as many equal parts of each pair as are one round of blocks. 250 nodes over
+             * 16384 tokens: four of 32 units, not three of 37 and one of 17, 189 and 215 us. Of ragged ones the short rests fill the gaps. */
+            const long long most = wave_most(q->pairs ? q->units : 0);
+            if (8 * most * pairs <= 9 * (long long)total) {
+                *equal = true;
+                const int parts = a.splits / (int)pairs, size = ((int)most + parts - 1) / parts;
+                return size < a.least ? a.least : size;
+            }
+        }
+        return each < a.least ? a.least : each > kMostUnits ? kMostUnits : (int)each;
+    }
+    return each < 1 ? 1 : each > kMostUnits ? kMostUnits : (int)each;
 }
 
 /* The part of this block (PAIR false) or the (tile, head) pair of number `index` (true): the tile, its head, its number of
@@ -244,7 +257,8 @@ __device__ __forceinline__ int part_units(const AttnArgs &a, Seqs *q) {
 template <int RM, bool PAIR, bool TREE>
 __device__ __forceinline__ bool find_part(const AttnArgs &a, int index, Tile *t, int *head, int *first_part) {
     Seqs q;
-    const int each = part_units<RM, TREE>(a, &q);
+    bool equal; /* TREE: a pair's parts are alike */
+    const int each = part_units<RM, TREE>(a, &q, &equal);
     int left = index, before = 0; /* parts of the sequences before */
     for (int base = 0;;) {
         const int per = (q.units + each - 1) / each, parts = q.pairs * per;
@@ -265,8 +279,11 @@ __device__ __forceinline__ bool find_part(const AttnArgs &a, int index, Tile *t,
             *head = pair % a.kv.heads;
             t->start = pair / a.kv.heads * RM;
             fill_tile<RM, TREE>(a, t);
-            t->begin = from + part * each * kUnit;
-            t->end = part + 1 < t->active && t->begin + each * kUnit < t->hi ? t->begin + each * kUnit : t->hi;
+            int size = each;
+            if constexpr (TREE)
+                if (equal) size = (__builtin_amdgcn_readlane(q.units, l) + t->active - 1) / t->active;
+            t->begin = from + part * size * kUnit;
+            t->end = part + 1 < t->active && t->begin + size * kUnit < t->hi ? t->begin + size * kUnit : t->hi;
             return true;
         }
         left -= __builtin_amdgcn_readlane(upto, 63);
