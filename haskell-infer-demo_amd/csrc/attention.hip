@@ -104,29 +104,57 @@ __device__ __forceinline__ void fill_tile(const AttnArgs &a, Tile *t) {
     if (t->hi <= t->lo) t->hi = t->lo = 0; /* the window may begin behind the last key */
 }
 
-/* TREE: which of the 32 tokens from `at` on the sequence's row `token` sees (none: -1), bit k for token at + k. Everything that it
- * follows from is found anew at each step that needs it: kept over a loop it would cost registers that there are not. */
-__device__ __forceinline__ uint32_t tree_sees(const AttnArgs &a, const Tile &t, int token, int at) {
-    if (token < 0) return 0u;
-    const int row = t.first_row + token, place = t.old + token;
+/* TREE: what a tile's rows see of their tree, in LDS: a row's words of bits, its position and its token in the sequence (-1: no row). Steps
+ * that hold nodes come last, when nothing is left to hide a load behind. */
+constexpr int kTreeWords = 8, kTreePosition = kTreeWords, kTreeToken = kTreeWords + 1, kTreeRow = kTreeWords + 2;
+
+/* Fills the ROWS rows from row `first` of a tile on, by the wave that reads them: GROUPS lanes a row. In two parts, for the loads to be
+ * on their way meanwhile. */
+template <int ROWS>
+struct TreeLoad {
+    static constexpr int kGroups = 64 / ROWS, kWords = kTreeWords / kGroups;
+    uint32_t words[kWords];
+    int position, token;
+
+    __device__ __forceinline__ void load(const AttnArgs &a, const Tile &t, int first) {
+        const int lane = threadIdx.x & 63, i = first + lane % ROWS, group = lane / ROWS;
+        token = i < t.rows ? (t.start + i) / a.group : -1;
+        const long long row = t.first_row + (token < 0 ? 0 : token);
+        const int held = (a.tree.nodes + 63) >> 6 << 1;
+        const uint32_t *bits = reinterpret_cast<const uint32_t *>(a.tree.seen) + row * held;
+#pragma unroll
+        for (int w = 0; w < kWords; ++w) words[w] = group + w * kGroups < held ? bits[group + w * kGroups] : 0u;
+        position = t.window ? a.tree.positions[row] : 0;
+    }
+    __device__ __forceinline__ void store(uint32_t *rows, int first) const {
+        const int lane = threadIdx.x & 63, group = lane / ROWS;
+        uint32_t *to = rows + (first + lane % ROWS) * kTreeRow;
+#pragma unroll
+        for (int w = 0; w < kWords; ++w) to[group + w * kGroups] = words[w];
+        if (group == 0) {
+            to[kTreePosition] = position;
+            to[kTreeToken] = token;
+        }
+    }
+};
+
+/* Which of the 32 tokens from `at` on a row sees, bit k for token at + k. What it follows from is found anew at each step that needs it: kept
+ * over a loop it would cost registers that there are not. */
+__device__ __forceinline__ uint32_t tree_sees(const AttnArgs &a, const Tile &t, const uint32_t *row, int at) {
+    const int token = (int)row[kTreeToken], place = t.old + token;
     /* [from, to) of the 32 */
-    const int to = row_end(a, t, place) - at;
+    const int to = token < 0 ? 0 : row_end(a, t, place) - at;
     int from = 0;
     if (t.window) {
         /* a node's position lies between its tree's first token and its place */
-        int position = place;
-        if (place >= t.base) {
-            const int p = a.tree.positions[row];
-            position = p < t.base ? t.base : p > place ? place : p;
-        }
-        from = position - t.window + 1 - at;
+        const int p = (int)row[kTreePosition];
+        from = (place < t.base || p > place ? place : p < t.base ? t.base : p) - t.window + 1 - at;
     }
     uint32_t sees = (to >= 32 ? 0xFFFFFFFFu : to > 0 ? (1u << to) - 1u : 0u) & (from <= 0 ? 0xFFFFFFFFu : from < 32 ? 0xFFFFFFFFu << from : 0u);
     const int node = at - t.base; /* of the first of them; the tokens before node 0 are no nodes */
     if (node > -32) {
-        const int words = (a.tree.nodes + 63) >> 6 << 1, w = node >> 5;
-        const uint32_t *bits = reinterpret_cast<const uint32_t *>(a.tree.seen) + (long long)row * words;
-        const uint32_t low = w < 0 ? 0xFFFFFFFFu : w < words ? bits[w] : 0u, high = w + 1 < words ? bits[w + 1] : 0u;
+        const int w = node >> 5;
+        const uint32_t low = w < 0 ? 0xFFFFFFFFu : w < kTreeWords ? row[w] : 0u, high = w + 1 < kTreeWords ? row[w + 1] : 0u;
         sees &= __builtin_amdgcn_alignbit(high, low, node & 31);
     }
     return sees;
@@ -502,6 +530,11 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
             }
         }
     };
+    /* TREE: the rows of the tile that this wave's steps are cut for, if they are; a copy for each wave. They set out ahead of keys and values. */
+    __shared__ uint32_t tree_rows[TREE ? 4 * RM * kTreeRow : 1];
+    uint32_t *const own_rows = tree_rows + (TREE ? wave * RM * kTreeRow : 0);
+    TreeLoad<RM> of_tree;
+    if constexpr (TREE) of_tree.load(a, t, 0);
     int t0 = t.begin + 32 * wave;
     if (t0 < t.end) {
         load_pages(t0);
@@ -543,10 +576,14 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
 
     f4 acc[RT][E];
     float m[RT], l[RT];
-    auto token_of = [&](int r) { /* TREE: of this lane's row */
+    if constexpr (TREE) {
+        of_tree.store(own_rows, 0);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); /* the wave's own: no other reads it */
+    }
+    auto tree_row = [&](int r) { /* TREE: of this lane's row */
         int i = r * 16 + n;
         asm volatile("" : "+v"(i)); /* or it is kept */
-        return i < t.rows ? (t.start + i) / a.group : -1;
+        return own_rows + i * kTreeRow;
     };
     float spoiled[RT] = {}; /* 1: this lane's row has seen a scale that is no number */
     int v_exp = kLift + 1; /* biased exponent of the power of two that the weights are over (8-bit caches) */
@@ -588,7 +625,7 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
 #pragma unroll
                     for (int r = 0; r < RT; ++r) {
                         uint32_t row_sees = 0;
-                        if constexpr (TREE) row_sees = tree_sees(a, t, token_of(r), t0) >> (4 * g);
+                        if constexpr (TREE) row_sees = tree_sees(a, t, tree_row(r), t0) >> (4 * g);
 #pragma unroll
                         for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -698,7 +735,7 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
         for (int r = 0; r < RT; ++r) {
             uint32_t row_sees = 0;
             if constexpr (TREE)
-                if (cut) row_sees = tree_sees(a, t, token_of(r), t0) >> (4 * g);
+                if (cut) row_sees = tree_sees(a, t, tree_row(r), t0) >> (4 * g);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 if constexpr (kCoded) s[r][c] *= ks[c];
@@ -749,7 +786,7 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
                 uint32_t row_sees[RT];
                 if constexpr (TREE)
 #pragma unroll
-                    for (int r = 0; r < RT; ++r) row_sees[r] = tree_sees(a, t, token_of(r), t0);
+                    for (int r = 0; r < RT; ++r) row_sees[r] = tree_sees(a, t, tree_row(r), t0);
 #pragma unroll
                 for (int x = 0; x < 8; ++x) {
                     bool some = false;
@@ -935,14 +972,14 @@ struct Chunk {
     static constexpr int kPieces = D / 8;                              /* of 8 values a token */
     static constexpr int kLoads = BN * D * (kCoded ? 1 : 2) / (256 * 16); /* 16-byte loads a thread and matrix */
     static constexpr int kSwizzle = kPieces < 16 ? kPieces - 1 : 15;
-    /* LDS: [2]{K, V}, then scales [2][2][BN], pages [3][BN], flags, queries, rows' tokens (TREE) */
+    /* LDS: [2]{K, V}, then scales [2][2][BN], pages [3][BN], flags, queries, rows of the tree (TREE) */
     static constexpr int kTile = BN * D * 2;
     static constexpr int kScales = 4 * kTile, kPages = kScales + (kCoded ? 4 * BN * 4 : 0);
     static constexpr int kFlags = kPages + 3 * BN * 4, kQueries = kFlags + 32; /* bad[3], exponents[2] */
     /* the last steps' queries of a K product that stand in LDS, [step][half][row]: the registers of 8-bit
      * codes on their way leave no room for all of 256 values, or of 64 where four blocks are to fit */
-    static constexpr int kStored = !kCoded || (!TIGHT && !TREE) ? 0 : D == 256 ? 3 : D == 64 ? 1 : 0;
-    static constexpr int kTokens = kQueries + kStored * 2 * kRows * 16, kBytes = kTokens + (TREE ? kRows * 4 : 0);
+    static constexpr int kStored = !kCoded || (!TIGHT && !TREE) ? 0 : D == 256 ? TREE ? 2 : 3 : D == 64 ? TREE ? 2 : 1 : 0;
+    static constexpr int kTree = kQueries + kStored * 2 * kRows * 16, kBytes = kTree + (TREE ? kRows * kTreeRow * 4 : 0);
 };
 
 /* 16 bytes a lane from memory to LDS, lane after lane from `to` (the same on every lane). */
@@ -1101,6 +1138,11 @@ __global__ __launch_bounds__(256, chunk_blocks(D, TIGHT)) void attn_chunk_kernel
         }
     };
 
+    /* TREE: a wave without any rows only helps with the tiles. Which waves have the rows goes round with the blocks, so that those of the
+     * blocks that share a CU are on different SIMDs. */
+    const int turn = TREE ? (blockIdx.x + 2 * (blockIdx.x >> 8)) & 3 : 0;
+    TreeLoad<32> of_tree;
+    if constexpr (TREE) of_tree.load(a, t, ((wave + turn) & 3) * 32);
     if (steps > 0) {
         if (tid < 64) {
             const int first = entry_of(0), second = entry_of(steps > 1 ? 1 : 0);
@@ -1112,25 +1154,24 @@ __global__ __launch_bounds__(256, chunk_blocks(D, TIGHT)) void attn_chunk_kernel
     }
 
     /* this lane's row: its queries and the keys it sees */
-    /* TREE: a wave without any rows only helps with the tiles. Which waves have the rows goes round with the blocks, so that those of the
-     * blocks that share a CU are on different SIMDs. */
-    const int turn = TREE ? (blockIdx.x + 2 * (blockIdx.x >> 8)) & 3 : 0;
     int i_row = ((wave + turn) & 3) * 32 + n, token = (t.start + i_row) / a.group, h = head * a.group + (t.start + i_row) % a.group;
     bool real = i_row < t.rows;
     const int place = t.old + token;
     /* TREE: unused, tree_sees instead */
     const int hi = !real ? 0 : row_end(a, t, place), lo = t.window ? place - t.window + 1 : 0;
     const uint32_t seen = hi > lo ? hi - lo : 0; /* this row sees a key where its place less lo, unsigned, is below this */
-    /* TREE: rows' tokens, -1 where there is none; read by the waves that wrote them */
-    int *tokens = reinterpret_cast<int *>(smem + C::kTokens);
-    if constexpr (TREE) tokens[i_row] = real ? token : -1;
+    uint32_t *const tree_rows = reinterpret_cast<uint32_t *>(smem + C::kTree); /* TREE; read by the waves that wrote them */
     auto row_of = [&] {
         int tid = threadIdx.x;
         asm volatile("" : "+v"(tid)); /* or it is kept over the loop, and what follows from it */
         return (((tid >> 6) + turn) & 3) * 32 + (tid & 31);
     };
     const bool idle = TREE && __builtin_amdgcn_readfirstlane(i_row) >= t.rows;
-    auto token_of = [&] { return tokens[row_of()]; };
+    auto tree_row = [&] { return tree_rows + row_of() * kTreeRow; };
+    if constexpr (TREE) {
+        of_tree.store(tree_rows, __builtin_amdgcn_readfirstlane(i_row) & ~31);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
     constexpr int kHeld = KS - C::kStored;
     bf8 q[kHeld], *const q_stored = reinterpret_cast<bf8 *>(smem + C::kQueries) + half * RM + i_row;
 #pragma unroll
@@ -1170,7 +1211,7 @@ __global__ __launch_bounds__(256, chunk_blocks(D, TIGHT)) void attn_chunk_kernel
                 float *of = scales + (step & 1) * 2 * BN + BN;
 #pragma unroll 1
                 for (int in = 0; in < BN; ++in) {
-                    const bool shown = TREE ? tree_sees(a, t, token_of(), t0 + in) & 1u : (uint32_t)(t0 + in - lo) < seen;
+                    const bool shown = TREE ? tree_sees(a, t, tree_row(), t0 + in) & 1u : (uint32_t)(t0 + in - lo) < seen;
                     spoiled |= shown & !(fabsf(of[in]) < __builtin_inff());
                 }
                 __syncthreads();
@@ -1214,7 +1255,7 @@ __global__ __launch_bounds__(256, chunk_blocks(D, TIGHT)) void attn_chunk_kernel
 #pragma unroll
             for (int c = 0; c < kHalves; ++c) {
                 uint32_t row_sees = 0;
-                if constexpr (TREE) row_sees = tree_sees(a, t, token_of(), t0 + 32 * c) >> (4 * half);
+                if constexpr (TREE) row_sees = tree_sees(a, t, tree_row(), t0 + 32 * c) >> (4 * half);
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
                     const int in = 32 * c + 8 * b + 4 * half;
@@ -1289,7 +1330,7 @@ __global__ __launch_bounds__(256, chunk_blocks(D, TIGHT)) void attn_chunk_kernel
                 }
                 if (__syncthreads_or(odd)) {
                     for (int in = 0; in < BN; ++in) {
-                        const bool sees = TREE ? tree_sees(a, t, token_of(), t0 + in) & 1u : (uint32_t)(t0 + in - lo) < seen;
+                        const bool sees = TREE ? tree_sees(a, t, tree_row(), t0 + in) & 1u : (uint32_t)(t0 + in - lo) < seen;
 #pragma unroll
                         for (int d = 0; d < DB; ++d)
 #pragma unroll
