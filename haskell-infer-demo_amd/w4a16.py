@@ -1066,21 +1066,19 @@ def beam_select(logits, scores, take, workspace=None, stream=None):
     need = _select_workspace(groups, beams, vocab)
     if not 1 <= take <= 128:
         _refuse(f"beam_select: take={take} is not 1 to 128")
-    # one allocation for the three
-    out = torch.empty((3, groups, take), dtype=torch.float32, device=device)
-    whole = out.view(torch.int32)
+    out = torch.empty((groups, take), dtype=torch.float32, device=device)
+    parents, tokens = torch.empty((2, groups, take), dtype=torch.int32, device=device).unbind(0)
     if workspace is None:
         workspace = torch.empty(need, dtype=torch.uint8, device=device)
         wp = workspace.data_ptr()
     else:
         wp = _dev(workspace, need, 1, "beam_select workspace", device)
     call = lib.w4a16_beam_select_f32 if logits.dtype == torch.float32 else lib.w4a16_beam_select_bf16
-    at, size = out.data_ptr(), groups * take * 4
-    st = call(logits.data_ptr(), logits.stride(0), logits.stride(1), sp, groups, beams, vocab, take, at, at + size, at + 2 * size, wp, need,
-              _raw_stream(None, index))
+    st = call(logits.data_ptr(), logits.stride(0), logits.stride(1), sp, groups, beams, vocab, take, out.data_ptr(), parents.data_ptr(),
+              tokens.data_ptr(), wp, need, _raw_stream(None, index))
     if st:
         _check(st, "beam_select")
-    return out[0], whole[1], whole[2]
+    return out, parents, tokens
 
 
 def beam_tables(page_table, kv_lens, parents, page_size, out=None, stream=None):
@@ -1205,9 +1203,8 @@ def verify_tree(target, node_tokens, parents, uniforms, sizes=None, workspace=No
     up = _exactly(uniforms, shape, torch.float32, device, "verify_tree uniforms")
     sp = None if sizes is None else _exactly(sizes, (seqs,), torch.int32, device, "verify_tree sizes")
     need = _tree_workspace(seqs, nodes, vocab)
-    # one allocation for the three
-    out = torch.empty(seqs * (2 * nodes + 1), dtype=torch.int32, device=device)
-    path, tokens, accepted = out[:seqs * nodes].view(shape), out[seqs * nodes:2 * seqs * nodes].view(shape), out[2 * seqs * nodes:]
+    accepted = torch.empty(seqs, dtype=torch.int32, device=device)
+    path, tokens = torch.empty((2, seqs, nodes), dtype=torch.int32, device=device).unbind(0)
     wp = None
     if need == 0:
         pass
@@ -1216,9 +1213,8 @@ def verify_tree(target, node_tokens, parents, uniforms, sizes=None, workspace=No
         wp = workspace.data_ptr()
     else:
         wp = _dev(workspace, need, 1, "verify_tree workspace", device)
-    at, size = out.data_ptr(), 4 * seqs * nodes
-    st = lib.w4a16_verify_tree_f32(tp, t_seq, t_row, ip, pp, sp, up, at + 2 * size, at, at + size, seqs, nodes, vocab, wp, need,
-                                   _raw_stream(None, index))
+    st = lib.w4a16_verify_tree_f32(tp, t_seq, t_row, ip, pp, sp, up, accepted.data_ptr(), path.data_ptr(), tokens.data_ptr(), seqs, nodes,
+                                   vocab, wp, need, _raw_stream(None, index))
     if st:
         _check(st, "verify_tree")
     return accepted, path, tokens
