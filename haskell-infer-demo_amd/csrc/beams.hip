@@ -15,6 +15,10 @@
  * and numbers unique, so the order is too. Where more are collected than there is room for, which takes rows of equal values, the
  * picks are made one after another instead.
  *
+ * The scan is bound by memory: 16 groups of 10 beams, 128257 words in FP32, 16.2 us (82 MB at 5.1 TB/s, a large copy's rate), 94 % of the VALU's
+ * cycles beside it. The pick is one block's chain of dependent steps: 8 of 4 beams' words 9.2 us, 40 of 10 beams' 16.4; four BF16 rows of 151936
+ * words are scanned in 4.3.
+ *
  * Exponentials are FP32 with the rounding of their arguments made good (2^-23), the sums of a load's four or eight too (2^-24 for each of two
  * or three additions), the sums of those FP64: 2^-21 in all.
  */
@@ -51,7 +55,7 @@ struct SelectArgs {
 template <bool BF16>
 __device__ __forceinline__ u4 load_raw(const void *row, int i, int n) {
     constexpr int kValues = values_a_load(BF16);
-    if (i + kValues <= n) return *reinterpret_cast<const u4_loose *>(static_cast<const uint8_t *>(row) + (long long)i * (BF16 ? 2 : 4));
+    if (i <= n - kValues) return *reinterpret_cast<const u4_loose *>(static_cast<const uint8_t *>(row) + (long long)i * (BF16 ? 2 : 4));
     constexpr uint32_t kLeast = BF16 ? 0xFF80FF80u : 0xFF800000u;
     u4 v = {kLeast, kLeast, kLeast, kLeast};
 #pragma unroll
@@ -424,7 +428,7 @@ int select(const char *what, bool bf16, const void *logits, long long group_stri
     a.beams = beams;
     a.vocab = vocab;
     a.take = take;
-    a.chunks = (vocab + chunk_values(bf16) - 1) / chunk_values(bf16);
+    a.chunks = (vocab - 1) / chunk_values(bf16) + 1;
     a.pieces = (a.chunks + kLoads - 1) / kLoads;
     const size_t rows = (size_t)groups * beams;
     a.sums = static_cast<double *>(ws);

@@ -278,3 +278,17 @@ def test_keep_path(cuda, dim, heads, page, fmt):
         for name in "kv":
             for a, b in zip(held(cache, name), expected[name]):
                 assert a is None or torch.equal(a.view(torch.uint8) if a.element_size() == 1 else a, b.view(torch.uint8) if b.element_size() == 1 else b)
+
+
+def test_the_longest_row(cuda):
+    """2^31 - 1 words: the last of a lane's eight is none. All of a value but a few, so that the sum is known."""
+    vocab = 2**31 - 1
+    logits = torch.full((1, 1, vocab), -1.0, dtype=torch.bfloat16, device=cuda)
+    some = {0: 24.0, vocab - 1: 26.0, vocab - 8: 25.0, 1 << 30: 23.0}
+    for at, x in some.items():
+        logits[0, 0, at] = x
+    got, parents, tokens = w4a16.beam_select(logits, torch.full((1, 1), 0.5, device=cuda), 4)
+    assert tokens.tolist() == [[vocab - 1, vocab - 8, 0, 1 << 30]] and parents.tolist() == [[0] * 4]
+    lse = np.log((vocab - 4) * np.exp(-1.0) + sum(np.exp(x) for x in some.values()))
+    want = 0.5 + np.array([26.0, 25.0, 24.0, 23.0]) - lse
+    assert (np.abs(got[0].cpu().numpy() - want) <= 2.0**-21 + np.abs(want) * 2.0**-23).all()
