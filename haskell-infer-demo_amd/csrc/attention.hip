@@ -446,7 +446,8 @@ constexpr int rows_blocks(int dim, int format, int rt) {
  *
  * Bound by memory: 32 sequences of 8192 tokens, one row of 32 heads each (16 of 256 values), the join included:
  * BF16 D = 64 102 us (5.2 TB/s), D = 128 192 (5.6), D = 256 200 (5.4); FP8 66 (4.4), 108 (5.1), 107 (5.1); INT8
- * 70, 110, 109.
+ * 70, 110, 109. Trees: two of which 5 rows grow over 100003 tokens, 24 heads over 4 of 256, INT8, 102 us (4.2 TB/s; VALU 50 %, one
+ * block a CU) and 7.2 for the join; one of 26 over 1500 tokens, 32 over 8 heads of 128, BF16, 12.9 and 4.0.
  */
 template <int D, int FMT, int RT, bool TREE>
 __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel(AttnArgs a) {
@@ -963,7 +964,9 @@ __device__ __forceinline__ uint32_t widen_f16(uint32_t codes) {
  * Every wave reads the whole tile, so the LDS reads of 32 rows take as long as their products; above
  * that it is bound by the weights' VALU work (five instructions each, and for 8-bit caches the widening
  * of a tile over 128 rows). 4096 rows over 16384 tokens, 32 heads (16 of 256 values): BF16 D = 64 671 us, 717
- * TFLOP/s; D = 128 979, 983; D = 256 1017, 946; INT8 859, 1193, 1308; FP8 748, 1134, 1269.
+ * TFLOP/s; D = 128 979, 983; D = 256 1017, 946; INT8 859, 1193, 1308; FP8 748, 1134, 1269. Trees: 16 of up to 60 over up to
+ * 8192 tokens, 32 heads over 8 of 128, FP8, 87.5 us, VALU 39 % and MFMA 22 % busy, 1.7 waves a SIMD: a tile's way through the registers to
+ * LDS is waited for; 8 of up to 251 over up to 16384, window 4096, 32 over 4 of 64, BF16, 90.6, VALU 58 %.
  */
 template <int D, int FMT, bool TIGHT, bool TREE>
 struct Chunk {
@@ -1226,95 +1229,95 @@ __global__ __launch_bounds__(256, chunk_blocks(D, TIGHT)) void attn_chunk_kernel
         const float *sc = scales + (step & 1) * 2 * BN;
         uint32_t p[kHalves][8];
         if (!idle) {
-        f16v s[kHalves];
-#pragma unroll
-        for (int c = 0; c < kHalves; ++c) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[c][i] = 0.0f;
-#pragma unroll
-            for (int j = 0; j < KS; ++j) {
-                const bf8 k = *reinterpret_cast<const bf8 *>(kt + (k_at ^ (32 * j)) + 32 * c * 2 * D);
-                const bf8 y = j < kHeld ? q[j < kHeld ? j : 0] : q_stored[(j - kHeld) * 2 * RM];
-                s[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, y, s[c], 0, 0, 0);
-            }
-        }
-        interleave<kHalves * KS, 1, kFar>();
-        /* scores over the maximum that the sums stand at: the exponents of the weights */
-        float base = m == -__builtin_inff() ? 0.0f : m;
-#pragma unroll
-        for (int c = 0; c < kHalves; ++c)
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                f4 x = {a.scale, a.scale, a.scale, a.scale};
-                if constexpr (kCoded) x = *reinterpret_cast<const f4 *>(sc + 32 * c + 8 * b + 4 * half);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) s[c][4 * b + i] = fmaf(s[c][4 * b + i], x[i], -base);
-            }
-        if (cut) {
-            const uint32_t at = t0 - lo;
+            f16v s[kHalves];
 #pragma unroll
             for (int c = 0; c < kHalves; ++c) {
-                uint32_t row_sees = 0;
-                if constexpr (TREE) row_sees = tree_sees(a, t, tree_row(), t0 + 32 * c) >> (4 * half);
 #pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    const int in = 32 * c + 8 * b + 4 * half;
-                    const int4 page = *reinterpret_cast<const int4 *>(pages + (step % 3) * BN + in);
-                    const int each[4] = {page.x, page.y, page.z, page.w};
+                for (int i = 0; i < 16; ++i) s[c][i] = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const bool hidden = TREE ? (each[i] < 0) | !(row_sees >> (8 * b + i) & 1u)
-                                                 : ((at + in + i) | (each[i] & 0x80000000u)) >= seen; /* a page of -1 as well */
-                        s[c][4 * b + i] = hidden ? -__builtin_inff() : s[c][4 * b + i];
-                    }
+                for (int j = 0; j < KS; ++j) {
+                    const bf8 k = *reinterpret_cast<const bf8 *>(kt + (k_at ^ (32 * j)) + 32 * c * 2 * D);
+                    const bf8 y = j < kHeld ? q[j < kHeld ? j : 0] : q_stored[(j - kHeld) * 2 * RM];
+                    s[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, y, s[c], 0, 0, 0);
                 }
             }
-        }
-        float most = s[0][0];
-#pragma unroll
-        for (int c = 0; c < kHalves; ++c)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) most = fmaxf(most, s[c][i]);
-        if (__any((most > 8.0f) | (m == -__builtin_inff()))) {
-            /* a new maximum: for rows that have none yet, or whose weights would pass 2^8 */
-            most = lane_max32(most);
-            const bool none = m == -__builtin_inff();
-            const float rise = most > (none ? -__builtin_inff() : 8.0f) ? most : 0.0f;
-            const float grow = none ? 0.0f : __builtin_amdgcn_exp2f(-rise);
-            m = none && rise == 0.0f && most != 0.0f ? m : base + rise;
-            l *= grow;
-#pragma unroll
-            for (int d = 0; d < DB; ++d) acc[d] *= grow;
+            interleave<kHalves * KS, 1, kFar>();
+            /* scores over the maximum that the sums stand at: the exponents of the weights */
+            float base = m == -__builtin_inff() ? 0.0f : m;
 #pragma unroll
             for (int c = 0; c < kHalves; ++c)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[c][i] -= rise;
-        }
-        if constexpr (kCoded) {
-            const int now = __builtin_amdgcn_readfirstlane(exponents[step & 1]) & 255;
-            if (now != v_exp) {
-                const float by = power_of_two(now - v_exp > 126 ? 1 : 127 - (now - v_exp));
+                for (int b = 0; b < 4; ++b) {
+                    f4 x = {a.scale, a.scale, a.scale, a.scale};
+                    if constexpr (kCoded) x = *reinterpret_cast<const f4 *>(sc + 32 * c + 8 * b + 4 * half);
 #pragma unroll
-                for (int d = 0; d < DB; ++d) acc[d] *= by;
-                v_exp = now;
-            }
-        }
-#pragma unroll
-        for (int c = 0; c < kHalves; ++c)
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                float w[4];
-                f4 x = {1.0f, 1.0f, 1.0f, 1.0f};
-                if constexpr (kCoded) x = *reinterpret_cast<const f4 *>(sc + BN + 32 * c + 8 * b + 4 * half);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    w[i] = __builtin_amdgcn_exp2f(s[c][4 * b + i]);
-                    l += w[i];
-                    if constexpr (kCoded) w[i] *= x[i];
+                    for (int i = 0; i < 4; ++i) s[c][4 * b + i] = fmaf(s[c][4 * b + i], x[i], -base);
                 }
-                p[c][2 * b] = kCoded ? pack_f16(w[0], w[1]) : kv_pack_bf16(w[0], w[1]);
-                p[c][2 * b + 1] = kCoded ? pack_f16(w[2], w[3]) : kv_pack_bf16(w[2], w[3]);
+            if (cut) {
+                const uint32_t at = t0 - lo;
+#pragma unroll
+                for (int c = 0; c < kHalves; ++c) {
+                    uint32_t row_sees = 0;
+                    if constexpr (TREE) row_sees = tree_sees(a, t, tree_row(), t0 + 32 * c) >> (4 * half);
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) {
+                        const int in = 32 * c + 8 * b + 4 * half;
+                        const int4 page = *reinterpret_cast<const int4 *>(pages + (step % 3) * BN + in);
+                        const int each[4] = {page.x, page.y, page.z, page.w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const bool hidden = TREE ? (each[i] < 0) | !(row_sees >> (8 * b + i) & 1u)
+                                                     : ((at + in + i) | (each[i] & 0x80000000u)) >= seen; /* a page of -1 as well */
+                            s[c][4 * b + i] = hidden ? -__builtin_inff() : s[c][4 * b + i];
+                        }
+                    }
+                }
             }
+            float most = s[0][0];
+#pragma unroll
+            for (int c = 0; c < kHalves; ++c)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) most = fmaxf(most, s[c][i]);
+            if (__any((most > 8.0f) | (m == -__builtin_inff()))) {
+                /* a new maximum: for rows that have none yet, or whose weights would pass 2^8 */
+                most = lane_max32(most);
+                const bool none = m == -__builtin_inff();
+                const float rise = most > (none ? -__builtin_inff() : 8.0f) ? most : 0.0f;
+                const float grow = none ? 0.0f : __builtin_amdgcn_exp2f(-rise);
+                m = none && rise == 0.0f && most != 0.0f ? m : base + rise;
+                l *= grow;
+#pragma unroll
+                for (int d = 0; d < DB; ++d) acc[d] *= grow;
+#pragma unroll
+                for (int c = 0; c < kHalves; ++c)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[c][i] -= rise;
+            }
+            if constexpr (kCoded) {
+                const int now = __builtin_amdgcn_readfirstlane(exponents[step & 1]) & 255;
+                if (now != v_exp) {
+                    const float by = power_of_two(now - v_exp > 126 ? 1 : 127 - (now - v_exp));
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) acc[d] *= by;
+                    v_exp = now;
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < kHalves; ++c)
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    float w[4];
+                    f4 x = {1.0f, 1.0f, 1.0f, 1.0f};
+                    if constexpr (kCoded) x = *reinterpret_cast<const f4 *>(sc + BN + 32 * c + 8 * b + 4 * half);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        w[i] = __builtin_amdgcn_exp2f(s[c][4 * b + i]);
+                        l += w[i];
+                        if constexpr (kCoded) w[i] *= x[i];
+                    }
+                    p[c][2 * b] = kCoded ? pack_f16(w[0], w[1]) : kv_pack_bf16(w[0], w[1]);
+                    p[c][2 * b + 1] = kCoded ? pack_f16(w[2], w[3]) : kv_pack_bf16(w[2], w[3]);
+                }
         }
         if constexpr (!kCoded) {
             /* Tokens that are not there weigh nothing, and what memory holds for them is taken
@@ -1358,27 +1361,27 @@ __global__ __launch_bounds__(256, chunk_blocks(D, TIGHT)) void attn_chunk_kernel
         /* O^T: 16 tokens and 32 values a product */
         if (!idle) {
 #pragma unroll
-        for (int u = 0; u < BN / 16; ++u) {
-            const uint32_t *w = &p[u / 2][4 * (u % 2)];
+            for (int u = 0; u < BN / 16; ++u) {
+                const uint32_t *w = &p[u / 2][4 * (u % 2)];
 #pragma unroll
-            for (int d = 0; d < DB; ++d) {
-                uint32_t v[4];
+                for (int d = 0; d < DB; ++d) {
+                    uint32_t v[4];
 #pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                    const uint2 got = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (__attribute__((address_space(3))) s4 *)(vt + (v_at ^ (64 * d)) + (16 * u + 8 * y) * 2 * D)));
-                    v[2 * y] = got.x;
-                    v[2 * y + 1] = got.y;
-                }
-                if constexpr (kCoded) {
-                    acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, make_uint4(v[0], v[1], v[2], v[3])),
-                                                                    __builtin_bit_cast(h8, make_uint4(w[0], w[1], w[2], w[3])), acc[d], 0, 0, 0);
-                } else {
-                    acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf8(v[0], v[1], v[2], v[3]), as_bf8(w[0], w[1], w[2], w[3]), acc[d], 0, 0, 0);
+                    for (int y = 0; y < 2; ++y) {
+                        const uint2 got = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (__attribute__((address_space(3))) s4 *)(vt + (v_at ^ (64 * d)) + (16 * u + 8 * y) * 2 * D)));
+                        v[2 * y] = got.x;
+                        v[2 * y + 1] = got.y;
+                    }
+                    if constexpr (kCoded) {
+                        acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, make_uint4(v[0], v[1], v[2], v[3])),
+                                                                        __builtin_bit_cast(h8, make_uint4(w[0], w[1], w[2], w[3])), acc[d], 0, 0, 0);
+                    } else {
+                        acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf8(v[0], v[1], v[2], v[3]), as_bf8(w[0], w[1], w[2], w[3]), acc[d], 0, 0, 0);
+                    }
                 }
             }
-        }
-        interleave<BN / 16 * DB, 2, kFar>();
+            interleave<BN / 16 * DB, 2, kFar>();
         }
         if (more) store_tile(step + 1);
         if (look && tid < 64) put_page(step + 2, entry);

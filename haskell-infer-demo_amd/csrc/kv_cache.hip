@@ -167,6 +167,9 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvView kv, uint16_t *k, ui
  *
  * Work beyond the row's place comes in steps of 64 lanes (1 KiB): heads of K, of V, of q, in this order, kAhead of them on
  * their way at a time.
+ *
+ * Bound by memory: 8198 rows of 32 queries and 8 keys of 128, BF16, 41 us, 203 MB at 4.9 TB/s (a large copy's rate). 592 rows
+ * of 24 + 4 heads of 256, INT8, 6.1 us; four rows 3.8, a launch and four dependent round trips.
  */
 struct AppendArgs {
     const uint16_t *k, *v, *q;
@@ -298,7 +301,8 @@ template <int D>
 void launch_append(int format, const KvView &kv, const AppendArgs &a, hipStream_t s) {
     constexpr int kHeads = 512 / D;
     const int steps = 2 * ((kv.heads + kHeads - 1) / kHeads) + (a.q_heads + kHeads - 1) / kHeads;
-    /* every step a wave of its own where there are few rows; a wave's angles serve all of its steps */
+    /* Every step a wave of its own where there are few rows; where there are many, a wave's angles serve all of its steps. 32 + 8 + 8 heads of
+     * 128, BF16, one wave a row, four, a step each (12): 4 rows 7.5, 3.8, 3.1 us; 2048 rows 12.0, 10.0, 13.9; 8192 rows 33.4, 33.2, 43.5. */
     const int blocks = (kv.rows + 3) / 4, most = (8 * device_cus() + blocks - 1) / blocks;
     const dim3 grid(blocks, steps < most ? steps : most), block(256);
     auto kernel = format == W4A16_KV_BF16   ? kv_append_kernel<D, W4A16_KV_BF16>
