@@ -12,6 +12,9 @@ This module mirrors the reference's operator interface for the path:
 * ``KvCache``, ``KvBatch``, ``paged_attention``, ``verify_drafts`` - a paged KV cache, attention over
   it and the verification of drafted tokens, around the FFN in a decode or verify step (no
   counterpart in the reference's C interface).
+* ``Rope``, ``KvCache.append``; ``KvTree``, ``paged_attention(tree=)``, ``verify_tree``, ``KvCache.keep_path``;
+  ``beam_select``, ``beam_tables``, ``KvCache.copy_tails`` - keys turned as they are written, trees of drafted tokens, and beam
+  search (no counterpart either).
 
 Device tensors are torch CUDA tensors (on ROCm, HIP memory); torch is used only for device memory
 and streams. There is no CPU fallback: if the library is missing the import fails.
