@@ -19,8 +19,9 @@
  * cycles beside it. The pick is one block's chain of dependent steps: 8 of 4 beams' words 9.2 us, 40 of 10 beams' 16.4; four BF16 rows of 151936
  * words are scanned in 4.3.
  *
- * Exponentials are FP32 with the rounding of their arguments made good (2^-23), the sums of a load's four or eight too (2^-24 for each of two
- * or three additions), the sums of those FP64: 2^-21 in all.
+ * Exponentials are FP32 (1.5 * 2^-23 with their product's rounding made good; of FP32 logits' difference from their piece's largest another 2^-22
+ * at most, over those of a piece that count), the sums of a load's four or eight too (2^-24 for each of two or three additions), the sums of
+ * those FP64: 2^-20 in all.
  */
 #include "launch.h"
 #include "wave.h"

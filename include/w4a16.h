@@ -483,7 +483,7 @@ int w4a16_kv_keep_path(const W4A16KvCache *cache, const W4A16KvBatch *batch, con
 
 /* Beam search. The `take` best continuations of each of `groups` groups of `beams` beams: of all (b, v) the largest
  *   scores[b] + logits[b][v] - log(sum over w of exp(logits[b][w])),
- * the best first, and of equal ones those of the lowest b * vocab + v. The sum of exponentials is exact to 2^-21, everything behind it FP64;
+ * the best first, and of equal ones those of the lowest b * vocab + v. The sum of exponentials is exact to 2^-20, everything behind it FP64;
  * scores are rounded to FP32 at the end. Logits of -infinity are no candidates, nor is any of a beam
  * whose score is not finite (a beam that is not to go on: -infinity) or that has an infinite or NaN logit: where there are fewer than
  * `take`, the rest have a score of -infinity and -1 for parent and token. logits [groups][beams][vocab], rows on any
