@@ -1114,6 +1114,12 @@ def beam_tables(page_table, kv_lens, parents, page_size, out=None, stream=None):
 def _floats3(t, what, device):
     import torch
 
+    try:
+        seq, row, one = t.stride()
+        if one == 1 and t.dtype == torch.float32 and t.device == device and t.is_cuda:
+            return t.data_ptr(), seq, row
+    except (AttributeError, TypeError, ValueError):
+        pass  # named below
     if not hasattr(t, "is_cuda") or not t.is_cuda or t.device != device:
         _refuse(f"{what}: expected a tensor on {device}")
     if t.dtype != torch.float32 or t.dim() != 3 or (t.shape[-1] > 1 and t.stride(-1) != 1):
@@ -1207,7 +1213,7 @@ def verify_tree(target, node_tokens, parents, uniforms, sizes=None, workspace=No
     sp = None if sizes is None else _exactly(sizes, (seqs,), torch.int32, device, "verify_tree sizes")
     need = _tree_workspace(seqs, nodes, vocab)
     accepted = torch.empty(seqs, dtype=torch.int32, device=device)
-    path, tokens = torch.empty((2, seqs, nodes), dtype=torch.int32, device=device).unbind(0)
+    path, tokens = torch.empty_like(parents), torch.empty_like(node_tokens)
     wp = None
     if need == 0:
         pass
