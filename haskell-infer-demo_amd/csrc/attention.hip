@@ -1615,6 +1615,14 @@ Plan plan_of(const W4A16KvCache *c, const W4A16KvBatch *b, int q_heads, bool tre
 template <int D, int RM, bool EVEN, bool TREE>
 void launch_join(int parts, const AttnArgs &a, hipStream_t s) {
     const unsigned x = a.kv.heads * a.items;
+    if constexpr (TREE && RM == kChunkRows) {
+        /* Side by side only where there are fewer blocks than CUs else, however many parts there are. FP8, 128 values, 60 nodes, one part after
+         * another and four at a time: 16 sequences of 2048 tokens 63 and 77 us, four of 8192 62 and 63, one of 100000 166 and 154 (16
+         * at a time 144, 77, 153). */
+        if (x * (RM / 16) < (unsigned)device_cus()) launch_k(attn_join_kernel<D, RM, 4, EVEN, TREE>, dim3(x, RM / 4), dim3(256), 0, s, a);
+        else launch_k(attn_join_kernel<D, RM, 1, EVEN, TREE>, dim3(x, RM / 16), dim3(256), 0, s, a);
+        return;
+    }
     if (parts > 16) launch_k(attn_join_kernel<D, RM, 16, EVEN, TREE>, dim3(x, RM), dim3(256), 0, s, a);
     else if (parts > 4) launch_k(attn_join_kernel<D, RM, 4, EVEN, TREE>, dim3(x, RM / 4), dim3(256), 0, s, a);
     else if (parts > 1) launch_k(attn_join_kernel<D, RM, 1, EVEN, TREE>, dim3(x, RM / 16), dim3(256), 0, s, a);
