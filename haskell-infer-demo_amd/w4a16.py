@@ -810,8 +810,8 @@ class KvCache:
             shape = (rows, q_heads, dim)
             qp, q_row, q_head = _rows3(q, shape, self.device, "KvCache.append q")
             if out is None:
-                make = torch.zeros if batch.padded else torch.empty
-                out = make(shape, dtype=q.dtype, device=self.device)
+                make = torch.zeros_like if batch.padded else torch.empty_like
+                out = make(q, memory_format=torch.contiguous_format)
                 op, o_row, o_head = out.data_ptr(), q_heads * dim, dim
             else:
                 op, o_row, o_head = _rows3(out, shape, self.device, "KvCache.append out")
