@@ -1035,6 +1035,16 @@ def _tables(page_table, kv_lens, third, device, what):
     pages."""
     import torch
 
+    kind = torch.int32
+    try:
+        seqs, pages = page_table.shape
+        stride, one = page_table.stride()
+        if (one == 1 and page_table.dtype == kind and page_table.device == device and kv_lens.shape == (seqs,) and kv_lens.dtype == kind and
+                kv_lens.device == device and kv_lens.is_contiguous() and third.numel() == seqs and 1 <= third.dim() <= 2 and third.dtype == kind and
+                third.device == device and third.is_contiguous()):
+            return page_table.data_ptr(), stride if seqs > 1 else pages, pages, kv_lens.data_ptr(), third.data_ptr()
+    except (AttributeError, TypeError, ValueError):
+        pass  # named below
     if not hasattr(page_table, "is_cuda") or page_table.device != device or page_table.dtype != torch.int32 or page_table.dim() != 2 or \
             (page_table.shape[1] > 1 and page_table.stride(1) != 1):
         _refuse(f"{what}: the table is no int32 tensor [seqs, pages] on {device} with a dense last axis")
@@ -1100,10 +1110,10 @@ def beam_tables(page_table, kv_lens, parents, page_size, out=None, stream=None):
     tp, stride, pages, lp, pp = _tables(page_table, kv_lens, parents, device, "beam_tables")
     groups, beams = parents.shape
     if out is None:
-        out = torch.empty((groups * beams, pages), dtype=torch.int32, device=device)
+        out = torch.empty_like(page_table, memory_format=torch.contiguous_format)
     elif out.shape != page_table.shape or out.dtype != torch.int32 or out.device != device or (pages > 1 and out.stride(1) != 1):
         _refuse(f"beam_tables: out is no int32 tensor {tuple(page_table.shape)} on {device} with a dense last axis")
-    source = torch.empty(groups * beams, dtype=torch.int32, device=device)
+    source = torch.empty_like(kv_lens)
     st = lib.w4a16_beam_tables(tp, stride, pages, lp, pp, groups, beams, page_size, out.data_ptr(),
                                out.stride(0) if groups * beams > 1 else pages, source.data_ptr(), _raw_stream(None, index))
     if st:
