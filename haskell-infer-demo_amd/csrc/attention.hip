@@ -210,7 +210,8 @@ __device__ __forceinline__ bool find_tile(const AttnArgs &a, int item, int split
  * all (tile, head) pairs and a.splits blocks wanted, every pair is cut into parts of
  * ceil(N / a.splits) units, so that long sequences have many parts and none is much longer
  * than another. The parts are counted through the sequences; a part is a block's, and its place in
- * the workspace.
+ * the workspace. With trees only the parts of pairs that are cut have places: ceil(u / each) of a pair of u > each units are fewer than
+ * 2 u / each, so all of them fewer than 2 N / each <= 2 a.splits, however many pairs there are, and such pairs fewer than a.splits.
  */
 struct Seqs { /* 64 sequences, one a lane */
     int first, news, old, from; /* old: position of its first row; from: where the first key that any of its rows sees is cut */
@@ -280,17 +281,19 @@ __device__ __forceinline__ int part_units(const AttnArgs &a, Seqs *q, bool *equa
     return each < 1 ? 1 : each > kMostUnits ? kMostUnits : (int)each;
 }
 
-/* The part of this block (PAIR false) or the (tile, head) pair of number `index` (true): the tile, its head, its number of
- * parts, and the number of its first one. */
+/* The part of this block (PAIR false) or the (tile, head) pair of number `index` (true; with trees, among those that are cut): the
+ * tile, its head, its number of parts, and the number of its first one. TREE: *place is the part's (PAIR: its first part's) in the workspace, -1
+ * where it has none. */
 template <int RM, bool PAIR, bool TREE>
-__device__ __forceinline__ bool find_part(const AttnArgs &a, int index, Tile *t, int *head, int *first_part) {
+__device__ __forceinline__ bool find_part(const AttnArgs &a, int index, Tile *t, int *head, int *first_part, int *place) {
     Seqs q;
     bool equal; /* TREE: a pair's parts are alike */
     const int each = part_units<RM, TREE>(a, &q, &equal);
-    int left = index, before = 0; /* parts of the sequences before */
+    int left = index, before = 0, places = 0; /* parts of the sequences before, and those that have places */
     for (int base = 0;;) {
         const int per = (q.units + each - 1) / each, parts = q.pairs * per;
-        const int upto_parts = wave_upto(parts), upto = PAIR ? wave_upto(q.pairs) : upto_parts;
+        const int pairs = TREE && per < 2 ? 0 : q.pairs, stored = pairs * per; /* TREE: that are cut */
+        const int upto_parts = wave_upto(parts), upto = PAIR ? wave_upto(pairs) : upto_parts, upto_stored = TREE ? wave_upto(stored) : 0;
         const unsigned long long here = __ballot(upto > left);
         if (here) {
             const int l = __ffsll((long long)here) - 1;
@@ -301,9 +304,11 @@ __device__ __forceinline__ bool find_part(const AttnArgs &a, int index, Tile *t,
             if constexpr (TREE) t->nodes = __builtin_amdgcn_readlane(q.nodes, l);
             const int from = __builtin_amdgcn_readlane(q.from, l);
             t->active = __builtin_amdgcn_readlane(per, l);
-            const int in_seq = left - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(PAIR ? q.pairs : parts, l));
+            const int in_seq = left - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(PAIR ? pairs : parts, l));
             const int pair = PAIR ? in_seq : in_seq / t->active, part = PAIR ? 0 : in_seq - pair * t->active;
             *first_part = before + __builtin_amdgcn_readlane(upto_parts, l) - __builtin_amdgcn_readlane(parts, l) + pair * t->active;
+            if constexpr (TREE)
+                *place = t->active < 2 ? -1 : places + __builtin_amdgcn_readlane(upto_stored, l) - __builtin_amdgcn_readlane(stored, l) + pair * t->active + part;
             *head = pair % a.kv.heads;
             t->start = pair / a.kv.heads * RM;
             fill_tile<RM, TREE>(a, t);
@@ -316,6 +321,7 @@ __device__ __forceinline__ bool find_part(const AttnArgs &a, int index, Tile *t,
         }
         left -= __builtin_amdgcn_readlane(upto, 63);
         before += __builtin_amdgcn_readlane(upto_parts, 63);
+        if constexpr (TREE) places += __builtin_amdgcn_readlane(upto_stored, 63);
         base += 64;
         if (base >= a.kv.seqs) return false;
         q = load_seqs<RM, TREE>(a, base);
@@ -457,8 +463,8 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
     const int mask = (1 << a.kv.shift) - 1;
     Tile t;
-    int head, first_part;
-    if (!find_part<RM, false, TREE>(a, blockIdx.x, &t, &head, &first_part)) return;
+    int head, first_part, place_of_part;
+    if (!find_part<RM, false, TREE>(a, blockIdx.x, &t, &head, &first_part, &place_of_part)) return;
 
     const int32_t *table = a.kv.table + (long long)t.seq * a.kv.table_stride;
     /* Pages of this lane's K tokens and V tokens (page sizes are multiples of 8, so four
@@ -867,7 +873,7 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
     constexpr int kPart = D < 128 ? D : 128, kPad = kPart + 4, kPer = kPart / 16;
     __shared__ float o_all[4][16][kPad];
     __shared__ float m_all[4][16], l_all[4][16];
-    float *partial = t.active > 1 ? partial_at<D, RM>(a, blockIdx.x) : nullptr;
+    float *partial = (TREE ? place_of_part >= 0 : t.active > 1) ? partial_at<D, RM>(a, TREE ? place_of_part : blockIdx.x) : nullptr;
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
         const float sum = lane_sum32(lane_sum16(l[r]));
@@ -1033,10 +1039,11 @@ __global__ __launch_bounds__(256, chunk_blocks(D, TIGHT)) void attn_chunk_kernel
     int *exponents = bad + 3;                                      /* [step % 2]: V's scales are over 2 to this, biased; + 256: one is not finite */
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 31, half = lane >> 5;
     /* the last tiles of a sequence see the most keys: those first */
-    int head = blockIdx.x % a.kv.heads, split = blockIdx.y, item = a.items - 1 - (int)(blockIdx.x / a.kv.heads), first_part;
+    int head = blockIdx.x % a.kv.heads, split = blockIdx.y, item = a.items - 1 - (int)(blockIdx.x / a.kv.heads);
+    int first_part, place_of_part;
     Tile t;
     if constexpr (TREE) {
-        if (!find_part<RM, false, TREE>(a, blockIdx.x, &t, &head, &first_part)) return;
+        if (!find_part<RM, false, TREE>(a, blockIdx.x, &t, &head, &first_part, &place_of_part)) return;
     } else {
         if (!find_tile<RM>(a, item, split, &t)) return;
         if (split >= t.active) return;
@@ -1398,7 +1405,8 @@ __global__ __launch_bounds__(256, chunk_blocks(D, TIGHT)) void attn_chunk_kernel
     }
     if (!real) return;
     float by = !kCoded ? 1.0f : spoiled ? __builtin_nanf("") : times_power(v_exp);
-    float *partial = t.active > 1 ? partial_at<D, RM>(a, TREE ? blockIdx.x : ((long long)item * a.kv.heads + head) * a.splits + split) : nullptr;
+    float *partial = (TREE ? place_of_part >= 0 : t.active > 1)
+                         ? partial_at<D, RM>(a, TREE ? place_of_part : ((long long)item * a.kv.heads + head) * a.splits + split) : nullptr;
     if (partial) {
 #pragma unroll
         for (int d = 0; d < DB; ++d)
@@ -1433,10 +1441,11 @@ template <int D, int RM, int SUB, bool EVEN, bool TREE>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     constexpr int kPer = D / 16, kRows = 16 / SUB;
     Tile t;
-    int head, first_part = 0;
+    int head, first_part = 0, first_place = 0;
     if constexpr (EVEN) {
-        if (!find_part<RM, true, TREE>(a, blockIdx.x, &t, &head, &first_part)) return;
+        if (!find_part<RM, true, TREE>(a, blockIdx.x, &t, &head, &first_part, &first_place)) return;
         if (first_part + t.active > a.blocks) return; /* sequences that overlap: not all parts were worked on */
+        if constexpr (!TREE) first_place = first_part;
     } else {
         head = blockIdx.x % a.kv.heads;
         if (!find_tile<RM>(a, blockIdx.x / a.kv.heads, 0, &t)) return;
@@ -1444,7 +1453,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     if (t.active < 2 || (int)blockIdx.y * kRows >= t.rows) return;
     const int lane = threadIdx.x & 15, unit = threadIdx.x >> 4, sub = unit / kRows, i = blockIdx.y * kRows + unit % kRows;
     const int row = i < t.rows ? i : t.rows - 1;
-    auto part_of = [&](int s) { return partial_at<D, RM>(a, (EVEN ? first_part : (long long)blockIdx.x * a.splits) + s); };
+    auto part_of = [&](int s) { return partial_at<D, RM>(a, (EVEN ? first_place : (long long)blockIdx.x * a.splits) + s); };
     /* Of many parts the first ones' values are on their way beside the maxima: 64 parts of 256 values 8.6
      * and 7.4 us; of few that costs more than it gives. */
     constexpr int kFirst = SUB == 16 ? 2 : 0;
@@ -1529,6 +1538,9 @@ struct Plan {
 
 constexpr int kChunkRows = 128;
 
+/* Places that parts of a call with trees may need: of those that are cut (find_part), and no more than there are blocks. */
+long long tree_places(const Part &p) { return 2LL * p.splits < p.blocks ? 2LL * p.splits : p.blocks; }
+
 Plan plan_of(const W4A16KvCache *c, const W4A16KvBatch *b, int q_heads, bool tree) {
     Plan p = {};
     const int group = q_heads / c->kv_heads, dim = c->head_dim;
@@ -1573,9 +1585,9 @@ Plan plan_of(const W4A16KvCache *c, const W4A16KvBatch *b, int q_heads, bool tre
          * 8 key heads of 128, BF16, cut and whole, in a graph: 512 tokens 10.5 and 9.2 us, 768 10.6 and 11.6;
          * sixteen sequences: 768 16.9 and 14.9, 1024 18.6 and 18.1, 1536 22.9 and 24.8. */
         if (tokens <= (pairs >= device_cus() / 2 ? 1024 : 512)) p.few.splits = 0;
-        if (pairs > 65536) p.few.splits = 0; /* places for their parts would take gigabytes */
+        if (!tree && pairs > 65536) p.few.splits = 0; /* places for their parts would take gigabytes */
         p.few.blocks = p.few.splits + pairs;
-        if (p.few.splits) p.ws_bytes = (size_t)p.few.blocks * rm * (dim + 2) * 4;
+        if (p.few.splits) p.ws_bytes = (size_t)(tree ? tree_places(p.few) : p.few.blocks) * rm * (dim + 2) * 4;
     }
     if (p.many.items && tree) {
         /* A tree's rows see all of what stands before them, and sequences are as long as they are: parts of equal size, one round
@@ -1583,11 +1595,10 @@ Plan plan_of(const W4A16KvCache *c, const W4A16KvBatch *b, int q_heads, bool tre
         const long long blocks = (long long)chunk_blocks(dim, dim == 256) * device_cus();
         const long long pairs = (long long)p.many.items * c->kv_heads, units = pairs * ((tokens + kUnit - 1) / kUnit);
         p.many.splits = (int)(units < 1 ? 1 : units < blocks ? units : blocks);
-        if (pairs > 65536) p.many.splits = 0;
         p.many.least = 2;
         p.many.blocks = p.many.splits + pairs;
         p.many.ws_at = p.ws_bytes;
-        if (p.many.splits) p.ws_bytes += (size_t)p.many.blocks * kChunkRows * (dim + 2) * 4;
+        p.ws_bytes += (size_t)tree_places(p.many) * kChunkRows * (dim + 2) * 4;
     } else if (p.many.items) {
         /* Two blocks a CU, by the tiles there are if max_new holds (`items` can be up to twice as many);
          * one, or parts of `least` tokens, where two would make those shorter, since a part's results
@@ -1614,7 +1625,8 @@ Plan plan_of(const W4A16KvCache *c, const W4A16KvBatch *b, int q_heads, bool tre
 
 template <int D, int RM, bool EVEN, bool TREE>
 void launch_join(int parts, const AttnArgs &a, hipStream_t s) {
-    const unsigned x = a.kv.heads * a.items;
+    unsigned x = a.kv.heads * a.items;
+    if (TREE && x > (unsigned)a.splits) x = a.splits; /* pairs that are cut */
     if constexpr (TREE && RM == kChunkRows) {
         /* Side by side only where there are fewer blocks than CUs else, however many parts there are. FP8, 128 values, 60 nodes, one part after
          * another and four at a time: 16 sequences of 2048 tokens 63 and 77 us, four of 8192 62 and 63, one of 100000 166 and 154 (16
@@ -1656,7 +1668,7 @@ void launch_format(const Plan &p, const AttnArgs &all, hipStream_t s) {
             }
         if constexpr (TREE) {
             launch_k(kernel, dim3((unsigned)p.many.blocks), dim3(256), lds, s, a);
-            if (a.splits) launch_join<D, kChunkRows, true, TREE>(parts_of(a), a, s);
+            launch_join<D, kChunkRows, true, TREE>(parts_of(a), a, s);
         } else {
             launch_k(kernel, dim3(a.kv.heads * a.items, a.splits), dim3(256), lds, s, a);
             launch_join<D, kChunkRows, false, TREE>(a.splits, a, s);
