@@ -69,9 +69,10 @@ struct Tile {
     int base, nodes;        /* TREE: the tree's first token, and how many it has */
 };
 
-/* The end of the keys that a row at `place` sees. */
+/* The end of the keys that a row at `place` sees; with trees, none behind its own place. */
+template <bool TREE>
 __device__ __forceinline__ int row_end(const AttnArgs &a, const Tile &t, int place) {
-    const int end = a.causal ? place + 1 : t.length;
+    const int end = TREE || a.causal ? place + 1 : t.length;
     return end < t.length ? end : t.length;
 }
 
@@ -90,8 +91,8 @@ __device__ __forceinline__ void fill_tile(const AttnArgs &a, Tile *t) {
     /* the same on every lane, and kept as such: in lanes it costs the few-row kernels registers that they do not have */
     t->length = __builtin_amdgcn_readfirstlane(kv_held(a.kv, t->old + t->news));
     t->window = a.window <= t->old + t->news ? a.window : 0;
-    t->hi = row_end(a, *t, t->old + t1);
-    t->all_hi = row_end(a, *t, t->old + t0);
+    t->hi = row_end<TREE>(a, *t, t->old + t1);
+    t->all_hi = row_end<TREE>(a, *t, t->old + t0);
     int least = t->old + t0; /* position of any of the tile's rows */
     if constexpr (TREE) {
         t->base = t->old + t->news - t->nodes;
@@ -143,7 +144,7 @@ struct TreeLoad {
 __device__ __forceinline__ uint32_t tree_sees(const AttnArgs &a, const Tile &t, const uint32_t *row, int at) {
     const int token = (int)row[kTreeToken], place = t.old + token;
     /* [from, to) of the 32 */
-    const int to = token < 0 ? 0 : row_end(a, t, place) - at;
+    const int to = token < 0 ? 0 : row_end<true>(a, t, place) - at;
     int from = 0;
     if (t.window) {
         /* a node's position lies between its tree's first token and its place */
@@ -317,6 +318,12 @@ __device__ __forceinline__ bool find_part(const AttnArgs &a, int index, Tile *t,
                 if (equal) size = (__builtin_amdgcn_readlane(q.units, l) + t->active - 1) / t->active;
             t->begin = from + part * size * kUnit;
             t->end = part + 1 < t->active && t->begin + size * kUnit < t->hi ? t->begin + size * kUnit : t->hi;
+            if constexpr (TREE) {
+                /* Rows before the tree: a tile's window may begin far behind its sequence's. By whole steps (of 64 tokens at most), which end with
+                 * the part, and what is left of it may be nothing. 4096 rows over 8192 tokens, window 256, 32 heads over 8 of 128, BF16:
+                 * 60 us, and 491 from the part's own begin. */
+                if (t->begin < t->lo) t->begin += (t->lo - t->begin) & ~63;
+            }
             return true;
         }
         left -= __builtin_amdgcn_readlane(upto, 63);
@@ -567,7 +574,7 @@ __global__ __launch_bounds__(256, rows_blocks(D, FMT, RT)) void attn_rows_kernel
         const bool real = i < t.rows;
         const int place = t.old + token;
         const uint16_t *row = a.q + (t.first_row + (real ? token : 0)) * a.q_row + h * a.q_head;
-        hi[r] = !real ? 0 : row_end(a, t, place);
+        hi[r] = !real ? 0 : row_end<TREE>(a, t, place);
         lo[r] = t.window ? place - t.window + 1 : 0;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
@@ -1168,7 +1175,7 @@ __global__ __launch_bounds__(256, chunk_blocks(D, TIGHT)) void attn_chunk_kernel
     bool real = i_row < t.rows;
     const int place = t.old + token;
     /* TREE: unused, tree_sees instead */
-    const int hi = !real ? 0 : row_end(a, t, place), lo = t.window ? place - t.window + 1 : 0;
+    const int hi = !real ? 0 : row_end<TREE>(a, t, place), lo = t.window ? place - t.window + 1 : 0;
     const uint32_t seen = hi > lo ? hi - lo : 0; /* this row sees a key where its place less lo, unsigned, is below this */
     uint32_t *const tree_rows = reinterpret_cast<uint32_t *>(smem + C::kTree); /* TREE; read by the waves that wrote them */
     auto row_of = [&] {
