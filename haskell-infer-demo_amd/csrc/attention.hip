@@ -1640,11 +1640,11 @@ void launch_join(int parts, const AttnArgs &a, hipStream_t s) {
          * at a time 144, 77, 153). */
         if (x * (RM / 16) < (unsigned)device_cus()) launch_k(attn_join_kernel<D, RM, 4, EVEN, TREE>, dim3(x, RM / 4), dim3(256), 0, s, a);
         else launch_k(attn_join_kernel<D, RM, 1, EVEN, TREE>, dim3(x, RM / 16), dim3(256), 0, s, a);
-        return;
+    } else {
+        if (parts > 16) launch_k(attn_join_kernel<D, RM, 16, EVEN, TREE>, dim3(x, RM), dim3(256), 0, s, a);
+        else if (parts > 4) launch_k(attn_join_kernel<D, RM, 4, EVEN, TREE>, dim3(x, RM / 4), dim3(256), 0, s, a);
+        else if (parts > 1) launch_k(attn_join_kernel<D, RM, 1, EVEN, TREE>, dim3(x, RM / 16), dim3(256), 0, s, a);
     }
-    if (parts > 16) launch_k(attn_join_kernel<D, RM, 16, EVEN, TREE>, dim3(x, RM), dim3(256), 0, s, a);
-    else if (parts > 4) launch_k(attn_join_kernel<D, RM, 4, EVEN, TREE>, dim3(x, RM / 4), dim3(256), 0, s, a);
-    else if (parts > 1) launch_k(attn_join_kernel<D, RM, 1, EVEN, TREE>, dim3(x, RM / 16), dim3(256), 0, s, a);
 }
 
 /* Parts of a (tile, head), about. */
