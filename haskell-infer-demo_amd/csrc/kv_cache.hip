@@ -241,8 +241,8 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvView kv, AppendArgs a)
                 f[2 * i] = __builtin_bit_cast(float, w[i] << 16);
                 f[2 * i + 1] = __builtin_bit_cast(float, w[i] & 0xFFFF0000u);
             }
-            if (!is_v) {
-                float y[8];
+            float y[8];
+            auto turn = [&] {
                 if (a.interleaved) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
@@ -256,6 +256,9 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvView kv, AppendArgs a)
                         y[4 + i] = f[4 + i] * c[i] + f[i] * s[i];
                     }
                 }
+            };
+            if (FMT != W4A16_KV_BF16 && !is_v) {
+                turn();
 #pragma unroll
                 for (int i = 0; i < 8; ++i) f[i] = turned ? y[i] : f[i];
             }
@@ -264,8 +267,14 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvView kv, AppendArgs a)
                 const long long slot = (((long long)at.page * kv.heads + h) << kv.shift) + at.inside;
                 uint16_t *to = which == 2 ? a.q_out + row * a.o_row + h * a.o_head
                                           : static_cast<uint16_t *>(is_v ? kv.v : kv.k) + slot * D;
-                *reinterpret_cast<uint2 *>(to + first) = make_uint2(kv_pack_bf16(f[0], f[1]), kv_pack_bf16(f[2], f[3]));
-                *reinterpret_cast<uint2 *>(to + second) = make_uint2(kv_pack_bf16(f[4], f[5]), kv_pack_bf16(f[6], f[7]));
+                uint32_t o[4] = {w[0], w[1], w[2], w[3]}; /* what is not turned goes as it came: a conversion would quiet a NaN */
+                if (!is_v) {
+                    if constexpr (FMT == W4A16_KV_BF16) turn();
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[i] = turned ? kv_pack_bf16(y[2 * i], y[2 * i + 1]) : w[i];
+                }
+                *reinterpret_cast<uint2 *>(to + first) = make_uint2(o[0], o[1]);
+                *reinterpret_cast<uint2 *>(to + second) = make_uint2(o[2], o[3]);
             } else {
                 float most = 0.0f;
                 bool finite = true;
