@@ -852,7 +852,8 @@ class KvCache:
 
     def keep_path(self, batch, path, stream=None):
         """Token j of each sequence's rows takes what its token path[s, j] (int32, more than j) holds: verify_tree's path goes to the
-        front of its tree. Entries that are not more than their place leave it as it is."""
+        front of its tree, if the batch's rows are the trees' nodes, all of them and no others. Entries that are not more than their
+        place leave it as it is."""
         import torch
 
         index = _on_current(self.device, "KvCache.keep_path")

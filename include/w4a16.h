@@ -478,7 +478,9 @@ int w4a16_paged_tree_attention_bf16(const W4A16KvCache *cache, const W4A16KvBatc
 
 /* Moves the tokens of a tree's path to its front: token j of sequence s's new ones (rows of the batch; j < width) takes what its token
  * path[s * width + j] holds, for entries of more than j; the others (-1 among them) leave their tokens as they are. What is
- * moved are codes and scales as they stand. The lengths are the caller's to cut back behind the path. */
+ * moved are codes and scales as they stand. w4a16_verify_tree_f32's paths count from the tree's root: for them the batch's rows are the nodes of
+ * the trees, all of them and no others, also where they were appended in several calls or in one with other rows. The lengths are the caller's
+ * to cut back behind the path: a tree of n nodes of which a were taken leaves n - 1 - a tokens less. */
 int w4a16_kv_keep_path(const W4A16KvCache *cache, const W4A16KvBatch *batch, const int32_t *path, int width, void *stream);
 
 /* Beam search. The `take` best continuations of each of `groups` groups of `beams` beams: of all (b, v) the largest
