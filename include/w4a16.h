@@ -468,7 +468,10 @@ int w4a16_kv_tree_plan(const W4A16KvBatch *batch, const int32_t *parents, int pa
 /* w4a16_paged_attention_bf16 for such rows: a row sees the tokens before its sequence's tree, and of the tree the nodes that
  * its bits name, none behind its own place. window > 0 (at least `nodes`): none of the tokens before the tree whose position is
  * `window` or more before the row's (positions outside base .. the row's place count as the nearer of the two, base being the
- * tokens before the tree). The workspace is as w4a16_paged_attention_bf16's, of the bytes w4a16_paged_tree_attention_workspace gives. */
+ * tokens before the tree). With a BF16 cache the weights are rounded to 2^-15 in calls where no sequence, by max_new, has more than 32 rows (new
+ * tokens times the query heads of a key head); in others to 2^-8 at most, and which rows are rounded less depends on the call's bounds, max_kv
+ * among them, not on the rows alone: a sequence of few rows may be rounded otherwise beside one of many. With an 8-bit cache all are as
+ * there. The workspace is as w4a16_paged_attention_bf16's, of the bytes w4a16_paged_tree_attention_workspace gives. */
 int w4a16_paged_tree_attention_workspace(const W4A16KvCache *cache, const W4A16KvBatch *batch, int q_heads, size_t *bytes);
 int w4a16_paged_tree_attention_bf16(const W4A16KvCache *cache, const W4A16KvBatch *batch, const W4A16KvTree *tree,
                                     const uint16_t *q, long long q_row_stride, long long q_head_stride,
