@@ -660,6 +660,9 @@ class _KvTreeStruct(ctypes.Structure):
     _fields_ = [("seen", _vp), ("positions", _vp), ("sizes", _vp), ("nodes", _i)]
 
 
+_INT_MAX = 2**31 - 1  # ctypes cuts a C int off without a word
+
+
 def _refuse(what):
     raise W4A16Error(W4A16_ERR_CONFIG, what)
 
@@ -925,6 +928,8 @@ class KvBatch:
         self.page_table, self.kv_lens, self.starts = page_table, kv_lens, starts
         self.device, self.rows, self.padded = kv_lens.device, rows, padded
         stride = page_table.stride(0) if seqs > 1 else pages
+        if stride > _INT_MAX:
+            _refuse(f"KvBatch: the table's rows are {stride} entries apart")
         self._c = _KvBatchStruct(page_table.data_ptr(), kv_lens.data_ptr(), starts.data_ptr(), seqs, rows, pages,
                                  stride, max_new, max_kv)
         self._ref = ctypes.addressof(self._c)
@@ -961,6 +966,8 @@ class KvTree:
         self._c = _KvTreeStruct(self.seen.data_ptr(), self.positions.data_ptr(), self._sizes, nodes)
         self._ref = ctypes.addressof(self._c)
         self._stride = parents.stride(0) if seqs > 1 else nodes
+        if self._stride > _INT_MAX:
+            _refuse(f"KvTree: the rows of parents are {self._stride} entries apart")
         self.update(stream)
 
     def update(self, stream=None):
@@ -1040,15 +1047,15 @@ def _tables(page_table, kv_lens, third, device, what):
     try:
         seqs, pages = page_table.shape
         stride, one = page_table.stride()
-        if (one == 1 and page_table.dtype == kind and page_table.device == device and kv_lens.shape == (seqs,) and kv_lens.dtype == kind and
+        if (one == 1 and stride <= _INT_MAX and page_table.dtype == kind and page_table.device == device and kv_lens.shape == (seqs,) and kv_lens.dtype == kind and
                 kv_lens.device == device and kv_lens.is_contiguous() and third.numel() == seqs and 1 <= third.dim() <= 2 and third.dtype == kind and
                 third.device == device and third.is_contiguous()):
             return page_table.data_ptr(), stride if seqs > 1 else pages, pages, kv_lens.data_ptr(), third.data_ptr()
     except (AttributeError, TypeError, ValueError):
         pass  # named below
     if not hasattr(page_table, "is_cuda") or page_table.device != device or page_table.dtype != torch.int32 or page_table.dim() != 2 or \
-            (page_table.shape[1] > 1 and page_table.stride(1) != 1):
-        _refuse(f"{what}: the table is no int32 tensor [seqs, pages] on {device} with a dense last axis")
+            (page_table.shape[1] > 1 and page_table.stride(1) != 1) or (page_table.shape[0] > 1 and page_table.stride(0) > _INT_MAX):
+        _refuse(f"{what}: the table is no int32 tensor [seqs, pages] on {device} with a dense last axis, rows under 2^31 apart")
     seqs, pages = page_table.shape
     return (page_table.data_ptr(), page_table.stride(0) if seqs > 1 else pages, pages,
             _exactly(kv_lens, (seqs,), torch.int32, device, f"{what} kv_lens"),
@@ -1112,7 +1119,8 @@ def beam_tables(page_table, kv_lens, parents, page_size, out=None, stream=None):
     groups, beams = parents.shape
     if out is None:
         out = torch.empty_like(page_table, memory_format=torch.contiguous_format)
-    elif out.shape != page_table.shape or out.dtype != torch.int32 or out.device != device or (pages > 1 and out.stride(1) != 1):
+    elif out.shape != page_table.shape or out.dtype != torch.int32 or out.device != device or (pages > 1 and out.stride(1) != 1) or \
+            (groups * beams > 1 and out.stride(0) > _INT_MAX):
         _refuse(f"beam_tables: out is no int32 tensor {tuple(page_table.shape)} on {device} with a dense last axis")
     source = torch.empty_like(kv_lens)
     st = lib.w4a16_beam_tables(tp, stride, pages, lp, pp, groups, beams, page_size, out.data_ptr(),
