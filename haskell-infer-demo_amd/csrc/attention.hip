@@ -459,7 +459,7 @@ constexpr int rows_blocks(int dim, int format, int rt) {
  *
  * Bound by memory: 32 sequences of 8192 tokens, one row of 32 heads each (16 of 256 values), the join included:
  * BF16 D = 64 102 us (5.2 TB/s), D = 128 192 (5.6), D = 256 200 (5.4); FP8 66 (4.4), 108 (5.1), 107 (5.1); INT8
- * 70, 110, 109. Trees: two of which 5 rows grow over 100003 tokens, 24 heads over 4 of 256, INT8, 102 us (4.2 TB/s; VALU 50 %, one
+ * 70, 110, 109. Trees: two of which 5 rows grow over 100003 tokens, 24 heads over 4 of 256, INT8, 100 us (4.2 TB/s; VALU 52 %, one
  * block a CU) and 7.2 for the join; one of 26 over 1500 tokens, 32 over 8 heads of 128, BF16, 12.9 and 4.0.
  */
 template <int D, int FMT, int RT, bool TREE>
@@ -978,8 +978,8 @@ __device__ __forceinline__ uint32_t widen_f16(uint32_t codes) {
  * that it is bound by the weights' VALU work (five instructions each, and for 8-bit caches the widening
  * of a tile over 128 rows). 4096 rows over 16384 tokens, 32 heads (16 of 256 values): BF16 D = 64 671 us, 717
  * TFLOP/s; D = 128 979, 983; D = 256 1017, 946; INT8 859, 1193, 1308; FP8 748, 1134, 1269. Trees: 16 of up to 60 over up to
- * 8192 tokens, 32 heads over 8 of 128, FP8, 87.5 us, VALU 39 % and MFMA 22 % busy, 1.7 waves a SIMD: a tile's way through the registers to
- * LDS is waited for; 8 of up to 251 over up to 16384, window 4096, 32 over 4 of 64, BF16, 90.6, VALU 58 %.
+ * 8192 tokens, 32 heads over 8 of 128, FP8, 86.9 us, VALU 39 % and MFMA 22 % busy, 1.7 waves a SIMD: a tile's way through the registers to
+ * LDS is waited for; 8 of up to 251 over up to 16384, window 4096, 32 over 4 of 64, BF16, 88.2, VALU 58 %.
  */
 template <int D, int FMT, bool TIGHT, bool TREE>
 struct Chunk {

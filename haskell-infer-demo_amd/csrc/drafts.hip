@@ -9,7 +9,8 @@
  * the probability that it has among what its refused siblings leave, p(x) / (1 - sum of theirs), and behind the last taken
  * node one token is drawn from its row without its children. Every wave goes through the tree by itself: a
  * lane has a node (four with more than 64) and its probability, all gathered at once, and a step down is ballots and lane reads. A tree of
- * 26 over 151936 words: 5.3 + 4.2 us, 24 of 40 over 100003: 7.0 + 5.1; bound as below.
+ * 26 over 151936 words, four of them taken: 5.5 + 3.8 us (none: 5.0 + 4.2); 24 of 40 over 100003, three taken: 9.4 + 4.2 (none: 8.5 + 4.4, and 7.0
+ * where the targets stand in a cache); bound as below.
  *
  * Up to kSmall words: one launch of one block a sequence that holds the row's weights in registers.
  * More: two launches. drafts_sum_kernel: every block finds its sequence's first refused token (a few

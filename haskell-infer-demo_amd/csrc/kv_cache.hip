@@ -168,8 +168,8 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvView kv, uint16_t *k, ui
  * Work beyond the row's place comes in steps of 64 lanes (1 KiB): heads of K, of V, of q, in this order, kAhead of them on
  * their way at a time.
  *
- * Bound by memory: 8198 rows of 32 queries and 8 keys of 128, BF16, 41 us, 203 MB at 4.9 TB/s (a large copy's rate). 592 rows
- * of 24 + 4 heads of 256, INT8, 6.1 us; four rows 3.8, a launch and four dependent round trips.
+ * Bound by memory: 8198 rows of 32 queries and 8 keys of 128, BF16, 40 us, 203 MB at 5.0 TB/s (a large copy's rate). 592 rows
+ * of 24 + 4 heads of 256, INT8, 6.2 us; four rows 3.8, a launch and four dependent round trips.
  */
 struct AppendArgs {
     const uint16_t *k, *v, *q;
