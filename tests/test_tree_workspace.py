@@ -87,3 +87,35 @@ def test_sequences_that_overlap(cuda, news, q_heads):
     out = w4a16.paged_attention(q, of, held, tree=tree, workspace=space[:need])
     torch.cuda.synchronize()
     assert (space[need:] == 171).all() and out.shape == q.shape
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["bf16", "fp8"])
+@pytest.mark.parametrize("news", [2, 33])
+def test_very_many_sequences(cuda, news, fmt):
+    """More than 65536 pairs, and one long sequence that is cut all the same: it, and some of the others, against FP64."""
+    print(f"very many: {fmt} {news}", flush=True)
+    count, page, heads, q_heads, dim, longest, held_pages = 8300, 16, 8, 8, 64, 4000, 300
+    kv_lens = [news + i % 11 for i in range(count)]
+    kv_lens[5000] = longest
+    columns = -(-longest // page)
+    table = (torch.arange(count)[:, None] * 7 + torch.arange(columns) * 11) % held_pages  # pages are shared: nothing writes
+    starts = torch.arange(count + 1, dtype=torch.int32) * news
+    batch_of = w4a16.KvBatch(table.to(torch.int32).to(cuda), torch.tensor(kv_lens, dtype=torch.int32, device=cuda), starts.to(cuda), count * news,
+                             max_new=news, max_kv=longest)
+    of = filled(held_pages, page, heads, dim, fmt, cuda, seed=2)
+    parents = short.random_parents(count, news, news, "random")
+    tree = w4a16.KvTree(parents.to(cuda), batch_of)
+    q = (2 * torch.randn(count * news, q_heads, dim, generator=torch.Generator().manual_seed(1))).to(torch.bfloat16)
+    need = asked(of._c, batch_of._c, q_heads)
+    space = torch.full((need + GUARD,), 171, dtype=torch.uint8, device=cuda)
+    out, lse = w4a16.paged_attention(q.to(cuda), of, batch_of, return_lse=True, tree=tree, workspace=space[:need])
+    assert (space[need:] == 171).all()
+    some = [0, 1, 63, 64, 4999, 5000, 5001, 8255, 8256, count - 1]
+    rows = torch.cat([torch.arange(s * news, (s + 1) * news) for s in some])
+    lens, tables = [kv_lens[s] for s in some], [table[s].tolist() for s in some]
+    (seen, positions), sizes = short.plan_of(parents[some], None, lens, [news] * len(some))
+    k, v, there = whole(of, tables, lens, page, held_pages)
+    seen_by = tree_oracle.visible(seen, positions, sizes, lens, [news] * len(some), news, 0)
+    tree_oracle.check(out.cpu()[rows], lse.cpu()[rows], tree_oracle.attention(q[rows], k, v, there, seen_by, dim**-0.5,
+                                                                              kv_check.sizes(of, tables, lens, page, held_pages)))
